@@ -485,6 +485,92 @@ int kf_sparse_wgrad(const float* x, const float* dy, const float* coef, const fl
                     const float* grid, float* dcoef, float* dbase, float* dscale, float* dbias, float* workspace,
                     int64_t B, int32_t I, int32_t O, const kf_basis_desc* basis, void* stream);
 
+/* ---- residual norm: the join between two blocks of a transformer ------------
+ * u = N_b(branch) w_b + s_b (branch_norm) or the branch itself,
+ * y = residual_scale x + gate u,  h = N(y) w + s, with N(v) = (v - mean) /
+ * sqrt(var + eps) (layer != 0) or v / sqrt(mean(v^2) + eps); float32 between
+ * the loads and the stores.  x, y, dy, dx (rows, width) in x_dtype; branch, h,
+ * dh, dbranch and a token gate (rows, width) in branch_dtype (x_dtype bf16 with
+ * a float32 branch is refused); w, s, bw, bs and a channel gate (width) in
+ * param_dtype.  s, bs, gate may be null; branch null: h = N(x) w + s alone, y
+ * is x.  stats (rows, 4) float32 receives mean and 1/std of y and of the
+ * branch for the backward (null: not written).  width 1 .. 8192.
+ * Backward: y is formed again from x and the branch; dy or dh may be null (no gradient); dw, ds, dbw, dbs and a channel
+ * gate's dgate may be null when not wanted; their sums over rows run in a fixed
+ * order through workspace (kf_residual_norm_workspace floats). */
+typedef struct kf_residual_norm_desc {
+  int32_t width;
+  int32_t layer;       /* 1: layer norm, 0: root mean square */
+  int32_t branch_norm; /* 1: the branch is normed first */
+  int32_t gate_token;  /* 1: gate (rows, width), 0: gate (width) */
+  int32_t x_dtype, branch_dtype, param_dtype;
+  float residual_scale, eps;
+} kf_residual_norm_desc;
+
+int kf_residual_norm_fwd(const void* x, const void* branch, const void* gate, const void* w, const void* s,
+                         const void* bw, const void* bs, void* y, void* h, float* stats, int64_t rows,
+                         const kf_residual_norm_desc* desc, void* stream);
+int64_t kf_residual_norm_workspace(int64_t rows, int32_t width);
+int kf_residual_norm_bwd(const void* x, const void* branch, const void* gate, const void* w, const void* bw,
+                         const void* bs, const float* stats, const void* dy, const void* dh, void* dx, void* dbranch,
+                         void* dgate, void* dw, void* ds, void* dbw, void* dbs, float* workspace,
+                         int64_t rows, const kf_residual_norm_desc* desc, void* stream);
+
+/* ---- attention over packed sequences ----------------------------------------
+ * Sequence s owns q_len rows of q from q_start and k_len rows of k and v from
+ * k_start; its queries stand at the last q_len of its k_len positions.  For a
+ * query at position p, head h (key head h / (heads / kv_heads)) and key j:
+ *   S_j = scale q.k_j + table[buckets[clamp(p - j, -span, span) + span]][h],
+ * over j < k_len, and j <= p when causal; o = sum_j softmax(S)_j v_j, 0 where
+ * no key is visible.  Keys and values outside a sequence never enter, whatever
+ * they hold.  Scores, softmax and sums are float32; bf16 inputs round the
+ * probabilities (and dS in the backward) to bf16 for the tensor cores.
+ *   seqs    (n_seqs, 4) int32: q_start, q_len, k_start, k_len
+ *   q_tiles (n_q_tiles, 2) int32: sequence and tile of its query rows, one entry
+ *           for every kf_attention_tile_rows() rows of every sequence, any
+ *           order; k_tiles likewise for the key rows
+ *   table   (n_buckets, heads) in table_dtype, buckets (2 span + 1) int32; null: no bias
+ *   o       (tq, heads, dim) contiguous; lse (heads, tq) float32, base 2 (null: not written)
+ * q, k, v in dtype with the strides of the descriptor (elements; head width
+ * contiguous).  Backward: dout like o; dq, dk, dv contiguous; dtable
+ * (n_buckets, heads) in table_dtype or null; workspace
+ * kf_attention_bwd_workspace floats.  Every sum runs in a fixed order. */
+typedef struct kf_attention_desc {
+  int64_t tq, tk;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  int32_t heads, kv_heads, dim, n_seqs;
+  int32_t dtype, causal;
+  int32_t span, n_buckets, table_dtype;
+  float scale;
+} kf_attention_desc;
+
+int kf_attention_tile_rows(const kf_attention_desc* desc);
+int kf_attention_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* q_tiles,
+                     int32_t n_q_tiles, const void* table, const int32_t* buckets, void* o, float* lse,
+                     const kf_attention_desc* desc, void* stream);
+int64_t kf_attention_bwd_workspace(int32_t n_q_tiles, const kf_attention_desc* desc);
+int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
+                     const int32_t* seqs, const int32_t* q_tiles, int32_t n_q_tiles, const int32_t* k_tiles,
+                     int32_t n_k_tiles, const void* table, const int32_t* buckets, void* dq, void* dk, void* dv,
+                     void* dtable, float* workspace, const kf_attention_desc* desc, void* stream);
+
+/* One new token per sequence over its cache: q (batch, heads, dim) attends to
+ * the first lengths[b] (clamped to [0, capacity]) rows of k, v (batch,
+ * capacity, kv_heads, dim) and stands at the last of them.  Slots past the
+ * length are not read.  o (batch, heads, dim) contiguous; workspace: batch *
+ * heads * splits * (dim + 2) floats with splits = kf_attention_decode_splits()
+ * (none for one split). */
+typedef struct kf_decode_desc {
+  int64_t q_batch, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head;
+  int32_t batch, capacity, heads, kv_heads, dim;
+  int32_t dtype, span, table_dtype;
+  float scale;
+} kf_decode_desc;
+
+int kf_attention_decode_splits(const kf_decode_desc* desc);
+int kf_attention_decode(const void* q, const void* k, const void* v, const int32_t* lengths, const void* table,
+                        const int32_t* buckets, void* o, float* workspace, const kf_decode_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

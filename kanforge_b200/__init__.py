@@ -11,11 +11,13 @@ The forward and backward passes, the closed derivative primitives and
 """
 
 from . import bases, convert, kernels
+from .attention import PackedSequences, RelativeBias, attention, attention_decode
 from .bases import *  # noqa: F401,F403
 from .bases import __all__ as _bases_all
 from .conv import KANConv1d, KANConv2d, KANConv3d
 from .convert import load, save
 from .layers import GRKAN, KAN, KANLinear, layer_inputs, rebuild_kan
+from .norm import ResidualNorm, residual_norm
 from .plan import KernelPlan, plan_for
 from .transformer import KANFFN
 
@@ -31,6 +33,11 @@ __all__ = [
     "KANFFN",
     "KANLinear",
     "KernelPlan",
+    "PackedSequences",
+    "RelativeBias",
+    "ResidualNorm",
+    "attention",
+    "attention_decode",
     "bases",
     "convert",
     "kernels",
@@ -38,6 +45,7 @@ __all__ = [
     "load",
     "plan_for",
     "rebuild_kan",
+    "residual_norm",
     "save",
     "__version__",
 ]

@@ -81,6 +81,35 @@ class FitBasis(ctypes.Structure):
     ]
 
 
+class ResidualNormDesc(ctypes.Structure):
+    """``kf_residual_norm_desc`` (include/kanforge_b200.h)."""
+
+    _fields_ = [(n, _c_i32) for n in ("width", "layer", "branch_norm", "gate_token", "x_dtype", "branch_dtype", "param_dtype")] + [
+        ("residual_scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class AttentionDesc(ctypes.Structure):
+    """``kf_attention_desc`` (include/kanforge_b200.h)."""
+
+    _fields_ = (
+        [(n, _c_i64) for n in ("tq", "tk", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
+        + [(n, _c_i32) for n in ("heads", "kv_heads", "dim", "n_seqs", "dtype", "causal", "span", "n_buckets", "table_dtype")]
+        + [("scale", ctypes.c_float)]
+    )
+
+
+class DecodeDesc(ctypes.Structure):
+    """``kf_decode_desc`` (include/kanforge_b200.h)."""
+
+    _fields_ = (
+        [(n, _c_i64) for n in ("q_batch", "q_head", "k_batch", "k_row", "k_head", "v_batch", "v_row", "v_head")]
+        + [(n, _c_i32) for n in ("batch", "capacity", "heads", "kv_heads", "dim", "dtype", "span", "table_dtype")]
+        + [("scale", ctypes.c_float)]
+    )
+
+
 KF_GRID_MAX_POINTS, KF_FIT_MAX_SIZE = 192, 256
 
 _GEOM = ctypes.POINTER(ConvGeom)
@@ -202,6 +231,21 @@ PROTOTYPES = {
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, ctypes.POINTER(BasisDesc), _vp],
     ),
+    "kf_residual_norm_fwd": (ctypes.c_int, [_vp] * 10 + [_c_i64, ctypes.POINTER(ResidualNormDesc), _vp]),
+    "kf_residual_norm_workspace": (_c_i64, [_c_i64, _c_i32]),
+    "kf_residual_norm_bwd": (ctypes.c_int, [_vp] * 17 + [_c_i64, ctypes.POINTER(ResidualNormDesc), _vp]),
+    "kf_attention_tile_rows": (ctypes.c_int, [ctypes.POINTER(AttentionDesc)]),
+    "kf_attention_fwd": (
+        ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _vp, _vp, _vp, ctypes.POINTER(AttentionDesc), _vp],
+    ),
+    "kf_attention_bwd_workspace": (_c_i64, [_c_i32, ctypes.POINTER(AttentionDesc)]),
+    "kf_attention_bwd": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+         ctypes.POINTER(AttentionDesc), _vp],
+    ),
+    "kf_attention_decode_splits": (ctypes.c_int, [ctypes.POINTER(DecodeDesc)]),
+    "kf_attention_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(DecodeDesc), _vp]),
     "kf_rational_bwd_noalloc": (
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i32, ctypes.POINTER(BasisDesc), ctypes.c_int, _vp],

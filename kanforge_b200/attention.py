@@ -1,0 +1,306 @@
+"""Attention of a KAN transformer: packed sequences, a learned relative position
+bias, and the single-token form over a cache.
+
+``attention`` runs whole prompts of different lengths packed into one batch,
+causal or both ways, with query heads that share key heads, forward and
+backward (``kf_attention_fwd`` / ``kf_attention_bwd``); ``RelativeBias`` adds
+its bucketed bias to the scores inside those kernels, so that no (query, key)
+matrix ever exists; ``attention_decode`` answers with one token per sequence
+(``kf_attention_decode``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .kernels import _check_cuda, _launch, _ptr, _stream
+
+ATTENTION_MAX_DIM = 128
+BIAS_MAX_DISTANCE, BIAS_MAX_BUCKETS = 2048, 256
+
+_DTYPE_CODE = {torch.float32: _lib.KF_DTYPE_F32, torch.bfloat16: _lib.KF_DTYPE_BF16}
+
+
+class PackedSequences:
+    """The lengths of sequences packed one after another, as the kernels read them.
+
+    ``q_lens`` are the query rows of each sequence and ``kv_lens`` (default: the
+    same) its key and value rows; a sequence's queries stand at the last of its
+    positions.  Zero lengths are allowed.  Build it once for a batch layout and
+    pass it to every layer's call; the tables lie on ``device``.
+    """
+
+    def __init__(self, q_lens, kv_lens=None, device="cuda"):
+        self.q_lens = [int(n) for n in q_lens]
+        self.kv_lens = list(self.q_lens) if kv_lens is None else [int(n) for n in kv_lens]
+        if len(self.q_lens) != len(self.kv_lens):
+            raise ValueError(f"{len(self.q_lens)} query lengths and {len(self.kv_lens)} key lengths")
+        if any(n < 0 for n in self.q_lens + self.kv_lens):
+            raise ValueError("lengths must not be negative")
+        self.total_q, self.total_kv = sum(self.q_lens), sum(self.kv_lens)
+        if max(self.total_q, self.total_kv) >= 2**31:
+            raise ValueError("a batch holds fewer than 2**31 rows")
+        rows, q0, k0 = [], 0, 0
+        for lq, lk in zip(self.q_lens, self.kv_lens):
+            rows.append((q0, lq, k0, lk))
+            q0, k0 = q0 + lq, k0 + lk
+        self.device = torch.device(device)
+        self.table = torch.tensor(rows, dtype=torch.int32).reshape(-1, 4).to(self.device)
+        self.device = self.table.device
+        self._tiles: dict = {}
+
+    def __len__(self) -> int:
+        return len(self.q_lens)
+
+    def tiles(self, side: str, rows: int, causal: bool) -> torch.Tensor:
+        """(n, 2) int32 (sequence, tile): every ``rows`` rows of the query ("q") or
+        key ("k") side, those with the most work first."""
+        key = (side, rows, causal)
+        if key not in self._tiles:
+            found = []
+            for s, (lq, lk) in enumerate(zip(self.q_lens, self.kv_lens)):
+                off = lk - lq
+                for t in range(-(-(lq if side == "q" else lk) // rows)):
+                    if not causal:
+                        cost = lk if side == "q" else lq
+                    elif side == "q":
+                        cost = max(0, min(lk, (t + 1) * rows + off))
+                    else:
+                        cost = max(0, lq - max(0, t * rows - off))
+                    found.append((-cost, s, t))
+            found.sort()
+            self._tiles[key] = torch.tensor([f[1:] for f in found], dtype=torch.int32).reshape(-1, 2).to(self.device)
+        return self._tiles[key]
+
+
+def relative_buckets(num_buckets: int, max_distance: int, bidirectional: bool) -> list[int]:
+    """Bucket of every distance position - key from -max_distance to max_distance.
+
+    One way (causal), keys after the query share bucket 0; both ways, keys after
+    the query take the upper half of the buckets.  Of the n buckets of a
+    direction the first e = n // 2 hold one distance each and the others grow
+    geometrically: bucket e + floor(log(d / e) / log(max_distance / e) * (n - e)),
+    at most n - 1.  The floor is exact (integers are compared)."""
+    n = num_buckets // 2 if bidirectional else num_buckets
+    exact = n // 2
+    steps = n - exact
+
+    def one_way(d: int) -> int:
+        if d < exact:
+            return d
+        b = 0
+        while b + 1 < steps and d**steps >= exact ** (steps - b - 1) * max_distance ** (b + 1):
+            b += 1
+        return exact + b
+
+    out = []
+    for d in range(-max_distance, max_distance + 1):
+        if bidirectional:
+            out.append(one_way(abs(d)) + (n if d < 0 else 0))
+        else:
+            out.append(one_way(max(0, d)))
+    return out
+
+
+class RelativeBias(nn.Module):
+    """A learned bias per (bucket of the distance query - key, head), added to the
+    attention scores; distances from ``max_distance`` on share a bucket (see
+    ``relative_buckets``).  ``weight`` is (num_buckets, heads)."""
+
+    def __init__(self, heads: int, num_buckets: int = 32, max_distance: int = 128, bidirectional: bool = True, *,
+                 device=None, dtype=None):
+        super().__init__()
+        n = num_buckets // 2 if bidirectional else num_buckets
+        if n < 2 or num_buckets > BIAS_MAX_BUCKETS or (bidirectional and num_buckets % 2):
+            raise ValueError(f"num_buckets must be 2 to {BIAS_MAX_BUCKETS} (an even number from 4 when bidirectional)")
+        if not n // 2 < max_distance <= BIAS_MAX_DISTANCE:
+            raise ValueError(f"max_distance must exceed {n // 2} and be at most {BIAS_MAX_DISTANCE}")
+        if heads < 1:
+            raise ValueError("heads must be positive")
+        self.heads, self.num_buckets, self.max_distance, self.bidirectional = heads, num_buckets, max_distance, bidirectional
+        self.weight = nn.Parameter(torch.zeros(num_buckets, heads, device=device, dtype=dtype))
+        buckets = torch.tensor(relative_buckets(num_buckets, max_distance, bidirectional), dtype=torch.int32)
+        self.register_buffer("buckets", buckets if device is None else buckets.to(device), persistent=False)
+
+    def forward(self, distance: torch.Tensor) -> torch.Tensor:
+        """(..., heads): the bias of integer distances query - key."""
+        at = distance.clamp(-self.max_distance, self.max_distance) + self.max_distance
+        return self.weight[self.buckets[at].long()]
+
+
+def _vectors(t: torch.Tensor) -> torch.Tensor:
+    """t, or a contiguous copy when its rows cannot be read in 16-byte vectors."""
+    per = 16 // t.element_size()
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+        s % per == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_heads(q, k, v, bias) -> tuple[int, int, int]:
+    _check_cuda(q, k, v)
+    heads, dim, kv_heads = q.shape[-2], q.shape[-1], k.shape[-2]
+    if q.dtype not in _DTYPE_CODE:
+        raise TypeError(f"attention takes float32 or bfloat16, not {q.dtype}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k and v must have one type (got {q.dtype}, {k.dtype}, {v.dtype})")
+    if k.shape != v.shape or k.shape[-1] != dim:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    if dim % 8 or not 8 <= dim <= ATTENTION_MAX_DIM:
+        raise ValueError(f"the head width must be a multiple of 8 up to {ATTENTION_MAX_DIM}, not {dim}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads do not divide over {kv_heads} key heads")
+    if heads > 65535:
+        raise ValueError("at most 65535 heads")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError(f"tensors lie on {q.device}, {k.device} and {v.device}")
+    if bias is not None:
+        if bias.heads != heads:
+            raise ValueError(f"the bias has {bias.heads} heads, the queries {heads}")
+        if bias.weight.device != q.device:
+            raise ValueError(f"the bias lies on {bias.weight.device}, the queries on {q.device}")
+        if bias.weight.dtype not in _DTYPE_CODE:
+            raise TypeError(f"the bias must be float32 or bfloat16, not {bias.weight.dtype}")
+    return heads, kv_heads, dim
+
+
+class _Call:
+    """The operands of one packed attention call as the kernels take them."""
+
+    __slots__ = ("q", "k", "v", "seqs", "causal", "desc", "table", "buckets")
+
+    def __init__(self, q, k, v, table, seqs, causal, scale, bias):
+        self.q, self.k, self.v = (_vectors(t.detach()) for t in (q, k, v))
+        self.seqs, self.causal = seqs, causal
+        self.table = None if table is None else table.detach().contiguous()
+        self.buckets = None if table is None else bias.buckets
+        q, k, v = self.q, self.k, self.v
+        self.desc = _lib.AttentionDesc(
+            q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            q.shape[1], k.shape[1], q.shape[2], len(seqs), _DTYPE_CODE[q.dtype], int(causal),
+            0 if table is None else bias.max_distance, 0 if table is None else bias.num_buckets,
+            0 if table is None else _DTYPE_CODE[table.dtype], scale)
+
+    def tiles(self, side: str) -> torch.Tensor:
+        rows = _lib.load().kf_attention_tile_rows(ctypes.byref(self.desc))
+        return self.seqs.tiles(side, rows, self.causal)
+
+    def forward(self, with_lse: bool):
+        q = self.q
+        o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        lse = torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32) if with_lse else None
+        tiles = self.tiles("q")
+        if tiles.shape[0]:
+            _launch("kf_attention_fwd", _ptr(q), _ptr(self.k), _ptr(self.v), _ptr(self.seqs.table), _ptr(tiles),
+                    tiles.shape[0], _ptr(self.table), _ptr(self.buckets), _ptr(o), _ptr(lse), ctypes.byref(self.desc),
+                    _stream(q))
+        return o, lse
+
+    def backward(self, o, lse, dout, want_table: bool):
+        q, k = self.q, self.k
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
+        dtable = torch.empty_like(self.table) if want_table else None
+        q_tiles, k_tiles = self.tiles("q"), self.tiles("k")
+        n_ws = int(_lib.load().kf_attention_bwd_workspace(q_tiles.shape[0], ctypes.byref(self.desc)))
+        ws = torch.empty(max(n_ws, 1), device=q.device, dtype=torch.float32)
+        if q_tiles.shape[0] or k_tiles.shape[0] or want_table:
+            _launch("kf_attention_bwd", _ptr(q), _ptr(k), _ptr(self.v), _ptr(o), _ptr(dout), _ptr(lse),
+                    _ptr(self.seqs.table), _ptr(q_tiles), q_tiles.shape[0], _ptr(k_tiles), k_tiles.shape[0],
+                    _ptr(self.table), _ptr(self.buckets), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), _ptr(ws),
+                    ctypes.byref(self.desc), _stream(q), kernels=3 + int(want_table))
+        return dq, dk, dv, dtable
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, seqs, causal, scale, bias):
+        o, lse = _Call(q, k, v, table, seqs, causal, scale, bias).forward(with_lse=True)
+        ctx.save_for_backward(q, k, v, table, o, lse)
+        ctx.options = (seqs, causal, scale, bias)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, o, lse = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        call = _Call(q, k, v, table, *ctx.options)
+        dout = dout.to(q.dtype).contiguous()
+        dout = _vectors(dout)
+        dq, dk, dv, dtable = call.backward(o, lse, dout, table is not None and need[3])
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None, None, None)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: PackedSequences, *, causal: bool = True,
+              scale: float | None = None, bias: RelativeBias | None = None) -> torch.Tensor:
+    """softmax(scale q k^T + bias) v over each packed sequence: (Tq, heads, dim).
+
+    ``q`` is (Tq, heads, dim), ``k`` and ``v`` (Tk, kv_heads, dim), float32 or
+    bfloat16, strided as they come (views of one projection's output are read
+    in place); query head h uses key head h // (heads / kv_heads).  ``scale``
+    defaults to 1/sqrt(dim).  ``causal`` queries see the keys up to their own
+    position; a query that sees no key gives 0 and passes no gradient.  Rows
+    of other sequences never enter a result, whatever they hold; a non-finite
+    value of a later key of the same sequence may reach a causal query near it.
+    Gradients reach q, k, v and ``bias.weight``; every sum runs in a fixed order.
+    """
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("q, k and v must be (tokens, heads, dim)")
+    _heads, _kv_heads, dim = _check_heads(q, k, v, bias)
+    if not isinstance(seqs, PackedSequences):
+        raise TypeError("seqs must be a PackedSequences")
+    if q.shape[0] != seqs.total_q or k.shape[0] != seqs.total_kv:
+        raise ValueError(f"the sequences hold {seqs.total_q} query and {seqs.total_kv} key rows, the tensors {q.shape[0]} "
+                         f"and {k.shape[0]}")
+    if seqs.device != q.device:
+        raise ValueError(f"the sequences lie on {seqs.device}, the queries on {q.device}")
+    table = None if bias is None else bias.weight
+    args = (q, k, v, table, seqs, bool(causal), 1.0 / math.sqrt(dim) if scale is None else float(scale), bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        return _Attention.apply(*args)
+    return _Call(*args).forward(with_lse=False)[0]
+
+
+def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, *,
+                     scale: float | None = None, bias: RelativeBias | None = None) -> torch.Tensor:
+    """One new token per sequence over its cache: (batch, heads, dim).
+
+    ``q`` is (batch, heads, dim), the caches (batch, capacity, kv_heads, dim) and
+    ``lengths`` (batch,) int32 on the device: how many slots of each cache are
+    filled, the new token's own last.  Slots past the length are never read; a
+    length of 0 gives 0, one above the capacity counts as the capacity.
+    Inference only: tensors that require a gradient raise.
+    """
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("q must be (batch, heads, dim), the caches (batch, capacity, kv_heads, dim)")
+    heads, kv_heads, dim = _check_heads(q, k_cache, v_cache, bias)
+    batch, capacity = k_cache.shape[:2]
+    if q.shape[0] != batch or batch > 65535:
+        raise ValueError(f"q holds {q.shape[0]} sequences, the caches {batch} (at most 65535)")
+    if lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.device != q.device:
+        raise ValueError(f"lengths must be ({batch},) int32 on {q.device}")
+    tracked = [q, k_cache, v_cache] + ([bias.weight] if bias is not None else [])
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tracked):
+        raise RuntimeError("attention_decode has no backward: call it under torch.no_grad(), or use attention")
+    q, k, v = _vectors(q.detach()), _vectors(k_cache.detach()), _vectors(v_cache.detach())
+    lengths = lengths.contiguous()
+    table = None if bias is None else bias.weight.detach().contiguous()
+    desc = _lib.DecodeDesc(q.stride(0), q.stride(1), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1),
+                           v.stride(2), batch, capacity, heads, kv_heads, dim, _DTYPE_CODE[q.dtype],
+                           0 if bias is None else bias.max_distance, 0 if bias is None else _DTYPE_CODE[table.dtype],
+                           1.0 / math.sqrt(dim) if scale is None else float(scale))
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    if batch == 0:
+        return o
+    splits = _lib.load().kf_attention_decode_splits(ctypes.byref(desc))
+    ws = torch.empty(batch * heads * splits * (dim + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
+    _launch("kf_attention_decode", _ptr(q), _ptr(k), _ptr(v), _ptr(lengths), _ptr(table),
+            _ptr(None if bias is None else bias.buckets), _ptr(o), _ptr(ws), ctypes.byref(desc), _stream(q),
+            kernels=1 + (splits > 1))
+    return o

@@ -1,0 +1,75 @@
+// What the attention kernels share: the packed sequences, the launch operands
+// and the learned relative position bias.
+//
+// Query i of a sequence with Lq queries and Lk keys stands at position
+// i + Lk - Lq; with d = position - key, scores are kept in base 2:
+//   t = scale log2(e) q.k + log2(e) B[bucket(d), head],  P = 2^(t - lse),
+// and lse = max + log2(sum) is what the forward keeps for the backward.
+#pragma once
+
+#include <math_constants.h>
+
+#include "common.cuh"
+
+namespace kf {
+namespace attn {
+
+constexpr int kMaxDim = 128;
+constexpr int kMaxSpan = 2048;    // largest distance with a bias of its own
+constexpr int kMaxBuckets = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Seq {  // one row of the table of sequences
+  int q0, lq, k0, lk;
+};
+
+struct Strided {  // (tokens, heads, dim), last dimension contiguous; strides in elements
+  const void* p;
+  int64_t row, head;
+};
+
+struct Args {
+  Strided q, k, v, dout;
+  void* o;      // (Tq, H, D) contiguous; read by the backward
+  void *dq, *dk, *dv;
+  float* lse;   // (H, Tq)
+  float* delta; // (H, Tq): dO . O
+  const int4* seqs;
+  const int2* tiles;  // (sequence, tile of its rows)
+  const void* table;  // (buckets, H) bias, or null
+  const int* buckets; // (2 span + 1): bucket of distance index - span
+  float* dtable_part; // (tiles, H, buckets)
+  int64_t tq;
+  int heads, kv_heads, dim, span, n_buckets;
+  bool causal, table_bf16;
+  float scale;
+};
+
+__device__ __forceinline__ Seq load_seq(const Args& a, int s) {
+  const int4 v = a.seqs[s];
+  return Seq{v.x, v.y, v.z, v.w};
+}
+
+// A query that sees one key has P = 1 whatever its score: dS = 0, without the
+// rounding of dP - delta.
+__device__ __forceinline__ bool one_key(const Args& a, const Seq& s, int pos) { return s.lk == 1 || (a.causal && pos == 0); }
+
+// A bias in base 2; the lowest and highest finite values stay finite.
+__device__ __forceinline__ float bias_base2(float b) {
+  return isinf(b) ? b : fminf(fmaxf(b * kLog2e, -CUDART_MAX_NORMAL_F), CUDART_MAX_NORMAL_F);
+}
+
+// Bias of one head in base 2, by clamped distance.
+__device__ __forceinline__ void expand_bias(const Args& a, int head, float* out, int thread, int n_threads) {
+  for (int i = thread; i < 2 * a.span + 1; i += n_threads) {
+    const int64_t at = (int64_t)a.buckets[i] * a.heads + head;
+    const float b = a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[at])
+                                 : static_cast<const float*>(a.table)[at];
+    out[i] = bias_base2(b);
+  }
+}
+
+__device__ __forceinline__ int clamp_dist(int d, int span) { return min(max(d, -span), span) + span; }
+
+}  // namespace attn
+}  // namespace kf

@@ -1,0 +1,501 @@
+// Attention over packed sequences on the CUDA cores: float32 forward and
+// backward.
+//
+// A CTA of 16 x 16 threads owns 64 rows (queries, or keys in dK/dV) and walks
+// over tiles of 64 of the other side.  A thread holds a 4 x 4 block of the
+// scores and, of each output row, 4 x D/16 sums; operands are in shared memory
+// with rows 4 floats longer than D, so that the 16-byte reads of 16 rows fall
+// into different banks.  64 multiply-adds per eight 16-byte reads: the kernels
+// are bound by the FMA pipe.  The backward runs dK/dV (rows = keys, sums over
+// the heads that share a key head) and dQ (rows = queries) separately: both
+// recompute the scores, and every sum has one order.
+#include <type_traits>
+
+#include "attention.cuh"
+
+namespace kf {
+namespace {
+
+using namespace attn;
+
+constexpr int kTile = 64, kThreads = 256;
+
+template <int D>
+struct Ld {
+  static constexpr int row = D + 4;
+};
+constexpr int kLdP = kTile + 4;
+
+// A tile of up to 64 rows into shared memory as float32; rows past `n` and
+// columns past `dim` are zero, so nothing outside the sequence enters a sum.
+template <typename T, int D>
+__device__ __forceinline__ void load_tile(float* dst, const Strided& s, int64_t row0, int n, int head, int dim) {
+  const T* p = static_cast<const T*>(s.p) + head * s.head;
+  for (int i = threadIdx.x; i < kTile * D; i += kThreads) {
+    const int r = i / D, c = i % D;
+    dst[r * Ld<D>::row + c] = (r < n && c < dim) ? to_f32<T>(p[(row0 + r) * s.row + c]) : 0.f;
+  }
+}
+
+// acc[i][j] += a(row ty*4+i) . b(row tx+16j)
+template <int D>
+__device__ __forceinline__ void dot_rows(const float* a, const float* b, int ty, int tx, float (&acc)[4][4]) {
+#pragma unroll 4
+  for (int d = 0; d < D; d += 4) {
+    float4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty * 4 + i) * Ld<D>::row + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * Ld<D>::row + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
+        acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
+        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
+        acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+      }
+  }
+}
+
+// acc[i][c] += sum_k p(row ty*4+i, k) m(row k, column): columns tx*4 + 64 q + (0..3)
+template <int D>
+__device__ __forceinline__ void dot_cols(const float* p, const float* m, int ty, int tx, float (&acc)[4][D / 16]) {
+#pragma unroll 4
+  for (int k = 0; k < kTile; ++k) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = p[(ty * 4 + i) * kLdP + k];
+#pragma unroll
+    for (int q = 0; q < D / 64; ++q) {
+      const float4 y = *reinterpret_cast<const float4*>(m + k * Ld<D>::row + tx * 4 + 64 * q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[i][4 * q] = fmaf(x[i], y.x, acc[i][4 * q]);
+        acc[i][4 * q + 1] = fmaf(x[i], y.y, acc[i][4 * q + 1]);
+        acc[i][4 * q + 2] = fmaf(x[i], y.z, acc[i][4 * q + 2]);
+        acc[i][4 * q + 3] = fmaf(x[i], y.w, acc[i][4 * q + 3]);
+      }
+    }
+  }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void store_rows(T* out, int64_t row0, int n, int heads, int head, int dim, int ty, int tx,
+                                           const float (&acc)[4][D / 16], const float (&mul)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = ty * 4 + i;
+    if (r >= n) continue;
+    T* p = out + ((row0 + r) * heads + head) * dim;
+#pragma unroll
+    for (int q = 0; q < D / 64; ++q)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int col = tx * 4 + 64 * q + c;
+        if (col < dim) p[col] = from_f32<T>(acc[i][4 * q + c] * mul[i]);
+      }
+  }
+}
+
+__device__ __forceinline__ float half_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float half_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
+  extern __shared__ __align__(16) float smem[];
+  float* sq = smem;
+  float* sk = sq + kTile * Ld<D>::row;
+  float* sv = sk + kTile * Ld<D>::row;
+  float* sp = sv + kTile * Ld<D>::row;
+  float* sbias = sp + kTile * kLdP;
+  const int2 tile = a.tiles[blockIdx.x];
+  const Seq s = load_seq(a, tile.x);
+  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+  const int r0 = tile.y * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  load_tile<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
+  if (a.table != nullptr) expand_bias(a, head, sbias, threadIdx.x, kThreads);
+  float m[4], l[4], o[4][D / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -CUDART_INF_F, l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) o[i][c] = 0.f;
+  }
+  const int k_end = a.causal ? min(s.lk, r0 + n_rows + off) : s.lk;
+  const float c2 = a.scale * kLog2e;
+  for (int k0 = 0; k0 < k_end; k0 += kTile) {
+    const int n_keys = min(kTile, s.lk - k0);
+    __syncthreads();
+    load_tile<T, D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_tile<T, D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
+    __syncthreads();
+    float t[4][4] = {};
+    dot_rows<D>(sq, sk, ty, tx, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = r0 + ty * 4 + i + off;
+      float top = -CUDART_INF_F;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + tx + 16 * j;
+        float v = t[i][j] * c2;
+        if (a.table != nullptr) v += sbias[clamp_dist(pos - key, a.span)];
+        t[i][j] = (key < s.lk && (!a.causal || key <= pos)) ? v : -CUDART_INF_F;
+        top = fmaxf(top, t[i][j]);
+      }
+      const float m_new = fmaxf(m[i], half_max(top));
+      const float base = m_new == -CUDART_INF_F ? 0.f : m_new;  // no visible key yet
+      const float fix = exp2f(m[i] - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t[i][j] = exp2f(t[i][j] - base);
+        sum += t[i][j];
+        sp[(ty * 4 + i) * kLdP + tx + 16 * j] = t[i][j];
+      }
+      l[i] = l[i] * fix + half_sum(sum);
+      m[i] = m_new;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) o[i][c] *= fix;
+    }
+    __syncwarp();  // a warp reads back its own rows of P only
+    dot_cols<D>(sp, sv, ty, tx, o);
+  }
+  float inv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    inv[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
+    const int r = ty * 4 + i;
+    if (a.lse != nullptr && tx == 0 && r < n_rows)
+      a.lse[head * a.tq + s.q0 + r0 + r] = l[i] == 0.f ? 0.f : m[i] + log2f(l[i]);
+  }
+  store_rows<T, D>(static_cast<T*>(a.o), s.q0 + r0, n_rows, a.heads, head, a.dim, ty, tx, o, inv);
+}
+
+// delta[h][i] = dO_i . O_i: one warp per (token, head).
+template <typename T>
+__global__ void __launch_bounds__(256) attention_delta(const Args a) {
+  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= a.tq * a.heads) return;
+  const int64_t tok = i / a.heads;
+  const int head = (int)(i - tok * a.heads), lane = threadIdx.x & 31;
+  const T* o = static_cast<const T*>(a.o) + i * a.dim;
+  const T* g = static_cast<const T*>(a.dout.p) + tok * a.dout.row + head * a.dout.head;
+  float v = 0.f;
+  for (int c = lane; c < a.dim; c += 32) v = fmaf(to_f32<T>(o[c]), to_f32<T>(g[c]), v);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+  if (lane == 0) a.delta[head * a.tq + tok] = v;
+}
+
+// Rows = queries: dQ = scale dS K, and the bias gradient's sums by distance.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
+  extern __shared__ __align__(16) float smem[];
+  float* sq = smem;
+  float* sg = sq + kTile * Ld<D>::row;
+  float* sk = sg + kTile * Ld<D>::row;
+  float* sv = sk + kTile * Ld<D>::row;
+  float* sp = sv + kTile * Ld<D>::row;
+  float* sbias = sp + kTile * kLdP;
+  float* ssum = sbias + 2 * a.span + 1;  // gradient sums by clamped distance
+  const int2 tile = a.tiles[blockIdx.x];
+  const Seq s = load_seq(a, tile.x);
+  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+  const int r0 = tile.y * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  load_tile<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
+  load_tile<T, D>(sg, a.dout, s.q0 + r0, n_rows, head, a.dim);
+  if (a.table != nullptr) {
+    expand_bias(a, head, sbias, threadIdx.x, kThreads);
+    for (int i = threadIdx.x; i < 2 * a.span + 1; i += kThreads) ssum[i] = 0.f;
+  }
+  float lse[4], delta[4], dq[4][D / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = ty * 4 + i;
+    lse[i] = r < n_rows ? a.lse[head * a.tq + s.q0 + r0 + r] : 0.f;
+    delta[i] = r < n_rows ? a.delta[head * a.tq + s.q0 + r0 + r] : 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) dq[i][c] = 0.f;
+  }
+  const int k_end = a.causal ? min(s.lk, r0 + n_rows + off) : s.lk;
+  const float c2 = a.scale * kLog2e;
+  for (int k0 = 0; k0 < k_end; k0 += kTile) {
+    const int n_keys = min(kTile, s.lk - k0);
+    __syncthreads();
+    load_tile<T, D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_tile<T, D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
+    __syncthreads();
+    float t[4][4] = {}, dp[4][4] = {};
+    dot_rows<D>(sq, sk, ty, tx, t);
+    dot_rows<D>(sg, sv, ty, tx, dp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = r0 + ty * 4 + i + off;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + tx + 16 * j;
+        float v = t[i][j] * c2;
+        if (a.table != nullptr) v += sbias[clamp_dist(pos - key, a.span)];
+        const bool visible = ty * 4 + i < n_rows && key < s.lk && (!a.causal || key <= pos) && !one_key(a, s, pos);
+        sp[(ty * 4 + i) * kLdP + tx + 16 * j] = visible ? exp2f(v - lse[i]) * (dp[i][j] - delta[i]) : 0.f;
+      }
+    }
+    __syncwarp();
+    dot_cols<D>(sp, sk, ty, tx, dq);
+    if (a.dtable_part != nullptr) {
+      // thread d sums the diagonal row - column = d - 63 of dS
+      __syncthreads();
+      float sum = 0.f;
+      const int d = (int)threadIdx.x - (kTile - 1);
+      if (threadIdx.x < 2 * kTile - 1)
+        for (int r = max(0, d); r < min(kTile, kTile + d); ++r) sum += sp[r * kLdP + r - d];
+      __syncthreads();
+      // distances beyond the span share its last entry: those sums go one after another
+      if (threadIdx.x < 2 * kTile - 1) sp[threadIdx.x] = sum;
+      __syncthreads();
+      const int d0 = r0 + off - k0;  // distance of the main diagonal
+      for (int e = threadIdx.x; e < 2 * a.span + 1; e += kThreads) {
+        const int dist = e - a.span;
+        int first = dist - d0 + kTile - 1, last = first;
+        if (dist == -a.span) first = 0;
+        if (dist == a.span) last = 2 * kTile - 2;
+        for (int i = max(0, first); i <= min(last, 2 * kTile - 2); ++i) ssum[e] += sp[i];
+      }
+    }
+  }
+  const float mul[4] = {a.scale, a.scale, a.scale, a.scale};
+  store_rows<T, D>(static_cast<T*>(a.dq), s.q0 + r0, n_rows, a.heads, head, a.dim, ty, tx, dq, mul);
+  if (a.dtable_part != nullptr) {
+    __syncthreads();
+    float* out = a.dtable_part + ((int64_t)blockIdx.x * a.heads + head) * a.n_buckets;
+    for (int b = threadIdx.x; b < a.n_buckets; b += kThreads) {
+      float sum = 0.f;
+      for (int e = 0; e < 2 * a.span + 1; ++e)
+        if (a.buckets[e] == b) sum += ssum[e];
+      out[b] = sum;
+    }
+  }
+}
+
+// Rows = keys: dV = P^T dO and dK = scale dS^T Q, summed over the heads of the group.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
+  extern __shared__ __align__(16) float smem[];
+  float* sk = smem;
+  float* sv = sk + kTile * Ld<D>::row;
+  float* sq = sv + kTile * Ld<D>::row;
+  float* sg = sq + kTile * Ld<D>::row;
+  float* sp = sg + kTile * Ld<D>::row;
+  float* sds = sp + kTile * kLdP;
+  float* slse = sds + kTile * kLdP;
+  float* sdelta = slse + kTile;
+  float* sbias = sdelta + kTile;
+  const int2 tile = a.tiles[blockIdx.x];
+  const Seq s = load_seq(a, tile.x);
+  const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
+  const int r0 = tile.y * kTile, n_rows = min(kTile, s.lk - r0), off = s.lk - s.lq;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  load_tile<T, D>(sk, a.k, s.k0 + r0, n_rows, kv_head, a.dim);
+  load_tile<T, D>(sv, a.v, s.k0 + r0, n_rows, kv_head, a.dim);
+  float dk[4][D / 16], dv[4][D / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
+  const int q_first = a.causal ? max(0, r0 - off) / kTile * kTile : 0;  // earlier queries see none of these keys
+  const float c2 = a.scale * kLog2e;
+  for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
+    __syncthreads();
+    if (a.table != nullptr) expand_bias(a, head, sbias, threadIdx.x, kThreads);
+    for (int q0 = q_first; q0 < s.lq; q0 += kTile) {
+      const int n_q = min(kTile, s.lq - q0);
+      __syncthreads();
+      load_tile<T, D>(sq, a.q, s.q0 + q0, n_q, head, a.dim);
+      load_tile<T, D>(sg, a.dout, s.q0 + q0, n_q, head, a.dim);
+      if (threadIdx.x < kTile) {
+        const bool in = (int)threadIdx.x < n_q;
+        slse[threadIdx.x] = in ? a.lse[head * a.tq + s.q0 + q0 + threadIdx.x] : 0.f;
+        sdelta[threadIdx.x] = in ? a.delta[head * a.tq + s.q0 + q0 + threadIdx.x] : 0.f;
+      }
+      __syncthreads();
+      float t[4][4] = {}, dp[4][4] = {};
+      dot_rows<D>(sk, sq, ty, tx, t);
+      dot_rows<D>(sv, sg, ty, tx, dp);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = r0 + ty * 4 + i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = tx + 16 * j, pos = q0 + c + off;
+          float v = t[i][j] * c2;
+          if (a.table != nullptr) v += sbias[clamp_dist(pos - key, a.span)];
+          const bool visible = c < n_q && key < s.lk && (!a.causal || key <= pos);
+          const float p = visible ? exp2f(v - slse[c]) : 0.f;
+          sp[(ty * 4 + i) * kLdP + c] = p;
+          sds[(ty * 4 + i) * kLdP + c] = visible && !one_key(a, s, pos) ? p * (dp[i][j] - sdelta[c]) : 0.f;
+        }
+      }
+      __syncwarp();
+      dot_cols<D>(sp, sg, ty, tx, dv);
+      dot_cols<D>(sds, sq, ty, tx, dk);
+    }
+  }
+  const float one[4] = {1.f, 1.f, 1.f, 1.f}, mul[4] = {a.scale, a.scale, a.scale, a.scale};
+  store_rows<T, D>(static_cast<T*>(a.dv), s.k0 + r0, n_rows, a.kv_heads, kv_head, a.dim, ty, tx, dv, one);
+  store_rows<T, D>(static_cast<T*>(a.dk), s.k0 + r0, n_rows, a.kv_heads, kv_head, a.dim, ty, tx, dk, mul);
+}
+
+// The bias gradient: the tiles' sums of one (bucket, head) in tile order, over 32 lanes.
+__global__ void __launch_bounds__(256) attention_dtable(const float* part, int n_tiles, int heads, int n_buckets, void* out,
+                                                        bool bf16) {
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;  // head * n_buckets + bucket
+  if (i >= heads * n_buckets) return;
+  float v = 0.f;
+  for (int t = lane; t < n_tiles; t += 32) v += part[(int64_t)t * heads * n_buckets + i];
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+  if (lane != 0) return;
+  const int64_t at = (int64_t)(i % n_buckets) * heads + i / n_buckets;
+  if (bf16)
+    static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else
+    static_cast<float*>(out)[at] = v;
+}
+
+template <typename K>
+int run(K* kernel, dim3 grid, size_t floats, const Args& a, cudaStream_t st, const char* what) {
+  KF_CUDA_RET(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(floats * sizeof(float))));
+  kernel<<<grid, kThreads, floats * sizeof(float), st>>>(a);
+  return check_launch(what);
+}
+
+template <typename T, int D>
+int fwd(const Args& a, int n_tiles, cudaStream_t st) {
+  const size_t bias = a.table != nullptr ? 2 * a.span + 1 : 0;
+  return run(attention_fwd<T, D>, dim3(n_tiles, a.heads), 3 * kTile * Ld<D>::row + kTile * kLdP + bias, a, st, "kf_attention_fwd");
+}
+
+template <typename T, int D>
+int bwd(const Args& a0, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+  Args a = a0;
+  const size_t bias = a.table != nullptr ? 2 * a.span + 1 : 0;
+  if (a.tq > 0) {
+    attention_delta<T><<<(unsigned)cdiv(a.tq * a.heads, 8), 256, 0, st>>>(a);
+    if (int rc = check_launch("kf_attention_bwd")) return rc;
+  }
+  if (n_q > 0)
+    if (int rc = run(attention_dq<T, D>, dim3(n_q, a.heads), 4 * kTile * Ld<D>::row + kTile * kLdP + 2 * bias, a, st, "kf_attention_bwd"))
+      return rc;
+  a.tiles = k_tiles;
+  if (n_k > 0)
+    return run(attention_dkdv<T, D>, dim3(n_k, a.kv_heads), 4 * kTile * Ld<D>::row + 2 * kTile * kLdP + 2 * kTile + bias, a, st,
+               "kf_attention_bwd");
+  return KF_OK;
+}
+
+int check_attention(const char* fn, const kf_attention_desc* d) {
+  KF_CHECK_ARG(d != nullptr, "%s: null descriptor", fn);
+  KF_CHECK_ARG(d->heads >= 1 && d->kv_heads >= 1 && d->heads % d->kv_heads == 0, "%s: %d heads do not divide over %d key heads", fn,
+               d->heads, d->kv_heads);
+  KF_CHECK_ARG(d->heads <= 65535, "%s: %d heads", fn, d->heads);
+  KF_CHECK_ARG(d->dim >= 8 && d->dim <= kMaxDim && d->dim % 8 == 0, "%s: head width %d is not a multiple of 8 up to %d", fn, d->dim,
+               kMaxDim);
+  KF_CHECK_ARG(d->dtype == KF_DTYPE_F32 || d->dtype == KF_DTYPE_BF16, "%s: types must be float32 or bfloat16", fn);
+  KF_CHECK_ARG(d->tq >= 0 && d->tk >= 0 && d->n_seqs >= 0, "%s: negative size", fn);
+  KF_CHECK_ARG(d->span >= 0 && d->span <= kMaxSpan, "%s: bias distances up to %d are outside [0, %d]", fn, d->span, kMaxSpan);
+  KF_CHECK_ARG(d->n_buckets >= 0 && d->n_buckets <= kMaxBuckets, "%s: %d buckets exceed %d", fn, d->n_buckets, kMaxBuckets);
+  return KF_OK;
+}
+
+Args make_args(const kf_attention_desc* d) {
+  Args a{};
+  a.heads = d->heads, a.kv_heads = d->kv_heads, a.dim = d->dim, a.span = d->span, a.n_buckets = d->n_buckets;
+  a.causal = d->causal != 0, a.table_bf16 = d->table_dtype == KF_DTYPE_BF16;
+  a.scale = d->scale, a.tq = d->tq;
+  a.q = {nullptr, d->q_row, d->q_head};
+  a.k = {nullptr, d->k_row, d->k_head};
+  a.v = {nullptr, d->v_row, d->v_head};
+  a.dout = {nullptr, (int64_t)d->heads * d->dim, d->dim};
+  return a;
+}
+
+template <typename F>
+int by_type(const kf_attention_desc* d, F&& f) {
+  using bf = __nv_bfloat16;
+  if (d->dtype == KF_DTYPE_BF16)
+    return d->dim <= 64 ? f(bf{}, std::integral_constant<int, 64>{}) : f(bf{}, std::integral_constant<int, 128>{});
+  return d->dim <= 64 ? f(float{}, std::integral_constant<int, 64>{}) : f(float{}, std::integral_constant<int, 128>{});
+}
+
+}  // namespace
+}  // namespace kf
+
+extern "C" int kf_attention_tile_rows(const kf_attention_desc* d) {
+  (void)d;
+  return kf::kTile;
+}
+
+extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* q_tiles,
+                                int32_t n_q_tiles, const void* table, const int32_t* buckets, void* o, float* lse,
+                                const kf_attention_desc* d, void* stream) {
+  using namespace kf;
+  clear_error();
+  if (int rc = check_attention("kf_attention_fwd", d)) return rc;
+  if (n_q_tiles == 0) return KF_OK;
+  KF_CHECK_ARG(n_q_tiles > 0, "kf_attention_fwd: negative tile count");
+  KF_CHECK_ARG(q && o && seqs && q_tiles && (d->tk == 0 || (k && v)), "kf_attention_fwd: null argument");
+  KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_fwd: the bias needs a table and buckets");
+  if (int rc = bind_device(q)) return rc;
+  Args a = make_args(d);
+  a.q.p = q, a.k.p = k, a.v.p = v, a.o = o, a.lse = lse, a.table = table, a.buckets = buckets;
+  a.seqs = reinterpret_cast<const int4*>(seqs), a.tiles = reinterpret_cast<const int2*>(q_tiles);
+  return by_type(d, [&](auto t, auto dim) { return fwd<decltype(t), decltype(dim)::value>(a, n_q_tiles, static_cast<cudaStream_t>(stream)); });
+}
+
+extern "C" int64_t kf_attention_bwd_workspace(int32_t n_q_tiles, const kf_attention_desc* d) {
+  if (d == nullptr || n_q_tiles < 0) return 0;
+  return (int64_t)d->heads * d->tq + (int64_t)n_q_tiles * d->heads * d->n_buckets;
+}
+
+extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
+                                const int32_t* seqs, const int32_t* q_tiles, int32_t n_q_tiles, const int32_t* k_tiles,
+                                int32_t n_k_tiles, const void* table, const int32_t* buckets, void* dq, void* dk, void* dv,
+                                void* dtable, float* workspace, const kf_attention_desc* d, void* stream) {
+  using namespace kf;
+  clear_error();
+  if (int rc = check_attention("kf_attention_bwd", d)) return rc;
+  KF_CHECK_ARG(n_q_tiles >= 0 && n_k_tiles >= 0, "kf_attention_bwd: negative tile count");
+  KF_CHECK_ARG(n_q_tiles == 0 || (q && o && dout && lse && dq && workspace && q_tiles && seqs), "kf_attention_bwd: null argument");
+  KF_CHECK_ARG(n_k_tiles == 0 || (k && v && dk && dv && k_tiles && seqs), "kf_attention_bwd: null argument");
+  KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_bwd: the bias needs a table and buckets");
+  KF_CHECK_ARG(dtable == nullptr || (table != nullptr && workspace != nullptr), "kf_attention_bwd: dtable needs a table and workspace");
+  if (n_q_tiles == 0 && n_k_tiles == 0 && dtable == nullptr) return KF_OK;
+  if (int rc = bind_device(n_q_tiles ? q : n_k_tiles ? k : dtable)) return rc;
+  Args a = make_args(d);
+  a.q.p = q, a.k.p = k, a.v.p = v, a.dout.p = dout, a.o = const_cast<void*>(o), a.lse = const_cast<float*>(lse);
+  a.dq = dq, a.dk = dk, a.dv = dv, a.table = table, a.buckets = buckets;
+  a.seqs = reinterpret_cast<const int4*>(seqs), a.tiles = reinterpret_cast<const int2*>(q_tiles);
+  a.delta = workspace;
+  a.dtable_part = dtable != nullptr ? workspace + (int64_t)d->heads * d->tq : nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc = by_type(d, [&](auto t, auto dim) {
+    return bwd<decltype(t), decltype(dim)::value>(a, reinterpret_cast<const int2*>(k_tiles), n_q_tiles, n_k_tiles, st);
+  });
+  if (rc || dtable == nullptr) return rc;
+  attention_dtable<<<(unsigned)cdiv(d->heads * d->n_buckets, 8), 256, 0, st>>>(a.dtable_part, n_q_tiles, d->heads, d->n_buckets, dtable,
+                                                                               a.table_bf16);
+  return check_launch("kf_attention_bwd");
+}

@@ -1,0 +1,192 @@
+"""The norms around a transformer block, fused with its gate and residual scale.
+
+``residual_norm`` joins two blocks in one pass over the rows:
+
+    u = N_b(branch) * branch_weight + branch_bias     (or the branch itself)
+    y = residual_scale * x + gate * u                 (the residual stream)
+    h = N(y) * weight + bias                          (the next block's input)
+
+with N a layer norm or a root-mean-square norm.  The kernels are
+``kf_residual_norm_fwd`` / ``kf_residual_norm_bwd`` (csrc/norm.cu).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .kernels import _aligned16, _check_cuda, _launch, _ptr, _stream
+
+NORM_KINDS = ("layer", "rms")
+NORM_MAX_WIDTH = 8192
+
+_DTYPE_CODE = {torch.float32: _lib.KF_DTYPE_F32, torch.bfloat16: _lib.KF_DTYPE_BF16}
+
+
+def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    return t.reshape(-1, width).contiguous()
+
+
+class _Call:
+    """The operands of one residual norm as the kernels take them."""
+
+    __slots__ = ("x", "branch", "gate", "w", "s", "bw", "bs", "desc", "rows", "width", "gate_token")
+
+    def __init__(self, x, branch, weight, bias, branch_weight, branch_bias, gate, kind, residual_scale, eps):
+        self.width = width = x.shape[-1]
+        self.x = _rows(x.detach(), width)
+        self.rows = self.x.shape[0]
+        self.branch = None if branch is None else _rows(branch.detach(), width)
+        self.gate_token = gate is not None and gate.dim() > 1
+        params = [weight, bias, branch_weight, branch_bias, None if self.gate_token else gate]
+        dtypes = {p.dtype for p in params if p is not None}
+        # parameters of one type are read as they are; mixed or other types as float32
+        dtype = dtypes.pop() if len(dtypes) == 1 and dtypes <= set(_DTYPE_CODE) else torch.float32
+        params = [None if p is None else _aligned16(p.detach().to(dtype).contiguous()) for p in params]
+        self.w, self.s, self.bw, self.bs, self.gate = params
+        if self.gate_token:
+            self.gate = _rows(gate.detach(), width)
+        out = self.x.dtype if self.branch is None else self.branch.dtype
+        self.desc = _lib.ResidualNormDesc(width, int(kind == "layer"), int(branch_weight is not None),
+                                          int(self.gate_token), _DTYPE_CODE[self.x.dtype], _DTYPE_CODE[out],
+                                          _DTYPE_CODE[dtype], residual_scale, eps)
+
+    def forward(self, with_stats: bool):
+        """(y, h, stats) as (rows, width) matrices; y is x where there is no branch."""
+        x = self.x
+        y = x if self.branch is None else torch.empty_like(x)
+        h = torch.empty_like(x if self.branch is None else self.branch)
+        stats = torch.empty(self.rows, 4, device=x.device, dtype=torch.float32) if with_stats else None
+        if self.rows:
+            _launch("kf_residual_norm_fwd", _ptr(x), _ptr(self.branch), _ptr(self.gate), _ptr(self.w), _ptr(self.s),
+                    _ptr(self.bw), _ptr(self.bs), _ptr(None if self.branch is None else y), _ptr(h), _ptr(stats),
+                    self.rows, ctypes.byref(self.desc), _stream(x))
+        return y, h, stats
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, weight, bias, branch_weight, branch_bias, gate, kind, residual_scale, eps):
+        call = _Call(x, branch, weight, bias, branch_weight, branch_bias, gate, kind, residual_scale, eps)
+        y, h, stats = call.forward(with_stats=True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, branch, weight, bias, branch_weight, branch_bias, gate, stats)
+        ctx.options = (kind, residual_scale, eps)
+        h = h.view(x.shape)
+        if branch is None:
+            return h
+        return y.view(x.shape), h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        x, branch, weight, bias, branch_weight, branch_bias, gate, stats = ctx.saved_tensors
+        dy, dh = (None, grads[0]) if branch is None else grads
+        if dy is None and dh is None:
+            return (None,) * 10
+        need = ctx.needs_input_grad
+        call = _Call(x, branch, weight, bias, branch_weight, branch_bias, gate, *ctx.options)
+        shape, rows = x.shape, call.x
+        dev, width = rows.device, call.width
+        mat = lambda g, like: None if g is None else _rows(g.to(like.dtype), width)  # noqa: E731
+        out_like = rows if branch is None else call.branch
+        dy, dh = mat(dy, rows), mat(dh, out_like)
+        dx = torch.empty_like(rows)
+        dbranch = None if branch is None else torch.empty_like(call.branch)
+        dgate = None
+        if gate is not None:
+            dgate = torch.empty_like(call.gate)
+        dw, ds, dbw, dbs = (None if p is None else torch.empty_like(p) for p in (call.w, call.s, call.bw, call.bs))
+        n_ws = int(_lib.load().kf_residual_norm_workspace(call.rows, width))
+        ws = torch.empty(n_ws, device=dev, dtype=torch.float32)
+        _launch("kf_residual_norm_bwd", _ptr(rows), _ptr(call.branch), _ptr(call.gate), _ptr(call.w), _ptr(call.bw),
+                _ptr(call.bs), _ptr(stats), _ptr(dy), _ptr(dh), _ptr(dx), _ptr(dbranch), _ptr(dgate),
+                _ptr(dw), _ptr(ds), _ptr(dbw), _ptr(dbs), _ptr(ws), call.rows, ctypes.byref(call.desc), _stream(rows),
+                kernels=2 if call.rows else 1)
+        like = lambda g, p, n: g.to(p.dtype).view(p.shape) if n and p is not None else None  # noqa: E731
+        return (dx.view(shape) if need[0] else None, dbranch.view(shape) if need[1] and branch is not None else None,
+                like(dw, weight, need[2]), like(ds, bias, need[3]), like(dbw, branch_weight, need[4]),
+                like(dbs, branch_bias, need[5]), like(dgate, gate, need[6]), None, None, None)
+
+
+def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                  kind: str = "layer", gate: torch.Tensor | None = None, branch_norm: bool = False,
+                  branch_weight: torch.Tensor | None = None, branch_bias: torch.Tensor | None = None,
+                  residual_scale: float = 1.0, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """(y, h) of the formulas at the head of this module, on (..., width) tensors.
+
+    ``x`` is the residual stream and ``branch`` a block's output, both float32
+    or bfloat16 (a float32 stream may take a bfloat16 branch); ``y`` has the
+    type of ``x``, ``h`` that of the branch.  ``gate`` is (width,), one factor
+    per channel, or broadcasts to the branch's shape.  ``branch=None`` norms
+    ``x`` alone, the start of a stack: y is x.  Sums and statistics are
+    float32; ``h`` comes from y before its rounding.  Gradients reach every
+    tensor argument; the sums over rows run in a fixed order.
+    """
+    if kind not in NORM_KINDS:
+        raise ValueError(f"kind must be one of {NORM_KINDS}")
+    if eps < 0:
+        raise ValueError("eps must not be negative")
+    _check_cuda(x, branch, weight, bias, gate, branch_weight, branch_bias)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= NORM_MAX_WIDTH:
+        raise ValueError(f"rows must have 1 to {NORM_MAX_WIDTH} elements (got a tensor of shape {tuple(x.shape)})")
+    width = x.shape[-1]
+    for what, t in (("x", x), ("branch", branch)):
+        if t is not None and t.dtype not in _DTYPE_CODE:
+            raise TypeError(f"{what} must be float32 or bfloat16, not {t.dtype}")
+    for what, t in (("weight", weight), ("bias", bias), ("branch_weight", branch_weight), ("branch_bias", branch_bias)):
+        if t is not None and t.shape != (width,):
+            raise ValueError(f"{what} must have shape ({width},), not {tuple(t.shape)}")
+    for t in (branch, weight, bias, gate, branch_weight, branch_bias):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"tensors lie on {x.device} and {t.device}")
+    if branch is None:
+        if gate is not None or branch_norm or residual_scale != 1.0:
+            raise ValueError("a gate, a branch norm or a residual scale needs a branch")
+    else:
+        if branch.shape != x.shape:
+            raise ValueError(f"x {tuple(x.shape)} and branch {tuple(branch.shape)} differ in shape")
+        if x.dtype == torch.bfloat16 and branch.dtype == torch.float32:
+            raise TypeError("a bfloat16 residual stream takes no float32 branch")
+    if branch_norm != (branch_weight is not None) or (branch_bias is not None and not branch_norm):
+        raise ValueError("branch_norm, branch_weight and branch_bias belong together")
+    if gate is not None and (gate.dim() > 1 or gate.shape != (width,)):
+        gate = gate.expand(branch.shape).to(branch.dtype)  # their gradients: autograd's
+        if gate.dim() < 2:
+            gate = gate.reshape(1, width)
+    args = (x, branch, weight, bias, branch_weight, branch_bias, gate, kind, float(residual_scale), float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:7]):
+        out = _ResidualNorm.apply(*args)
+        return (x, out) if branch is None else out
+    y, h, _ = _Call(*args).forward(with_stats=False)
+    return (x if branch is None else y.view(x.shape)), h.view(x.shape)
+
+
+class ResidualNorm(nn.Module):
+    """``residual_norm`` with its parameters: ``weight`` (and ``bias`` for a layer
+    norm), ``branch_weight`` (``branch_bias``) with ``branch_norm``, and ``gate``
+    (one factor per channel, starting at ``gate_init``) unless that is None."""
+
+    def __init__(self, dim: int, kind: str = "layer", *, branch_norm: bool = False, gate_init: float | None = None,
+                 residual_scale: float = 1.0, eps: float = 1e-6, device=None, dtype=None):
+        super().__init__()
+        if kind not in NORM_KINDS:
+            raise ValueError(f"kind must be one of {NORM_KINDS}")
+        if not 1 <= dim <= NORM_MAX_WIDTH:
+            raise ValueError(f"dim must be 1 to {NORM_MAX_WIDTH}")
+        self.dim, self.kind, self.branch_norm = dim, kind, branch_norm
+        self.residual_scale, self.eps = residual_scale, eps
+        make = lambda on, v: nn.Parameter(torch.full((dim,), v, device=device, dtype=dtype)) if on else None  # noqa: E731
+        self.weight, self.bias = make(True, 1.0), make(kind == "layer", 0.0)
+        self.branch_weight = make(branch_norm, 1.0)
+        self.branch_bias = make(branch_norm and kind == "layer", 0.0)
+        self.gate = make(gate_init is not None, gate_init)
+
+    def forward(self, x: torch.Tensor, branch: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        return residual_norm(x, branch, self.weight, self.bias, kind=self.kind, gate=self.gate,
+                             branch_norm=self.branch_norm, branch_weight=self.branch_weight,
+                             branch_bias=self.branch_bias, residual_scale=self.residual_scale, eps=self.eps)

@@ -1,0 +1,99 @@
+"""Host side of packed attention and the residual norm, without a GPU: lengths,
+tiles, buckets and the refusals that come before any launch."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import kanforge_b200 as kb
+from kanforge_b200.attention import relative_buckets
+
+
+def test_sequences_tables_and_refusals():
+    s = kb.PackedSequences([3, 0, 5], [4, 2, 5], device="cpu")
+    assert s.table.tolist() == [[0, 3, 0, 4], [3, 0, 4, 2], [3, 5, 6, 5]]
+    assert (s.total_q, s.total_kv, len(s)) == (8, 11, 3)
+    with pytest.raises(ValueError):
+        kb.PackedSequences([1, -1], device="cpu")
+    with pytest.raises(ValueError):
+        kb.PackedSequences([1], [1, 2], device="cpu")
+    with pytest.raises(ValueError):
+        kb.PackedSequences([1 << 30, 1 << 30], device="cpu")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("rows", [1, 16, 64])
+def test_tiles_cover_every_row_once_with_the_most_work_first(rows, causal):
+    q_lens, kv_lens = [0, 1, 64, 65, 200], [3, 9, 64, 30, 300]
+    s = kb.PackedSequences(q_lens, kv_lens, device="cpu")
+    for side, lens in (("q", q_lens), ("k", kv_lens)):
+        tiles = [tuple(t) for t in s.tiles(side, rows, causal).tolist()]
+        assert sorted(tiles) == [(i, t) for i, n in enumerate(lens) for t in range(-(-n // rows))]
+        cost = []
+        for i, t in tiles:
+            off = kv_lens[i] - q_lens[i]
+            if side == "q":
+                cost.append(max(0, min(kv_lens[i], (t + 1) * rows + off)) if causal else kv_lens[i])
+            else:
+                cost.append(max(0, q_lens[i] - max(0, t * rows - off)) if causal else q_lens[i])
+        assert cost == sorted(cost, reverse=True)
+
+
+@pytest.mark.parametrize("n,span,both", [(32, 128, True), (32, 128, False), (8, 20, True), (4, 3, True), (2, 2, False),
+                                         (64, 2048, False)])
+def test_buckets_follow_the_logarithm(n, span, both):
+    got = relative_buckets(n, span, both)
+    assert len(got) == 2 * span + 1 and min(got) == 0 and max(got) == n - 1
+    one = n // 2 if both else n
+    exact = one // 2
+    for d in range(-span, span + 1):
+        dist = abs(d) if both else max(0, d)
+        if dist < exact:
+            want = dist
+        else:
+            # 1e-9: the exact floor where the logarithm is a whole number
+            want = min(one - 1, exact + int(math.log(dist / exact) / math.log(span / exact) * (one - exact) + 1e-9))
+        assert got[d + span] == want + (one if both and d < 0 else 0), d
+
+
+def test_bias_module_looks_up_and_refuses():
+    b = kb.RelativeBias(3, 8, 16, bidirectional=False)
+    with torch.no_grad():
+        b.weight.copy_(torch.arange(24.0).reshape(8, 3))
+    assert b(torch.tensor([0, 1, 500, -4])).tolist() == [[0, 1, 2], [3, 4, 5], [21, 22, 23], [0, 1, 2]]
+    assert set(b.state_dict()) == {"weight"}
+    for args in ((3, 1), (3, 7), (3, 300), (3, 32, 8), (3, 32, 4096), (0, 32)):
+        with pytest.raises(ValueError):
+            kb.RelativeBias(*args)
+
+
+def test_cpu_tensors_raise():
+    t = torch.randn(4, 2, 16)
+    with pytest.raises(RuntimeError):
+        kb.attention(t, t, t, kb.PackedSequences([4], device="cpu"))
+    with pytest.raises(RuntimeError):
+        kb.attention_decode(t, t[None], t[None], torch.ones(4, dtype=torch.int32))
+    with pytest.raises(RuntimeError):
+        kb.residual_norm(t, t, torch.ones(16))
+
+
+def test_entry_points_check_their_arguments_before_any_cuda_call():
+    import ctypes
+
+    from kanforge_b200 import _lib
+
+    lib = _lib.load()
+    d = _lib.AttentionDesc(heads=4, kv_heads=3, dim=64)
+    assert lib.kf_attention_fwd(*[None] * 5, 1, *[None] * 4, ctypes.byref(d), None) == 1
+    assert "do not divide" in _lib.last_error()
+    d = _lib.AttentionDesc(heads=4, kv_heads=2, dim=65)
+    assert lib.kf_attention_fwd(*[None] * 5, 1, *[None] * 4, ctypes.byref(d), None) == 1
+    d = _lib.DecodeDesc(heads=4, kv_heads=2, dim=64, batch=1, capacity=8)
+    assert lib.kf_attention_decode(*[None] * 8, ctypes.byref(d), None) == 1
+    d = _lib.ResidualNormDesc(width=9000)
+    x = ctypes.c_void_p(16)
+    assert lib.kf_residual_norm_fwd(x, *[None] * 2, x, *[None] * 6, 1, ctypes.byref(d), None) == 1
+    assert "outside" in _lib.last_error()

@@ -1,0 +1,380 @@
+"""Attention over packed sequences, its relative position bias and the
+single-token form against the formulas in float64.
+
+Tolerance, max|a - b| / max|b| over a tensor: bfloat16 2e-2, about ten roundings
+of 2^-9 (the inputs are taken as exact; the probabilities, dS, the output that
+delta is made of and the results are each rounded once).  float32 1e-5, 168
+roundings of 2^-24: sums of up to 1000 terms with errors of either sign.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import kanforge_b200 as kb
+from kanforge_b200.attention import relative_buckets
+
+pytestmark = pytest.mark.gpu
+TOL = {torch.float32: 1e-5, torch.bfloat16: 2e-2}
+
+
+def close(got, want, tol, what, floor=0.0):
+    assert got.shape == want.shape, what
+    if got.numel() == 0:
+        return
+    assert got.isfinite().all(), f"{what} is not finite"
+    top = max(want.abs().max().item(), floor)
+    err = (got.double() - want).abs().max().item()
+    assert err <= tol * max(top, 1e-30), f"{what}: {err:.3e} of {top:.3e}"
+
+
+def formula(q, k, v, q_lens, kv_lens, causal, scale, table=None, buckets=None, span=0):
+    """float64, differentiable; rows that see no key give 0."""
+    rep = q.shape[1] // k.shape[1]
+    outs, q0, k0 = [], 0, 0
+    for lq, lk in zip(q_lens, kv_lens):
+        qs, ks, vs = q[q0:q0 + lq], k[k0:k0 + lk].repeat_interleave(rep, 1), v[k0:k0 + lk].repeat_interleave(rep, 1)
+        s = torch.einsum("ihd,jhd->hij", qs, ks) * scale
+        dist = torch.arange(lq, device=q.device)[:, None] + (lk - lq) - torch.arange(lk, device=q.device)[None, :]
+        if table is not None:
+            s = s + table[buckets[dist.clamp(-span, span) + span].long()].permute(2, 0, 1)
+        seen = (dist >= 0) if causal else torch.ones_like(dist, dtype=torch.bool)
+        e = torch.where(seen, (s - s.detach().masked_fill(~seen, -1e300).amax(-1, keepdim=True) if lk else s), -1e4).exp()
+        e = e * seen
+        outs.append(torch.einsum("hij,jhd->ihd", e / e.sum(-1, keepdim=True).clamp(min=1e-300), vs))
+        q0, k0 = q0 + lq, k0 + lk
+    return torch.cat(outs) if outs else q * 0
+
+
+def make(q_lens, kv_lens, heads, kv_heads, dim, dtype, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda n, h: (scale * torch.randn(n, h, dim, generator=g, device="cuda")).to(dtype)  # noqa: E731
+    return r(sum(q_lens), heads), r(sum(kv_lens), kv_heads), r(sum(kv_lens), kv_heads), r(sum(q_lens), heads)
+
+
+def check(q, k, v, dout, q_lens, kv_lens, causal, bias=None, scale=None, tol=None):
+    dtype = q.dtype
+    seqs = kb.PackedSequences(q_lens, kv_lens)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)] + ([bias.weight] if bias is not None else [])
+    out = kb.attention(*leaves[:3], seqs, causal=causal, bias=bias, scale=scale)
+    assert out.dtype == dtype and out.shape == q.shape
+    grads = torch.autograd.grad(out, leaves, dout)
+    with torch.no_grad():
+        infer = kb.attention(q, k, v, seqs, causal=causal, bias=bias, scale=scale)
+    assert torch.equal(infer, out)
+    ref = [t.detach().double().requires_grad_() for t in leaves]
+    want = formula(*ref[:3], q_lens, kv_lens, causal, scale or 1 / math.sqrt(q.shape[-1]), *(
+        (ref[3], bias.buckets, bias.max_distance) if bias is not None else ()))
+    wants = torch.autograd.grad((want * dout.double()).sum(), ref, allow_unused=True)
+    tol = tol or TOL[dtype]
+    close(out, want.detach(), tol, "out")
+    # a sequence of one visible key has dS = 0 exactly: then compare with the size of its terms
+    for name, g, w, leaf in zip(("dq", "dk", "dv", "dbias"), grads, wants, leaves):
+        w = torch.zeros_like(leaf, dtype=torch.float64) if w is None else w
+        close(g, w, TOL[g.dtype] if name != "dbias" else TOL[dtype], name, floor=0.1)
+    return out, grads
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [8, 24, 40, 64, 80, 128])
+def test_head_widths(dim, causal, dtype):
+    lens = [70, 1, 129, 256, 33]
+    check(*make(lens, lens, 4, 2, dim, dtype), lens, lens, causal)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (6, 6), (6, 2), (8, 1), (12, 4), (20, 1), (33, 11)])
+def test_shared_heads(heads, kv_heads, dtype):
+    lens = [65, 200, 3]
+    check(*make(lens, lens, heads, kv_heads, 64, dtype), lens, lens, True)
+
+
+LAYOUTS = [
+    ([1], [1]), ([0], [0]), ([], []), ([0, 5, 0], [0, 5, 0]), ([1] * 9, [1] * 9), ([64, 128, 192], [64, 128, 192]),
+    ([127, 129, 255, 257], [127, 129, 255, 257]), ([600], [600]),
+    ([1, 1, 1], [500, 1, 77]), ([5, 70, 130], [300, 70, 514]),  # queries behind a past
+    ([10, 200, 64], [4, 130, 0]), ([150], [20]), ([3, 0], [0, 9]),  # causal rows that see nothing, no keys, no queries
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("layout", LAYOUTS, ids=lambda x: f"{x[0]}over{x[1]}")
+def test_lengths(layout, causal, dtype):
+    q_lens, kv_lens = layout
+    out, grads = check(*make(q_lens, kv_lens, 6, 3, 64, dtype), q_lens, kv_lens, causal)
+    q0 = 0
+    for lq, lk in zip(q_lens, kv_lens):
+        empty = lq if lk == 0 else (max(0, lq - lk) if causal else 0)
+        assert (out[q0:q0 + empty] == 0).all() and (grads[0][q0:q0 + empty] == 0).all()
+        q0 += lq
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("buckets,span", [(32, 128), (8, 20), (4, 3), (64, 500)])
+def test_bias(buckets, span, causal, dtype):
+    lens = [1, 90, 260, 300]
+    heads = 6
+    bias = kb.RelativeBias(heads, buckets, span, bidirectional=not causal, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        bias.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
+    check(*make(lens, lens, heads, 3, 64, dtype), lens, lens, causal, bias=bias)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_bias_behind_a_past_and_wide_heads(dtype):
+    q_lens, kv_lens = [5, 140, 1], [400, 141, 700]
+    bias = kb.RelativeBias(4, 32, 128, bidirectional=False, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        bias.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
+    check(*make(q_lens, kv_lens, 4, 4, 128, dtype), q_lens, kv_lens, True, bias=bias)
+
+
+def test_a_bias_that_closes_a_bucket():
+    # the lowest finite value keeps keys out of the softmax wherever another key is open
+    lens = [200]
+    for low in (torch.finfo(torch.float32).min, -float("inf")):
+        q, k, v, dout = make(lens, lens, 2, 2, 64, torch.float32)
+        bias = kb.RelativeBias(2, 8, 16, bidirectional=False, device="cuda")
+        with torch.no_grad():
+            bias.weight[-1] = low  # distances from the last bucket's first on
+        first = relative_buckets(8, 16, False)[16:].index(7)
+        out = kb.attention(q, k, v, kb.PackedSequences(lens), causal=True, bias=bias)
+        s = torch.einsum("ihd,jhd->hij", q.double(), k.double()) / 8
+        d = torch.arange(200, device="cuda")[:, None] - torch.arange(200, device="cuda")[None, :]
+        p = s.masked_fill((d < 0) | (d >= first), -math.inf).softmax(-1)
+        close(out.detach(), torch.einsum("hij,jhd->ihd", p, v.double()), 1e-5, "out")
+        g = torch.autograd.grad(out, bias.weight, dout)[0]
+        assert g.isfinite().all() and (g[-1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_scores(dtype):
+    # one key takes nearly all the weight; sums stay finite and exact at the top.  The scores reach some hundreds:
+    # float32 holds them to 2^-24 * 2^9, so the probabilities to 3e-5
+    lens = [150, 40]
+    q, k, v, dout = make(lens, lens, 4, 4, 64, dtype, scale=6.0)
+    check(q, k, v / 6, dout / 6, lens, lens, True, tol=1e-4 if dtype == torch.float32 else None)
+
+
+def test_views_of_one_projection_and_odd_alignment():
+    lens = [100, 57]
+    g = torch.Generator(device="cuda").manual_seed(0)
+    qkv = torch.randn(157, 8 + 2 * 2, 64, generator=g, device="cuda").bfloat16()
+    q, k, v = qkv.split([8, 2, 2], 1)
+    seqs = kb.PackedSequences(lens)
+    want = kb.attention(q.contiguous(), k.contiguous(), v.contiguous(), seqs)
+    assert torch.equal(kb.attention(q, k, v, seqs), want)
+    odd = torch.empty(157 * 8 * 64 + 3, device="cuda", dtype=torch.bfloat16)[3:].view(157, 8, 64).copy_(q)
+    assert torch.equal(kb.attention(odd, k, v, seqs), want)
+    heads_first = q.permute(1, 0, 2).contiguous().permute(1, 0, 2)
+    assert torch.equal(kb.attention(heads_first, k, v, seqs), want)
+    # a gradient that comes as a broadcast view
+    ql = q.contiguous().requires_grad_()
+    a = torch.autograd.grad(kb.attention(ql, k, v, seqs).sum(), ql)[0]
+    b = torch.autograd.grad(kb.attention(ql, k, v, seqs), ql, torch.ones_like(ql))[0]
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_other_sequences_never_enter(causal, dtype):
+    lens = [100, 30, 77]
+    q, k, v, dout = make(lens, lens, 4, 2, 64, dtype)
+    seqs = kb.PackedSequences(lens)
+
+    def step(q, k, v, dout):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = kb.attention(*leaves, seqs, causal=causal)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    want = step(q, k, v, dout)
+    for t, bad in ((q, float("nan")), (k, float("inf")), (v, float("nan")), (dout, float("-inf"))):
+        t[100:130] = bad
+    got = step(q, k, v, dout)
+    for a, b in zip(got, want):
+        assert torch.equal(a[:100], b[:100]) and torch.equal(a[130:], b[130:])
+
+
+def test_gradient_matches_differences():
+    q_lens, kv_lens = [5, 9], [7, 6]
+    q, k, v, dout = make(q_lens, kv_lens, 4, 2, 16, torch.float32)
+    bias = kb.RelativeBias(4, 8, 6, bidirectional=True, device="cuda")
+    with torch.no_grad():
+        bias.weight.normal_(0, 0.5, generator=torch.Generator(device="cuda").manual_seed(1))
+    seqs = kb.PackedSequences(q_lens, kv_lens)
+    leaves = [t.requires_grad_() for t in (q, k, v)] + [bias.weight]
+
+    def loss():
+        return (kb.attention(*leaves[:3], seqs, causal=False, bias=bias).double() * dout.double()).sum()
+
+    grads = torch.autograd.grad(loss(), leaves)
+    for t, g in zip(leaves, grads):
+        d = torch.randn_like(t)
+        d /= d.norm()
+        step = 2e-2
+        with torch.no_grad():
+            t += step * d
+            hi = loss()
+            t -= 2 * step * d
+            lo = loss()
+            t += step * d
+        assert abs((hi - lo).item() / (2 * step) - (g.double() * d.double()).sum().item()) < 5e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_same_bits_every_run_and_on_another_stream(dtype):
+    lens = [400, 333, 90]
+    q, k, v, dout = make(lens, lens, 8, 2, 64, dtype)
+    bias = kb.RelativeBias(8, 32, 64, bidirectional=False, device="cuda", dtype=dtype)
+    seqs = kb.PackedSequences(lens)
+
+    def step():
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = kb.attention(*leaves, seqs, bias=bias)
+        return [out.detach(), *torch.autograd.grad(out, leaves + [bias.weight], dout)]
+
+    first = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = step()
+    side.synchronize()
+    kb.kernels.check_device_errors()
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+
+
+def test_refusals():
+    q, k, v, _ = make([4], [4], 4, 2, 16, torch.float32)
+    seqs = kb.PackedSequences([4])
+    with pytest.raises(ValueError):
+        kb.attention(q[:3], k, v, seqs)
+    with pytest.raises(ValueError):
+        kb.attention(q, k, v[:, :1], seqs)
+    with pytest.raises(ValueError):
+        kb.attention(q[:, :3], k, v, seqs)
+    with pytest.raises(TypeError):
+        kb.attention(q, k.bfloat16(), v, seqs)
+    with pytest.raises(TypeError):
+        kb.attention(q.half(), k.half(), v.half(), seqs)
+    with pytest.raises(TypeError):
+        kb.attention(q, k, v, [4])
+    with pytest.raises(RuntimeError):
+        kb.attention(q.cpu(), k.cpu(), v.cpu(), seqs)
+    with pytest.raises(ValueError):
+        kb.attention(q, k, v, kb.PackedSequences([4], device="cpu"))
+    with pytest.raises(ValueError):
+        kb.attention(q, k, v, seqs, bias=kb.RelativeBias(3, device="cuda"))
+    with pytest.raises(ValueError):
+        kb.attention(q, k, v, seqs, bias=kb.RelativeBias(4))
+    for dim in (12, 136):
+        with pytest.raises(ValueError):
+            kb.attention(*make([4], [4], 4, 2, dim, torch.float32)[:3], seqs)
+    q.requires_grad_()
+    g = torch.autograd.grad(kb.attention(q, k, v, seqs).sum(), q, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+# --- one token over a cache ---------------------------------------------------
+
+
+def decode_case(batch, capacity, heads, kv_heads, dim, dtype, lengths, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dtype)  # noqa: E731
+    return (r(batch, heads, dim), r(batch, capacity, kv_heads, dim), r(batch, capacity, kv_heads, dim),
+            torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+
+
+def decode_want(q, k, v, lengths, bias):
+    cap = k.shape[1]
+    lens = [min(max(n, 0), cap) for n in lengths]
+    packed = [torch.cat([t[b, :n] for b, n in enumerate(lens)]).double() for t in (k, v)]
+    return formula(q.double(), *packed, [1] * len(lens), lens, True, 1 / math.sqrt(q.shape[-1]), *(
+        (bias.weight.double(), bias.buckets, bias.max_distance) if bias is not None else ()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 8), (5, 5, 40), (12, 4, 64), (8, 1, 128), (40, 2, 80), (17, 1, 64)])
+def test_decode(heads, kv_heads, dim, with_bias, dtype):
+    lengths = [1, 2, 15, 16, 17, 63, 64, 65, 300, 511, 512, 0, 700, -3]
+    q, k, v, n = decode_case(len(lengths), 512, heads, kv_heads, dim, dtype, lengths)
+    bias = None
+    if with_bias:
+        bias = kb.RelativeBias(heads, 32, 100, bidirectional=False, device="cuda", dtype=dtype).requires_grad_(False)
+        bias.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
+    got = kb.attention_decode(q, k, v, n, bias=bias)
+    close(got, decode_want(q, k, v, lengths, bias), TOL[dtype], "decode")
+    assert (got[11] == 0).all() and (got[13] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,capacity", [(1, 1), (1, 33), (1, 9000), (3, 4096), (200, 70)])
+def test_decode_sizes(batch, capacity, dtype):
+    lengths = [capacity - (b * 7) % max(1, capacity // 2) for b in range(batch)]
+    q, k, v, n = decode_case(batch, capacity, 8, 2, 64, dtype, lengths)
+    close(kb.attention_decode(q, k, v, n), decode_want(q, k, v, lengths, None), TOL[dtype], "decode")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_reads_no_slot_past_the_length(dtype):
+    lengths = [1, 40, 129]
+    q, k, v, n = decode_case(3, 130, 6, 3, 64, dtype, lengths)
+    want = kb.attention_decode(q, k, v, n)
+    for b, m in enumerate(lengths):
+        k[b, m:], v[b, m:] = float("nan"), float("inf")
+    assert torch.equal(kb.attention_decode(q, k, v, n), want)
+
+
+def test_decode_cache_in_another_order():
+    # (batch, kv_heads, capacity, dim) storage, viewed in the call's order
+    q, k, v, n = decode_case(4, 100, 4, 2, 64, torch.bfloat16, [100, 3, 50, 77])
+    kt, vt = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (k, v))
+    assert torch.equal(kb.attention_decode(q, kt, vt, n), kb.attention_decode(q, k, v, n))
+
+
+def test_decode_past_32_bit_offsets():
+    # the cache holds more than 2^31 elements; only the last sequence's end is looked at
+    cap, kv_heads, dim = 1 << 20, 8, 128
+    k = torch.zeros(3, cap, kv_heads, dim, device="cuda", dtype=torch.bfloat16)
+    v = torch.zeros_like(k)
+    q = torch.randn(3, kv_heads, dim, device="cuda").bfloat16()
+    k[2, cap - 1] = q[2] * 4
+    v[2, cap - 1] = torch.randn(kv_heads, dim, device="cuda").bfloat16()
+    n = torch.tensor([1, 1, cap], dtype=torch.int32, device="cuda")
+    got = kb.attention_decode(q, k, v, n)
+    s = 4 * q[2].double().square().sum(-1, keepdim=True) / math.sqrt(dim)
+    p = s.exp() / (s.exp() + cap - 1)
+    assert (got[:2] == 0).all()
+    close(got[2], p * v[2, cap - 1].double(), 2e-2, "last slot")
+
+
+def test_decode_agrees_with_attention():
+    lens = [30, 200, 77]
+    q, k, v, n = decode_case(3, 256, 8, 2, 64, torch.bfloat16, lens)
+    packed = [torch.cat([t[b, :m] for b, m in enumerate(lens)]) for t in (k, v)]
+    want = kb.attention(q, *packed, kb.PackedSequences([1, 1, 1], lens))
+    close(kb.attention_decode(q, k, v, n), want.double(), 2e-2, "decode")
+
+
+def test_decode_refusals():
+    q, k, v, n = decode_case(2, 8, 4, 2, 16, torch.float32, [1, 2])
+    with pytest.raises(ValueError):
+        kb.attention_decode(q, k, v, n.long())
+    with pytest.raises(ValueError):
+        kb.attention_decode(q[:1], k, v, n)
+    with pytest.raises(ValueError):
+        kb.attention_decode(q, k, v, n[:1])
+    with pytest.raises(TypeError):
+        kb.attention_decode(q, k.bfloat16(), v.bfloat16(), n)
+    with pytest.raises(RuntimeError):
+        kb.attention_decode(q.requires_grad_(), k, v, n)
+    with pytest.raises(RuntimeError):
+        kb.attention_decode(q.detach().cpu(), k.cpu(), v.cpu(), n.cpu())
