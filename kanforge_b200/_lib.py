@@ -234,14 +234,16 @@ PROTOTYPES = {
     "kf_residual_norm_fwd": (ctypes.c_int, [_vp] * 10 + [_c_i64, ctypes.POINTER(ResidualNormDesc), _vp]),
     "kf_residual_norm_workspace": (_c_i64, [_c_i64, _c_i32]),
     "kf_residual_norm_bwd": (ctypes.c_int, [_vp] * 17 + [_c_i64, ctypes.POINTER(ResidualNormDesc), _vp]),
-    "kf_attention_tile_rows": (ctypes.c_int, [ctypes.POINTER(AttentionDesc)]),
+    "kf_attention_tiling": (
+        ctypes.c_int, [ctypes.POINTER(AttentionDesc), ctypes.c_int, ctypes.POINTER(_c_i32), ctypes.POINTER(_c_i32)],
+    ),
     "kf_attention_fwd": (
-        ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _vp, _vp, _vp, ctypes.POINTER(AttentionDesc), _vp],
+        ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(AttentionDesc), _vp],
     ),
     "kf_attention_bwd_workspace": (_c_i64, [_c_i32, ctypes.POINTER(AttentionDesc)]),
     "kf_attention_bwd": (
         ctypes.c_int,
-        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
          ctypes.POINTER(AttentionDesc), _vp],
     ),
     "kf_attention_decode_splits": (ctypes.c_int, [ctypes.POINTER(DecodeDesc)]),

@@ -58,19 +58,19 @@ class PackedSequences:
     def __len__(self) -> int:
         return len(self.q_lens)
 
-    def tiles(self, side: str, rows: int, causal: bool) -> torch.Tensor:
+    def tiles(self, side: str, rows: int, causal: bool, pack: int = 1) -> torch.Tensor:
         """(n, 2) int32 (sequence, tile): every ``rows`` rows of the query ("q") or
-        key ("k") side, those with the most work first."""
-        key = (side, rows, causal)
+        key ("k") side, ``pack`` rows to a token, those with the most work first."""
+        key = (side, rows, causal, pack)
         if key not in self._tiles:
             found = []
             for s, (lq, lk) in enumerate(zip(self.q_lens, self.kv_lens)):
                 off = lk - lq
-                for t in range(-(-(lq if side == "q" else lk) // rows)):
+                for t in range(-(-(lq if side == "q" else lk) * pack // rows)):
                     if not causal:
                         cost = lk if side == "q" else lq
                     elif side == "q":
-                        cost = max(0, min(lk, (t + 1) * rows + off))
+                        cost = max(0, min(lk, -(-(t + 1) * rows // pack) + off))
                     else:
                         cost = max(0, lq - max(0, t * rows - off))
                     found.append((-cost, s, t))
@@ -186,32 +186,36 @@ class _Call:
             0 if table is None else bias.max_distance, 0 if table is None else bias.num_buckets,
             0 if table is None else _DTYPE_CODE[table.dtype], scale)
 
-    def tiles(self, side: str) -> torch.Tensor:
-        rows = _lib.load().kf_attention_tile_rows(ctypes.byref(self.desc))
-        return self.seqs.tiles(side, rows, self.causal)
+    def tiles(self, what: int) -> torch.Tensor:
+        """The tiles of the forward's queries (0), the backward's queries (1) or its keys (2)."""
+        rows, pack = ctypes.c_int32(), ctypes.c_int32()
+        _lib.call("kf_attention_tiling", ctypes.byref(self.desc), what, ctypes.byref(rows), ctypes.byref(pack))
+        return self.seqs.tiles("k" if what == 2 else "q", rows.value, self.causal, pack.value)
 
     def forward(self, with_lse: bool):
         q = self.q
         o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         lse = torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32) if with_lse else None
-        tiles = self.tiles("q")
+        # bf16: what the rounding of o leaves out, so that delta = dout . o keeps float32's digits
+        rest = torch.empty_like(o) if with_lse and q.dtype == torch.bfloat16 else None
+        tiles = self.tiles(0)
         if tiles.shape[0]:
             _launch("kf_attention_fwd", _ptr(q), _ptr(self.k), _ptr(self.v), _ptr(self.seqs.table), _ptr(tiles),
-                    tiles.shape[0], _ptr(self.table), _ptr(self.buckets), _ptr(o), _ptr(lse), ctypes.byref(self.desc),
-                    _stream(q))
-        return o, lse
+                    tiles.shape[0], _ptr(self.table), _ptr(self.buckets), _ptr(o), _ptr(rest), _ptr(lse),
+                    ctypes.byref(self.desc), _stream(q))
+        return o, rest, lse
 
-    def backward(self, o, lse, dout, want_table: bool):
+    def backward(self, o, rest, lse, dout, want_table: bool):
         q, k = self.q, self.k
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
         dtable = torch.empty_like(self.table) if want_table else None
-        q_tiles, k_tiles = self.tiles("q"), self.tiles("k")
+        q_tiles, k_tiles = self.tiles(1), self.tiles(2)
         n_ws = int(_lib.load().kf_attention_bwd_workspace(q_tiles.shape[0], ctypes.byref(self.desc)))
         ws = torch.empty(max(n_ws, 1), device=q.device, dtype=torch.float32)
         if q_tiles.shape[0] or k_tiles.shape[0] or want_table:
-            _launch("kf_attention_bwd", _ptr(q), _ptr(k), _ptr(self.v), _ptr(o), _ptr(dout), _ptr(lse),
-                    _ptr(self.seqs.table), _ptr(q_tiles), q_tiles.shape[0], _ptr(k_tiles), k_tiles.shape[0],
+            _launch("kf_attention_bwd", _ptr(q), _ptr(k), _ptr(self.v), _ptr(o), _ptr(rest), _ptr(dout),
+                    _ptr(lse), _ptr(self.seqs.table), _ptr(q_tiles), q_tiles.shape[0], _ptr(k_tiles), k_tiles.shape[0],
                     _ptr(self.table), _ptr(self.buckets), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), _ptr(ws),
                     ctypes.byref(self.desc), _stream(q), kernels=3 + int(want_table))
         return dq, dk, dv, dtable
@@ -220,20 +224,20 @@ class _Call:
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, seqs, causal, scale, bias):
-        o, lse = _Call(q, k, v, table, seqs, causal, scale, bias).forward(with_lse=True)
-        ctx.save_for_backward(q, k, v, table, o, lse)
+        o, rest, lse = _Call(q, k, v, table, seqs, causal, scale, bias).forward(with_lse=True)
+        ctx.save_for_backward(q, k, v, table, o, rest, lse)
         ctx.options = (seqs, causal, scale, bias)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, o, lse = ctx.saved_tensors
+        q, k, v, table, o, rest, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
         call = _Call(q, k, v, table, *ctx.options)
         dout = dout.to(q.dtype).contiguous()
         dout = _vectors(dout)
-        dq, dk, dv, dtable = call.backward(o, lse, dout, table is not None and need[3])
+        dq, dk, dv, dtable = call.backward(o, rest, lse, dout, table is not None and need[3])
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None, None, None)
 
 
@@ -260,6 +264,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: PackedSeq
                          f"and {k.shape[0]}")
     if seqs.device != q.device:
         raise ValueError(f"the sequences lie on {seqs.device}, the queries on {q.device}")
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive, not {scale}")
     table = None if bias is None else bias.weight
     args = (q, k, v, table, seqs, bool(causal), 1.0 / math.sqrt(dim) if scale is None else float(scale), bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
@@ -288,6 +294,8 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     tracked = [q, k_cache, v_cache] + ([bias.weight] if bias is not None else [])
     if torch.is_grad_enabled() and any(t.requires_grad for t in tracked):
         raise RuntimeError("attention_decode has no backward: call it under torch.no_grad(), or use attention")
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive, not {scale}")
     q, k, v = _vectors(q.detach()), _vectors(k_cache.detach()), _vectors(v_cache.detach())
     lengths = lengths.contiguous()
     table = None if bias is None else bias.weight.detach().contiguous()

@@ -1,0 +1,134 @@
+// C ABI of packed attention: checks, tiling and dispatch by type, and the
+// last step of the bias gradient.
+#include "attention_tc.cuh"
+
+namespace kf {
+namespace {
+
+using namespace attn;
+
+// The bias gradient: the tiles' sums of one (bucket, head) in tile order, over 32 lanes.
+__global__ void __launch_bounds__(256) attention_dtable(const float* part, int n_tiles, int heads, int n_buckets, void* out,
+                                                        bool bf16) {
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;  // head * n_buckets + bucket
+  if (i >= heads * n_buckets) return;
+  float v = 0.f;
+  for (int t = lane; t < n_tiles; t += 32) v += part[(int64_t)t * heads * n_buckets + i];
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+  if (lane != 0) return;
+  const int64_t at = (int64_t)(i % n_buckets) * heads + i / n_buckets;
+  if (bf16)
+    static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else
+    static_cast<float*>(out)[at] = v;
+}
+
+int check_attention(const char* fn, const kf_attention_desc* d) {
+  KF_CHECK_ARG(d != nullptr, "%s: null descriptor", fn);
+  KF_CHECK_ARG(d->heads >= 1 && d->kv_heads >= 1 && d->heads % d->kv_heads == 0, "%s: %d heads do not divide over %d key heads", fn,
+               d->heads, d->kv_heads);
+  KF_CHECK_ARG(d->heads <= 65535, "%s: %d heads", fn, d->heads);
+  KF_CHECK_ARG(d->dim >= 8 && d->dim <= kMaxDim && d->dim % 8 == 0, "%s: head width %d is not a multiple of 8 up to %d", fn, d->dim,
+               kMaxDim);
+  KF_CHECK_ARG(d->dtype == KF_DTYPE_F32 || d->dtype == KF_DTYPE_BF16, "%s: types must be float32 or bfloat16", fn);
+  KF_CHECK_ARG(d->tq >= 0 && d->tk >= 0 && d->n_seqs >= 0, "%s: negative size", fn);
+  KF_CHECK_ARG(d->span >= 0 && d->span <= kMaxSpan, "%s: bias distances up to %d are outside [0, %d]", fn, d->span, kMaxSpan);
+  KF_CHECK_ARG(d->n_buckets >= 0 && d->n_buckets <= kMaxBuckets, "%s: %d buckets exceed %d", fn, d->n_buckets, kMaxBuckets);
+  return KF_OK;
+}
+
+// Rows of a tile of the forward's queries (pass 0), the backward's queries (1)
+// and its keys (2), and how many neighbouring rows are heads of one token.
+// bf16 packs the heads that share a key head, unless their bias tables would
+// not fit in shared memory.
+void tiling(const kf_attention_desc* d, int pass, int32_t* rows, int32_t* pack) {
+  *pack = 1;
+  if (d->dtype == KF_DTYPE_F32 || pass > 0) {
+    *rows = 64;
+    return;
+  }
+  *rows = 256;
+  const int group = d->heads / d->kv_heads;
+  if (d->n_buckets == 0 || group * bias_floats(d->span) * (int)sizeof(float) <= kBiasBytes) *pack = group;
+}
+
+Args make_args(const kf_attention_desc* d) {
+  Args a{};
+  a.heads = d->heads, a.kv_heads = d->kv_heads, a.dim = d->dim, a.span = d->span, a.n_buckets = d->n_buckets;
+  a.causal = d->causal != 0, a.table_bf16 = d->table_dtype == KF_DTYPE_BF16;
+  a.scale = d->scale, a.tq = d->tq;
+  a.q = {nullptr, d->q_row, d->q_head};
+  a.k = {nullptr, d->k_row, d->k_head};
+  a.v = {nullptr, d->v_row, d->v_head};
+  a.dout = {nullptr, (int64_t)d->heads * d->dim, d->dim};
+  return a;
+}
+
+}  // namespace
+}  // namespace kf
+
+extern "C" int kf_attention_tiling(const kf_attention_desc* d, int pass, int32_t* rows, int32_t* pack) {
+  using namespace kf;
+  clear_error();
+  if (int rc = check_attention("kf_attention_tiling", d)) return rc;
+  KF_CHECK_ARG(pass >= 0 && pass <= 2 && rows && pack, "kf_attention_tiling: bad argument");
+  tiling(d, pass, rows, pack);
+  return KF_OK;
+}
+
+extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* q_tiles,
+                                int32_t n_q_tiles, const void* table, const int32_t* buckets, void* o, void* o_rest,
+                                float* lse, const kf_attention_desc* d, void* stream) {
+  using namespace kf;
+  clear_error();
+  if (int rc = check_attention("kf_attention_fwd", d)) return rc;
+  if (n_q_tiles == 0) return KF_OK;
+  KF_CHECK_ARG(n_q_tiles > 0, "kf_attention_fwd: negative tile count");
+  KF_CHECK_ARG(q && o && seqs && q_tiles && (d->tk == 0 || (k && v)), "kf_attention_fwd: null argument");
+  KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_fwd: the bias needs a table and buckets");
+  if (int rc = bind_device(q)) return rc;
+  Args a = make_args(d);
+  a.q.p = q, a.k.p = k, a.v.p = v, a.o = o, a.o_rest = o_rest, a.lse = lse, a.table = table, a.buckets = buckets;
+  a.seqs = reinterpret_cast<const int4*>(seqs), a.tiles = reinterpret_cast<const int2*>(q_tiles);
+  int rows;
+  tiling(d, 0, &rows, &a.pack);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return d->dtype == KF_DTYPE_BF16 ? fwd_bf16(a, n_q_tiles, st) : fwd_f32(a, n_q_tiles, st);
+}
+
+extern "C" int64_t kf_attention_bwd_workspace(int32_t n_q_tiles, const kf_attention_desc* d) {
+  if (d == nullptr || n_q_tiles < 0) return 0;
+  return (int64_t)d->heads * d->tq + (int64_t)n_q_tiles * d->heads * d->n_buckets;
+}
+
+extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout, const float* lse,
+                                const int32_t* seqs, const int32_t* q_tiles, int32_t n_q_tiles, const int32_t* k_tiles,
+                                int32_t n_k_tiles, const void* table, const int32_t* buckets, void* dq, void* dk, void* dv,
+                                void* dtable, float* workspace, const kf_attention_desc* d, void* stream) {
+  using namespace kf;
+  clear_error();
+  if (int rc = check_attention("kf_attention_bwd", d)) return rc;
+  KF_CHECK_ARG(n_q_tiles >= 0 && n_k_tiles >= 0, "kf_attention_bwd: negative tile count");
+  KF_CHECK_ARG(n_q_tiles == 0 || (q && o && dout && lse && dq && workspace && q_tiles && seqs), "kf_attention_bwd: null argument");
+  KF_CHECK_ARG(n_k_tiles == 0 || (k && v && dk && dv && k_tiles && seqs), "kf_attention_bwd: null argument");
+  KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_bwd: the bias needs a table and buckets");
+  KF_CHECK_ARG(dtable == nullptr || (table != nullptr && workspace != nullptr), "kf_attention_bwd: dtable needs a table and workspace");
+  if (n_q_tiles == 0 && n_k_tiles == 0 && dtable == nullptr) return KF_OK;
+  if (int rc = bind_device(n_q_tiles ? q : n_k_tiles ? k : dtable)) return rc;
+  Args a = make_args(d);
+  a.q.p = q, a.k.p = k, a.v.p = v, a.dout.p = dout, a.o = const_cast<void*>(o), a.o_rest = const_cast<void*>(o_rest), a.lse = const_cast<float*>(lse);
+  a.dq = dq, a.dk = dk, a.dv = dv, a.table = table, a.buckets = buckets;
+  a.seqs = reinterpret_cast<const int4*>(seqs), a.tiles = reinterpret_cast<const int2*>(q_tiles);
+  a.delta = workspace;
+  a.dtable_part = dtable != nullptr ? workspace + (int64_t)d->heads * d->tq : nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int2* kt = reinterpret_cast<const int2*>(k_tiles);
+  int rows;
+  tiling(d, 1, &rows, &a.pack);
+  int rc = d->dtype == KF_DTYPE_BF16 ? bwd_bf16(a, kt, n_q_tiles, n_k_tiles, st) : bwd_f32(a, kt, n_q_tiles, n_k_tiles, st);
+  if (rc || dtable == nullptr) return rc;
+  attention_dtable<<<(unsigned)cdiv(d->heads * d->n_buckets, 8), 256, 0, st>>>(a.dtable_part, n_q_tiles, d->heads, d->n_buckets, dtable,
+                                                                               a.table_bf16);
+  return check_launch("kf_attention_bwd");
+}

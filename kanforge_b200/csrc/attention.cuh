@@ -31,6 +31,7 @@ struct Strided {  // (tokens, heads, dim), last dimension contiguous; strides in
 struct Args {
   Strided q, k, v, dout;
   void* o;      // (Tq, H, D) contiguous; read by the backward
+  void* o_rest; // bf16: what the rounding of o left out, for delta; may be null
   void *dq, *dk, *dv;
   float* lse;   // (H, Tq)
   float* delta; // (H, Tq): dO . O
@@ -41,6 +42,7 @@ struct Args {
   float* dtable_part; // (tiles, H, buckets)
   int64_t tq;
   int heads, kv_heads, dim, span, n_buckets;
+  int pack;  // heads that are neighbouring rows of a tile (bf16)
   bool causal, table_bf16;
   float scale;
 };
@@ -68,6 +70,12 @@ __device__ __forceinline__ void expand_bias(const Args& a, int head, float* out,
     out[i] = bias_base2(b);
   }
 }
+
+// attention_f32.cu, attention_fwd.cu, attention_bwd.cu
+int fwd_f32(const Args& a, int n_tiles, cudaStream_t st);
+int bwd_f32(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st);
+int fwd_bf16(const Args& a, int n_tiles, cudaStream_t st);
+int bwd_bf16(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st);
 
 __device__ __forceinline__ int clamp_dist(int d, int span) { return min(max(d, -span), span) + span; }
 

@@ -9,8 +9,6 @@
 // are bound by the FMA pipe.  The backward runs dK/dV (rows = keys, sums over
 // the heads that share a key head) and dQ (rows = queries) separately: both
 // recompute the scores, and every sum has one order.
-#include <type_traits>
-
 #include "attention.cuh"
 
 namespace kf {
@@ -193,7 +191,8 @@ __global__ void __launch_bounds__(256) attention_delta(const Args a) {
   const T* o = static_cast<const T*>(a.o) + i * a.dim;
   const T* g = static_cast<const T*>(a.dout.p) + tok * a.dout.row + head * a.dout.head;
   float v = 0.f;
-  for (int c = lane; c < a.dim; c += 32) v = fmaf(to_f32<T>(o[c]), to_f32<T>(g[c]), v);
+  const T* rest = a.o_rest == nullptr ? nullptr : static_cast<const T*>(a.o_rest) + i * a.dim;
+  for (int c = lane; c < a.dim; c += 32) v = fmaf(to_f32<T>(o[c]) + (rest ? to_f32<T>(rest[c]) : 0.f), to_f32<T>(g[c]), v);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
   if (lane == 0) a.delta[head * a.tq + tok] = v;
@@ -358,23 +357,6 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
   store_rows<T, D>(static_cast<T*>(a.dk), s.k0 + r0, n_rows, a.kv_heads, kv_head, a.dim, ty, tx, dk, mul);
 }
 
-// The bias gradient: the tiles' sums of one (bucket, head) in tile order, over 32 lanes.
-__global__ void __launch_bounds__(256) attention_dtable(const float* part, int n_tiles, int heads, int n_buckets, void* out,
-                                                        bool bf16) {
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;  // head * n_buckets + bucket
-  if (i >= heads * n_buckets) return;
-  float v = 0.f;
-  for (int t = lane; t < n_tiles; t += 32) v += part[(int64_t)t * heads * n_buckets + i];
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-  if (lane != 0) return;
-  const int64_t at = (int64_t)(i % n_buckets) * heads + i / n_buckets;
-  if (bf16)
-    static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
-  else
-    static_cast<float*>(out)[at] = v;
-}
-
 template <typename K>
 int run(K* kernel, dim3 grid, size_t floats, const Args& a, cudaStream_t st, const char* what) {
   KF_CUDA_RET(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(floats * sizeof(float))));
@@ -406,96 +388,17 @@ int bwd(const Args& a0, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) 
   return KF_OK;
 }
 
-int check_attention(const char* fn, const kf_attention_desc* d) {
-  KF_CHECK_ARG(d != nullptr, "%s: null descriptor", fn);
-  KF_CHECK_ARG(d->heads >= 1 && d->kv_heads >= 1 && d->heads % d->kv_heads == 0, "%s: %d heads do not divide over %d key heads", fn,
-               d->heads, d->kv_heads);
-  KF_CHECK_ARG(d->heads <= 65535, "%s: %d heads", fn, d->heads);
-  KF_CHECK_ARG(d->dim >= 8 && d->dim <= kMaxDim && d->dim % 8 == 0, "%s: head width %d is not a multiple of 8 up to %d", fn, d->dim,
-               kMaxDim);
-  KF_CHECK_ARG(d->dtype == KF_DTYPE_F32 || d->dtype == KF_DTYPE_BF16, "%s: types must be float32 or bfloat16", fn);
-  KF_CHECK_ARG(d->tq >= 0 && d->tk >= 0 && d->n_seqs >= 0, "%s: negative size", fn);
-  KF_CHECK_ARG(d->span >= 0 && d->span <= kMaxSpan, "%s: bias distances up to %d are outside [0, %d]", fn, d->span, kMaxSpan);
-  KF_CHECK_ARG(d->n_buckets >= 0 && d->n_buckets <= kMaxBuckets, "%s: %d buckets exceed %d", fn, d->n_buckets, kMaxBuckets);
-  return KF_OK;
-}
-
-Args make_args(const kf_attention_desc* d) {
-  Args a{};
-  a.heads = d->heads, a.kv_heads = d->kv_heads, a.dim = d->dim, a.span = d->span, a.n_buckets = d->n_buckets;
-  a.causal = d->causal != 0, a.table_bf16 = d->table_dtype == KF_DTYPE_BF16;
-  a.scale = d->scale, a.tq = d->tq;
-  a.q = {nullptr, d->q_row, d->q_head};
-  a.k = {nullptr, d->k_row, d->k_head};
-  a.v = {nullptr, d->v_row, d->v_head};
-  a.dout = {nullptr, (int64_t)d->heads * d->dim, d->dim};
-  return a;
-}
-
-template <typename F>
-int by_type(const kf_attention_desc* d, F&& f) {
-  using bf = __nv_bfloat16;
-  if (d->dtype == KF_DTYPE_BF16)
-    return d->dim <= 64 ? f(bf{}, std::integral_constant<int, 64>{}) : f(bf{}, std::integral_constant<int, 128>{});
-  return d->dim <= 64 ? f(float{}, std::integral_constant<int, 64>{}) : f(float{}, std::integral_constant<int, 128>{});
-}
-
 }  // namespace
+
+namespace attn {
+int fwd_f32(const Args& a, int n_tiles, cudaStream_t st) {
+  return a.dim <= 64 ? fwd<float, 64>(a, n_tiles, st) : fwd<float, 128>(a, n_tiles, st);
+}
+int bwd_f32(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+  return a.dim <= 64 ? bwd<float, 64>(a, k_tiles, n_q, n_k, st) : bwd<float, 128>(a, k_tiles, n_q, n_k, st);
+}
+int bwd_bf16(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+  return a.dim <= 64 ? bwd<__nv_bfloat16, 64>(a, k_tiles, n_q, n_k, st) : bwd<__nv_bfloat16, 128>(a, k_tiles, n_q, n_k, st);
+}
+}  // namespace attn
 }  // namespace kf
-
-extern "C" int kf_attention_tile_rows(const kf_attention_desc* d) {
-  (void)d;
-  return kf::kTile;
-}
-
-extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* q_tiles,
-                                int32_t n_q_tiles, const void* table, const int32_t* buckets, void* o, float* lse,
-                                const kf_attention_desc* d, void* stream) {
-  using namespace kf;
-  clear_error();
-  if (int rc = check_attention("kf_attention_fwd", d)) return rc;
-  if (n_q_tiles == 0) return KF_OK;
-  KF_CHECK_ARG(n_q_tiles > 0, "kf_attention_fwd: negative tile count");
-  KF_CHECK_ARG(q && o && seqs && q_tiles && (d->tk == 0 || (k && v)), "kf_attention_fwd: null argument");
-  KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_fwd: the bias needs a table and buckets");
-  if (int rc = bind_device(q)) return rc;
-  Args a = make_args(d);
-  a.q.p = q, a.k.p = k, a.v.p = v, a.o = o, a.lse = lse, a.table = table, a.buckets = buckets;
-  a.seqs = reinterpret_cast<const int4*>(seqs), a.tiles = reinterpret_cast<const int2*>(q_tiles);
-  return by_type(d, [&](auto t, auto dim) { return fwd<decltype(t), decltype(dim)::value>(a, n_q_tiles, static_cast<cudaStream_t>(stream)); });
-}
-
-extern "C" int64_t kf_attention_bwd_workspace(int32_t n_q_tiles, const kf_attention_desc* d) {
-  if (d == nullptr || n_q_tiles < 0) return 0;
-  return (int64_t)d->heads * d->tq + (int64_t)n_q_tiles * d->heads * d->n_buckets;
-}
-
-extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,
-                                const int32_t* seqs, const int32_t* q_tiles, int32_t n_q_tiles, const int32_t* k_tiles,
-                                int32_t n_k_tiles, const void* table, const int32_t* buckets, void* dq, void* dk, void* dv,
-                                void* dtable, float* workspace, const kf_attention_desc* d, void* stream) {
-  using namespace kf;
-  clear_error();
-  if (int rc = check_attention("kf_attention_bwd", d)) return rc;
-  KF_CHECK_ARG(n_q_tiles >= 0 && n_k_tiles >= 0, "kf_attention_bwd: negative tile count");
-  KF_CHECK_ARG(n_q_tiles == 0 || (q && o && dout && lse && dq && workspace && q_tiles && seqs), "kf_attention_bwd: null argument");
-  KF_CHECK_ARG(n_k_tiles == 0 || (k && v && dk && dv && k_tiles && seqs), "kf_attention_bwd: null argument");
-  KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_bwd: the bias needs a table and buckets");
-  KF_CHECK_ARG(dtable == nullptr || (table != nullptr && workspace != nullptr), "kf_attention_bwd: dtable needs a table and workspace");
-  if (n_q_tiles == 0 && n_k_tiles == 0 && dtable == nullptr) return KF_OK;
-  if (int rc = bind_device(n_q_tiles ? q : n_k_tiles ? k : dtable)) return rc;
-  Args a = make_args(d);
-  a.q.p = q, a.k.p = k, a.v.p = v, a.dout.p = dout, a.o = const_cast<void*>(o), a.lse = const_cast<float*>(lse);
-  a.dq = dq, a.dk = dk, a.dv = dv, a.table = table, a.buckets = buckets;
-  a.seqs = reinterpret_cast<const int4*>(seqs), a.tiles = reinterpret_cast<const int2*>(q_tiles);
-  a.delta = workspace;
-  a.dtable_part = dtable != nullptr ? workspace + (int64_t)d->heads * d->tq : nullptr;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int rc = by_type(d, [&](auto t, auto dim) {
-    return bwd<decltype(t), decltype(dim)::value>(a, reinterpret_cast<const int2*>(k_tiles), n_q_tiles, n_k_tiles, st);
-  });
-  if (rc || dtable == nullptr) return rc;
-  attention_dtable<<<(unsigned)cdiv(d->heads * d->n_buckets, 8), 256, 0, st>>>(a.dtable_part, n_q_tiles, d->heads, d->n_buckets, dtable,
-                                                                               a.table_bf16);
-  return check_launch("kf_attention_bwd");
-}
