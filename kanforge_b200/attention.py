@@ -22,7 +22,7 @@ from . import _lib
 from .kernels import _check_cuda, _launch, _ptr, _stream
 
 ATTENTION_MAX_DIM = 128
-BIAS_MAX_DISTANCE, BIAS_MAX_BUCKETS = 2048, 256
+BIAS_MAX_DISTANCE, BIAS_MAX_BUCKETS = 1024, 256
 
 _DTYPE_CODE = {torch.float32: _lib.KF_DTYPE_F32, torch.bfloat16: _lib.KF_DTYPE_BF16}
 

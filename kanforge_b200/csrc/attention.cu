@@ -44,11 +44,8 @@ int check_attention(const char* fn, const kf_attention_desc* d) {
 // not fit in shared memory.
 void tiling(const kf_attention_desc* d, int pass, int32_t* rows, int32_t* pack) {
   *pack = 1;
-  if (d->dtype == KF_DTYPE_F32 || pass > 0) {
-    *rows = 64;
-    return;
-  }
-  *rows = 256;
+  *rows = d->dtype == KF_DTYPE_F32 ? 64 : pass == 0 ? 256 : 128;
+  if (d->dtype == KF_DTYPE_F32 || pass > 0) return;
   const int group = d->heads / d->kv_heads;
   if (d->n_buckets == 0 || group * bias_floats(d->span) * (int)sizeof(float) <= kBiasBytes) *pack = group;
 }

@@ -15,7 +15,7 @@ namespace kf {
 namespace attn {
 
 constexpr int kMaxDim = 128;
-constexpr int kMaxSpan = 2048;    // largest distance with a bias of its own
+constexpr int kMaxSpan = 1024;    // largest distance with a bias of its own
 constexpr int kMaxBuckets = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 

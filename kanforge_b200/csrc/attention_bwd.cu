@@ -1,0 +1,593 @@
+// Attention backward over packed sequences for bf16, on the tensor cores.
+//
+// Two kernels, so that every sum has one order without atomics: both form the
+// scores again, P = 2^(t - lse), and dS = P (dP - delta) with dP = dO V^T.
+//   dQ    rows = 128 queries of a head, walks over key tiles:
+//         S, dP -> dS -> dQ += dS K; first it makes delta = dO . O, which the
+//         second kernel reads, and it sums dS by distance for the bias gradient.
+//   dK dV rows = 128 keys of a key head, walks over the query tiles of all heads
+//         that share it: S^T, dP^T -> P^T, dS^T -> dV += P^T dO, dK += dS^T Q.
+// Seven products of 128 x 128 x D a tile pair against five with one kernel;
+// the five would add every dQ tile into memory in an order that varies.
+// All scores live in tensor memory; P and dS go back there as bf16 (2^-9 of
+// each term) and are the A operands of the products that sum them.  Of the 12
+// warps 0-7 do the softmax arithmetic (thread = row, a warpgroup per half of
+// the columns), 8-10 load, 11 issues the MMAs.
+#include "attention_tc.cuh"
+
+namespace kf {
+namespace {
+
+using namespace attn;
+
+constexpr int kThreads = 384, kLoaders = 96, kSoftmax = 256;
+
+template <int DP>
+struct Bwd {
+  static constexpr int kStages = DP == 64 ? 6 : 4;  // streamed tiles in flight
+  static constexpr int kTile = tile_bytes<DP>();
+  static constexpr int kFloats = 1024 + (2 + kStages) * kTile;  // offset of what follows the tiles
+};
+
+struct Ctl {
+  uint64_t fixed_full, fin, full[8], empty[8], s_full, dp_full, s_read, p_ready, ds_ready, dv_done, dk_done;
+  uint32_t tmem;
+  int abort;
+};
+
+__device__ __forceinline__ void init_barriers(Ctl* c, int stages) {
+  c->abort = 0;
+  mbar_init(&c->fixed_full, kLoaders);
+  mbar_init(&c->fin, 1);
+  for (int i = 0; i < stages; ++i) mbar_init(&c->full[i], kLoaders), mbar_init(&c->empty[i], 1);
+  mbar_init(&c->s_full, 1), mbar_init(&c->dp_full, 1), mbar_init(&c->dv_done, 1), mbar_init(&c->dk_done, 1);
+  mbar_init(&c->s_read, kSoftmax), mbar_init(&c->p_ready, kSoftmax), mbar_init(&c->ds_ready, kSoftmax);
+  fence_barrier_init();
+}
+
+// Barrier of the softmax warps.  A warp whose wait ran out calls it once with
+// false and leaves; the others learn of it at their next call and leave too.
+__device__ __forceinline__ bool softmax_sync(bool ok = true) { return named_bar_and(1, kSoftmax, ok); }
+
+// One row of a result: DP columns of this thread's lane times mul, dim of them stored.
+template <int DP>
+__device__ __forceinline__ void store_row(uint32_t lanes, __nv_bfloat16* out, int dim, float mul, bool zero, bool valid) {
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) {
+    float o[32];
+    __syncwarp();
+    if (!zero) {
+      tmem_ld32_issue(lanes + i * 32, o);
+      tmem_wait_ld(o);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (!valid || i * 32 + q * 8 >= dim) continue;
+      uint4 w;
+      uint32_t* u = &w.x;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) u[c] = zero ? 0u : pack_bf16x2(o[q * 8 + 2 * c] * mul, o[q * 8 + 2 * c + 1] * mul);
+      *reinterpret_cast<uint4*>(out + i * 32 + q * 8) = w;
+    }
+  }
+}
+
+// ---- dQ -------------------------------------------------------------------------
+// Tensor memory: S at 0, dP at 128, dQ at 256, two buffers of dS at 384.
+
+// Floats behind the tiles: bias table, sums by distance, block diagonals, bucket ids.
+constexpr int kDiag = 16 * 64;  // 4 x 4 blocks of 32 x 32 scores, 63 diagonals each
+__host__ __device__ constexpr int dq_floats(bool bias, bool grad, int span) {
+  return 2 * kRows + (bias ? bias_floats(span) : 0) + (grad ? 2 * span + 1 + kDiag + (2 * span + 4) / 4 : 0);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a) {
+  using F = Bwd<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Ctl ctl;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* sdelta = reinterpret_cast<float*>(smem + (2 + F::kStages) * F::kTile);  // (2, 128) halves of delta
+  float* sbias = sdelta + 2 * kRows;
+  float* ssum = sbias + (a.table != nullptr ? bias_floats(a.span) : 0);
+  float* sdiag = ssum + 2 * a.span + 1;
+  uint8_t* sbucket = reinterpret_cast<uint8_t*>(sdiag + kDiag);
+  volatile int* abort = &ctl.abort;
+
+  const int2 tile = a.tiles[blockIdx.x];
+  const Seq s = load_seq(a, tile.x);
+  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+  const int r0 = tile.y * kRows, off = s.lk - s.lq, n_rows = min(kRows, s.lq - r0);
+  const int keys = a.causal ? max(0, min(s.lk, r0 + n_rows + off)) : s.lk;
+  const int n = (keys + kRows - 1) / kRows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool grad = a.dtable_part != nullptr;
+
+  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages);
+  if (warp == 11) {
+    tmem_alloc(&ctl.tmem, 512);
+    tmem_relinquish();
+  }
+  if (a.table != nullptr) expand_bias_padded(a, head, 1, sbias, threadIdx.x, kThreads);
+  if (grad)
+    for (int i = threadIdx.x; i < 2 * a.span + 1; i += kThreads) ssum[i] = 0.f, sbucket[i] = (uint8_t)a.buckets[i];
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl.tmem, q_tile = smem_u32(smem), ring = q_tile + 2 * F::kTile;
+
+  // registers: 384 x 168 at launch = 256 x 208 + 128 x 88
+  if (warp >= 8) reg_dec<88>();
+  if (warp >= 8 && warp < 11) {
+    // ---- loads: Q and dO, then K and V tiles in turn
+    const int tid = threadIdx.x - 256;
+    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q.p) + (int64_t)s.q0 * a.q.row + head * a.q.head;
+    const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(a.dout.p) + (int64_t)s.q0 * a.dout.row + head * a.dout.head;
+    const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.k.p) + (int64_t)s.k0 * a.k.row + kv_head * a.k.head;
+    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v.p) + (int64_t)s.k0 * a.v.row + kv_head * a.v.head;
+    load_tile_async<DP, kLoaders>(q_tile, q, a.q.row, 0, 1, r0, n_rows, a.dim, tid);
+    load_tile_async<DP, kLoaders>(q_tile + F::kTile, g, a.dout.row, 0, 1, r0, n_rows, a.dim, tid);
+    feed_ring<F::kStages>(2 * n, &ctl.fixed_full, ctl.full, ctl.empty, abort, [&](int it) {
+      const bool is_v = it & 1;
+      const int j = it >> 1;
+      load_tile_async<DP, kLoaders>(ring + it % F::kStages * F::kTile, is_v ? v : k, is_v ? a.v.row : a.k.row, 0, 1, j * kRows,
+                                    min(kRows, s.lk - j * kRows), a.dim, tid);
+    });
+  } else if (warp == 11) {
+    // ---- MMAs: S and dP of the next tile go ahead of dQ of this one
+    if (lane == 0 && n > 0) {
+      const uint32_t idesc_s = idesc_bf16_f32(kRows, kRows, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
+      auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* done) {
+        if (!mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort)) return false;
+        tc_fence_after();
+        const uint32_t b = ring + (it % F::kStages) * F::kTile;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) mma_ss(d, desc_k(fixed, i), desc_k(b, i), idesc_s, i > 0);
+        mma_commit(done);
+        return true;
+      };
+      auto dp = [&](int j) {
+        if (!product(2 * j + 1, tmem + 128, q_tile + F::kTile, &ctl.dp_full)) return false;
+        mma_commit(&ctl.empty[(2 * j + 1) % F::kStages]);  // V has no other use
+        return true;
+      };
+      bool ok = mbar_wait(&ctl.fixed_full, 0, abort) && product(0, tmem, q_tile, &ctl.s_full) && dp(0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) {
+          ok = mbar_wait(&ctl.s_read, j & 1, abort);
+          tc_fence_after();
+          ok = ok && product(2 * (j + 1), tmem, q_tile, &ctl.s_full);
+        }
+        if (!ok || !(ok = mbar_wait(&ctl.ds_ready, j & 1, abort))) break;
+        tc_fence_after();
+        if (j + 1 < n && !(ok = dp(j + 1))) break;
+        const uint32_t kt = ring + (2 * j % F::kStages) * F::kTile;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          mma_ts(tmem + 256, tmem + 384 + (j & 1) * 64 + i * 8, desc_mn(kt, i), idesc_d, j > 0 || i > 0);
+        mma_commit(&ctl.empty[2 * j % F::kStages]);
+      }
+      mma_commit(&ctl.dk_done);
+      mma_commit(&ctl.fin);
+      mbar_drain(&ctl.fin, 0);
+    }
+  } else {
+    reg_inc<208>();
+    // ---- softmax arithmetic: thread = query, a warpgroup per half of a tile's keys
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
+    const bool valid = row < n_rows;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int pos = r + off;
+    const int limit = valid && a.causal ? min(s.lk, pos + 1) : s.lk;
+    const int64_t stat = (int64_t)head * a.tq + s.q0 + r;
+    // delta = dO . O, half of the columns each
+    float delta = 0.f;
+    if (valid) {
+      const int64_t at = ((int64_t)(s.q0 + r) * a.heads + head) * a.dim;
+      const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(a.dout.p) + (int64_t)(s.q0 + r) * a.dout.row + head * a.dout.head;
+      const __nv_bfloat16* o = static_cast<const __nv_bfloat16*>(a.o) + at;
+      const __nv_bfloat16* e = a.o_rest == nullptr ? nullptr : static_cast<const __nv_bfloat16*>(a.o_rest) + at;
+#pragma unroll 4
+      for (int c = half * 8; c < a.dim; c += 16) {
+        const uint4 gv = *reinterpret_cast<const uint4*>(g + c), ov = *reinterpret_cast<const uint4*>(o + c);
+        const uint4 ev = e == nullptr ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(e + c);
+        const uint32_t *gw = &gv.x, *ow = &ov.x, *ew = &ev.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          delta = fmaf(__uint_as_float(gw[i] << 16), __uint_as_float(ow[i] << 16) + __uint_as_float(ew[i] << 16), delta);
+          delta = fmaf(__uint_as_float(gw[i] & 0xffff0000u),
+                       __uint_as_float(ow[i] & 0xffff0000u) + __uint_as_float(ew[i] & 0xffff0000u), delta);
+        }
+      }
+    }
+    sdelta[half * kRows + row] = delta;
+    softmax_sync();
+    delta = sdelta[row] + sdelta[kRows + row];
+    if (valid && half == 0) a.delta[stat] = delta;
+    // a row that sees one key has dS = 0; rows past the sequence likewise
+    const float lse = valid && !one_key(a, s, pos) ? a.lse[stat] : CUDART_INF_F;
+    const float c2 = a.scale * kLog2e;
+    const float* bias = sbias + a.span + kBiasPad;
+    float far_sum[2] = {0.f, 0.f};  // dS at distances >= span, <= -span
+    bool ok = true, together = true;
+    for (int j = 0; j < n; ++j) {
+      if (!(ok = mbar_wait_warp(&ctl.s_full, j & 1, abort))) break;
+      tc_fence_after();
+      float x[64];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) tmem_ld32_issue(lanes + half * 64 + i * 32, x + i * 32);
+      tmem_wait_ld(x);
+      tc_fence_before();
+      mbar_arrive(&ctl.s_read);
+      const int k0 = j * kRows + half * 64;
+      const int dist = pos - k0;
+      bool near = false;
+      float base = -lse;
+      if (a.table != nullptr) {
+        near = !__all_sync(0xffffffffu, dist - 63 >= a.span || dist <= -a.span);
+        if (near) {
+          const float* b = bias + max(-a.span - kBiasPad + 63, min(dist, a.span + kBiasPad));
+#pragma unroll
+          for (int i = 0; i < 64; ++i) x[i] = fmaf(x[i], c2, b[-i] - lse);
+        } else {
+          base = (dist > 0 ? bias[a.span] : bias[-a.span]) - lse;
+        }
+      }
+      if (!near) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) x[i] = fmaf(x[i], c2, base);
+      }
+#pragma unroll
+      for (int i = 0; i < 64; ++i) x[i] = ex2(x[i]);
+      const bool masked = __any_sync(0xffffffffu, limit - k0 < 64);
+      if (!(ok = mbar_wait_warp(&ctl.dp_full, j & 1, abort))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float d[32];
+        tmem_ld32_issue(lanes + 128 + half * 64 + h * 32, d);
+        tmem_wait_ld(d);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[h * 32 + i] *= d[i] - delta;
+      }
+      if (masked) {
+        const int seen = limit - k0;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) x[i] = i < seen ? x[i] : 0.f;
+      }
+      uint32_t w[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+      tmem_st32(lanes + 384 + (j & 1) * 64 + half * 32, w);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&ctl.ds_ready);
+      if (!grad) continue;
+      // ---- the bias gradient.  A tile farther than the span from all its keys adds to one bucket.
+      const int d0 = r0 + off - j * kRows;  // distance of the tile's first query and key
+      if (d0 - (kRows - 1) >= a.span || d0 + kRows - 1 <= -a.span) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 64; ++i) sum[i & 3] += x[i];
+        far_sum[d0 > 0 ? 0 : 1] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      } else {
+        // A partial sum moves along its diagonal, one lane up for each column; lane 31's is complete.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float* out = sdiag + ((warp & 3) * 4 + half * 2 + h) * 64;  // index row - column + 31
+          float acc = 0.f;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            if (c > 0) {
+              acc = __shfl_up_sync(0xffffffffu, acc, 1);
+              if (lane == 0) acc = 0.f;
+            }
+            acc += x[h * 32 + c];
+            if (lane == 31) out[62 - c] = acc;
+          }
+          if (lane < 31) out[lane] = acc;
+        }
+        if (!(together = softmax_sync())) break;
+        // thread i takes the tile's diagonal row - column = i - 127 over the 4 x 4 blocks, in order
+        const int i = threadIdx.x - (kRows - 1);
+        if (threadIdx.x < 2 * kRows - 1) {
+          float sum = 0.f;
+#pragma unroll
+          for (int b = 0; b < 16; ++b) {
+            const int e = i - ((b >> 2) - (b & 3)) * 32 + 31;
+            if (e >= 0 && e < 63) sum += sdiag[b * 64 + e];
+          }
+          const int dd = d0 + i;
+          if (dd >= a.span)
+            far_sum[0] += sum;
+          else if (dd <= -a.span)
+            far_sum[1] += sum;
+          else
+            ssum[dd + a.span] += sum;  // this thread's alone
+        }
+        if (!(together = softmax_sync())) break;
+      }
+    }
+    if (ok && together && n > 0) ok = mbar_wait_warp(&ctl.dk_done, 0, abort);
+    if (grad && together) together = softmax_sync(ok);
+    if (ok && together) {
+      tc_fence_after();
+      if (half == 0)
+        store_row<DP>(lanes + 256, static_cast<__nv_bfloat16*>(a.dq) + ((int64_t)(s.q0 + r) * a.heads + head) * a.dim, a.dim,
+                      a.scale, n == 0, valid);
+      if (grad) {
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) far_sum[f] += __shfl_xor_sync(0xffffffffu, far_sum[f], o);
+          if (lane == 0) sdiag[f * 8 + warp] = far_sum[f];
+        }
+        softmax_sync();
+        if (threadIdx.x < 2) {
+          float sum = 0.f;
+          for (int w = 0; w < 8; ++w) sum += sdiag[threadIdx.x * 8 + w];
+          ssum[threadIdx.x == 0 ? 2 * a.span : 0] += sum;
+        }
+        softmax_sync();
+        // a warp per bucket in turn
+        float* out = a.dtable_part + ((int64_t)blockIdx.x * a.heads + head) * a.n_buckets;
+        for (int b = warp; b < a.n_buckets; b += 8) {
+          float sum = 0.f;
+          for (int e = lane; e < 2 * a.span + 1; e += 32)
+            if (sbucket[e] == b) sum += ssum[e];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (lane == 0) out[b] = sum;
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 11) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- dK, dV -----------------------------------------------------------------------
+// Tensor memory: S^T at 0, dP^T at 128, dV and dK from 256.  With DP = 64 P^T
+// and dS^T have columns of their own; with DP = 128 they lie in their scores'
+// columns, and the next scores wait for the product that reads them.
+template <int DP>
+struct KvCols {
+  static constexpr uint32_t dv = 256, dk = 256 + DP;
+  static constexpr uint32_t p = DP == 64 ? 384 : 0, ds = DP == 64 ? 448 : 128;
+  static constexpr uint32_t half = DP == 64 ? 32 : 64;  // second warpgroup's columns
+  __device__ static constexpr uint32_t step(int i) { return (i >> 2) * half + (i & 3) * 8; }
+};
+
+__host__ __device__ constexpr int dkdv_floats(bool bias, int span) { return 8 * 2 * kRows + (bias ? bias_floats(span) : 0); }
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a) {
+  using F = Bwd<DP>;
+  using C = KvCols<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Ctl ctl;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* sstat = reinterpret_cast<float*>(smem + (2 + F::kStages) * F::kTile);  // lse, delta of each stage in the ring
+  float* sbias = sstat + 8 * 2 * kRows;
+  volatile int* abort = &ctl.abort;
+
+  const int2 tile = a.tiles[blockIdx.x];
+  const Seq s = load_seq(a, tile.x);
+  const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
+  const int r0 = tile.y * kRows, off = s.lk - s.lq, n_rows = min(kRows, s.lk - r0);
+  const int first = a.causal ? max(0, r0 - off) / kRows : 0;  // earlier query tiles see none of these keys
+  const int per_head = max(0, (s.lq + kRows - 1) / kRows - first), n = group * per_head;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages);
+  if (warp == 11) {
+    tmem_alloc(&ctl.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl.tmem, k_tile = smem_u32(smem), ring = k_tile + 2 * F::kTile;
+
+  if (warp >= 8) reg_dec<88>();
+  if (warp >= 8 && warp < 11) {
+    // ---- loads: K and V, then Q (with lse and delta) and dO tiles in turn
+    const int tid = threadIdx.x - 256;
+    const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.k.p) + (int64_t)s.k0 * a.k.row + kv_head * a.k.head;
+    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v.p) + (int64_t)s.k0 * a.v.row + kv_head * a.v.head;
+    load_tile_async<DP, kLoaders>(k_tile, k, a.k.row, 0, 1, r0, n_rows, a.dim, tid);
+    load_tile_async<DP, kLoaders>(k_tile + F::kTile, v, a.v.row, 0, 1, r0, n_rows, a.dim, tid);
+    feed_ring<F::kStages>(2 * n, &ctl.fixed_full, ctl.full, ctl.empty, abort, [&](int it) {
+      const int st = it % F::kStages, i = it >> 1;
+      const int head = kv_head * group + i / per_head, q0 = (first + i % per_head) * kRows;
+      const int n_q = min(kRows, s.lq - q0);
+      const Strided& src = it & 1 ? a.dout : a.q;
+      const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(src.p) + (int64_t)s.q0 * src.row + head * src.head;
+      load_tile_async<DP, kLoaders>(ring + st * F::kTile, p, src.row, 0, 1, q0, n_q, a.dim, tid);
+      if (it & 1) return;
+      const int64_t stat = (int64_t)head * a.tq + s.q0 + q0;
+      for (int c = tid; c < 2 * kRows; c += kLoaders) {
+        const int col = c & (kRows - 1);
+        const bool in = col < n_q;
+        const float* f = (c < kRows ? a.lse : a.delta) + stat + (in ? col : 0);
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sstat + st * 2 * kRows + c)), "l"(f), "r"(in ? 4 : 0)
+                     : "memory");
+      }
+    });
+  } else if (warp == 11) {
+    // ---- MMAs
+    if (lane == 0 && n > 0) {
+      const uint32_t idesc_s = idesc_bf16_f32(kRows, kRows, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
+      auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* done) {
+        if (!mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort)) return false;
+        tc_fence_after();
+        const uint32_t b = ring + (it % F::kStages) * F::kTile;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) mma_ss(d, desc_k(fixed, i), desc_k(b, i), idesc_s, i > 0);
+        mma_commit(done);
+        return true;
+      };
+      auto sum = [&](int it, uint32_t d, uint32_t p, bool more, uint64_t* done) {
+        const uint32_t b = ring + (it % F::kStages) * F::kTile;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mma_ts(d, p + C::step(i), desc_mn(b, i), idesc_d, more || i > 0);
+        mma_commit(done);
+        mma_commit(&ctl.empty[it % F::kStages]);
+      };
+      bool ok = mbar_wait(&ctl.fixed_full, 0, abort) && product(0, tmem, k_tile, &ctl.s_full) &&
+                product(1, tmem + 128, k_tile + F::kTile, &ctl.dp_full);
+      for (int i = 0; i < n && ok; ++i) {
+        if (!(ok = mbar_wait(&ctl.p_ready, i & 1, abort))) break;
+        tc_fence_after();
+        sum(2 * i + 1, tmem + C::dv, tmem + C::p, i > 0, &ctl.dv_done);
+        if (i + 1 < n) {
+          if (DP == 128 && !(ok = mbar_wait(&ctl.dv_done, i & 1, abort))) break;
+          if (!(ok = product(2 * (i + 1), tmem, k_tile, &ctl.s_full))) break;
+        }
+        if (!(ok = mbar_wait(&ctl.ds_ready, i & 1, abort))) break;
+        tc_fence_after();
+        sum(2 * i, tmem + C::dk, tmem + C::ds, i > 0, &ctl.dk_done);
+        if (i + 1 < n) {
+          if (DP == 128 && !(ok = mbar_wait(&ctl.dk_done, i & 1, abort))) break;
+          ok = product(2 * (i + 1) + 1, tmem + 128, k_tile + F::kTile, &ctl.dp_full);
+        }
+      }
+      mma_commit(&ctl.fin);
+      mbar_drain(&ctl.fin, 0);
+    }
+  } else {
+    reg_inc<208>();
+    // ---- softmax arithmetic: thread = key, a warpgroup per half of a tile's queries
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane, key = r0 + row;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float c2 = a.scale * kLog2e;
+    const float* bias = sbias + a.span + kBiasPad;
+    bool ok = true, together = true;
+    for (int i = 0; i < n; ++i) {
+      const int st = 2 * i % F::kStages, q0 = (first + i % per_head) * kRows + half * 64;
+      if (a.table != nullptr && i % per_head == 0) {  // another head's table
+        if (!(together = softmax_sync())) break;
+        expand_bias_padded(a, kv_head * group + i / per_head, 1, sbias, threadIdx.x, kSoftmax);
+        if (!(together = softmax_sync())) break;
+      }
+      ok = mbar_wait_warp(&ctl.full[st], (2 * i / F::kStages) & 1, abort) && mbar_wait_warp(&ctl.s_full, i & 1, abort);
+      if (!ok) break;
+      tc_fence_after();
+      float x[64];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) tmem_ld32_issue(lanes + half * 64 + h * 32, x + h * 32);
+      tmem_wait_ld(x);
+      const float4* lse = reinterpret_cast<const float4*>(sstat + st * 2 * kRows + half * 64);
+      const float4* delta = lse + kRows / 4;
+      const int dist = q0 + off - key;  // of the first column
+      float mul = c2, add = 0.f;
+      if (a.table != nullptr) {
+        if (__all_sync(0xffffffffu, dist >= a.span || dist + 63 <= -a.span)) {
+          add = dist > 0 ? bias[a.span] : bias[-a.span];
+        } else {
+          const float* b = bias + max(-a.span - kBiasPad, min(dist, a.span + kBiasPad - 63));
+#pragma unroll
+          for (int c = 0; c < 64; ++c) x[c] = fmaf(x[c], c2, b[c]);
+          mul = 1.f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 e = lse[c / 4];
+        x[c] = ex2(fmaf(x[c], mul, add - e.x));
+        x[c + 1] = ex2(fmaf(x[c + 1], mul, add - e.y));
+        x[c + 2] = ex2(fmaf(x[c + 2], mul, add - e.z));
+        x[c + 3] = ex2(fmaf(x[c + 3], mul, add - e.w));
+      }
+      // columns of queries that see this key: [from, to)
+      const int from = a.causal ? key - off - q0 : 0, to = s.lq - q0;
+      const bool masked = __any_sync(0xffffffffu, from > 0 || to < 64 || s.lk == 1 || (a.causal && q0 + off <= 0));
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) x[c] = c >= from && c < to ? x[c] : 0.f;
+      }
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) w[c] = pack_bf16x2(x[2 * c], x[2 * c + 1]);
+      tmem_st32(lanes + C::p + half * C::half, w);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&ctl.p_ready);
+
+      if (!(ok = mbar_wait_warp(&ctl.dp_full, i & 1, abort))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float d[32];
+        tmem_ld32_issue(lanes + 128 + half * 64 + h * 32, d);
+        tmem_wait_ld(d);
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 e = delta[(h * 32 + c) / 4];
+          x[h * 32 + c] *= d[c] - e.x;
+          x[h * 32 + c + 1] *= d[c + 1] - e.y;
+          x[h * 32 + c + 2] *= d[c + 2] - e.z;
+          x[h * 32 + c + 3] *= d[c + 3] - e.w;
+        }
+      }
+      if (masked) {
+        const int one = a.causal ? -off - q0 : -1;  // the query that sees one key
+#pragma unroll
+        for (int c = 0; c < 64; ++c) x[c] = c >= from && c < to && c != one && s.lk > 1 ? x[c] : 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 32; ++c) w[c] = pack_bf16x2(x[2 * c], x[2 * c + 1]);
+      tmem_st32(lanes + C::ds + half * C::half, w);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&ctl.ds_ready);
+    }
+    if (ok && together && n > 0) ok = mbar_wait_warp(half == 0 ? &ctl.dv_done : &ctl.dk_done, (n - 1) & 1, abort);
+    if (a.table != nullptr && together) together = softmax_sync(ok);
+    if (ok && together) {
+      tc_fence_after();
+      const int64_t at = ((int64_t)(s.k0 + key) * a.kv_heads + kv_head) * a.dim;
+      store_row<DP>(lanes + (half == 0 ? C::dv : C::dk), static_cast<__nv_bfloat16*>(half == 0 ? a.dv : a.dk) + at, a.dim,
+                    half == 0 ? 1.f : a.scale, n == 0, row < n_rows);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 11) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int DP>
+int launch(const Args& a0, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+  Args a = a0;
+  const bool bias = a.table != nullptr;
+  if (n_q > 0) {
+    const size_t smem = Bwd<DP>::kFloats + dq_floats(bias, a.dtable_part != nullptr, a.span) * sizeof(float);
+    KF_CUDA_RET(cudaFuncSetAttribute(attention_dq_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    attention_dq_tc<DP><<<dim3(n_q, a.heads), kThreads, smem, st>>>(a);
+    if (int rc = check_launch("kf_attention_bwd")) return rc;
+  }
+  if (n_k > 0) {
+    a.tiles = k_tiles;
+    const size_t smem = Bwd<DP>::kFloats + dkdv_floats(bias, a.span) * sizeof(float);
+    KF_CUDA_RET(cudaFuncSetAttribute(attention_dkdv_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    attention_dkdv_tc<DP><<<dim3(n_k, a.kv_heads), kThreads, smem, st>>>(a);
+    return check_launch("kf_attention_bwd");
+  }
+  return KF_OK;
+}
+
+}  // namespace
+
+namespace attn {
+int bwd_bf16(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+  return a.dim <= 64 ? launch<64>(a, k_tiles, n_q, n_k, st) : launch<128>(a, k_tiles, n_q, n_k, st);
+}
+}  // namespace attn
+}  // namespace kf

@@ -397,8 +397,5 @@ int fwd_f32(const Args& a, int n_tiles, cudaStream_t st) {
 int bwd_f32(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
   return a.dim <= 64 ? bwd<float, 64>(a, k_tiles, n_q, n_k, st) : bwd<float, 128>(a, k_tiles, n_q, n_k, st);
 }
-int bwd_bf16(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
-  return a.dim <= 64 ? bwd<__nv_bfloat16, 64>(a, k_tiles, n_q, n_k, st) : bwd<__nv_bfloat16, 128>(a, k_tiles, n_q, n_k, st);
-}
 }  // namespace attn
 }  // namespace kf

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a) {
   // registers: 384 x 168 at launch = 256 x 208 + 128 x 88
   if (warp >= 8) reg_dec<88>();
   if (warp >= 8 && warp < 11) {
-    // ---- loads: Q, then K and V tiles in turn through the ring; up to three loads in flight
+    // ---- loads: Q, then K and V tiles in turn through the ring
     const int tid = threadIdx.x - 256;
     const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q.p) + (int64_t)s.q0 * a.q.row + head0 * a.q.head;
     const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.k.p) + (int64_t)s.k0 * a.k.row + kv_head * a.k.head;
@@ -93,30 +93,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
       load_tile_async<DP, kLoaders>(q_tile + t * F::kTile, q, a.q.row, a.q.head, pack, r0 + t * kRows, n_rows[t], a.dim, tid);
-    cp_async_commit();
-    auto landed = [&](int item) {  // item 0 is Q, item i the (i - 1)th tile of the ring
-      fence_proxy_async_smem();
-      mbar_arrive(item == 0 ? &ctl.q_full : &ctl.kv_full[(item - 1) % F::kStages]);
-    };
-    int item = 1;
-    bool ok = true;
-    for (; item <= 2 * n_max; ++item) {
-      const int it = item - 1, st = it % F::kStages, j = it >> 1;
-      if (!(ok = mbar_wait(&ctl.kv_empty[st], ((it / F::kStages) & 1) ^ 1, abort))) break;
+    feed_ring<F::kStages>(2 * n_max, &ctl.q_full, ctl.kv_full, ctl.kv_empty, abort, [&](int it) {
       const bool is_v = it & 1;
-      load_tile_async<DP, kLoaders>(kv_tile + st * F::kTile, is_v ? v : k, is_v ? a.v.row : a.k.row, 0, 1, j * kRows,
+      const int j = it >> 1;
+      load_tile_async<DP, kLoaders>(kv_tile + it % F::kStages * F::kTile, is_v ? v : k, is_v ? a.v.row : a.k.row, 0, 1, j * kRows,
                                     min(kRows, s.lk - j * kRows), a.dim, tid);
-      cp_async_commit();
-      if (item >= 2) {
-        cp_async_wait<2>();
-        landed(item - 2);
-      }
-    }
-    cp_async_wait<0>();
-    if (ok) {
-      if (item >= 2) landed(item - 2);
-      landed(item - 1);
-    }
+    });
   } else if (warp == 11) {
     // ---- MMAs
     if (lane == 0 && n_max > 0) {

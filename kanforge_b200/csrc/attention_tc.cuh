@@ -136,6 +136,49 @@ __device__ __forceinline__ void load_tile_async(uint32_t dst, const __nv_bfloat1
   }
 }
 
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// The loader's side of a ring of STAGES tiles.  Item 0 was issued before and
+// signals `fixed`; issue(it) starts the copies of tile it.  A thread keeps up to
+// three items in flight and signals an item once its own copies have landed;
+// before it blocks on a full ring it signals all it has, since the MMAs that
+// free a tile may need the ones just loaded.
+template <int STAGES, typename Issue>
+__device__ __forceinline__ void feed_ring(int n_items, uint64_t* fixed, uint64_t* full, uint64_t* empty, volatile int* abort,
+                                          Issue&& issue) {
+  cp_async_commit();
+  int sent = 0;  // items signalled
+  auto signal = [&](int upto) {
+    fence_proxy_async_smem();
+    for (; sent < upto; ++sent) mbar_arrive(sent == 0 ? fixed : full + (sent - 1) % STAGES);
+  };
+  bool ok = true;
+  for (int it = 0; it < n_items; ++it) {
+    const uint32_t parity = ((it / STAGES) & 1) ^ 1;
+    if (!mbar_test(empty + it % STAGES, parity)) {
+      cp_async_wait<0>();
+      signal(it + 1);
+      if (!(ok = mbar_wait(empty + it % STAGES, parity, abort))) break;
+    }
+    issue(it);
+    cp_async_commit();
+    cp_async_wait<2>();
+    if (it > 0) signal(it);  // items 0 .. it - 1 of it + 2
+  }
+  cp_async_wait<0>();
+  if (ok) signal(n_items + 1);
+}
+
 // K-major operand (rows x DP, contraction over DP), k-step j of 16
 __device__ __forceinline__ uint64_t desc_k(uint32_t tile, int j) { return smem_desc_sw128(tile + (j >> 2) * kPanel + (j & 3) * 32, 16, 1024); }
 // MN-major operand (contraction over its 128 rows), k-step j of 16 rows
