@@ -561,9 +561,7 @@ int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o,
 /* One new token per sequence over its cache: q (batch, heads, dim) attends to
  * the first lengths[b] (clamped to [0, capacity]) rows of k, v (batch,
  * capacity, kv_heads, dim) and stands at the last of them.  Slots past the
- * length are not read.  o (batch, heads, dim) contiguous; workspace: batch *
- * heads * splits * (dim + 2) floats with splits = kf_attention_decode_splits()
- * (none for one split). */
+ * length are not read.  o (batch, heads, dim) contiguous.  One launch. */
 typedef struct kf_decode_desc {
   int64_t q_batch, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head;
   int32_t batch, capacity, heads, kv_heads, dim;
@@ -571,9 +569,8 @@ typedef struct kf_decode_desc {
   float scale;
 } kf_decode_desc;
 
-int kf_attention_decode_splits(const kf_decode_desc* desc);
 int kf_attention_decode(const void* q, const void* k, const void* v, const int32_t* lengths, const void* table,
-                        const int32_t* buckets, void* o, float* workspace, const kf_decode_desc* desc, void* stream);
+                        const int32_t* buckets, void* o, const kf_decode_desc* desc, void* stream);
 
 #ifdef __cplusplus
 }

@@ -246,8 +246,7 @@ PROTOTYPES = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
          ctypes.POINTER(AttentionDesc), _vp],
     ),
-    "kf_attention_decode_splits": (ctypes.c_int, [ctypes.POINTER(DecodeDesc)]),
-    "kf_attention_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(DecodeDesc), _vp]),
+    "kf_attention_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(DecodeDesc), _vp]),
     "kf_rational_bwd_noalloc": (
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i32, ctypes.POINTER(BasisDesc), ctypes.c_int, _vp],

@@ -306,9 +306,6 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     if batch == 0:
         return o
-    splits = _lib.load().kf_attention_decode_splits(ctypes.byref(desc))
-    ws = torch.empty(batch * heads * splits * (dim + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
     _launch("kf_attention_decode", _ptr(q), _ptr(k), _ptr(v), _ptr(lengths), _ptr(table),
-            _ptr(None if bias is None else bias.buckets), _ptr(o), _ptr(ws), ctypes.byref(desc), _stream(q),
-            kernels=1 + (splits > 1))
+            _ptr(None if bias is None else bias.buckets), _ptr(o), ctypes.byref(desc), _stream(q))
     return o

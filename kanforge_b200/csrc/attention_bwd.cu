@@ -180,9 +180,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a) {
     const int pos = r + off;
     const int limit = valid && a.causal ? min(s.lk, pos + 1) : s.lk;
     const int64_t stat = (int64_t)head * a.tq + s.q0 + r;
-    // delta = dO . O, half of the columns each
+    // delta = dO . O, half of the columns each.  The rounding of P that is in O weighs
+    // most in short rows: where one tile holds all keys, delta = sum P dP below instead.
     float delta = 0.f;
-    if (valid) {
+    if (valid && n != 1) {
       const int64_t at = ((int64_t)(s.q0 + r) * a.heads + head) * a.dim;
       const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(a.dout.p) + (int64_t)(s.q0 + r) * a.dout.row + head * a.dout.head;
       const __nv_bfloat16* o = static_cast<const __nv_bfloat16*>(a.o) + at;
@@ -200,16 +201,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a) {
         }
       }
     }
-    sdelta[half * kRows + row] = delta;
-    softmax_sync();
-    delta = sdelta[row] + sdelta[kRows + row];
-    if (valid && half == 0) a.delta[stat] = delta;
+    if (n != 1) {
+      sdelta[half * kRows + row] = delta;
+      softmax_sync();
+      delta = sdelta[row] + sdelta[kRows + row];
+      if (valid && half == 0) a.delta[stat] = delta;
+    }
     // a row that sees one key has dS = 0; rows past the sequence likewise
     const float lse = valid && !one_key(a, s, pos) ? a.lse[stat] : CUDART_INF_F;
     const float c2 = a.scale * kLog2e;
     const float* bias = sbias + a.span + kBiasPad;
     float far_sum[2] = {0.f, 0.f};  // dS at distances >= span, <= -span
-    bool ok = true, together = true;
+    bool ok = true, together = true, owed = n == 1;  // owed: the barrier of delta is still ahead
     for (int j = 0; j < n; ++j) {
       if (!(ok = mbar_wait_warp(&ctl.s_full, j & 1, abort))) break;
       tc_fence_after();
@@ -242,16 +245,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a) {
       const bool masked = __any_sync(0xffffffffu, limit - k0 < 64);
       if (!(ok = mbar_wait_warp(&ctl.dp_full, j & 1, abort))) break;
       tc_fence_after();
+      float d[64];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float d[32];
-        tmem_ld32_issue(lanes + 128 + half * 64 + h * 32, d);
-        tmem_wait_ld(d);
+      for (int h = 0; h < 2; ++h) tmem_ld32_issue(lanes + 128 + half * 64 + h * 32, d + h * 32);
+      tmem_wait_ld(d);
+      const int seen = limit - k0;
+      if (n == 1) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[h * 32 + i] *= d[i] - delta;
+        for (int i = 0; i < 64; ++i) sum[i & 3] += i < seen ? x[i] * d[i] : 0.f;
+        sdelta[half * kRows + row] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (!(together = softmax_sync())) break;
+        owed = false;
+        delta = sdelta[row] + sdelta[kRows + row];
+        if (valid && half == 0) a.delta[stat] = delta;
       }
+#pragma unroll
+      for (int i = 0; i < 64; ++i) x[i] *= d[i] - delta;
       if (masked) {
-        const int seen = limit - k0;
 #pragma unroll
         for (int i = 0; i < 64; ++i) x[i] = i < seen ? x[i] : 0.f;
       }
@@ -309,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a) {
       }
     }
     if (ok && together && n > 0) ok = mbar_wait_warp(&ctl.dk_done, 0, abort);
-    if (grad && together) together = softmax_sync(ok);
+    if ((grad || owed) && together) together = softmax_sync(ok);
     if (ok && together) {
       tc_fence_after();
       if (half == 0)

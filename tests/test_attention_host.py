@@ -92,7 +92,7 @@ def test_entry_points_check_their_arguments_before_any_cuda_call():
     d = _lib.AttentionDesc(heads=4, kv_heads=2, dim=65)
     assert lib.kf_attention_fwd(*[None] * 5, 1, *[None] * 5, ctypes.byref(d), None) == 1
     d = _lib.DecodeDesc(heads=4, kv_heads=2, dim=64, batch=1, capacity=8)
-    assert lib.kf_attention_decode(*[None] * 8, ctypes.byref(d), None) == 1
+    assert lib.kf_attention_decode(*[None] * 7, ctypes.byref(d), None) == 1
     d = _lib.ResidualNormDesc(width=9000)
     x = ctypes.c_void_p(16)
     assert lib.kf_residual_norm_fwd(x, *[None] * 2, x, *[None] * 6, 1, ctypes.byref(d), None) == 1
