@@ -19,7 +19,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernels import _check_cuda, _launch, _ptr, _stream
+from .kernels import _check_cuda, _launch
 
 ATTENTION_MAX_DIM = 128
 BIAS_MAX_DISTANCE, BIAS_MAX_BUCKETS = 1024, 256
@@ -54,6 +54,7 @@ class PackedSequences:
         self.table = torch.tensor(rows, dtype=torch.int32).reshape(-1, 4).to(self.device)
         self.device = self.table.device
         self._tiles: dict = {}
+        self._plans: dict = {}  # by a call's shapes, strides and types
 
     def __len__(self) -> int:
         return len(self.q_lens)
@@ -135,20 +136,27 @@ class RelativeBias(nn.Module):
 
 
 def _vectors(t: torch.Tensor) -> torch.Tensor:
-    """t, or a contiguous copy when its rows cannot be read in 16-byte vectors."""
-    per = 16 // t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-        s % per == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    """t, or a contiguous copy when its rows cannot be read in 16-byte vectors
+    (contiguous tensors can: the head width is a multiple of 8)."""
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        per = 16 // t.element_size()
+        if t.stride(-1) == 1 and all(s % per == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+            return t
+    return t.detach().clone(memory_format=torch.contiguous_format)
 
 
-def _check_heads(q, k, v, bias) -> tuple[int, int, int]:
-    _check_cuda(q, k, v)
-    heads, dim, kv_heads = q.shape[-2], q.shape[-1], k.shape[-2]
-    if q.dtype not in _DTYPE_CODE:
-        raise TypeError(f"attention takes float32 or bfloat16, not {q.dtype}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"q, k and v must have one type (got {q.dtype}, {k.dtype}, {v.dtype})")
+def _check_heads(q, k, v, bias, scale) -> tuple[int, int, int]:
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        _check_cuda(q, k, v)
+    dtype, device = q.dtype, q.device
+    heads, dim = q.shape[-2:]
+    kv_heads = k.shape[-2]
+    if dtype not in _DTYPE_CODE:
+        raise TypeError(f"attention takes float32 or bfloat16, not {dtype}")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"q, k and v must have one type (got {dtype}, {k.dtype}, {v.dtype})")
     if k.shape != v.shape or k.shape[-1] != dim:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
     if dim % 8 or not 8 <= dim <= ATTENTION_MAX_DIM:
@@ -157,74 +165,83 @@ def _check_heads(q, k, v, bias) -> tuple[int, int, int]:
         raise ValueError(f"{heads} query heads do not divide over {kv_heads} key heads")
     if heads > 65535:
         raise ValueError("at most 65535 heads")
-    if k.device != q.device or v.device != q.device:
-        raise ValueError(f"tensors lie on {q.device}, {k.device} and {v.device}")
+    if k.device != device or v.device != device:
+        raise ValueError(f"tensors lie on {device}, {k.device} and {v.device}")
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive, not {scale}")
     if bias is not None:
+        weight = bias.weight
         if bias.heads != heads:
             raise ValueError(f"the bias has {bias.heads} heads, the queries {heads}")
-        if bias.weight.device != q.device:
-            raise ValueError(f"the bias lies on {bias.weight.device}, the queries on {q.device}")
-        if bias.weight.dtype not in _DTYPE_CODE:
-            raise TypeError(f"the bias must be float32 or bfloat16, not {bias.weight.dtype}")
+        if weight.device != device:
+            raise ValueError(f"the bias lies on {weight.device}, the queries on {device}")
+        if weight.dtype not in _DTYPE_CODE:
+            raise TypeError(f"the bias must be float32 or bfloat16, not {weight.dtype}")
     return heads, kv_heads, dim
 
 
-class _Call:
-    """The operands of one packed attention call as the kernels take them."""
+def _raw_stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
-    __slots__ = ("q", "k", "v", "seqs", "causal", "desc", "table", "buckets")
 
-    def __init__(self, q, k, v, table, seqs, causal, scale, bias):
-        self.q, self.k, self.v = (_vectors(t.detach()) for t in (q, k, v))
-        self.seqs, self.causal = seqs, causal
-        self.table = None if table is None else table.detach().contiguous()
-        self.buckets = None if table is None else bias.buckets
-        q, k, v = self.q, self.k, self.v
+class _Plan:
+    """What a call's shapes decide: the descriptor, the tiles of the forward's
+    queries, the backward's queries and its keys, the backward's workspace."""
+
+    __slots__ = ("desc", "ref", "tiles", "workspace")
+
+    def __init__(self, seqs, q, k, v, causal, scale, bias):
+        has = bias is not None
         self.desc = _lib.AttentionDesc(
             q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
             q.shape[1], k.shape[1], q.shape[2], len(seqs), _DTYPE_CODE[q.dtype], int(causal),
-            0 if table is None else bias.max_distance, 0 if table is None else bias.num_buckets,
-            0 if table is None else _DTYPE_CODE[table.dtype], scale)
+            bias.max_distance if has else 0, bias.num_buckets if has else 0, _DTYPE_CODE[bias.weight.dtype] if has else 0,
+            scale)
+        self.ref = ctypes.byref(self.desc)
+        self.tiles = []
+        for what, side in enumerate("qqk"):
+            rows, pack = ctypes.c_int32(), ctypes.c_int32()
+            _lib.call("kf_attention_tiling", self.ref, what, ctypes.byref(rows), ctypes.byref(pack))
+            t = seqs.tiles(side, rows.value, causal, pack.value)
+            self.tiles.append((t.data_ptr(), t.shape[0]))
+        self.workspace = max(1, int(_lib.load().kf_attention_bwd_workspace(self.tiles[1][1], self.ref)))
 
-    def tiles(self, what: int) -> torch.Tensor:
-        """The tiles of the forward's queries (0), the backward's queries (1) or its keys (2)."""
-        rows, pack = ctypes.c_int32(), ctypes.c_int32()
-        _lib.call("kf_attention_tiling", ctypes.byref(self.desc), what, ctypes.byref(rows), ctypes.byref(pack))
-        return self.seqs.tiles("k" if what == 2 else "q", rows.value, self.causal, pack.value)
 
-    def forward(self, with_lse: bool):
-        q = self.q
-        o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        lse = torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32) if with_lse else None
-        # bf16: what the rounding of o leaves out, so that delta = dout . o keeps float32's digits
-        rest = torch.empty_like(o) if with_lse and q.dtype == torch.bfloat16 else None
-        tiles = self.tiles(0)
-        if tiles.shape[0]:
-            _launch("kf_attention_fwd", _ptr(q), _ptr(self.k), _ptr(self.v), _ptr(self.seqs.table), _ptr(tiles),
-                    tiles.shape[0], _ptr(self.table), _ptr(self.buckets), _ptr(o), _ptr(rest), _ptr(lse),
-                    ctypes.byref(self.desc), _stream(q))
-        return o, rest, lse
+def _plan(seqs, q, k, v, causal, scale, bias) -> _Plan:
+    key = (q.dtype, q.shape, q.stride(), k.shape, k.stride(), v.stride(), causal, scale,
+           None if bias is None else (bias.weight.dtype, bias.num_buckets, bias.max_distance))
+    plan = seqs._plans.get(key)
+    if plan is None:
+        plan = seqs._plans[key] = _Plan(seqs, q, k, v, causal, scale, bias)
+    return plan
 
-    def backward(self, o, rest, lse, dout, want_table: bool):
-        q, k = self.q, self.k
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
-        dtable = torch.empty_like(self.table) if want_table else None
-        q_tiles, k_tiles = self.tiles(1), self.tiles(2)
-        n_ws = int(_lib.load().kf_attention_bwd_workspace(q_tiles.shape[0], ctypes.byref(self.desc)))
-        ws = torch.empty(max(n_ws, 1), device=q.device, dtype=torch.float32)
-        if q_tiles.shape[0] or k_tiles.shape[0] or want_table:
-            _launch("kf_attention_bwd", _ptr(q), _ptr(k), _ptr(self.v), _ptr(o), _ptr(rest), _ptr(dout),
-                    _ptr(lse), _ptr(self.seqs.table), _ptr(q_tiles), q_tiles.shape[0], _ptr(k_tiles), k_tiles.shape[0],
-                    _ptr(self.table), _ptr(self.buckets), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable), _ptr(ws),
-                    ctypes.byref(self.desc), _stream(q), kernels=3 + int(want_table))
-        return dq, dk, dv, dtable
+
+def _forward(q, k, v, table, seqs, causal, scale, bias, train: bool):
+    """(o, rest, lse): the output, and for the backward what the rounding of a
+    bf16 output leaves out (delta = dout . o keeps float32's digits) and the
+    logarithms of the sums."""
+    q, k, v = _vectors(q), _vectors(k), _vectors(v)
+    plan = _plan(seqs, q, k, v, causal, scale, bias)
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    rest = lse = None
+    if train:
+        lse = torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32)
+        if q.dtype == torch.bfloat16:
+            rest = torch.empty_like(o)
+    tiles, n = plan.tiles[0]
+    if n:
+        table = None if table is None else table.detach().contiguous()
+        _launch("kf_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), seqs.table.data_ptr(), tiles, n,
+                None if table is None else table.data_ptr(), None if table is None else bias.buckets.data_ptr(),
+                o.data_ptr(), None if rest is None else rest.data_ptr(), None if lse is None else lse.data_ptr(),
+                plan.ref, _raw_stream(q))
+    return o, rest, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, seqs, causal, scale, bias):
-        o, rest, lse = _Call(q, k, v, table, seqs, causal, scale, bias).forward(with_lse=True)
+        o, rest, lse = _forward(q, k, v, table, seqs, causal, scale, bias, train=True)
         ctx.save_for_backward(q, k, v, table, o, rest, lse)
         ctx.options = (seqs, causal, scale, bias)
         return o
@@ -233,11 +250,27 @@ class _Attention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, table, o, rest, lse = ctx.saved_tensors
+        seqs, causal, scale, bias = ctx.options
         need = ctx.needs_input_grad
-        call = _Call(q, k, v, table, *ctx.options)
-        dout = dout.to(q.dtype).contiguous()
-        dout = _vectors(dout)
-        dq, dk, dv, dtable = call.backward(o, rest, lse, dout, table is not None and need[3])
+        q, k, v = _vectors(q), _vectors(k), _vectors(v)
+        plan = _plan(seqs, q, k, v, causal, scale, bias)
+        if dout.dtype != q.dtype or not dout.is_contiguous() or dout.data_ptr() % 16:
+            dout = dout.to(q.dtype).clone(memory_format=torch.contiguous_format)
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        dk = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+        dv = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+        want = table is not None and need[3]
+        tab = None if table is None else table.detach().contiguous()
+        dtable = torch.empty_like(tab) if want else None
+        (q_tiles, n_q), (k_tiles, n_k) = plan.tiles[1:]
+        if n_q or n_k or want:
+            ws = torch.empty(plan.workspace, device=q.device, dtype=torch.float32)
+            _launch("kf_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                    None if rest is None else rest.data_ptr(), dout.data_ptr(), lse.data_ptr(), seqs.table.data_ptr(),
+                    q_tiles, n_q, k_tiles, n_k, None if tab is None else tab.data_ptr(),
+                    None if tab is None else bias.buckets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                    None if dtable is None else dtable.data_ptr(), ws.data_ptr(), plan.ref, _raw_stream(q),
+                    kernels=2 + (q.dtype == torch.float32) + want)
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None, None, None)
 
 
@@ -256,7 +289,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: PackedSeq
     """
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v must be (tokens, heads, dim)")
-    _heads, _kv_heads, dim = _check_heads(q, k, v, bias)
+    dim = _check_heads(q, k, v, bias, scale)[2]
     if not isinstance(seqs, PackedSequences):
         raise TypeError("seqs must be a PackedSequences")
     if q.shape[0] != seqs.total_q or k.shape[0] != seqs.total_kv:
@@ -264,13 +297,32 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: PackedSeq
                          f"and {k.shape[0]}")
     if seqs.device != q.device:
         raise ValueError(f"the sequences lie on {seqs.device}, the queries on {q.device}")
-    if scale is not None and not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be positive, not {scale}")
     table = None if bias is None else bias.weight
     args = (q, k, v, table, seqs, bool(causal), 1.0 / math.sqrt(dim) if scale is None else float(scale), bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (table is not None and table.requires_grad)):
         return _Attention.apply(*args)
-    return _Call(*args).forward(with_lse=False)[0]
+    return _forward(*args, train=False)[0]
+
+
+_DECODE_PLANS_MAX = 512
+_decode_plans: dict = {}  # descriptors by shapes, strides and types
+
+
+def _decode_plan(q, k, v, scale, bias):
+    key = (q.dtype, q.shape, q.stride(), k.shape, k.stride(), v.stride(), scale,
+           None if bias is None else (bias.weight.dtype, bias.max_distance))
+    ref = _decode_plans.get(key)
+    if ref is None:
+        batch, capacity, kv_heads, dim = k.shape
+        desc = _lib.DecodeDesc(q.stride(0), q.stride(1), *k.stride()[:3], *v.stride()[:3], batch, capacity, q.shape[1],
+                               kv_heads, dim, _DTYPE_CODE[q.dtype], 0 if bias is None else bias.max_distance,
+                               0 if bias is None else _DTYPE_CODE[bias.weight.dtype],
+                               1.0 / math.sqrt(dim) if scale is None else float(scale))
+        if len(_decode_plans) >= _DECODE_PLANS_MAX:
+            _decode_plans.clear()
+        ref = _decode_plans[key] = ctypes.byref(desc)
+    return ref
 
 
 def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, *,
@@ -285,27 +337,22 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("q must be (batch, heads, dim), the caches (batch, capacity, kv_heads, dim)")
-    heads, kv_heads, dim = _check_heads(q, k_cache, v_cache, bias)
-    batch, capacity = k_cache.shape[:2]
+    _check_heads(q, k_cache, v_cache, bias, scale)
+    batch = k_cache.shape[0]
     if q.shape[0] != batch or batch > 65535:
         raise ValueError(f"q holds {q.shape[0]} sequences, the caches {batch} (at most 65535)")
     if lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.device != q.device:
         raise ValueError(f"lengths must be ({batch},) int32 on {q.device}")
-    tracked = [q, k_cache, v_cache] + ([bias.weight] if bias is not None else [])
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tracked):
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
+                                    (bias is not None and bias.weight.requires_grad)):
         raise RuntimeError("attention_decode has no backward: call it under torch.no_grad(), or use attention")
-    if scale is not None and not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be positive, not {scale}")
-    q, k, v = _vectors(q.detach()), _vectors(k_cache.detach()), _vectors(v_cache.detach())
-    lengths = lengths.contiguous()
-    table = None if bias is None else bias.weight.detach().contiguous()
-    desc = _lib.DecodeDesc(q.stride(0), q.stride(1), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1),
-                           v.stride(2), batch, capacity, heads, kv_heads, dim, _DTYPE_CODE[q.dtype],
-                           0 if bias is None else bias.max_distance, 0 if bias is None else _DTYPE_CODE[table.dtype],
-                           1.0 / math.sqrt(dim) if scale is None else float(scale))
+    q, k, v = _vectors(q), _vectors(k_cache), _vectors(v_cache)
     o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     if batch == 0:
         return o
-    _launch("kf_attention_decode", _ptr(q), _ptr(k), _ptr(v), _ptr(lengths), _ptr(table),
-            _ptr(None if bias is None else bias.buckets), _ptr(o), ctypes.byref(desc), _stream(q))
+    lengths = lengths.contiguous()
+    table = None if bias is None else bias.weight.detach().contiguous()
+    _launch("kf_attention_decode", q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths.data_ptr(),
+            None if table is None else table.data_ptr(), None if bias is None else bias.buckets.data_ptr(), o.data_ptr(),
+            _decode_plan(q, k, v, scale, bias), _raw_stream(q))
     return o

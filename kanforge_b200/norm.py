@@ -19,7 +19,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernels import _aligned16, _check_cuda, _launch, _ptr, _stream
+from .kernels import _check_cuda, _launch
 
 NORM_KINDS = ("layer", "rms")
 NORM_MAX_WIDTH = 8192
@@ -27,8 +27,25 @@ NORM_MAX_WIDTH = 8192
 _DTYPE_CODE = {torch.float32: _lib.KF_DTYPE_F32, torch.bfloat16: _lib.KF_DTYPE_BF16}
 
 
-def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
-    return t.reshape(-1, width).contiguous()
+_descs: dict = {}  # descriptors by their values
+_DESCS_MAX = 512
+
+
+def _desc(*values):
+    ref = _descs.get(values)
+    if ref is None:
+        if len(_descs) >= _DESCS_MAX:
+            _descs.clear()
+        ref = _descs[values] = ctypes.byref(_lib.ResidualNormDesc(*values))
+    return ref
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 class _Call:
@@ -38,33 +55,32 @@ class _Call:
 
     def __init__(self, x, branch, weight, bias, branch_weight, branch_bias, gate, kind, residual_scale, eps):
         self.width = width = x.shape[-1]
-        self.x = _rows(x.detach(), width)
-        self.rows = self.x.shape[0]
-        self.branch = None if branch is None else _rows(branch.detach(), width)
-        self.gate_token = gate is not None and gate.dim() > 1
-        params = [weight, bias, branch_weight, branch_bias, None if self.gate_token else gate]
-        dtypes = {p.dtype for p in params if p is not None}
+        self.x = x.contiguous()
+        self.rows = x.numel() // width
+        self.branch = None if branch is None else branch.contiguous()
+        self.gate_token = token = gate is not None and gate.dim() > 1
+        params = (weight, bias, branch_weight, branch_bias, None if token else gate)
         # parameters of one type are read as they are; mixed or other types as float32
-        dtype = dtypes.pop() if len(dtypes) == 1 and dtypes <= set(_DTYPE_CODE) else torch.float32
-        params = [None if p is None else _aligned16(p.detach().to(dtype).contiguous()) for p in params]
-        self.w, self.s, self.bw, self.bs, self.gate = params
-        if self.gate_token:
-            self.gate = _rows(gate.detach(), width)
-        out = self.x.dtype if self.branch is None else self.branch.dtype
-        self.desc = _lib.ResidualNormDesc(width, int(kind == "layer"), int(branch_weight is not None),
-                                          int(self.gate_token), _DTYPE_CODE[self.x.dtype], _DTYPE_CODE[out],
-                                          _DTYPE_CODE[dtype], residual_scale, eps)
+        dtype = weight.dtype
+        if dtype not in _DTYPE_CODE or any(p is not None and p.dtype != dtype for p in params):
+            dtype = torch.float32
+        self.w, self.s, self.bw, self.bs, self.gate = (
+            p if p is None or (p.dtype == dtype and p.is_contiguous()) else p.detach().to(dtype).contiguous() for p in params)
+        if token:
+            self.gate = gate.contiguous()
+        out = x.dtype if branch is None else branch.dtype
+        self.desc = _desc(width, int(kind == "layer"), int(branch_weight is not None), int(token), _DTYPE_CODE[x.dtype],
+                          _DTYPE_CODE[out], _DTYPE_CODE[dtype], residual_scale, eps)
 
     def forward(self, with_stats: bool):
-        """(y, h, stats) as (rows, width) matrices; y is x where there is no branch."""
-        x = self.x
-        y = x if self.branch is None else torch.empty_like(x)
-        h = torch.empty_like(x if self.branch is None else self.branch)
+        """(y, h, stats); y is None where there is no branch (it is x)."""
+        x, branch = self.x, self.branch
+        y = None if branch is None else torch.empty_like(x)
+        h = torch.empty_like(x if branch is None else branch)
         stats = torch.empty(self.rows, 4, device=x.device, dtype=torch.float32) if with_stats else None
         if self.rows:
-            _launch("kf_residual_norm_fwd", _ptr(x), _ptr(self.branch), _ptr(self.gate), _ptr(self.w), _ptr(self.s),
-                    _ptr(self.bw), _ptr(self.bs), _ptr(None if self.branch is None else y), _ptr(h), _ptr(stats),
-                    self.rows, ctypes.byref(self.desc), _stream(x))
+            _launch("kf_residual_norm_fwd", x.data_ptr(), _ptr(branch), _ptr(self.gate), self.w.data_ptr(), _ptr(self.s),
+                    _ptr(self.bw), _ptr(self.bs), _ptr(y), h.data_ptr(), _ptr(stats), self.rows, self.desc, _raw_stream(x))
         return y, h, stats
 
 
@@ -76,10 +92,7 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, branch, weight, bias, branch_weight, branch_bias, gate, stats)
         ctx.options = (kind, residual_scale, eps)
-        h = h.view(x.shape)
-        if branch is None:
-            return h
-        return y.view(x.shape), h
+        return h if branch is None else (y, h)
 
     @staticmethod
     @once_differentiable
@@ -90,27 +103,21 @@ class _ResidualNorm(torch.autograd.Function):
             return (None,) * 10
         need = ctx.needs_input_grad
         call = _Call(x, branch, weight, bias, branch_weight, branch_bias, gate, *ctx.options)
-        shape, rows = x.shape, call.x
-        dev, width = rows.device, call.width
-        mat = lambda g, like: None if g is None else _rows(g.to(like.dtype), width)  # noqa: E731
-        out_like = rows if branch is None else call.branch
-        dy, dh = mat(dy, rows), mat(dh, out_like)
-        dx = torch.empty_like(rows)
-        dbranch = None if branch is None else torch.empty_like(call.branch)
-        dgate = None
-        if gate is not None:
-            dgate = torch.empty_like(call.gate)
-        dw, ds, dbw, dbs = (None if p is None else torch.empty_like(p) for p in (call.w, call.s, call.bw, call.bs))
-        n_ws = int(_lib.load().kf_residual_norm_workspace(call.rows, width))
-        ws = torch.empty(n_ws, device=dev, dtype=torch.float32)
-        _launch("kf_residual_norm_bwd", _ptr(rows), _ptr(call.branch), _ptr(call.gate), _ptr(call.w), _ptr(call.bw),
-                _ptr(call.bs), _ptr(stats), _ptr(dy), _ptr(dh), _ptr(dx), _ptr(dbranch), _ptr(dgate),
-                _ptr(dw), _ptr(ds), _ptr(dbw), _ptr(dbs), _ptr(ws), call.rows, ctypes.byref(call.desc), _stream(rows),
-                kernels=2 if call.rows else 1)
-        like = lambda g, p, n: g.to(p.dtype).view(p.shape) if n and p is not None else None  # noqa: E731
-        return (dx.view(shape) if need[0] else None, dbranch.view(shape) if need[1] and branch is not None else None,
-                like(dw, weight, need[2]), like(ds, bias, need[3]), like(dbw, branch_weight, need[4]),
-                like(dbs, branch_bias, need[5]), like(dgate, gate, need[6]), None, None, None)
+        x2 = call.x
+        mat = lambda g, like: None if g is None else g.to(like.dtype).contiguous()  # noqa: E731
+        dy, dh = mat(dy, x2), mat(dh, x2 if branch is None else call.branch)
+        dx = torch.empty_like(x2)
+        new = lambda p: None if p is None else torch.empty_like(p)  # noqa: E731
+        dbranch, dgate, dw, ds, dbw, dbs = map(new, (call.branch, call.gate, call.w, call.s, call.bw, call.bs))
+        n_ws = int(_lib.load().kf_residual_norm_workspace(call.rows, call.width))
+        ws = torch.empty(n_ws, device=x2.device, dtype=torch.float32)
+        _launch("kf_residual_norm_bwd", _ptr(x2), _ptr(call.branch), _ptr(call.gate), _ptr(call.w), _ptr(call.bw),
+                _ptr(call.bs), _ptr(stats), _ptr(dy), _ptr(dh), _ptr(dx), _ptr(dbranch), _ptr(dgate), _ptr(dw), _ptr(ds),
+                _ptr(dbw), _ptr(dbs), _ptr(ws), call.rows, call.desc, _raw_stream(x2), kernels=2 if call.rows else 1)
+        like = lambda g, p, n: g.to(p.dtype) if n and p is not None else None  # noqa: E731
+        return (dx if need[0] else None, dbranch if need[1] else None, like(dw, weight, need[2]), like(ds, bias, need[3]),
+                like(dbw, branch_weight, need[4]), like(dbs, branch_bias, need[5]), like(dgate, gate, need[6]), None, None,
+                None)
 
 
 def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -131,19 +138,22 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, weight: torch.Te
         raise ValueError(f"kind must be one of {NORM_KINDS}")
     if eps < 0:
         raise ValueError("eps must not be negative")
-    _check_cuda(x, branch, weight, bias, gate, branch_weight, branch_bias)
+    tensors = (x, branch, weight, bias, branch_weight, branch_bias, gate)
+    given = [t for t in tensors if t is not None]
+    device = x.device
+    for t in given:
+        if not t.is_cuda:
+            _check_cuda(t)
+        if t.device != device:
+            raise ValueError(f"tensors lie on {device} and {t.device}")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= NORM_MAX_WIDTH:
         raise ValueError(f"rows must have 1 to {NORM_MAX_WIDTH} elements (got a tensor of shape {tuple(x.shape)})")
     width = x.shape[-1]
-    for what, t in (("x", x), ("branch", branch)):
-        if t is not None and t.dtype not in _DTYPE_CODE:
-            raise TypeError(f"{what} must be float32 or bfloat16, not {t.dtype}")
-    for what, t in (("weight", weight), ("bias", bias), ("branch_weight", branch_weight), ("branch_bias", branch_bias)):
+    if x.dtype not in _DTYPE_CODE or (branch is not None and branch.dtype not in _DTYPE_CODE):
+        raise TypeError(f"x and branch must be float32 or bfloat16, not {x.dtype} and {None if branch is None else branch.dtype}")
+    for t in (weight, bias, branch_weight, branch_bias):
         if t is not None and t.shape != (width,):
-            raise ValueError(f"{what} must have shape ({width},), not {tuple(t.shape)}")
-    for t in (branch, weight, bias, gate, branch_weight, branch_bias):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"tensors lie on {x.device} and {t.device}")
+            raise ValueError(f"norm parameters must have shape ({width},), not {tuple(t.shape)}")
     if branch is None:
         if gate is not None or branch_norm or residual_scale != 1.0:
             raise ValueError("a gate, a branch norm or a residual scale needs a branch")
@@ -154,16 +164,16 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, weight: torch.Te
             raise TypeError("a bfloat16 residual stream takes no float32 branch")
     if branch_norm != (branch_weight is not None) or (branch_bias is not None and not branch_norm):
         raise ValueError("branch_norm, branch_weight and branch_bias belong together")
-    if gate is not None and (gate.dim() > 1 or gate.shape != (width,)):
+    if gate is not None and gate.shape != (width,):
         gate = gate.expand(branch.shape).to(branch.dtype)  # their gradients: autograd's
         if gate.dim() < 2:
             gate = gate.reshape(1, width)
     args = (x, branch, weight, bias, branch_weight, branch_bias, gate, kind, float(residual_scale), float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:7]):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         out = _ResidualNorm.apply(*args)
         return (x, out) if branch is None else out
     y, h, _ = _Call(*args).forward(with_stats=False)
-    return (x if branch is None else y.view(x.shape)), h.view(x.shape)
+    return (x if branch is None else y), h
 
 
 class ResidualNorm(nn.Module):
