@@ -54,7 +54,7 @@ Args make_args(const kf_attention_desc* d) {
   Args a{};
   a.heads = d->heads, a.kv_heads = d->kv_heads, a.dim = d->dim, a.span = d->span, a.n_buckets = d->n_buckets;
   a.causal = d->causal != 0, a.table_bf16 = d->table_dtype == KF_DTYPE_BF16;
-  a.scale = d->scale, a.tq = d->tq;
+  a.scale = d->scale, a.tq = d->tq, a.tk = d->tk;
   a.q = {nullptr, d->q_row, d->q_head};
   a.k = {nullptr, d->k_row, d->k_head};
   a.v = {nullptr, d->v_row, d->v_head};
@@ -64,6 +64,32 @@ Args make_args(const kf_attention_desc* d) {
 
 }  // namespace
 }  // namespace kf
+
+int kf::attn::make_tile_map(CUtensorMap* map, const void* p, int64_t rows, int heads, int dim, int64_t row_stride,
+                            int64_t head_stride) {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn) : nullptr;
+  }();
+  if (encode == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from the driver");
+    return KF_ERR_CUDA;
+  }
+  // the stride of a dimension of size one is never used, but it is checked
+  const cuuint64_t pitch = (cuuint64_t)(dim + 7) / 8 * 16;
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {heads > 1 ? (cuuint64_t)head_stride * 2 : pitch, rows > 1 ? (cuuint64_t)row_stride * 2 : pitch};
+  cuuint32_t box[3] = {64, 1, (cuuint32_t)kRows}, step[3] = {1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  KF_CHECK_ARG(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (%d) for %lld rows x %d heads x %d, strides %lld and %lld", (int)r,
+               (long long)rows, heads, dim, (long long)row_stride, (long long)head_stride);
+  return KF_OK;
+}
 
 extern "C" int kf_attention_tiling(const kf_attention_desc* d, int pass, int32_t* rows, int32_t* pack) {
   using namespace kf;

@@ -40,7 +40,7 @@ struct Args {
   const void* table;  // (buckets, H) bias, or null
   const int* buckets; // (2 span + 1): bucket of distance index - span
   float* dtable_part; // (tiles, H, buckets)
-  int64_t tq;
+  int64_t tq, tk;
   int heads, kv_heads, dim, span, n_buckets;
   int pack;  // heads that are neighbouring rows of a tile (bf16)
   bool causal, table_bf16;

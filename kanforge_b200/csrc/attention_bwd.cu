@@ -12,7 +12,7 @@
 // All scores live in tensor memory; P and dS go back there as bf16 (2^-9 of
 // each term) and are the A operands of the products that sum them.  Of the 12
 // warps 0-7 do the softmax arithmetic (thread = row, a warpgroup per half of
-// the columns), 8-10 load, 11 issues the MMAs.
+// the columns), 8 loads, 10 and 11 issue the MMAs of one chain each.
 #include "attention_tc.cuh"
 
 namespace kf {
@@ -20,7 +20,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int kThreads = 384, kLoaders = 96, kSoftmax = 256;
+constexpr int kThreads = 384, kSoftmax = 256;
 
 template <int DP>
 struct Bwd {
@@ -30,18 +30,20 @@ struct Bwd {
 };
 
 struct Ctl {
-  uint64_t fixed_full, fin, full[8], empty[8], s_full, dp_full, s_read, p_ready, ds_ready, dv_done, dk_done;
+  uint64_t fixed_full, part, full[8], empty[8], stat_full[8], s_full, dp_full, s_read, p_ready, ds_ready, dv_done, dk_done, fin[2];
   uint32_t tmem;
   int abort;
 };
 
-__device__ __forceinline__ void init_barriers(Ctl* c, int stages) {
+// `users`: how many MMA warps read a streamed tile
+__device__ __forceinline__ void init_barriers(Ctl* c, int stages, int users) {
   c->abort = 0;
-  mbar_init(&c->fixed_full, kLoaders);
-  mbar_init(&c->fin, 1);
-  for (int i = 0; i < stages; ++i) mbar_init(&c->full[i], kLoaders), mbar_init(&c->empty[i], 1);
+  mbar_init(&c->fixed_full, 2);
+  mbar_init(&c->part, 1);
+  for (int i = 0; i < stages; ++i) mbar_init(&c->full[i], 1), mbar_init(&c->empty[i], users), mbar_init(&c->stat_full[i], 32);
   mbar_init(&c->s_full, 1), mbar_init(&c->dp_full, 1), mbar_init(&c->dv_done, 1), mbar_init(&c->dk_done, 1);
   mbar_init(&c->s_read, kSoftmax), mbar_init(&c->p_ready, kSoftmax), mbar_init(&c->ds_ready, kSoftmax);
+  mbar_init(&c->fin[0], 1), mbar_init(&c->fin[1], 1);
   fence_barrier_init();
 }
 
@@ -82,7 +84,10 @@ __host__ __device__ constexpr int dq_floats(bool bias, bool grad, int span) {
 }
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a) {
+__global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, const __grid_constant__ CUtensorMap q_map,
+                                                               const __grid_constant__ CUtensorMap g_map,
+                                                               const __grid_constant__ CUtensorMap k_map,
+                                                               const __grid_constant__ CUtensorMap v_map) {
   using F = Bwd<DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
@@ -103,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool grad = a.dtable_part != nullptr;
 
-  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages);
+  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, 1);
   if (warp == 11) {
     tmem_alloc(&ctl.tmem, 512);
     tmem_relinquish();
@@ -118,60 +123,55 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a) {
 
   // registers: 384 x 168 at launch = 256 x 208 + 128 x 88
   if (warp >= 8) reg_dec<88>();
-  if (warp >= 8 && warp < 11) {
+  if (warp == 8) {
     // ---- loads: Q and dO, then K and V tiles in turn
-    const int tid = threadIdx.x - 256;
-    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q.p) + (int64_t)s.q0 * a.q.row + head * a.q.head;
-    const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(a.dout.p) + (int64_t)s.q0 * a.dout.row + head * a.dout.head;
-    const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.k.p) + (int64_t)s.k0 * a.k.row + kv_head * a.k.head;
-    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v.p) + (int64_t)s.k0 * a.v.row + kv_head * a.v.head;
-    load_tile_async<DP, kLoaders>(q_tile, q, a.q.row, 0, 1, r0, n_rows, a.dim, tid);
-    load_tile_async<DP, kLoaders>(q_tile + F::kTile, g, a.dout.row, 0, 1, r0, n_rows, a.dim, tid);
-    feed_ring<F::kStages>(2 * n, &ctl.fixed_full, ctl.full, ctl.empty, abort, [&](int it) {
-      const bool is_v = it & 1;
-      const int j = it >> 1;
-      load_tile_async<DP, kLoaders>(ring + it % F::kStages * F::kTile, is_v ? v : k, is_v ? a.v.row : a.k.row, 0, 1, j * kRows,
-                                    min(kRows, s.lk - j * kRows), a.dim, tid);
-    });
-  } else if (warp == 11) {
-    // ---- MMAs: S and dP of the next tile go ahead of dQ of this one
-    if (lane == 0 && n > 0) {
+    TileLoader<DP> loader{&ctl.part, abort};
+    if (loader.load(q_tile, &q_map, &ctl.fixed_full, head, s.q0 + r0, n_rows) &&
+        loader.load(q_tile + F::kTile, &g_map, &ctl.fixed_full, head, s.q0 + r0, n_rows))
+      feed_ring<F::kStages>(2 * n, ctl.full, ctl.empty, abort, [&](int it, int st) {
+        const int j = it >> 1;
+        return loader.load(ring + st * F::kTile, it & 1 ? &v_map : &k_map, &ctl.full[st], kv_head, s.k0 + j * kRows,
+                           min(kRows, s.lk - j * kRows));
+      });
+    mbar_drain(&ctl.fixed_full, 0);
+  } else if (warp >= 10) {
+    // ---- MMAs: warp 10 S, then dQ; warp 11 dP.  S of the next tile goes ahead of dQ of this one.
+    if (lane == 0) {
       const uint32_t idesc_s = idesc_bf16_f32(kRows, kRows, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
       auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* done) {
         if (!mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort)) return false;
         tc_fence_after();
-        const uint32_t b = ring + (it % F::kStages) * F::kTile;
+        const uint32_t ad = desc_k(fixed), bd = desc_k(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) mma_ss(d, desc_k(fixed, i), desc_k(b, i), idesc_s, i > 0);
+        for (int i = 0; i < DP / 16; ++i) mma_ss(d, ad + step_k(i), bd + step_k(i), idesc_s, i > 0);
         mma_commit(done);
         return true;
       };
-      auto dp = [&](int j) {
-        if (!product(2 * j + 1, tmem + 128, q_tile + F::kTile, &ctl.dp_full)) return false;
-        mma_commit(&ctl.empty[(2 * j + 1) % F::kStages]);  // V has no other use
-        return true;
-      };
-      bool ok = mbar_wait(&ctl.fixed_full, 0, abort) && product(0, tmem, q_tile, &ctl.s_full) && dp(0);
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) {
-          ok = mbar_wait(&ctl.s_read, j & 1, abort);
+      bool ok = mbar_wait(&ctl.fixed_full, 0, abort);
+      if (warp == 10) {
+        if (ok && n > 0) ok = product(0, tmem, q_tile, &ctl.s_full);
+        for (int j = 0; j < n && ok; ++j) {
+          if (j + 1 < n && !(ok = mbar_wait(&ctl.s_read, j & 1, abort) && product(2 * (j + 1), tmem, q_tile, &ctl.s_full))) break;
+          if (!(ok = mbar_wait(&ctl.ds_ready, j & 1, abort))) break;
           tc_fence_after();
-          ok = ok && product(2 * (j + 1), tmem, q_tile, &ctl.s_full);
-        }
-        if (!ok || !(ok = mbar_wait(&ctl.ds_ready, j & 1, abort))) break;
-        tc_fence_after();
-        if (j + 1 < n && !(ok = dp(j + 1))) break;
-        const uint32_t kt = ring + (2 * j % F::kStages) * F::kTile;
+          const uint32_t kd = desc_mn(ring + (2 * j % F::kStages) * F::kTile);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          mma_ts(tmem + 256, tmem + 384 + (j & 1) * 64 + i * 8, desc_mn(kt, i), idesc_d, j > 0 || i > 0);
-        mma_commit(&ctl.empty[2 * j % F::kStages]);
+          for (int i = 0; i < 8; ++i)
+            mma_ts(tmem + 256, tmem + 384 + (j & 1) * 64 + i * 8, kd + step_mn(i), idesc_d, j > 0 || i > 0);
+          mma_commit(&ctl.empty[2 * j % F::kStages]);
+        }
+        mma_commit(&ctl.dk_done);
+      } else {
+        for (int j = 0; j < n && ok; ++j) {
+          if (j > 0 && !(ok = mbar_wait(&ctl.ds_ready, (j - 1) & 1, abort))) break;
+          ok = product(2 * j + 1, tmem + 128, q_tile + F::kTile, &ctl.dp_full);
+          if (ok) mma_commit(&ctl.empty[(2 * j + 1) % F::kStages]);
+        }
       }
-      mma_commit(&ctl.dk_done);
-      mma_commit(&ctl.fin);
-      mbar_drain(&ctl.fin, 0);
+      mma_commit(&ctl.fin[warp - 10]);
+      mbar_drain(&ctl.fin[warp - 10], 0);
     }
-  } else {
+  } else if (warp < 8) {
     reg_inc<208>();
     // ---- softmax arithmetic: thread = query, a warpgroup per half of a tile's keys
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
@@ -376,7 +376,10 @@ struct KvCols {
 __host__ __device__ constexpr int dkdv_floats(bool bias, int span) { return 8 * 2 * kRows + (bias ? bias_floats(span) : 0); }
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a) {
+__global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a, const __grid_constant__ CUtensorMap q_map,
+                                                                 const __grid_constant__ CUtensorMap g_map,
+                                                                 const __grid_constant__ CUtensorMap k_map,
+                                                                 const __grid_constant__ CUtensorMap v_map) {
   using F = Bwd<DP>;
   using C = KvCols<DP>;
   extern __shared__ uint8_t smem_raw[];
@@ -394,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a) {
   const int per_head = max(0, (s.lq + kRows - 1) / kRows - first), n = group * per_head;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages);
+  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, 2);
   if (warp == 11) {
     tmem_alloc(&ctl.tmem, 512);
     tmem_relinquish();
@@ -405,72 +408,67 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a) {
   const uint32_t tmem = ctl.tmem, k_tile = smem_u32(smem), ring = k_tile + 2 * F::kTile;
 
   if (warp >= 8) reg_dec<88>();
-  if (warp >= 8 && warp < 11) {
+  if (warp == 8) {
     // ---- loads: K and V, then Q (with lse and delta) and dO tiles in turn
-    const int tid = threadIdx.x - 256;
-    const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.k.p) + (int64_t)s.k0 * a.k.row + kv_head * a.k.head;
-    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v.p) + (int64_t)s.k0 * a.v.row + kv_head * a.v.head;
-    load_tile_async<DP, kLoaders>(k_tile, k, a.k.row, 0, 1, r0, n_rows, a.dim, tid);
-    load_tile_async<DP, kLoaders>(k_tile + F::kTile, v, a.v.row, 0, 1, r0, n_rows, a.dim, tid);
-    feed_ring<F::kStages>(2 * n, &ctl.fixed_full, ctl.full, ctl.empty, abort, [&](int it) {
-      const int st = it % F::kStages, i = it >> 1;
-      const int head = kv_head * group + i / per_head, q0 = (first + i % per_head) * kRows;
-      const int n_q = min(kRows, s.lq - q0);
-      const Strided& src = it & 1 ? a.dout : a.q;
-      const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(src.p) + (int64_t)s.q0 * src.row + head * src.head;
-      load_tile_async<DP, kLoaders>(ring + st * F::kTile, p, src.row, 0, 1, q0, n_q, a.dim, tid);
-      if (it & 1) return;
-      const int64_t stat = (int64_t)head * a.tq + s.q0 + q0;
-      for (int c = tid; c < 2 * kRows; c += kLoaders) {
-        const int col = c & (kRows - 1);
-        const bool in = col < n_q;
-        const float* f = (c < kRows ? a.lse : a.delta) + stat + (in ? col : 0);
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sstat + st * 2 * kRows + c)), "l"(f), "r"(in ? 4 : 0)
-                     : "memory");
-      }
-    });
-  } else if (warp == 11) {
-    // ---- MMAs
-    if (lane == 0 && n > 0) {
+    TileLoader<DP> loader{&ctl.part, abort};
+    if (loader.load(k_tile, &k_map, &ctl.fixed_full, kv_head, s.k0 + r0, n_rows) &&
+        loader.load(k_tile + F::kTile, &v_map, &ctl.fixed_full, kv_head, s.k0 + r0, n_rows))
+      feed_ring<F::kStages>(2 * n, ctl.full, ctl.empty, abort, [&](int it, int st) {
+        const int i = it >> 1, head = kv_head * group + i / per_head, q0 = (first + i % per_head) * kRows;
+        const int n_q = min(kRows, s.lq - q0);
+        if (!(it & 1)) {
+          const int64_t stat = (int64_t)head * a.tq + s.q0 + q0;
+          for (int c = lane; c < 2 * kRows; c += 32) {
+            const int col = c & (kRows - 1);
+            const bool in = col < n_q;
+            const float* f = (c < kRows ? a.lse : a.delta) + stat + (in ? col : 0);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sstat + st * 2 * kRows + c)), "l"(f),
+                         "r"(in ? 4 : 0)
+                         : "memory");
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl.stat_full[st])) : "memory");
+        }
+        return loader.load(ring + st * F::kTile, it & 1 ? &g_map : &q_map, &ctl.full[st], head, s.q0 + q0, n_q);
+      });
+    cp_async_wait<0>();
+    mbar_drain(&ctl.fixed_full, 0);
+  } else if (warp >= 10) {
+    // ---- MMAs: warp 10 S^T and dV, warp 11 dP^T and dK
+    if (lane == 0) {
       const uint32_t idesc_s = idesc_bf16_f32(kRows, kRows, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
-      auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* done) {
-        if (!mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort)) return false;
+      const int w = warp - 10;  // the product takes item 2 i + w, the sum item 2 i + 1 - w
+      const uint32_t d = tmem + w * 128, fixed = desc_k(k_tile + w * F::kTile), acc = tmem + (w == 0 ? C::dv : C::dk),
+                     p = tmem + (w == 0 ? C::p : C::ds);
+      uint64_t *made = w == 0 ? &ctl.s_full : &ctl.dp_full, *ready = w == 0 ? &ctl.p_ready : &ctl.ds_ready,
+               *done = w == 0 ? &ctl.dv_done : &ctl.dk_done;
+      auto full = [&](int it) { return mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort); };
+      auto product = [&](int it) {
+        if (!full(it)) return false;
         tc_fence_after();
-        const uint32_t b = ring + (it % F::kStages) * F::kTile;
+        const uint32_t bd = desc_k(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) mma_ss(d, desc_k(fixed, i), desc_k(b, i), idesc_s, i > 0);
-        mma_commit(done);
+        for (int i = 0; i < DP / 16; ++i) mma_ss(d, fixed + step_k(i), bd + step_k(i), idesc_s, i > 0);
+        mma_commit(made);
+        mma_commit(&ctl.empty[it % F::kStages]);
         return true;
       };
-      auto sum = [&](int it, uint32_t d, uint32_t p, bool more, uint64_t* done) {
-        const uint32_t b = ring + (it % F::kStages) * F::kTile;
+      bool ok = mbar_wait(&ctl.fixed_full, 0, abort) && (n == 0 || product(w));
+      for (int i = 0; i < n && ok; ++i) {
+        const int it = 2 * i + 1 - w;
+        if (!(ok = mbar_wait(ready, i & 1, abort) && full(it))) break;
+        tc_fence_after();
+        const uint32_t bd = desc_mn(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mma_ts(d, p + C::step(i), desc_mn(b, i), idesc_d, more || i > 0);
+        for (int c = 0; c < 8; ++c) mma_ts(acc, p + C::step(c), bd + step_mn(c), idesc_d, i > 0 || c > 0);
         mma_commit(done);
         mma_commit(&ctl.empty[it % F::kStages]);
-      };
-      bool ok = mbar_wait(&ctl.fixed_full, 0, abort) && product(0, tmem, k_tile, &ctl.s_full) &&
-                product(1, tmem + 128, k_tile + F::kTile, &ctl.dp_full);
-      for (int i = 0; i < n && ok; ++i) {
-        if (!(ok = mbar_wait(&ctl.p_ready, i & 1, abort))) break;
-        tc_fence_after();
-        sum(2 * i + 1, tmem + C::dv, tmem + C::p, i > 0, &ctl.dv_done);
-        if (i + 1 < n) {
-          if (DP == 128 && !(ok = mbar_wait(&ctl.dv_done, i & 1, abort))) break;
-          if (!(ok = product(2 * (i + 1), tmem, k_tile, &ctl.s_full))) break;
-        }
-        if (!(ok = mbar_wait(&ctl.ds_ready, i & 1, abort))) break;
-        tc_fence_after();
-        sum(2 * i, tmem + C::dk, tmem + C::ds, i > 0, &ctl.dk_done);
-        if (i + 1 < n) {
-          if (DP == 128 && !(ok = mbar_wait(&ctl.dk_done, i & 1, abort))) break;
-          ok = product(2 * (i + 1) + 1, tmem + 128, k_tile + F::kTile, &ctl.dp_full);
-        }
+        // DP = 128: the next scores take the columns this sum reads
+        if (i + 1 < n) ok = (DP == 64 || mbar_wait(done, i & 1, abort)) && product(2 * (i + 1) + w);
       }
-      mma_commit(&ctl.fin);
-      mbar_drain(&ctl.fin, 0);
+      mma_commit(&ctl.fin[w]);
+      mbar_drain(&ctl.fin[w], 0);
     }
-  } else {
+  } else if (warp < 8) {
     reg_inc<208>();
     // ---- softmax arithmetic: thread = key, a warpgroup per half of a tile's queries
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, key = r0 + row;
@@ -485,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a) {
         expand_bias_padded(a, kv_head * group + i / per_head, 1, sbias, threadIdx.x, kSoftmax);
         if (!(together = softmax_sync())) break;
       }
-      ok = mbar_wait_warp(&ctl.full[st], (2 * i / F::kStages) & 1, abort) && mbar_wait_warp(&ctl.s_full, i & 1, abort);
+      ok = mbar_wait_warp(&ctl.stat_full[st], (2 * i / F::kStages) & 1, abort) && mbar_wait_warp(&ctl.s_full, i & 1, abort);
       if (!ok) break;
       tc_fence_after();
       float x[64];
@@ -578,17 +576,27 @@ template <int DP>
 int launch(const Args& a0, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
   Args a = a0;
   const bool bias = a.table != nullptr;
+  // a side without rows has no tiles, but the map of its tensor must be valid
+  auto map = [&](CUtensorMap* m, const Strided& t, int64_t rows, int heads) {
+    return rows > 0 ? make_tile_map(m, t.p, rows, heads, a.dim, t.row, t.head)
+                    : make_tile_map(m, n_q > 0 ? a.q.p : a.k.p, 1, 1, a.dim, 0, 0);
+  };
+  CUtensorMap q_map, g_map, k_map, v_map;
+  if (int rc = map(&q_map, a.q, a.tq, a.heads)) return rc;
+  if (int rc = map(&g_map, a.dout, a.tq, a.heads)) return rc;
+  if (int rc = map(&k_map, a.k, a.tk, a.kv_heads)) return rc;
+  if (int rc = map(&v_map, a.v, a.tk, a.kv_heads)) return rc;
   if (n_q > 0) {
     const size_t smem = Bwd<DP>::kFloats + dq_floats(bias, a.dtable_part != nullptr, a.span) * sizeof(float);
     KF_CUDA_RET(cudaFuncSetAttribute(attention_dq_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attention_dq_tc<DP><<<dim3(n_q, a.heads), kThreads, smem, st>>>(a);
+    attention_dq_tc<DP><<<dim3(n_q, a.heads), kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     if (int rc = check_launch("kf_attention_bwd")) return rc;
   }
   if (n_k > 0) {
     a.tiles = k_tiles;
     const size_t smem = Bwd<DP>::kFloats + dkdv_floats(bias, a.span) * sizeof(float);
     KF_CUDA_RET(cudaFuncSetAttribute(attention_dkdv_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attention_dkdv_tc<DP><<<dim3(n_k, a.kv_heads), kThreads, smem, st>>>(a);
+    attention_dkdv_tc<DP><<<dim3(n_k, a.kv_heads), kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     return check_launch("kf_attention_bwd");
   }
   return KF_OK;
@@ -598,6 +606,7 @@ int launch(const Args& a0, const int2* k_tiles, int n_q, int n_k, cudaStream_t s
 
 namespace attn {
 int bwd_bf16(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+  if (n_q == 0 && n_k == 0) return KF_OK;
   return a.dim <= 64 ? launch<64>(a, k_tiles, n_q, n_k, st) : launch<128>(a, k_tiles, n_q, n_k, st);
 }
 }  // namespace attn

@@ -2,17 +2,20 @@
 //
 // A CTA owns 256 rows of one sequence and key head as two MMA tiles of 128.
 // Rows are (query, head) pairs: the heads that share a key head are neighbouring
-// rows, so each K and V tile serves all of them.  Per tile of 128 keys:
+// rows, so each K and V tile serves all of them.  Per 64 keys (half a tile):
 //   S = Q K^T into tensor memory; a softmax thread owns one row (a TMEM lane),
-//   reads its 128 scores, keeps the running maximum and sum in registers and
+//   reads its 64 scores, keeps the running maximum and sum in registers and
 //   writes P = 2^(t - m) back to tensor memory as bf16; O += P V with P as the
 //   A operand from there.
 // P is rounded to bf16 for the tensor cores (2^-9 of each weight, summed with
 // either sign); the sum that divides O is the float32 one.  The maximum in use
 // moves only when a row's true one is more than 8 above it (2^8 times the sum
 // in float32 and bf16 loses nothing), so O is rarely rescaled.
-// While one tile's softmax runs, the tensor cores work for the other tile.
-// Warps 0-7 softmax (one warpgroup a tile), 8-10 load, 11 issues the MMAs.
+// Four half tiles are in flight, two per row tile, each with scores of its own:
+// the chain S -> softmax -> P V -> next S of one half runs under the softmax of
+// the other, and under the other row tile.  Tensor memory has no room for more.
+// Warps 0-7 softmax (one warpgroup a row tile), 8 loads, 10 and 11 issue the
+// MMAs of one row tile each.
 #include "attention_tc.cuh"
 
 namespace kf {
@@ -20,7 +23,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int kThreads = 384, kLoaders = 96;
+constexpr int kThreads = 384, kHalf = kRows / 2;
 constexpr float kLazy = 8.f;
 
 template <int DP>
@@ -28,19 +31,21 @@ struct Fwd {
   static constexpr int kStages = DP == 64 ? 6 : 4;  // K and V tiles in flight
   static constexpr int kTile = tile_bytes<DP>();
   static constexpr int kSmem = 1024 + (2 + kStages) * kTile;  // + bias tables
-  // tensor memory columns; with DP = 64 there is room for P beside S
-  static constexpr uint32_t o(int t) { return 256 + t * DP; }
-  static constexpr uint32_t p(int t) { return DP == 64 ? 384 + t * 64 : t * 128; }
+  // tensor memory columns; with DP = 64 there is room for P beside S, with 128 it takes the columns of its scores
+  __device__ static constexpr uint32_t s(int t, int h) { return t * kRows + h * kHalf; }
+  __device__ static constexpr uint32_t o(int t) { return 256 + t * DP; }
+  __device__ static constexpr uint32_t p(int t, int h) { return DP == 64 ? 384 + t * 64 + h * 32 : s(t, h); }
 };
 
 struct Ctl {
-  uint64_t q_full, fin, kv_full[8], kv_empty[8], s_full[2], p_ready[2], o_done[2];
+  uint64_t q_full, part, kv_full[8], kv_empty[8], s_full[2][2], p_ready[2][2], pv_done[2], o_done[2];
   uint32_t tmem;
   int abort;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a) {
+__global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a, const __grid_constant__ CUtensorMap k_map,
+                                                                const __grid_constant__ CUtensorMap v_map) {
   using F = Fwd<DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
@@ -66,10 +71,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a) {
 
   if (threadIdx.x == 0) {
     ctl.abort = 0;
-    mbar_init(&ctl.q_full, kLoaders);
-    mbar_init(&ctl.fin, 1);
-    for (int i = 0; i < F::kStages; ++i) mbar_init(&ctl.kv_full[i], kLoaders), mbar_init(&ctl.kv_empty[i], 1);
-    for (int t = 0; t < 2; ++t) mbar_init(&ctl.s_full[t], 1), mbar_init(&ctl.p_ready[t], kRows), mbar_init(&ctl.o_done[t], 1);
+    mbar_init(&ctl.q_full, 2 * kRows);
+    mbar_init(&ctl.part, 1);
+    for (int i = 0; i < F::kStages; ++i) mbar_init(&ctl.kv_full[i], 1), mbar_init(&ctl.kv_empty[i], 2);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&ctl.pv_done[t], 1), mbar_init(&ctl.o_done[t], 1);
+      for (int h = 0; h < 2; ++h) mbar_init(&ctl.s_full[t][h], 1), mbar_init(&ctl.p_ready[t][h], kRows);
+    }
     fence_barrier_init();
   }
   if (warp == 11) {
@@ -84,62 +92,61 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a) {
 
   // registers: 384 x 168 at launch = 256 x 208 + 128 x 88
   if (warp >= 8) reg_dec<88>();
-  if (warp >= 8 && warp < 11) {
-    // ---- loads: Q, then K and V tiles in turn through the ring
-    const int tid = threadIdx.x - 256;
-    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q.p) + (int64_t)s.q0 * a.q.row + head0 * a.q.head;
-    const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.k.p) + (int64_t)s.k0 * a.k.row + kv_head * a.k.head;
-    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v.p) + (int64_t)s.k0 * a.v.row + kv_head * a.v.head;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-      load_tile_async<DP, kLoaders>(q_tile + t * F::kTile, q, a.q.row, a.q.head, pack, r0 + t * kRows, n_rows[t], a.dim, tid);
-    feed_ring<F::kStages>(2 * n_max, &ctl.q_full, ctl.kv_full, ctl.kv_empty, abort, [&](int it) {
-      const bool is_v = it & 1;
+  if (warp == 8) {
+    // ---- loads: K and V tiles in turn
+    TileLoader<DP> loader{&ctl.part, abort};
+    feed_ring<F::kStages>(2 * n_max, ctl.kv_full, ctl.kv_empty, abort, [&](int it, int st) {
       const int j = it >> 1;
-      load_tile_async<DP, kLoaders>(kv_tile + it % F::kStages * F::kTile, is_v ? v : k, is_v ? a.v.row : a.k.row, 0, 1, j * kRows,
-                                    min(kRows, s.lk - j * kRows), a.dim, tid);
+      return loader.load(kv_tile + st * F::kTile, it & 1 ? &v_map : &k_map, &ctl.kv_full[st], kv_head, s.k0 + j * kRows,
+                         min(kRows, s.lk - j * kRows));
     });
-  } else if (warp == 11) {
-    // ---- MMAs
+  } else if (warp >= 10) {
+    // ---- MMAs of row tile t
     if (lane == 0 && n_max > 0) {
-      const uint32_t idesc_s = idesc_bf16_f32(kRows, kRows, false, false), idesc_o = idesc_bf16_f32(kRows, DP, false, true);
+      const int t = warp - 10, n = n_kv[t];
+      const uint32_t idesc_s = idesc_bf16_f32(kRows, kHalf, false, false), idesc_o = idesc_bf16_f32(kRows, DP, false, true);
+      const uint32_t qd = desc_k(q_tile + t * F::kTile);
       auto full = [&](int it) { return mbar_wait(&ctl.kv_full[it % F::kStages], (it / F::kStages) & 1, abort); };
-      auto last_user = [&](int j) { return n_kv[1] > j ? 1 : 0; };
-      auto scores = [&](int t, int j) {
-        if (!full(2 * j)) return false;
-        tc_fence_after();
-        const uint32_t kt = kv_tile + (2 * j % F::kStages) * F::kTile;
+      auto scores = [&](int j, int h) {
+        const uint32_t kd = desc_k(kv_tile + (2 * j % F::kStages) * F::kTile) + h * (kHalf * 128 >> 4);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) mma_ss(tmem + t * 128, desc_k(q_tile + t * F::kTile, i), desc_k(kt, i), idesc_s, i > 0);
-        mma_commit(&ctl.s_full[t]);
-        if (t == last_user(j)) mma_commit(&ctl.kv_empty[2 * j % F::kStages]);
-        return true;
+        for (int i = 0; i < DP / 16; ++i) mma_ss(tmem + F::s(t, h), qd + step_k(i), kd + step_k(i), idesc_s, i > 0);
+        mma_commit(&ctl.s_full[t][h]);
+        if (h == 1) mma_commit(&ctl.kv_empty[2 * j % F::kStages]);
       };
       bool ok = mbar_wait(&ctl.q_full, 0, abort);
-      for (int t = 0; t < 2; ++t)
-        if (ok && n_kv[t] > 0) ok = scores(t, 0);
-      for (int j = 0; j < n_max && ok; ++j) {
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j >= n_kv[t]) continue;
-          const int it = 2 * j + 1;
-          if (!(ok = mbar_wait(&ctl.p_ready[t], j & 1, abort) && full(it))) break;
-          tc_fence_after();
-          const uint32_t vt = kv_tile + (it % F::kStages) * F::kTile;
+      if (ok && n > 0 && (ok = full(0))) {
+        tc_fence_after();
+        scores(0, 0);
+        scores(0, 1);
+      }
+      for (int j = 0; j < n && ok; ++j) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) mma_ts(tmem + F::o(t), tmem + F::p(t) + i * 8, desc_mn(vt, i), idesc_o, j > 0 || i > 0);
-          mma_commit(&ctl.o_done[t]);
-          if (t == last_user(j)) mma_commit(&ctl.kv_empty[it % F::kStages]);
-          if (j + 1 < n_kv[t]) {
+        for (int h = 0; h < 2; ++h) {
+          const int it = 2 * j + 1;
+          if (!(ok = mbar_wait(&ctl.p_ready[t][h], j & 1, abort) && (h == 1 || full(it)))) break;
+          tc_fence_after();
+          const uint32_t vd = desc_mn(kv_tile + (it % F::kStages) * F::kTile);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mma_ts(tmem + F::o(t), tmem + F::p(t, h) + i * 8, vd + step_mn(h * 4 + i), idesc_o, j > 0 || h > 0 || i > 0);
+          mma_commit(&ctl.pv_done[t]);
+          if (h == 1) mma_commit(&ctl.kv_empty[it % F::kStages]);
+          if (j + 1 < n) {
             // DP = 128: the next scores take P's columns, so P V has to be done
-            if (DP == 128 && !(ok = mbar_wait(&ctl.o_done[t], j & 1, abort))) break;
-            ok = scores(t, j + 1);
+            if (!(ok = (h == 1 || full(it + 1)) && (DP == 64 || mbar_wait(&ctl.pv_done[t], h, abort)))) break;
+            tc_fence_after();
+            scores(j + 1, h);
           }
         }
       }
-      mma_commit(&ctl.fin);
-      mbar_drain(&ctl.fin, 0);
+      mma_commit(&ctl.o_done[t]);
+      // tiles that only the other row tile uses
+      for (int it = 2 * n; it < 2 * n_max && ok; ++it)
+        if ((ok = full(it))) mbar_arrive(&ctl.kv_empty[it % F::kStages]);
+      mbar_drain(&ctl.o_done[t], 0);
     }
-  } else {
+  } else if (warp < 8) {
     reg_inc<208>();
     // ---- softmax: thread = row
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
@@ -152,75 +159,81 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a) {
     const float* bias = sbias + (a.table != nullptr ? (r - tok * pack) * bias_floats(a.span) + a.span + kBiasPad : 0);
     float m = -CUDART_INF_F, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      if (!(ok = mbar_wait_warp(&ctl.s_full[t], j & 1, abort))) break;
+    load_tile_async<DP, kRows>(q_tile + t * F::kTile, static_cast<const __nv_bfloat16*>(a.q.p) + (int64_t)s.q0 * a.q.row + head0 * a.q.head,
+                               a.q.row, a.q.head, pack, r0 + t * kRows, n_rows[t], a.dim, row);
+    cp_async_commit();
+    cp_async_wait<0>();
+    fence_proxy_async_smem();
+    mbar_arrive(&ctl.q_full);
+    for (int i = 0; i < 2 * n; ++i) {
+      const int j = i >> 1, h = i & 1;
+      if (!(ok = mbar_wait_warp(&ctl.s_full[t][h], j & 1, abort))) break;
       tc_fence_after();
-      float x[128];
+      float x[kHalf];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32_issue(lanes + t * 128 + i * 32, x + i * 32);
+      for (int c = 0; c < 2; ++c) tmem_ld32_issue(lanes + F::s(t, h) + c * 32, x + c * 32);
       tmem_wait_ld(x);
-      const int k0 = j * kRows;
+      const int k0 = j * kRows + h * kHalf;
       float mul = c2, add = 0.f;
       if (a.table != nullptr) {
-        const int dist = pos - k0;  // to the tile's first key
-        const bool far = dist - (kRows - 1) >= a.span || dist <= -a.span;
+        const int dist = pos - k0;  // to the first of the keys
+        const bool far = dist - (kHalf - 1) >= a.span || dist <= -a.span;
         if (__all_sync(0xffffffffu, far)) {
           add = dist > 0 ? bias[a.span] : bias[-a.span];
         } else {
-          const float* b = bias + max(-a.span - kBiasPad + kRows - 1, min(dist, a.span + kBiasPad));
+          const float* b = bias + max(-a.span - kBiasPad + kHalf - 1, min(dist, a.span + kBiasPad));
 #pragma unroll
-          for (int i = 0; i < 128; ++i) x[i] = fmaf(x[i], c2, b[-i]);
+          for (int c = 0; c < kHalf; ++c) x[c] = fmaf(x[c], c2, b[-c]);
           mul = 1.f;
         }
       }
-      if (__any_sync(0xffffffffu, limit - k0 < kRows)) {
+      if (__any_sync(0xffffffffu, limit - k0 < kHalf)) {
         const int seen = limit - k0;
 #pragma unroll
-        for (int i = 0; i < 128; ++i) x[i] = i < seen ? x[i] : -CUDART_INF_F;
+        for (int c = 0; c < kHalf; ++c) x[c] = c < seen ? x[c] : -CUDART_INF_F;
       }
       float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], x[i]);
+      for (int c = 4; c < kHalf; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
       const float high = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mul, add);
       if (__any_sync(0xffffffffu, high > m + kLazy)) {
-        // some row's maximum moves: its sum and output follow (O is idle: S came after the last P V)
+        // some row's maximum moves: its sum and, once the last P V is done, its output follow
         const float m_new = fmaxf(m, high);
         const float fix = m == -CUDART_INF_F ? 0.f : ex2(m - m_new);
         m = m_new;
         l *= fix;
-        if (j > 0) {
+        if (i > 0) {
+          if (!(ok = mbar_wait_warp(&ctl.pv_done[t], (i - 1) & 1, abort))) break;
+          tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < DP / 32; ++i) {
+          for (int c = 0; c < DP / 32; ++c) {
             float o[32];
-            tmem_ld32_issue(lanes + F::o(t) + i * 32, o);
+            tmem_ld32_issue(lanes + F::o(t) + c * 32, o);
             tmem_wait_ld(o);
 #pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] *= fix;
-            tmem_st32(lanes + F::o(t) + i * 32, reinterpret_cast<uint32_t*>(o));
+            for (int e = 0; e < 32; ++e) o[e] *= fix;
+            tmem_st32(lanes + F::o(t) + c * 32, reinterpret_cast<uint32_t*>(o));
           }
         }
       }
       const float base = add - (m == -CUDART_INF_F ? 0.f : m);  // a row without a visible key yet: 2^-inf = 0
       float sum[2] = {0.f, 0.f};
+      uint32_t p[kHalf / 2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t p[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float e0 = ex2(fmaf(x[h * 64 + 2 * i], mul, base)), e1 = ex2(fmaf(x[h * 64 + 2 * i + 1], mul, base));
-          sum[0] += e0;
-          sum[1] += e1;
-          p[i] = pack_bf16x2(e0, e1);
-        }
-        tmem_st32(lanes + F::p(t) + h * 32, p);
+      for (int c = 0; c < kHalf / 2; ++c) {
+        const float e0 = ex2(fmaf(x[2 * c], mul, base)), e1 = ex2(fmaf(x[2 * c + 1], mul, base));
+        sum[0] += e0;
+        sum[1] += e1;
+        p[c] = pack_bf16x2(e0, e1);
       }
+      tmem_st32(lanes + F::p(t, h), p);
       l += sum[0] + sum[1];
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&ctl.p_ready[t]);
+      mbar_arrive(&ctl.p_ready[t][h]);
     }
     // ---- O / l, and the logarithm of the sum
-    if (ok && n > 0) ok = mbar_wait_warp(&ctl.o_done[t], (n - 1) & 1, abort);
+    if (ok && n > 0) ok = mbar_wait_warp(&ctl.o_done[t], 0, abort);
     if (ok) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -270,7 +283,11 @@ template <int DP>
 int launch(const Args& a, int n_tiles, cudaStream_t st) {
   const size_t smem = Fwd<DP>::kSmem + (a.table != nullptr ? a.pack * bias_floats(a.span) * sizeof(float) : 0);
   KF_CUDA_RET(cudaFuncSetAttribute(attention_fwd_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  attention_fwd_tc<DP><<<dim3(n_tiles, a.heads / a.pack), kThreads, smem, st>>>(a);
+  CUtensorMap k_map, v_map;
+  const bool keys = a.tk > 0;  // without keys no tile is loaded
+  if (int rc = make_tile_map(&k_map, keys ? a.k.p : a.q.p, keys ? a.tk : 1, keys ? a.kv_heads : 1, a.dim, a.k.row, a.k.head)) return rc;
+  if (int rc = make_tile_map(&v_map, keys ? a.v.p : a.q.p, keys ? a.tk : 1, keys ? a.kv_heads : 1, a.dim, a.v.row, a.v.head)) return rc;
+  attention_fwd_tc<DP><<<dim3(n_tiles, a.heads / a.pack), kThreads, smem, st>>>(a, k_map, v_map);
   return check_launch("kf_attention_fwd");
 }
 

@@ -33,22 +33,30 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
+// A shared memory operand: the descriptor's low word (address) and the high
+// word, which all operands share; a step along the operand is an addition to
+// the low word, so that issuing an MMA costs a few instructions.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride 1024, version 1, 128-byte swizzle
+
 // D[tmem] (+)= A[smem] B[smem]^T
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHi)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem]^T: a lane holds a row of A, a column two neighbouring bf16 of it
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHi)
       : "memory");
 }
 // One arrival on `bar` when every MMA this thread has issued is complete.
@@ -136,53 +144,73 @@ __device__ __forceinline__ void load_tile_async(uint32_t dst, const __nv_bfloat1
   }
 }
 
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
+// 3-D tiled load (column, head, row) of 64 columns x 128 rows of one head.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
-  return ok != 0;
 }
 
-// The loader's side of a ring of STAGES tiles.  Item 0 was issued before and
-// signals `fixed`; issue(it) starts the copies of tile it.  A thread keeps up to
-// three items in flight and signals an item once its own copies have landed;
-// before it blocks on a full ring it signals all it has, since the MMAs that
-// free a tile may need the ones just loaded.
-template <int STAGES, typename Issue>
-__device__ __forceinline__ void feed_ring(int n_items, uint64_t* fixed, uint64_t* full, uint64_t* empty, volatile int* abort,
-                                          Issue&& issue) {
-  cp_async_commit();
-  int sent = 0;  // items signalled
-  auto signal = [&](int upto) {
-    fence_proxy_async_smem();
-    for (; sent < upto; ++sent) mbar_arrive(sent == 0 ? fixed : full + (sent - 1) % STAGES);
-  };
-  bool ok = true;
-  for (int it = 0; it < n_items; ++it) {
-    const uint32_t parity = ((it / STAGES) & 1) ^ 1;
-    if (!mbar_test(empty + it % STAGES, parity)) {
-      cp_async_wait<0>();
-      signal(it + 1);
-      if (!(ok = mbar_wait(empty + it % STAGES, parity, abort))) break;
+__device__ __forceinline__ void st_zero16(uint32_t dst) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+}
+
+// One warp's loads of 128-row tiles by TMA.  Rows past the sequence belong to
+// its neighbour in the packed tensor: a tile that has such rows lands on a
+// barrier of the warp's own and is signalled once they are overwritten by
+// zeros, so that nothing outside a sequence enters an MMA.
+template <int DP>
+struct TileLoader {
+  uint64_t* part;  // count 1
+  volatile int* abort;
+  uint32_t parity = 0;
+
+  // The n first rows of the tile at `row` of head `head`; one arrival on `full` when it is there.
+  __device__ __forceinline__ bool load(uint32_t dst, const CUtensorMap* map, uint64_t* full, int head, int row, int n) {
+    const int lane = threadIdx.x & 31;
+    uint64_t* bar = n < kRows ? part : full;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(bar, tile_bytes<DP>());
+#pragma unroll
+      for (int p = 0; p < DP / 64; ++p) tma_load_3d(dst + p * kPanel, map, bar, p * 64, head, row);
     }
-    issue(it);
-    cp_async_commit();
-    cp_async_wait<2>();
-    if (it > 0) signal(it);  // items 0 .. it - 1 of it + 2
+    if (n >= kRows) return true;
+    const bool ok = mbar_wait_warp(part, parity, abort);
+    if (!ok) mbar_drain(part, parity);
+    parity ^= 1;
+#pragma unroll
+    for (int p = 0; p < DP / 64; ++p)
+      for (int i = lane; i < (kRows - n) * 8; i += 32) st_zero16(dst + p * kPanel + n * 128 + i * 16);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(full);
+    return ok;
   }
-  cp_async_wait<0>();
-  if (ok) signal(n_items + 1);
+};
+
+// A ring of STAGES tiles: tile it goes to stage it % STAGES once that is free.
+// load(it, stage) starts one; after an abort the loads in flight are waited for.
+template <int STAGES, typename Load>
+__device__ __forceinline__ void feed_ring(int n_items, uint64_t* full, uint64_t* empty, volatile int* abort, Load&& load) {
+  int it = 0;
+  for (; it < n_items; ++it) {
+    if (!mbar_wait_warp(empty + it % STAGES, ((it / STAGES) & 1) ^ 1, abort)) break;
+    if (!load(it, it % STAGES)) break;
+  }
+  if (*abort)
+    for (int i = max(0, it - STAGES); i < it; ++i) mbar_drain(full + i % STAGES, (i / STAGES) & 1);
 }
 
-// K-major operand (rows x DP, contraction over DP), k-step j of 16
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int j) { return smem_desc_sw128(tile + (j >> 2) * kPanel + (j & 3) * 32, 16, 1024); }
-// MN-major operand (contraction over its 128 rows), k-step j of 16 rows
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int j) { return smem_desc_sw128(tile + j * 2048, kPanel, 1024); }
+// Low words.  K-major operand (rows x DP, contraction over DP): k-step j of 16 columns.
+__device__ __forceinline__ uint32_t desc_k(uint32_t tile) { return ((tile >> 4) & 0x3FFFu) | (1u << 16); }
+__host__ __device__ constexpr uint32_t step_k(int j) { return ((j >> 2) * kPanel + (j & 3) * 32) >> 4; }
+// MN-major operand (contraction over its 128 rows, panels of 64 columns): k-step j of 16 rows.
+__device__ __forceinline__ uint32_t desc_mn(uint32_t tile) { return ((tile >> 4) & 0x3FFFu) | ((uint32_t)(kPanel >> 4) << 16); }
+__host__ __device__ constexpr uint32_t step_mn(int j) { return j * (2048 >> 4); }
+
+// Map of a (tokens, heads, dim) bf16 tensor, boxes of 64 columns x 1 head x 128 rows.
+int make_tile_map(CUtensorMap* map, const void* p, int64_t rows, int heads, int dim, int64_t row_stride, int64_t head_stride);
 
 // ---- softmax arithmetic ---------------------------------------------------------
 
