@@ -525,12 +525,12 @@ int kf_residual_norm_bwd(const void* x, const void* branch, const void* gate, co
  * no key is visible.  Keys and values outside a sequence never enter, whatever
  * they hold.  Scores, softmax and sums are float32; bf16 inputs round the
  * probabilities (and dS in the backward) to bf16 for the tensor cores.
- *   seqs    (n_seqs, 4) int32: q_start, q_len, k_start, k_len
- *   q_tiles (n_q_tiles, 2) int32: sequence and tile of its query rows, one entry
- *           for every tile of every sequence, any order; k_tiles likewise for
- *           the key rows.  kf_attention_tiling() gives the rows of a tile for
- *           the forward's queries (pass 0), the backward's queries (1) and its
- *           keys (2), and pack: a sequence of n queries has n * pack rows
+ *   q_tiles (n_q_tiles, 8) int32: q_start, q_len, k_start, k_len of a sequence,
+ *           the index of a tile of its query rows, three unused; one entry for
+ *           every tile of every sequence, any order; k_tiles likewise for the key
+ *           rows.  kf_attention_tiling() gives the rows of a tile for the
+ *           forward's queries (pass 0), the backward's queries (1) and its keys
+ *           (2), and pack: a sequence of n queries has n * pack rows
  *   table   (n_buckets, heads) in table_dtype, buckets (2 span + 1) int32; null: no bias
  *   o       (tq, heads, dim) contiguous; lse (heads, tq) float32, base 2 (null: not written);
  *           o_rest like o, bf16 only: what o's rounding left out, which the
@@ -542,19 +542,19 @@ int kf_residual_norm_bwd(const void* x, const void* branch, const void* gate, co
 typedef struct kf_attention_desc {
   int64_t tq, tk;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
-  int32_t heads, kv_heads, dim, n_seqs;
+  int32_t heads, kv_heads, dim;
   int32_t dtype, causal;
   int32_t span, n_buckets, table_dtype;
   float scale;
 } kf_attention_desc;
 
 int kf_attention_tiling(const kf_attention_desc* desc, int pass, int32_t* rows, int32_t* pack);
-int kf_attention_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* q_tiles,
-                     int32_t n_q_tiles, const void* table, const int32_t* buckets, void* o, void* o_rest, float* lse,
+int kf_attention_fwd(const void* q, const void* k, const void* v, const int32_t* q_tiles, int32_t n_q_tiles,
+                     const void* table, const int32_t* buckets, void* o, void* o_rest, float* lse,
                      const kf_attention_desc* desc, void* stream);
 int64_t kf_attention_bwd_workspace(int32_t n_q_tiles, const kf_attention_desc* desc);
 int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout,
-                     const float* lse, const int32_t* seqs, const int32_t* q_tiles, int32_t n_q_tiles, const int32_t* k_tiles,
+                     const float* lse, const int32_t* q_tiles, int32_t n_q_tiles, const int32_t* k_tiles,
                      int32_t n_k_tiles, const void* table, const int32_t* buckets, void* dq, void* dk, void* dv,
                      void* dtable, float* workspace, const kf_attention_desc* desc, void* stream);
 

@@ -95,7 +95,7 @@ class AttentionDesc(ctypes.Structure):
 
     _fields_ = (
         [(n, _c_i64) for n in ("tq", "tk", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
-        + [(n, _c_i32) for n in ("heads", "kv_heads", "dim", "n_seqs", "dtype", "causal", "span", "n_buckets", "table_dtype")]
+        + [(n, _c_i32) for n in ("heads", "kv_heads", "dim", "dtype", "causal", "span", "n_buckets", "table_dtype")]
         + [("scale", ctypes.c_float)]
     )
 
@@ -238,12 +238,12 @@ PROTOTYPES = {
         ctypes.c_int, [ctypes.POINTER(AttentionDesc), ctypes.c_int, ctypes.POINTER(_c_i32), ctypes.POINTER(_c_i32)],
     ),
     "kf_attention_fwd": (
-        ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(AttentionDesc), _vp],
+        ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i32, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(AttentionDesc), _vp],
     ),
     "kf_attention_bwd_workspace": (_c_i64, [_c_i32, ctypes.POINTER(AttentionDesc)]),
     "kf_attention_bwd": (
         ctypes.c_int,
-        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i32, _vp, _c_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
          ctypes.POINTER(AttentionDesc), _vp],
     ),
     "kf_attention_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(DecodeDesc), _vp]),

@@ -50,34 +50,43 @@ class PackedSequences:
         for lq, lk in zip(self.q_lens, self.kv_lens):
             rows.append((q0, lq, k0, lk))
             q0, k0 = q0 + lq, k0 + lk
-        self.device = torch.device(device)
-        self.table = torch.tensor(rows, dtype=torch.int32).reshape(-1, 4).to(self.device)
+        self._rows = torch.tensor(rows, dtype=torch.int32).reshape(-1, 4)
+        self.table = self._rows.to(torch.device(device))
         self.device = self.table.device
         self._tiles: dict = {}
         self._plans: dict = {}  # by a call's shapes, strides and types
 
-    def __len__(self) -> int:
-        return len(self.q_lens)
-
     def tiles(self, side: str, rows: int, causal: bool, pack: int = 1) -> torch.Tensor:
         """(n, 2) int32 (sequence, tile): every ``rows`` rows of the query ("q") or
         key ("k") side, ``pack`` rows to a token, those with the most work first."""
+        found = []
+        for s, (lq, lk) in enumerate(zip(self.q_lens, self.kv_lens)):
+            off = lk - lq
+            for t in range(-(-(lq if side == "q" else lk) * pack // rows)):
+                if not causal:
+                    cost = lk if side == "q" else lq
+                elif side == "q":
+                    cost = max(0, min(lk, -(-(t + 1) * rows // pack) + off))
+                else:
+                    cost = max(0, lq - max(0, t * rows - off))
+                found.append((-cost, s, t))
+        found.sort()
+        return torch.tensor([f[1:] for f in found], dtype=torch.int32).reshape(-1, 2)
+
+    def _entries(self, side: str, rows: int, causal: bool, pack: int) -> torch.Tensor:
+        """``tiles`` as the kernels read them: (n, 8) int32 on the device, the rows of
+        the tile's sequence and its index."""
         key = (side, rows, causal, pack)
         if key not in self._tiles:
-            found = []
-            for s, (lq, lk) in enumerate(zip(self.q_lens, self.kv_lens)):
-                off = lk - lq
-                for t in range(-(-(lq if side == "q" else lk) * pack // rows)):
-                    if not causal:
-                        cost = lk if side == "q" else lq
-                    elif side == "q":
-                        cost = max(0, min(lk, -(-(t + 1) * rows // pack) + off))
-                    else:
-                        cost = max(0, lq - max(0, t * rows - off))
-                    found.append((-cost, s, t))
-            found.sort()
-            self._tiles[key] = torch.tensor([f[1:] for f in found], dtype=torch.int32).reshape(-1, 2).to(self.device)
+            tiles = self.tiles(side, rows, causal, pack)
+            out = torch.zeros(tiles.shape[0], 8, dtype=torch.int32)
+            out[:, :4] = self._rows[tiles[:, 0].long()]
+            out[:, 4] = tiles[:, 1]
+            self._tiles[key] = out.to(self.device)
         return self._tiles[key]
+
+    def __len__(self) -> int:
+        return len(self.q_lens)
 
 
 def relative_buckets(num_buckets: int, max_distance: int, bidirectional: bool) -> list[int]:
@@ -194,7 +203,7 @@ class _Plan:
         has = bias is not None
         self.desc = _lib.AttentionDesc(
             q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-            q.shape[1], k.shape[1], q.shape[2], len(seqs), _DTYPE_CODE[q.dtype], int(causal),
+            q.shape[1], k.shape[1], q.shape[2], _DTYPE_CODE[q.dtype], int(causal),
             bias.max_distance if has else 0, bias.num_buckets if has else 0, _DTYPE_CODE[bias.weight.dtype] if has else 0,
             scale)
         self.ref = ctypes.byref(self.desc)
@@ -202,7 +211,7 @@ class _Plan:
         for what, side in enumerate("qqk"):
             rows, pack = ctypes.c_int32(), ctypes.c_int32()
             _lib.call("kf_attention_tiling", self.ref, what, ctypes.byref(rows), ctypes.byref(pack))
-            t = seqs.tiles(side, rows.value, causal, pack.value)
+            t = seqs._entries(side, rows.value, causal, pack.value)
             self.tiles.append((t.data_ptr(), t.shape[0]))
         self.workspace = max(1, int(_lib.load().kf_attention_bwd_workspace(self.tiles[1][1], self.ref)))
 
@@ -231,7 +240,7 @@ def _forward(q, k, v, table, seqs, causal, scale, bias, train: bool):
     tiles, n = plan.tiles[0]
     if n:
         table = None if table is None else table.detach().contiguous()
-        _launch("kf_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), seqs.table.data_ptr(), tiles, n,
+        _launch("kf_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), tiles, n,
                 None if table is None else table.data_ptr(), None if table is None else bias.buckets.data_ptr(),
                 o.data_ptr(), None if rest is None else rest.data_ptr(), None if lse is None else lse.data_ptr(),
                 plan.ref, _raw_stream(q))
@@ -266,7 +275,7 @@ class _Attention(torch.autograd.Function):
         if n_q or n_k or want:
             ws = torch.empty(plan.workspace, device=q.device, dtype=torch.float32)
             _launch("kf_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                    None if rest is None else rest.data_ptr(), dout.data_ptr(), lse.data_ptr(), seqs.table.data_ptr(),
+                    None if rest is None else rest.data_ptr(), dout.data_ptr(), lse.data_ptr(),
                     q_tiles, n_q, k_tiles, n_k, None if tab is None else tab.data_ptr(),
                     None if tab is None else bias.buckets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                     None if dtable is None else dtable.data_ptr(), ws.data_ptr(), plan.ref, _raw_stream(q),

@@ -32,7 +32,7 @@ int check_attention(const char* fn, const kf_attention_desc* d) {
   KF_CHECK_ARG(d->dim >= 8 && d->dim <= kMaxDim && d->dim % 8 == 0, "%s: head width %d is not a multiple of 8 up to %d", fn, d->dim,
                kMaxDim);
   KF_CHECK_ARG(d->dtype == KF_DTYPE_F32 || d->dtype == KF_DTYPE_BF16, "%s: types must be float32 or bfloat16", fn);
-  KF_CHECK_ARG(d->tq >= 0 && d->tk >= 0 && d->n_seqs >= 0, "%s: negative size", fn);
+  KF_CHECK_ARG(d->tq >= 0 && d->tk >= 0, "%s: negative size", fn);
   KF_CHECK_ARG(d->span >= 0 && d->span <= kMaxSpan, "%s: bias distances up to %d are outside [0, %d]", fn, d->span, kMaxSpan);
   KF_CHECK_ARG(d->n_buckets >= 0 && d->n_buckets <= kMaxBuckets, "%s: %d buckets exceed %d", fn, d->n_buckets, kMaxBuckets);
   return KF_OK;
@@ -44,10 +44,10 @@ int check_attention(const char* fn, const kf_attention_desc* d) {
 // not fit in shared memory.
 void tiling(const kf_attention_desc* d, int pass, int32_t* rows, int32_t* pack) {
   *pack = 1;
-  *rows = d->dtype == KF_DTYPE_F32 ? 64 : pass == 0 ? 256 : 128;
+  *rows = d->dtype == KF_DTYPE_F32 ? 64 : pass == 0 && d->dim > 64 ? 256 : 128;
   if (d->dtype == KF_DTYPE_F32 || pass > 0) return;
   const int group = d->heads / d->kv_heads;
-  if (d->n_buckets == 0 || group * bias_floats(d->span) * (int)sizeof(float) <= kBiasBytes) *pack = group;
+  if (d->n_buckets == 0 || group * bias_floats(d->span) * (int)sizeof(float) <= fwd_bias_bytes(d->dim)) *pack = group;
 }
 
 Args make_args(const kf_attention_desc* d) {
@@ -82,7 +82,7 @@ int kf::attn::make_tile_map(CUtensorMap* map, const void* p, int64_t rows, int h
   const cuuint64_t pitch = (cuuint64_t)(dim + 7) / 8 * 16;
   cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
   cuuint64_t strides[2] = {heads > 1 ? (cuuint64_t)head_stride * 2 : pitch, rows > 1 ? (cuuint64_t)row_stride * 2 : pitch};
-  cuuint32_t box[3] = {64, 1, (cuuint32_t)kRows}, step[3] = {1, 1, 1};
+  cuuint32_t box[3] = {64, 1, (cuuint32_t)kBoxRows}, step[3] = {1, 1, 1};
   const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, step,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -100,20 +100,19 @@ extern "C" int kf_attention_tiling(const kf_attention_desc* d, int pass, int32_t
   return KF_OK;
 }
 
-extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, const int32_t* seqs, const int32_t* q_tiles,
-                                int32_t n_q_tiles, const void* table, const int32_t* buckets, void* o, void* o_rest,
+extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, const int32_t* q_tiles, int32_t n_q_tiles, const void* table, const int32_t* buckets, void* o, void* o_rest,
                                 float* lse, const kf_attention_desc* d, void* stream) {
   using namespace kf;
   clear_error();
   if (int rc = check_attention("kf_attention_fwd", d)) return rc;
   if (n_q_tiles == 0) return KF_OK;
   KF_CHECK_ARG(n_q_tiles > 0, "kf_attention_fwd: negative tile count");
-  KF_CHECK_ARG(q && o && seqs && q_tiles && (d->tk == 0 || (k && v)), "kf_attention_fwd: null argument");
+  KF_CHECK_ARG(q && o && q_tiles && (d->tk == 0 || (k && v)), "kf_attention_fwd: null argument");
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_fwd: the bias needs a table and buckets");
   if (int rc = bind_device(q)) return rc;
   Args a = make_args(d);
   a.q.p = q, a.k.p = k, a.v.p = v, a.o = o, a.o_rest = o_rest, a.lse = lse, a.table = table, a.buckets = buckets;
-  a.seqs = reinterpret_cast<const int4*>(seqs), a.tiles = reinterpret_cast<const int2*>(q_tiles);
+  a.tiles = reinterpret_cast<const Tile*>(q_tiles);
   int rows;
   tiling(d, 0, &rows, &a.pack);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -126,15 +125,15 @@ extern "C" int64_t kf_attention_bwd_workspace(int32_t n_q_tiles, const kf_attent
 }
 
 extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout, const float* lse,
-                                const int32_t* seqs, const int32_t* q_tiles, int32_t n_q_tiles, const int32_t* k_tiles,
+                                const int32_t* q_tiles, int32_t n_q_tiles, const int32_t* k_tiles,
                                 int32_t n_k_tiles, const void* table, const int32_t* buckets, void* dq, void* dk, void* dv,
                                 void* dtable, float* workspace, const kf_attention_desc* d, void* stream) {
   using namespace kf;
   clear_error();
   if (int rc = check_attention("kf_attention_bwd", d)) return rc;
   KF_CHECK_ARG(n_q_tiles >= 0 && n_k_tiles >= 0, "kf_attention_bwd: negative tile count");
-  KF_CHECK_ARG(n_q_tiles == 0 || (q && o && dout && lse && dq && workspace && q_tiles && seqs), "kf_attention_bwd: null argument");
-  KF_CHECK_ARG(n_k_tiles == 0 || (k && v && dk && dv && k_tiles && seqs), "kf_attention_bwd: null argument");
+  KF_CHECK_ARG(n_q_tiles == 0 || (q && o && dout && lse && dq && workspace && q_tiles), "kf_attention_bwd: null argument");
+  KF_CHECK_ARG(n_k_tiles == 0 || (k && v && dk && dv && k_tiles), "kf_attention_bwd: null argument");
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_bwd: the bias needs a table and buckets");
   KF_CHECK_ARG(dtable == nullptr || (table != nullptr && workspace != nullptr), "kf_attention_bwd: dtable needs a table and workspace");
   if (n_q_tiles == 0 && n_k_tiles == 0 && dtable == nullptr) return KF_OK;
@@ -142,11 +141,11 @@ extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, con
   Args a = make_args(d);
   a.q.p = q, a.k.p = k, a.v.p = v, a.dout.p = dout, a.o = const_cast<void*>(o), a.o_rest = const_cast<void*>(o_rest), a.lse = const_cast<float*>(lse);
   a.dq = dq, a.dk = dk, a.dv = dv, a.table = table, a.buckets = buckets;
-  a.seqs = reinterpret_cast<const int4*>(seqs), a.tiles = reinterpret_cast<const int2*>(q_tiles);
+  a.tiles = reinterpret_cast<const Tile*>(q_tiles);
   a.delta = workspace;
   a.dtable_part = dtable != nullptr ? workspace + (int64_t)d->heads * d->tq : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int2* kt = reinterpret_cast<const int2*>(k_tiles);
+  const Tile* kt = reinterpret_cast<const Tile*>(k_tiles);
   int rows;
   tiling(d, 1, &rows, &a.pack);
   int rc = d->dtype == KF_DTYPE_BF16 ? bwd_bf16(a, kt, n_q_tiles, n_k_tiles, st) : bwd_f32(a, kt, n_q_tiles, n_k_tiles, st);

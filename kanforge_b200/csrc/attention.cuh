@@ -19,8 +19,14 @@ constexpr int kMaxSpan = 1024;    // largest distance with a bias of its own
 constexpr int kMaxBuckets = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct Seq {  // one row of the table of sequences
-  int q0, lq, k0, lk;
+struct Seq {
+  int q0, lq, k0, lk;  // rows of the queries, of the keys
+};
+
+struct __align__(16) Tile {
+  Seq s;
+  int index;  // of the tile in its sequence
+  int unused[3];
 };
 
 struct Strided {  // (tokens, heads, dim), last dimension contiguous; strides in elements
@@ -35,8 +41,7 @@ struct Args {
   void *dq, *dk, *dv;
   float* lse;   // (H, Tq)
   float* delta; // (H, Tq): dO . O
-  const int4* seqs;
-  const int2* tiles;  // (sequence, tile of its rows)
+  const Tile* tiles;
   const void* table;  // (buckets, H) bias, or null
   const int* buckets; // (2 span + 1): bucket of distance index - span
   float* dtable_part; // (tiles, H, buckets)
@@ -47,8 +52,9 @@ struct Args {
   float scale;
 };
 
-__device__ __forceinline__ Seq load_seq(const Args& a, int s) {
-  const int4 v = a.seqs[s];
+__device__ __forceinline__ Seq load_tile(const Args& a, int i, int* index) {
+  const int4 v = *reinterpret_cast<const int4*>(&a.tiles[i].s);
+  *index = a.tiles[i].index;
   return Seq{v.x, v.y, v.z, v.w};
 }
 
@@ -73,9 +79,11 @@ __device__ __forceinline__ void expand_bias(const Args& a, int head, float* out,
 
 // attention_f32.cu, attention_fwd.cu, attention_bwd.cu
 int fwd_f32(const Args& a, int n_tiles, cudaStream_t st);
-int bwd_f32(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st);
+int bwd_f32(const Args& a, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st);
+// shared memory of the bf16 forward for bias tables
+constexpr int fwd_bias_bytes(int dim) { return dim <= 64 ? 12 * 1024 : 32 * 1024; }
 int fwd_bf16(const Args& a, int n_tiles, cudaStream_t st);
-int bwd_bf16(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st);
+int bwd_bf16(const Args& a, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st);
 
 __device__ __forceinline__ int clamp_dist(int d, int span) { return min(max(d, -span), span) + span; }
 

@@ -10,9 +10,11 @@
 // Seven products of 128 x 128 x D a tile pair against five with one kernel;
 // the five would add every dQ tile into memory in an order that varies.
 // All scores live in tensor memory; P and dS go back there as bf16 (2^-9 of
-// each term) and are the A operands of the products that sum them.  Of the 12
-// warps 0-7 do the softmax arithmetic (thread = row, a warpgroup per half of
-// the columns), 8 loads, 10 and 11 issue the MMAs of one chain each.
+// each term) and are the A operands of the products that sum them.  A streamed
+// tile has 128 rows with D = 128 and a CTA has an SM to itself; with D <= 64 it has
+// 64 and two CTAs share an SM, so that one's chain of products and softmax runs
+// under the other's.  Warps: softmax arithmetic (thread = row, a warpgroup for
+// each 64 columns), one that loads, two that issue the MMAs of one chain each.
 #include "attention_tc.cuh"
 
 namespace kf {
@@ -20,36 +22,42 @@ namespace {
 
 using namespace attn;
 
-constexpr int kThreads = 384, kSoftmax = 256;
-
 template <int DP>
 struct Bwd {
-  static constexpr int kStages = DP == 64 ? 6 : 4;  // streamed tiles in flight
-  static constexpr int kTile = tile_bytes<DP>();
-  static constexpr int kFloats = 1024 + (2 + kStages) * kTile;  // offset of what follows the tiles
+  static constexpr int kCols = DP == 64 ? 64 : 128;    // rows of a streamed tile, columns of the scores
+  static constexpr int kStages = DP == 64 ? 6 : 4;     // streamed tiles in flight
+  static constexpr int kFixed = tile_bytes<DP>(kRows), kTile = tile_bytes<DP>(kCols);
+  static constexpr int kRing = 2 * kFixed, kFloats = kRing + kStages * kTile;  // byte offsets behind the fixed tiles
+  static constexpr int kGroups = kCols / 64, kSoftmax = kGroups * 128;
+  static constexpr int kLoadWarp = kGroups * 4, kMmaWarp = DP == 64 ? 5 : 10;
+  static constexpr int kThreads = DP == 64 ? 224 : 384, kCtas = DP == 64 ? 2 : 1;
+  static constexpr uint32_t kTmem = DP == 64 ? 256 : 512;
 };
 
 struct Ctl {
-  uint64_t fixed_full, part, full[8], empty[8], stat_full[8], s_full, dp_full, s_read, p_ready, ds_ready, dv_done, dk_done, fin[2];
+  uint64_t fixed_full, part[2], full[8], empty[8], stat_full[8], s_full, dp_full, s_read, p_ready, ds_ready, dv_done, dk_done, fin[2];
   uint32_t tmem;
   int abort;
 };
 
 // `users`: how many MMA warps read a streamed tile
-__device__ __forceinline__ void init_barriers(Ctl* c, int stages, int users) {
+__device__ __forceinline__ void init_barriers(Ctl* c, int stages, int users, int softmax) {
   c->abort = 0;
   mbar_init(&c->fixed_full, 2);
-  mbar_init(&c->part, 1);
+  mbar_init(&c->part[0], 1), mbar_init(&c->part[1], 1);
   for (int i = 0; i < stages; ++i) mbar_init(&c->full[i], 1), mbar_init(&c->empty[i], users), mbar_init(&c->stat_full[i], 32);
   mbar_init(&c->s_full, 1), mbar_init(&c->dp_full, 1), mbar_init(&c->dv_done, 1), mbar_init(&c->dk_done, 1);
-  mbar_init(&c->s_read, kSoftmax), mbar_init(&c->p_ready, kSoftmax), mbar_init(&c->ds_ready, kSoftmax);
+  mbar_init(&c->s_read, softmax), mbar_init(&c->p_ready, softmax), mbar_init(&c->ds_ready, softmax);
   mbar_init(&c->fin[0], 1), mbar_init(&c->fin[1], 1);
   fence_barrier_init();
 }
 
 // Barrier of the softmax warps.  A warp whose wait ran out calls it once with
 // false and leaves; the others learn of it at their next call and leave too.
-__device__ __forceinline__ bool softmax_sync(bool ok = true) { return named_bar_and(1, kSoftmax, ok); }
+template <int DP>
+__device__ __forceinline__ bool softmax_sync(bool ok = true) {
+  return named_bar_and(1, Bwd<DP>::kSoftmax, ok);
+}
 
 // One row of a result: DP columns of this thread's lane times mul, dim of them stored.
 template <int DP>
@@ -75,104 +83,107 @@ __device__ __forceinline__ void store_row(uint32_t lanes, __nv_bfloat16* out, in
 }
 
 // ---- dQ -------------------------------------------------------------------------
-// Tensor memory: S at 0, dP at 128, dQ at 256, two buffers of dS at 384.
+// Tensor memory: S, dP, dQ, two buffers of dS.
+template <int DP>
+struct QCols {
+  static constexpr uint32_t s = 0, dp = Bwd<DP>::kCols, dq = 2 * Bwd<DP>::kCols, ds = dq + DP, ds_buffer = Bwd<DP>::kCols / 2;
+};
 
-// Floats behind the tiles: bias table, sums by distance, block diagonals, bucket ids.
-constexpr int kDiag = 16 * 64;  // 4 x 4 blocks of 32 x 32 scores, 63 diagonals each
+// Floats behind the tiles: halves of delta, bias table, sums by distance, block diagonals, bucket ids.
+constexpr int kDiag = 64;  // of a block of 32 x 32 scores: 63 diagonals
+template <int DP>
 __host__ __device__ constexpr int dq_floats(bool bias, bool grad, int span) {
-  return 2 * kRows + (bias ? bias_floats(span) : 0) + (grad ? 2 * span + 1 + kDiag + (2 * span + 4) / 4 : 0);
+  return 2 * kRows + (bias ? bias_floats(span) : 0) + (grad ? 2 * span + 1 + Bwd<DP>::kCols / 8 * kDiag + (2 * span + 4) / 4 : 0);
 }
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, const __grid_constant__ CUtensorMap q_map,
+__global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_dq_tc(const Args a, const __grid_constant__ CUtensorMap q_map,
                                                                const __grid_constant__ CUtensorMap g_map,
                                                                const __grid_constant__ CUtensorMap k_map,
                                                                const __grid_constant__ CUtensorMap v_map) {
   using F = Bwd<DP>;
+  using C = QCols<DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sdelta = reinterpret_cast<float*>(smem + (2 + F::kStages) * F::kTile);  // (2, 128) halves of delta
+  float* sdelta = reinterpret_cast<float*>(smem + F::kFloats);  // (groups, 128) parts of delta
   float* sbias = sdelta + 2 * kRows;
   float* ssum = sbias + (a.table != nullptr ? bias_floats(a.span) : 0);
   float* sdiag = ssum + 2 * a.span + 1;
-  uint8_t* sbucket = reinterpret_cast<uint8_t*>(sdiag + kDiag);
+  uint8_t* sbucket = reinterpret_cast<uint8_t*>(sdiag + F::kCols / 8 * kDiag);
   volatile int* abort = &ctl.abort;
 
-  const int2 tile = a.tiles[blockIdx.x];
-  const Seq s = load_seq(a, tile.x);
+  int tile;
+  const Seq s = load_tile(a, blockIdx.x, &tile);
   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-  const int r0 = tile.y * kRows, off = s.lk - s.lq, n_rows = min(kRows, s.lq - r0);
+  const int r0 = tile * kRows, off = s.lk - s.lq, n_rows = min(kRows, s.lq - r0);
   const int keys = a.causal ? max(0, min(s.lk, r0 + n_rows + off)) : s.lk;
-  const int n = (keys + kRows - 1) / kRows;
+  const int n = (keys + F::kCols - 1) / F::kCols;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool grad = a.dtable_part != nullptr;
 
-  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, 1);
-  if (warp == 11) {
-    tmem_alloc(&ctl.tmem, 512);
+  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, 1, F::kSoftmax);
+  if (warp == F::kMmaWarp) {
+    tmem_alloc(&ctl.tmem, F::kTmem);
     tmem_relinquish();
   }
-  if (a.table != nullptr) expand_bias_padded(a, head, 1, sbias, threadIdx.x, kThreads);
-  if (grad)
-    for (int i = threadIdx.x; i < 2 * a.span + 1; i += kThreads) ssum[i] = 0.f, sbucket[i] = (uint8_t)a.buckets[i];
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl.tmem, q_tile = smem_u32(smem), ring = q_tile + 2 * F::kTile;
+  const uint32_t tmem = ctl.tmem, q_tile = smem_u32(smem), ring = q_tile + F::kRing;
 
-  // registers: 384 x 168 at launch = 256 x 208 + 128 x 88
-  if (warp >= 8) reg_dec<88>();
-  if (warp == 8) {
+  // registers with D = 128: 384 x 168 at launch = 256 x 208 + 128 x 88
+  if (DP == 128 && warp >= 8) reg_dec<88>();
+  if (warp == F::kLoadWarp) {
     // ---- loads: Q and dO, then K and V tiles in turn
-    TileLoader<DP> loader{&ctl.part, abort};
-    if (loader.load(q_tile, &q_map, &ctl.fixed_full, head, s.q0 + r0, n_rows) &&
-        loader.load(q_tile + F::kTile, &g_map, &ctl.fixed_full, head, s.q0 + r0, n_rows))
-      feed_ring<F::kStages>(2 * n, ctl.full, ctl.empty, abort, [&](int it, int st) {
+    TileLoader<DP> loader(ctl.part, abort);
+    if (loader.template load<kRows>(q_tile, &q_map, &ctl.fixed_full, head, s.q0 + r0, n_rows) &&
+        loader.template load<kRows>(q_tile + F::kFixed, &g_map, &ctl.fixed_full, head, s.q0 + r0, n_rows))
+      feed_ring<F::kStages>(loader, 2 * n, ctl.full, ctl.empty, abort, [&](int it, int st) {
         const int j = it >> 1;
-        return loader.load(ring + st * F::kTile, it & 1 ? &v_map : &k_map, &ctl.full[st], kv_head, s.k0 + j * kRows,
-                           min(kRows, s.lk - j * kRows));
+        return loader.template load<F::kCols>(ring + st * F::kTile, it & 1 ? &v_map : &k_map, &ctl.full[st], kv_head,
+                                              s.k0 + j * F::kCols, s.lk - j * F::kCols);
       });
     mbar_drain(&ctl.fixed_full, 0);
-  } else if (warp >= 10) {
-    // ---- MMAs: warp 10 S, then dQ; warp 11 dP.  S of the next tile goes ahead of dQ of this one.
+  } else if (warp >= F::kMmaWarp) {
+    // ---- MMAs: one warp S, then dQ, the other dP.  S of the next tile goes ahead of dQ of this one.
     if (lane == 0) {
-      const uint32_t idesc_s = idesc_bf16_f32(kRows, kRows, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
+      const uint32_t idesc_s = idesc_bf16_f32(kRows, F::kCols, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
       auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* done) {
         if (!mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort)) return false;
         tc_fence_after();
         const uint32_t ad = desc_k(fixed), bd = desc_k(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) mma_ss(d, ad + step_k(i), bd + step_k(i), idesc_s, i > 0);
+        for (int i = 0; i < DP / 16; ++i) mma_ss(d, ad + step_k<kRows>(i), bd + step_k<F::kCols>(i), idesc_s, i > 0);
         mma_commit(done);
         return true;
       };
       bool ok = mbar_wait(&ctl.fixed_full, 0, abort);
-      if (warp == 10) {
-        if (ok && n > 0) ok = product(0, tmem, q_tile, &ctl.s_full);
+      if (warp == F::kMmaWarp) {
+        if (ok && n > 0) ok = product(0, tmem + C::s, q_tile, &ctl.s_full);
         for (int j = 0; j < n && ok; ++j) {
-          if (j + 1 < n && !(ok = mbar_wait(&ctl.s_read, j & 1, abort) && product(2 * (j + 1), tmem, q_tile, &ctl.s_full))) break;
+          if (j + 1 < n && !(ok = mbar_wait(&ctl.s_read, j & 1, abort) && product(2 * (j + 1), tmem + C::s, q_tile, &ctl.s_full))) break;
           if (!(ok = mbar_wait(&ctl.ds_ready, j & 1, abort))) break;
           tc_fence_after();
-          const uint32_t kd = desc_mn(ring + (2 * j % F::kStages) * F::kTile);
+          const uint32_t kd = desc_mn<F::kCols>(ring + (2 * j % F::kStages) * F::kTile);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            mma_ts(tmem + 256, tmem + 384 + (j & 1) * 64 + i * 8, kd + step_mn(i), idesc_d, j > 0 || i > 0);
+          for (int i = 0; i < F::kCols / 16; ++i)
+            mma_ts(tmem + C::dq, tmem + C::ds + (j & 1) * C::ds_buffer + i * 8, kd + step_mn(i), idesc_d, j > 0 || i > 0);
           mma_commit(&ctl.empty[2 * j % F::kStages]);
         }
         mma_commit(&ctl.dk_done);
       } else {
         for (int j = 0; j < n && ok; ++j) {
           if (j > 0 && !(ok = mbar_wait(&ctl.ds_ready, (j - 1) & 1, abort))) break;
-          ok = product(2 * j + 1, tmem + 128, q_tile + F::kTile, &ctl.dp_full);
+          ok = product(2 * j + 1, tmem + C::dp, q_tile + F::kFixed, &ctl.dp_full);
           if (ok) mma_commit(&ctl.empty[(2 * j + 1) % F::kStages]);
         }
       }
-      mma_commit(&ctl.fin[warp - 10]);
-      mbar_drain(&ctl.fin[warp - 10], 0);
+      mma_commit(&ctl.fin[warp - F::kMmaWarp]);
+      mbar_drain(&ctl.fin[warp - F::kMmaWarp], 0);
     }
-  } else if (warp < 8) {
-    reg_inc<208>();
+  } else if (warp < F::kLoadWarp) {
+    if (DP == 128) reg_inc<208>();
     // ---- softmax arithmetic: thread = query, a warpgroup per half of a tile's keys
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
     const bool valid = row < n_rows;
@@ -180,16 +191,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, con
     const int pos = r + off;
     const int limit = valid && a.causal ? min(s.lk, pos + 1) : s.lk;
     const int64_t stat = (int64_t)head * a.tq + s.q0 + r;
-    // delta = dO . O, half of the columns each.  The rounding of P that is in O weighs
-    // most in short rows: where one tile holds all keys, delta = sum P dP below instead.
+    if (a.table != nullptr) expand_bias_padded(a, head, 1, sbias, threadIdx.x, F::kSoftmax);
+    if (grad)
+      for (int i = threadIdx.x; i < 2 * a.span + 1; i += F::kSoftmax) ssum[i] = 0.f, sbucket[i] = (uint8_t)a.buckets[i];
+    // delta = dO . O, a part of the columns for each warpgroup
     float delta = 0.f;
-    if (valid && n != 1) {
+    if (valid) {
       const int64_t at = ((int64_t)(s.q0 + r) * a.heads + head) * a.dim;
       const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(a.dout.p) + (int64_t)(s.q0 + r) * a.dout.row + head * a.dout.head;
       const __nv_bfloat16* o = static_cast<const __nv_bfloat16*>(a.o) + at;
       const __nv_bfloat16* e = a.o_rest == nullptr ? nullptr : static_cast<const __nv_bfloat16*>(a.o_rest) + at;
 #pragma unroll 4
-      for (int c = half * 8; c < a.dim; c += 16) {
+      for (int c = half * 8; c < a.dim; c += F::kGroups * 8) {
         const uint4 gv = *reinterpret_cast<const uint4*>(g + c), ov = *reinterpret_cast<const uint4*>(o + c);
         const uint4 ev = e == nullptr ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(e + c);
         const uint32_t *gw = &gv.x, *ow = &ov.x, *ew = &ev.x;
@@ -201,28 +214,29 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, con
         }
       }
     }
-    if (n != 1) {
-      sdelta[half * kRows + row] = delta;
-      softmax_sync();
-      delta = sdelta[row] + sdelta[kRows + row];
-      if (valid && half == 0) a.delta[stat] = delta;
-    }
+    sdelta[half * kRows + row] = delta;
+    softmax_sync<DP>();  // the bias table is complete, too
+    if (F::kGroups == 2) delta = sdelta[row] + sdelta[kRows + row];
+    // O carries the rounding of P, which weighs most where a row sees few keys:
+    // rows whose keys all lie in the first tile get delta = sum P dP there.
+    const bool short_rows = (a.causal ? r0 + off + 1 : s.lk) <= F::kCols;
+    if (valid && half == 0 && !(short_rows && n > 0)) a.delta[stat] = delta;
     // a row that sees one key has dS = 0; rows past the sequence likewise
     const float lse = valid && !one_key(a, s, pos) ? a.lse[stat] : CUDART_INF_F;
     const float c2 = a.scale * kLog2e;
     const float* bias = sbias + a.span + kBiasPad;
     float far_sum[2] = {0.f, 0.f};  // dS at distances >= span, <= -span
-    bool ok = true, together = true, owed = n == 1;  // owed: the barrier of delta is still ahead
+    bool ok = true, together = true, owed = F::kGroups == 2 && short_rows && n > 0;  // owed: the barrier of delta is still ahead
     for (int j = 0; j < n; ++j) {
       if (!(ok = mbar_wait_warp(&ctl.s_full, j & 1, abort))) break;
       tc_fence_after();
       float x[64];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) tmem_ld32_issue(lanes + half * 64 + i * 32, x + i * 32);
+      for (int i = 0; i < 2; ++i) tmem_ld32_issue(lanes + C::s + half * 64 + i * 32, x + i * 32);
       tmem_wait_ld(x);
       tc_fence_before();
       mbar_arrive(&ctl.s_read);
-      const int k0 = j * kRows + half * 64;
+      const int k0 = j * F::kCols + half * 64;
       const int dist = pos - k0;
       bool near = false;
       float base = -lse;
@@ -245,23 +259,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, con
       const bool masked = __any_sync(0xffffffffu, limit - k0 < 64);
       if (!(ok = mbar_wait_warp(&ctl.dp_full, j & 1, abort))) break;
       tc_fence_after();
-      float d[64];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) tmem_ld32_issue(lanes + 128 + half * 64 + h * 32, d + h * 32);
-      tmem_wait_ld(d);
       const int seen = limit - k0;
-      if (n == 1) {
+      if (short_rows && j == 0) {
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 64; ++i) sum[i & 3] += i < seen ? x[i] * d[i] : 0.f;
-        sdelta[half * kRows + row] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (!(together = softmax_sync())) break;
-        owed = false;
-        delta = sdelta[row] + sdelta[kRows + row];
+        for (int h = 0; h < 2; ++h) {
+          float d[32];
+          tmem_ld32_issue(lanes + C::dp + half * 64 + h * 32, d);
+          tmem_wait_ld(d);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum[i & 3] += h * 32 + i < seen ? x[h * 32 + i] * d[i] : 0.f;
+        }
+        float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (F::kGroups == 2) {
+          sdelta[half * kRows + row] = all;
+          if (!(together = softmax_sync<DP>())) break;
+          owed = false;
+          all = sdelta[row] + sdelta[kRows + row];
+        }
+        if (limit <= F::kCols) delta = all;
         if (valid && half == 0) a.delta[stat] = delta;
       }
 #pragma unroll
-      for (int i = 0; i < 64; ++i) x[i] *= d[i] - delta;
+      for (int h = 0; h < 2; ++h) {
+        float d[32];
+        tmem_ld32_issue(lanes + C::dp + half * 64 + h * 32, d);
+        tmem_wait_ld(d);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[h * 32 + i] *= d[i] - delta;
+      }
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 64; ++i) x[i] = i < seen ? x[i] : 0.f;
@@ -269,14 +295,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, con
       uint32_t w[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-      tmem_st32(lanes + 384 + (j & 1) * 64 + half * 32, w);
+      tmem_st32(lanes + C::ds + (j & 1) * C::ds_buffer + half * 32, w);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&ctl.ds_ready);
       if (!grad) continue;
       // ---- the bias gradient.  A tile farther than the span from all its keys adds to one bucket.
-      const int d0 = r0 + off - j * kRows;  // distance of the tile's first query and key
-      if (d0 - (kRows - 1) >= a.span || d0 + kRows - 1 <= -a.span) {
+      const int d0 = r0 + off - j * F::kCols;  // distance of the tile's first query and key
+      if (d0 - (F::kCols - 1) >= a.span || d0 + kRows - 1 <= -a.span) {
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 64; ++i) sum[i & 3] += x[i];
@@ -285,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, con
         // A partial sum moves along its diagonal, one lane up for each column; lane 31's is complete.
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float* out = sdiag + ((warp & 3) * 4 + half * 2 + h) * 64;  // index row - column + 31
+          float* out = sdiag + ((warp & 3) * (F::kCols / 32) + half * 2 + h) * kDiag;  // index row - column + 31
           float acc = 0.f;
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
@@ -298,33 +324,32 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, con
           }
           if (lane < 31) out[lane] = acc;
         }
-        if (!(together = softmax_sync())) break;
-        // thread i takes the tile's diagonal row - column = i - 127 over the 4 x 4 blocks, in order
-        const int i = threadIdx.x - (kRows - 1);
-        if (threadIdx.x < 2 * kRows - 1) {
+        if (!(together = softmax_sync<DP>())) break;
+        // a thread takes the diagonal row - column = i of the tile over its blocks, in order; no other thread has it
+        for (int at = threadIdx.x; at < kRows + F::kCols - 1; at += F::kSoftmax) {
+          const int i = at - (F::kCols - 1), dd = d0 + i;
           float sum = 0.f;
 #pragma unroll
-          for (int b = 0; b < 16; ++b) {
-            const int e = i - ((b >> 2) - (b & 3)) * 32 + 31;
-            if (e >= 0 && e < 63) sum += sdiag[b * 64 + e];
+          for (int b = 0; b < 4 * (F::kCols / 32); ++b) {
+            const int e = i - (b / (F::kCols / 32) - b % (F::kCols / 32)) * 32 + 31;
+            if (e >= 0 && e < 63) sum += sdiag[b * kDiag + e];
           }
-          const int dd = d0 + i;
           if (dd >= a.span)
             far_sum[0] += sum;
           else if (dd <= -a.span)
             far_sum[1] += sum;
           else
-            ssum[dd + a.span] += sum;  // this thread's alone
+            ssum[dd + a.span] += sum;
         }
-        if (!(together = softmax_sync())) break;
+        if (!(together = softmax_sync<DP>())) break;
       }
     }
     if (ok && together && n > 0) ok = mbar_wait_warp(&ctl.dk_done, 0, abort);
-    if ((grad || owed) && together) together = softmax_sync(ok);
+    if ((grad || owed) && together) together = softmax_sync<DP>(ok);
     if (ok && together) {
       tc_fence_after();
       if (half == 0)
-        store_row<DP>(lanes + 256, static_cast<__nv_bfloat16*>(a.dq) + ((int64_t)(s.q0 + r) * a.heads + head) * a.dim, a.dim,
+        store_row<DP>(lanes + C::dq, static_cast<__nv_bfloat16*>(a.dq) + ((int64_t)(s.q0 + r) * a.heads + head) * a.dim, a.dim,
                       a.scale, n == 0, valid);
       if (grad) {
 #pragma unroll
@@ -333,16 +358,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, con
           for (int o = 16; o > 0; o >>= 1) far_sum[f] += __shfl_xor_sync(0xffffffffu, far_sum[f], o);
           if (lane == 0) sdiag[f * 8 + warp] = far_sum[f];
         }
-        softmax_sync();
+        softmax_sync<DP>();
         if (threadIdx.x < 2) {
           float sum = 0.f;
-          for (int w = 0; w < 8; ++w) sum += sdiag[threadIdx.x * 8 + w];
+          for (int w = 0; w < F::kLoadWarp; ++w) sum += sdiag[threadIdx.x * 8 + w];
           ssum[threadIdx.x == 0 ? 2 * a.span : 0] += sum;
         }
-        softmax_sync();
+        softmax_sync<DP>();
         // a warp per bucket in turn
         float* out = a.dtable_part + ((int64_t)blockIdx.x * a.heads + head) * a.n_buckets;
-        for (int b = warp; b < a.n_buckets; b += 8) {
+        for (int b = warp; b < a.n_buckets; b += F::kLoadWarp) {
           float sum = 0.f;
           for (int e = lane; e < 2 * a.span + 1; e += 32)
             if (sbucket[e] == b) sum += ssum[e];
@@ -355,28 +380,29 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dq_tc(const Args a, con
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 11) {
+  if (warp == F::kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, F::kTmem);
   }
 }
 
 // ---- dK, dV -----------------------------------------------------------------------
-// Tensor memory: S^T at 0, dP^T at 128, dV and dK from 256.  With DP = 64 P^T
-// and dS^T have columns of their own; with DP = 128 they lie in their scores'
-// columns, and the next scores wait for the product that reads them.
+// Tensor memory: S^T, dP^T, dV, dK.  P^T and dS^T lie in their scores' columns,
+// and the next scores wait for the product that reads them.
 template <int DP>
 struct KvCols {
-  static constexpr uint32_t dv = 256, dk = 256 + DP;
-  static constexpr uint32_t p = DP == 64 ? 384 : 0, ds = DP == 64 ? 448 : 128;
-  static constexpr uint32_t half = DP == 64 ? 32 : 64;  // second warpgroup's columns
-  __device__ static constexpr uint32_t step(int i) { return (i >> 2) * half + (i & 3) * 8; }
+  static constexpr uint32_t s = 0, dp = Bwd<DP>::kCols, dv = 2 * Bwd<DP>::kCols, dk = dv + DP;
+  // k-step i of 16 columns: a warpgroup's 64 scores become 32 columns at their start
+  __device__ static constexpr uint32_t step(int i) { return (i >> 2) * 64 + (i & 3) * 8; }
 };
 
-__host__ __device__ constexpr int dkdv_floats(bool bias, int span) { return 8 * 2 * kRows + (bias ? bias_floats(span) : 0); }
+template <int DP>
+__host__ __device__ constexpr int dkdv_floats(bool bias, int span) {
+  return Bwd<DP>::kStages * 2 * Bwd<DP>::kCols + (bias ? bias_floats(span) : 0);
+}
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a, const __grid_constant__ CUtensorMap q_map,
+__global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_dkdv_tc(const Args a, const __grid_constant__ CUtensorMap q_map,
                                                                  const __grid_constant__ CUtensorMap g_map,
                                                                  const __grid_constant__ CUtensorMap k_map,
                                                                  const __grid_constant__ CUtensorMap v_map) {
@@ -385,60 +411,59 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a, c
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sstat = reinterpret_cast<float*>(smem + (2 + F::kStages) * F::kTile);  // lse, delta of each stage in the ring
-  float* sbias = sstat + 8 * 2 * kRows;
+  float* sstat = reinterpret_cast<float*>(smem + F::kFloats);  // lse, delta of each stage in the ring
+  float* sbias = sstat + F::kStages * 2 * F::kCols;
   volatile int* abort = &ctl.abort;
 
-  const int2 tile = a.tiles[blockIdx.x];
-  const Seq s = load_seq(a, tile.x);
+  int tile;
+  const Seq s = load_tile(a, blockIdx.x, &tile);
   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
-  const int r0 = tile.y * kRows, off = s.lk - s.lq, n_rows = min(kRows, s.lk - r0);
-  const int first = a.causal ? max(0, r0 - off) / kRows : 0;  // earlier query tiles see none of these keys
-  const int per_head = max(0, (s.lq + kRows - 1) / kRows - first), n = group * per_head;
+  const int r0 = tile * kRows, off = s.lk - s.lq, n_rows = min(kRows, s.lk - r0);
+  const int first = a.causal ? max(0, r0 - off) / F::kCols : 0;  // earlier query tiles see none of these keys
+  const int per_head = max(0, (s.lq + F::kCols - 1) / F::kCols - first), n = group * per_head;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, 2);
-  if (warp == 11) {
-    tmem_alloc(&ctl.tmem, 512);
+  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, 2, F::kSoftmax);
+  if (warp == F::kMmaWarp) {
+    tmem_alloc(&ctl.tmem, F::kTmem);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl.tmem, k_tile = smem_u32(smem), ring = k_tile + 2 * F::kTile;
+  const uint32_t tmem = ctl.tmem, k_tile = smem_u32(smem), ring = k_tile + F::kRing;
 
-  if (warp >= 8) reg_dec<88>();
-  if (warp == 8) {
+  if (DP == 128 && warp >= 8) reg_dec<88>();
+  if (warp == F::kLoadWarp) {
     // ---- loads: K and V, then Q (with lse and delta) and dO tiles in turn
-    TileLoader<DP> loader{&ctl.part, abort};
-    if (loader.load(k_tile, &k_map, &ctl.fixed_full, kv_head, s.k0 + r0, n_rows) &&
-        loader.load(k_tile + F::kTile, &v_map, &ctl.fixed_full, kv_head, s.k0 + r0, n_rows))
-      feed_ring<F::kStages>(2 * n, ctl.full, ctl.empty, abort, [&](int it, int st) {
-        const int i = it >> 1, head = kv_head * group + i / per_head, q0 = (first + i % per_head) * kRows;
-        const int n_q = min(kRows, s.lq - q0);
+    TileLoader<DP> loader(ctl.part, abort);
+    if (loader.template load<kRows>(k_tile, &k_map, &ctl.fixed_full, kv_head, s.k0 + r0, n_rows) &&
+        loader.template load<kRows>(k_tile + F::kFixed, &v_map, &ctl.fixed_full, kv_head, s.k0 + r0, n_rows))
+      feed_ring<F::kStages>(loader, 2 * n, ctl.full, ctl.empty, abort, [&](int it, int st) {
+        const int i = it >> 1, head = kv_head * group + i / per_head, q0 = (first + i % per_head) * F::kCols;
+        const int n_q = min(F::kCols, s.lq - q0);
         if (!(it & 1)) {
           const int64_t stat = (int64_t)head * a.tq + s.q0 + q0;
-          for (int c = lane; c < 2 * kRows; c += 32) {
-            const int col = c & (kRows - 1);
+          for (int c = lane; c < 2 * F::kCols; c += 32) {
+            const int col = c & (F::kCols - 1);
             const bool in = col < n_q;
-            const float* f = (c < kRows ? a.lse : a.delta) + stat + (in ? col : 0);
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sstat + st * 2 * kRows + c)), "l"(f),
+            const float* f = (c < F::kCols ? a.lse : a.delta) + stat + (in ? col : 0);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sstat + st * 2 * F::kCols + c)), "l"(f),
                          "r"(in ? 4 : 0)
                          : "memory");
           }
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl.stat_full[st])) : "memory");
         }
-        return loader.load(ring + st * F::kTile, it & 1 ? &g_map : &q_map, &ctl.full[st], head, s.q0 + q0, n_q);
+        return loader.template load<F::kCols>(ring + st * F::kTile, it & 1 ? &g_map : &q_map, &ctl.full[st], head, s.q0 + q0, n_q);
       });
     cp_async_wait<0>();
     mbar_drain(&ctl.fixed_full, 0);
-  } else if (warp >= 10) {
-    // ---- MMAs: warp 10 S^T and dV, warp 11 dP^T and dK
+  } else if (warp >= F::kMmaWarp) {
+    // ---- MMAs: one warp S^T and dV, the other dP^T and dK
     if (lane == 0) {
-      const uint32_t idesc_s = idesc_bf16_f32(kRows, kRows, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
-      const int w = warp - 10;  // the product takes item 2 i + w, the sum item 2 i + 1 - w
-      const uint32_t d = tmem + w * 128, fixed = desc_k(k_tile + w * F::kTile), acc = tmem + (w == 0 ? C::dv : C::dk),
-                     p = tmem + (w == 0 ? C::p : C::ds);
+      const uint32_t idesc_s = idesc_bf16_f32(kRows, F::kCols, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
+      const int w = warp - F::kMmaWarp;  // the product takes item 2 i + w, the sum item 2 i + 1 - w
+      const uint32_t d = tmem + (w == 0 ? C::s : C::dp), fixed = desc_k(k_tile + w * F::kFixed), acc = tmem + (w == 0 ? C::dv : C::dk);
       uint64_t *made = w == 0 ? &ctl.s_full : &ctl.dp_full, *ready = w == 0 ? &ctl.p_ready : &ctl.ds_ready,
                *done = w == 0 ? &ctl.dv_done : &ctl.dk_done;
       auto full = [&](int it) { return mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort); };
@@ -447,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a, c
         tc_fence_after();
         const uint32_t bd = desc_k(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) mma_ss(d, fixed + step_k(i), bd + step_k(i), idesc_s, i > 0);
+        for (int i = 0; i < DP / 16; ++i) mma_ss(d, fixed + step_k<kRows>(i), bd + step_k<F::kCols>(i), idesc_s, i > 0);
         mma_commit(made);
         mma_commit(&ctl.empty[it % F::kStages]);
         return true;
@@ -457,19 +482,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a, c
         const int it = 2 * i + 1 - w;
         if (!(ok = mbar_wait(ready, i & 1, abort) && full(it))) break;
         tc_fence_after();
-        const uint32_t bd = desc_mn(ring + (it % F::kStages) * F::kTile);
+        const uint32_t bd = desc_mn<F::kCols>(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) mma_ts(acc, p + C::step(c), bd + step_mn(c), idesc_d, i > 0 || c > 0);
+        for (int c = 0; c < F::kCols / 16; ++c) mma_ts(acc, d + C::step(c), bd + step_mn(c), idesc_d, i > 0 || c > 0);
         mma_commit(done);
         mma_commit(&ctl.empty[it % F::kStages]);
-        // DP = 128: the next scores take the columns this sum reads
-        if (i + 1 < n) ok = (DP == 64 || mbar_wait(done, i & 1, abort)) && product(2 * (i + 1) + w);
+        // the next scores take the columns this sum reads
+        if (i + 1 < n) ok = mbar_wait(done, i & 1, abort) && product(2 * (i + 1) + w);
       }
       mma_commit(&ctl.fin[w]);
       mbar_drain(&ctl.fin[w], 0);
     }
-  } else if (warp < 8) {
-    reg_inc<208>();
+  } else if (warp < F::kLoadWarp) {
+    if (DP == 128) reg_inc<208>();
     // ---- softmax arithmetic: thread = key, a warpgroup per half of a tile's queries
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, key = r0 + row;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -477,21 +502,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a, c
     const float* bias = sbias + a.span + kBiasPad;
     bool ok = true, together = true;
     for (int i = 0; i < n; ++i) {
-      const int st = 2 * i % F::kStages, q0 = (first + i % per_head) * kRows + half * 64;
+      const int st = 2 * i % F::kStages, q0 = (first + i % per_head) * F::kCols + half * 64;
       if (a.table != nullptr && i % per_head == 0) {  // another head's table
-        if (!(together = softmax_sync())) break;
-        expand_bias_padded(a, kv_head * group + i / per_head, 1, sbias, threadIdx.x, kSoftmax);
-        if (!(together = softmax_sync())) break;
+        if (!(together = softmax_sync<DP>())) break;
+        expand_bias_padded(a, kv_head * group + i / per_head, 1, sbias, threadIdx.x, F::kSoftmax);
+        if (!(together = softmax_sync<DP>())) break;
       }
       ok = mbar_wait_warp(&ctl.stat_full[st], (2 * i / F::kStages) & 1, abort) && mbar_wait_warp(&ctl.s_full, i & 1, abort);
       if (!ok) break;
       tc_fence_after();
       float x[64];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) tmem_ld32_issue(lanes + half * 64 + h * 32, x + h * 32);
+      for (int h = 0; h < 2; ++h) tmem_ld32_issue(lanes + C::s + half * 64 + h * 32, x + h * 32);
       tmem_wait_ld(x);
-      const float4* lse = reinterpret_cast<const float4*>(sstat + st * 2 * kRows + half * 64);
-      const float4* delta = lse + kRows / 4;
+      const float4* lse = reinterpret_cast<const float4*>(sstat + st * 2 * F::kCols + half * 64);
+      const float4* delta = lse + F::kCols / 4;
       const int dist = q0 + off - key;  // of the first column
       float mul = c2, add = 0.f;
       if (a.table != nullptr) {
@@ -522,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a, c
       uint32_t w[32];
 #pragma unroll
       for (int c = 0; c < 32; ++c) w[c] = pack_bf16x2(x[2 * c], x[2 * c + 1]);
-      tmem_st32(lanes + C::p + half * C::half, w);
+      tmem_st32(lanes + C::s + half * 64, w);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&ctl.p_ready);
@@ -532,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a, c
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float d[32];
-        tmem_ld32_issue(lanes + 128 + half * 64 + h * 32, d);
+        tmem_ld32_issue(lanes + C::dp + half * 64 + h * 32, d);
         tmem_wait_ld(d);
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
@@ -550,30 +575,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_dkdv_tc(const Args a, c
       }
 #pragma unroll
       for (int c = 0; c < 32; ++c) w[c] = pack_bf16x2(x[2 * c], x[2 * c + 1]);
-      tmem_st32(lanes + C::ds + half * C::half, w);
+      tmem_st32(lanes + C::dp + half * 64, w);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&ctl.ds_ready);
     }
-    if (ok && together && n > 0) ok = mbar_wait_warp(half == 0 ? &ctl.dv_done : &ctl.dk_done, (n - 1) & 1, abort);
-    if (a.table != nullptr && together) together = softmax_sync(ok);
+    if (ok && together && n > 0)
+      ok = mbar_wait_warp(&ctl.dv_done, (n - 1) & 1, abort) && mbar_wait_warp(&ctl.dk_done, (n - 1) & 1, abort);
+    if (a.table != nullptr && together) together = softmax_sync<DP>(ok);
     if (ok && together) {
       tc_fence_after();
       const int64_t at = ((int64_t)(s.k0 + key) * a.kv_heads + kv_head) * a.dim;
-      store_row<DP>(lanes + (half == 0 ? C::dv : C::dk), static_cast<__nv_bfloat16*>(half == 0 ? a.dv : a.dk) + at, a.dim,
-                    half == 0 ? 1.f : a.scale, n == 0, row < n_rows);
+      if (half == 0)
+        store_row<DP>(lanes + C::dv, static_cast<__nv_bfloat16*>(a.dv) + at, a.dim, 1.f, n == 0, row < n_rows);
+      if (half == F::kGroups - 1)
+        store_row<DP>(lanes + C::dk, static_cast<__nv_bfloat16*>(a.dk) + at, a.dim, a.scale, n == 0, row < n_rows);
     }
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 11) {
+  if (warp == F::kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, F::kTmem);
   }
 }
 
 template <int DP>
-int launch(const Args& a0, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+int launch(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) {
   Args a = a0;
   const bool bias = a.table != nullptr;
   // a side without rows has no tiles, but the map of its tensor must be valid
@@ -587,16 +615,16 @@ int launch(const Args& a0, const int2* k_tiles, int n_q, int n_k, cudaStream_t s
   if (int rc = map(&k_map, a.k, a.tk, a.kv_heads)) return rc;
   if (int rc = map(&v_map, a.v, a.tk, a.kv_heads)) return rc;
   if (n_q > 0) {
-    const size_t smem = Bwd<DP>::kFloats + dq_floats(bias, a.dtable_part != nullptr, a.span) * sizeof(float);
+    const size_t smem = 1024 + Bwd<DP>::kFloats + dq_floats<DP>(bias, a.dtable_part != nullptr, a.span) * sizeof(float);
     KF_CUDA_RET(cudaFuncSetAttribute(attention_dq_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attention_dq_tc<DP><<<dim3(n_q, a.heads), kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
+    attention_dq_tc<DP><<<dim3(n_q, a.heads), Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     if (int rc = check_launch("kf_attention_bwd")) return rc;
   }
   if (n_k > 0) {
     a.tiles = k_tiles;
-    const size_t smem = Bwd<DP>::kFloats + dkdv_floats(bias, a.span) * sizeof(float);
+    const size_t smem = 1024 + Bwd<DP>::kFloats + dkdv_floats<DP>(bias, a.span) * sizeof(float);
     KF_CUDA_RET(cudaFuncSetAttribute(attention_dkdv_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attention_dkdv_tc<DP><<<dim3(n_k, a.kv_heads), kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
+    attention_dkdv_tc<DP><<<dim3(n_k, a.kv_heads), Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     return check_launch("kf_attention_bwd");
   }
   return KF_OK;
@@ -605,7 +633,7 @@ int launch(const Args& a0, const int2* k_tiles, int n_q, int n_k, cudaStream_t s
 }  // namespace
 
 namespace attn {
-int bwd_bf16(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+int bwd_bf16(const Args& a, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) {
   if (n_q == 0 && n_k == 0) return KF_OK;
   return a.dim <= 64 ? launch<64>(a, k_tiles, n_q, n_k, st) : launch<128>(a, k_tiles, n_q, n_k, st);
 }

@@ -27,7 +27,7 @@ constexpr int kLdP = kTile + 4;
 // A tile of up to 64 rows into shared memory as float32; rows past `n` and
 // columns past `dim` are zero, so nothing outside the sequence enters a sum.
 template <typename T, int D>
-__device__ __forceinline__ void load_tile(float* dst, const Strided& s, int64_t row0, int n, int head, int dim) {
+__device__ __forceinline__ void load_rows(float* dst, const Strided& s, int64_t row0, int n, int head, int dim) {
   const T* p = static_cast<const T*>(s.p) + head * s.head;
   for (int i = threadIdx.x; i < kTile * D; i += kThreads) {
     const int r = i / D, c = i % D;
@@ -116,12 +116,12 @@ __global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
   float* sv = sk + kTile * Ld<D>::row;
   float* sp = sv + kTile * Ld<D>::row;
   float* sbias = sp + kTile * kLdP;
-  const int2 tile = a.tiles[blockIdx.x];
-  const Seq s = load_seq(a, tile.x);
+  int tile;
+  const Seq s = load_tile(a, blockIdx.x, &tile);
   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-  const int r0 = tile.y * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
+  const int r0 = tile * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  load_tile<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
+  load_rows<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
   if (a.table != nullptr) expand_bias(a, head, sbias, threadIdx.x, kThreads);
   float m[4], l[4], o[4][D / 16];
 #pragma unroll
@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
   for (int k0 = 0; k0 < k_end; k0 += kTile) {
     const int n_keys = min(kTile, s.lk - k0);
     __syncthreads();
-    load_tile<T, D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
-    load_tile<T, D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_rows<T, D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_rows<T, D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
     __syncthreads();
     float t[4][4] = {};
     dot_rows<D>(sq, sk, ty, tx, t);
@@ -209,13 +209,13 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
   float* sp = sv + kTile * Ld<D>::row;
   float* sbias = sp + kTile * kLdP;
   float* ssum = sbias + 2 * a.span + 1;  // gradient sums by clamped distance
-  const int2 tile = a.tiles[blockIdx.x];
-  const Seq s = load_seq(a, tile.x);
+  int tile;
+  const Seq s = load_tile(a, blockIdx.x, &tile);
   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-  const int r0 = tile.y * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
+  const int r0 = tile * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  load_tile<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
-  load_tile<T, D>(sg, a.dout, s.q0 + r0, n_rows, head, a.dim);
+  load_rows<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
+  load_rows<T, D>(sg, a.dout, s.q0 + r0, n_rows, head, a.dim);
   if (a.table != nullptr) {
     expand_bias(a, head, sbias, threadIdx.x, kThreads);
     for (int i = threadIdx.x; i < 2 * a.span + 1; i += kThreads) ssum[i] = 0.f;
@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
   for (int k0 = 0; k0 < k_end; k0 += kTile) {
     const int n_keys = min(kTile, s.lk - k0);
     __syncthreads();
-    load_tile<T, D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
-    load_tile<T, D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_rows<T, D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_rows<T, D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
     __syncthreads();
     float t[4][4] = {}, dp[4][4] = {};
     dot_rows<D>(sq, sk, ty, tx, t);
@@ -302,13 +302,13 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
   float* slse = sds + kTile * kLdP;
   float* sdelta = slse + kTile;
   float* sbias = sdelta + kTile;
-  const int2 tile = a.tiles[blockIdx.x];
-  const Seq s = load_seq(a, tile.x);
+  int tile;
+  const Seq s = load_tile(a, blockIdx.x, &tile);
   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
-  const int r0 = tile.y * kTile, n_rows = min(kTile, s.lk - r0), off = s.lk - s.lq;
+  const int r0 = tile * kTile, n_rows = min(kTile, s.lk - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  load_tile<T, D>(sk, a.k, s.k0 + r0, n_rows, kv_head, a.dim);
-  load_tile<T, D>(sv, a.v, s.k0 + r0, n_rows, kv_head, a.dim);
+  load_rows<T, D>(sk, a.k, s.k0 + r0, n_rows, kv_head, a.dim);
+  load_rows<T, D>(sv, a.v, s.k0 + r0, n_rows, kv_head, a.dim);
   float dk[4][D / 16], dv[4][D / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -322,8 +322,8 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
     for (int q0 = q_first; q0 < s.lq; q0 += kTile) {
       const int n_q = min(kTile, s.lq - q0);
       __syncthreads();
-      load_tile<T, D>(sq, a.q, s.q0 + q0, n_q, head, a.dim);
-      load_tile<T, D>(sg, a.dout, s.q0 + q0, n_q, head, a.dim);
+      load_rows<T, D>(sq, a.q, s.q0 + q0, n_q, head, a.dim);
+      load_rows<T, D>(sg, a.dout, s.q0 + q0, n_q, head, a.dim);
       if (threadIdx.x < kTile) {
         const bool in = (int)threadIdx.x < n_q;
         slse[threadIdx.x] = in ? a.lse[head * a.tq + s.q0 + q0 + threadIdx.x] : 0.f;
@@ -371,7 +371,7 @@ int fwd(const Args& a, int n_tiles, cudaStream_t st) {
 }
 
 template <typename T, int D>
-int bwd(const Args& a0, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+int bwd(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) {
   Args a = a0;
   const size_t bias = a.table != nullptr ? 2 * a.span + 1 : 0;
   if (a.tq > 0) {
@@ -394,7 +394,7 @@ namespace attn {
 int fwd_f32(const Args& a, int n_tiles, cudaStream_t st) {
   return a.dim <= 64 ? fwd<float, 64>(a, n_tiles, st) : fwd<float, 128>(a, n_tiles, st);
 }
-int bwd_f32(const Args& a, const int2* k_tiles, int n_q, int n_k, cudaStream_t st) {
+int bwd_f32(const Args& a, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) {
   return a.dim <= 64 ? bwd<float, 64>(a, k_tiles, n_q, n_k, st) : bwd<float, 128>(a, k_tiles, n_q, n_k, st);
 }
 }  // namespace attn

@@ -1,8 +1,8 @@
 // Attention forward over packed sequences for bf16, on the tensor cores.
 //
-// A CTA owns 256 rows of one sequence and key head as two MMA tiles of 128.
+// A CTA owns one (D <= 64) or two row tiles of 128 of one sequence and key head.
 // Rows are (query, head) pairs: the heads that share a key head are neighbouring
-// rows, so each K and V tile serves all of them.  Per 64 keys (half a tile):
+// rows, so each K and V tile serves all of them.  Per 64 keys:
 //   S = Q K^T into tensor memory; a softmax thread owns one row (a TMEM lane),
 //   reads its 64 scores, keeps the running maximum and sum in registers and
 //   writes P = 2^(t - m) back to tensor memory as bf16; O += P V with P as the
@@ -11,11 +11,13 @@
 // either sign); the sum that divides O is the float32 one.  The maximum in use
 // moves only when a row's true one is more than 8 above it (2^8 times the sum
 // in float32 and bf16 loses nothing), so O is rarely rescaled.
-// Four half tiles are in flight, two per row tile, each with scores of its own:
-// the chain S -> softmax -> P V -> next S of one half runs under the softmax of
-// the other, and under the other row tile.  Tensor memory has no room for more.
-// Warps 0-7 softmax (one warpgroup a row tile), 8 loads, 10 and 11 issue the
-// MMAs of one row tile each.
+// Two scores of 64 keys are in flight for each row tile: the chain S -> softmax
+// -> P V -> next S of one runs under the softmax of the other.  An SM holds two
+// row tiles, all that tensor memory has room for: with D = 128 as one CTA, which
+// reads K and V once for both; with D <= 64, where the exponentials and not the
+// loads bound the loop, as two CTAs, so that one starts and ends under the other.
+// Warps: softmax (four a row tile), one that loads, one a row tile that issues
+// MMAs.
 #include "attention_tc.cuh"
 
 namespace kf {
@@ -23,122 +25,119 @@ namespace {
 
 using namespace attn;
 
-constexpr int kThreads = 384, kHalf = kRows / 2;
 constexpr float kLazy = 8.f;
+constexpr int kKeys = 64;  // of a streamed tile
 
 template <int DP>
 struct Fwd {
-  static constexpr int kStages = DP == 64 ? 6 : 4;  // K and V tiles in flight
-  static constexpr int kTile = tile_bytes<DP>();
-  static constexpr int kSmem = 1024 + (2 + kStages) * kTile;  // + bias tables
-  // tensor memory columns; with DP = 64 there is room for P beside S, with 128 it takes the columns of its scores
-  __device__ static constexpr uint32_t s(int t, int h) { return t * kRows + h * kHalf; }
-  __device__ static constexpr uint32_t o(int t) { return 256 + t * DP; }
-  __device__ static constexpr uint32_t p(int t, int h) { return DP == 64 ? 384 + t * 64 + h * 32 : s(t, h); }
+  static constexpr int NT = DP == 64 ? 1 : 2;          // row tiles
+  static constexpr int kStages = DP == 64 ? 10 : 8;    // K and V tiles in flight
+  static constexpr int kTile = tile_bytes<DP>(kKeys), kQTile = tile_bytes<DP>(kRows);
+  static constexpr int kSmem = 1024 + NT * kQTile + kStages * kTile;  // + bias tables
+  static constexpr int kSoftmax = NT * 128, kLoadWarp = NT * 4, kMmaWarp = DP == 64 ? 5 : 10;
+  static constexpr int kThreads = DP == 64 ? 192 : 384;
+  static constexpr uint32_t kCols = DP == 64 ? 256 : 512;
+  // tensor memory columns; with D <= 64 there is room for P beside S, with 128 it takes the columns of its scores
+  __device__ static constexpr uint32_t s(int t, int h) { return t * 128 + h * kKeys; }
+  __device__ static constexpr uint32_t o(int t) { return NT * 128 + t * DP; }
+  __device__ static constexpr uint32_t p(int t, int h) { return DP == 64 ? 192 + h * 32 : s(t, h); }
 };
 
 struct Ctl {
-  uint64_t q_full, part, kv_full[8], kv_empty[8], s_full[2][2], p_ready[2][2], pv_done[2], o_done[2];
+  uint64_t q_full, part[2], kv_full[10], kv_empty[10], s_full[2][2], p_ready[2][2], pv_done[2], o_done[2];
   uint32_t tmem;
   int abort;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a, const __grid_constant__ CUtensorMap k_map,
-                                                                const __grid_constant__ CUtensorMap v_map) {
+__global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
+    attention_fwd_tc(const Args a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using F = Fwd<DP>;
+  constexpr int NT = F::NT;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sbias = reinterpret_cast<float*>(smem + (2 + F::kStages) * F::kTile);
+  float* sbias = reinterpret_cast<float*>(smem + NT * F::kQTile + F::kStages * F::kTile);
   volatile int* abort = &ctl.abort;
 
-  const int2 tile = a.tiles[blockIdx.x];
-  const Seq s = load_seq(a, tile.x);
+  int tile;
+  const Seq s = load_tile(a, blockIdx.x, &tile);
   const int pack = a.pack, head0 = blockIdx.y * pack, kv_head = head0 / (a.heads / a.kv_heads);
-  const int r0 = tile.y * 2 * kRows, off = s.lk - s.lq, total = s.lq * pack;
-  // key tiles of each of the two row tiles
-  int n_rows[2], n_kv[2];
+  const int r0 = tile * NT * kRows, off = s.lk - s.lq, total = s.lq * pack;
+  // key tiles of each row tile
+  int n_rows[NT], n_kv[NT], n_max = 0;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < NT; ++t) {
     n_rows[t] = min(kRows, max(0, total - r0 - t * kRows));
     const int last = (r0 + t * kRows + n_rows[t] - 1) / pack;  // its last query
     const int keys = n_rows[t] == 0 ? 0 : a.causal ? min(s.lk, last + off + 1) : s.lk;
-    n_kv[t] = max(0, (keys + kRows - 1) / kRows);
+    n_kv[t] = max(0, (keys + kKeys - 1) / kKeys);
+    n_max = max(n_max, n_kv[t]);
   }
-  const int n_max = max(n_kv[0], n_kv[1]);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     ctl.abort = 0;
-    mbar_init(&ctl.q_full, 2 * kRows);
-    mbar_init(&ctl.part, 1);
-    for (int i = 0; i < F::kStages; ++i) mbar_init(&ctl.kv_full[i], 1), mbar_init(&ctl.kv_empty[i], 2);
-    for (int t = 0; t < 2; ++t) {
+    mbar_init(&ctl.q_full, F::kSoftmax);
+    mbar_init(&ctl.part[0], 1), mbar_init(&ctl.part[1], 1);
+    for (int i = 0; i < F::kStages; ++i) mbar_init(&ctl.kv_full[i], 1), mbar_init(&ctl.kv_empty[i], NT);
+    for (int t = 0; t < NT; ++t) {
       mbar_init(&ctl.pv_done[t], 1), mbar_init(&ctl.o_done[t], 1);
       for (int h = 0; h < 2; ++h) mbar_init(&ctl.s_full[t][h], 1), mbar_init(&ctl.p_ready[t][h], kRows);
     }
     fence_barrier_init();
   }
-  if (warp == 11) {
-    tmem_alloc(&ctl.tmem, 512);
+  if (warp == F::kMmaWarp) {
+    tmem_alloc(&ctl.tmem, F::kCols);
     tmem_relinquish();
   }
-  if (a.table != nullptr) expand_bias_padded(a, head0, pack, sbias, threadIdx.x, kThreads);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl.tmem, q_tile = smem_u32(smem), kv_tile = q_tile + 2 * F::kTile;
+  const uint32_t tmem = ctl.tmem, q_tile = smem_u32(smem), kv_tile = q_tile + NT * F::kQTile;
 
-  // registers: 384 x 168 at launch = 256 x 208 + 128 x 88
-  if (warp >= 8) reg_dec<88>();
-  if (warp == 8) {
+  // registers with D = 128: 384 x 168 at launch = 256 x 208 + 128 x 88
+  if (NT == 2 && warp >= F::kLoadWarp) reg_dec<88>();
+  if (warp == F::kLoadWarp) {
     // ---- loads: K and V tiles in turn
-    TileLoader<DP> loader{&ctl.part, abort};
-    feed_ring<F::kStages>(2 * n_max, ctl.kv_full, ctl.kv_empty, abort, [&](int it, int st) {
+    TileLoader<DP> loader(ctl.part, abort);
+    feed_ring<F::kStages>(loader, 2 * n_max, ctl.kv_full, ctl.kv_empty, abort, [&](int it, int st) {
       const int j = it >> 1;
-      return loader.load(kv_tile + st * F::kTile, it & 1 ? &v_map : &k_map, &ctl.kv_full[st], kv_head, s.k0 + j * kRows,
-                         min(kRows, s.lk - j * kRows));
+      return loader.template load<kKeys>(kv_tile + st * F::kTile, it & 1 ? &v_map : &k_map, &ctl.kv_full[st], kv_head,
+                                         s.k0 + j * kKeys, s.lk - j * kKeys);
     });
-  } else if (warp >= 10) {
+  } else if (warp >= F::kMmaWarp) {
     // ---- MMAs of row tile t
     if (lane == 0 && n_max > 0) {
-      const int t = warp - 10, n = n_kv[t];
-      const uint32_t idesc_s = idesc_bf16_f32(kRows, kHalf, false, false), idesc_o = idesc_bf16_f32(kRows, DP, false, true);
-      const uint32_t qd = desc_k(q_tile + t * F::kTile);
+      const int t = warp - F::kMmaWarp, n = NT == 1 ? n_max : n_kv[t];
+      const uint32_t idesc_s = idesc_bf16_f32(kRows, kKeys, false, false), idesc_o = idesc_bf16_f32(kRows, DP, false, true);
+      const uint32_t qd = desc_k(q_tile + t * F::kQTile);
       auto full = [&](int it) { return mbar_wait(&ctl.kv_full[it % F::kStages], (it / F::kStages) & 1, abort); };
-      auto scores = [&](int j, int h) {
-        const uint32_t kd = desc_k(kv_tile + (2 * j % F::kStages) * F::kTile) + h * (kHalf * 128 >> 4);
+      auto scores = [&](int j) {
+        if (!full(2 * j)) return false;
+        tc_fence_after();
+        const uint32_t kd = desc_k(kv_tile + (2 * j % F::kStages) * F::kTile);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) mma_ss(tmem + F::s(t, h), qd + step_k(i), kd + step_k(i), idesc_s, i > 0);
-        mma_commit(&ctl.s_full[t][h]);
-        if (h == 1) mma_commit(&ctl.kv_empty[2 * j % F::kStages]);
+        for (int i = 0; i < DP / 16; ++i)
+          mma_ss(tmem + F::s(t, j & 1), qd + step_k<kRows>(i), kd + step_k<kKeys>(i), idesc_s, i > 0);
+        mma_commit(&ctl.s_full[t][j & 1]);
+        mma_commit(&ctl.kv_empty[2 * j % F::kStages]);
+        return true;
       };
       bool ok = mbar_wait(&ctl.q_full, 0, abort);
-      if (ok && n > 0 && (ok = full(0))) {
-        tc_fence_after();
-        scores(0, 0);
-        scores(0, 1);
-      }
+      for (int j = 0; j < min(n, 2) && ok; ++j) ok = scores(j);
       for (int j = 0; j < n && ok; ++j) {
+        const int it = 2 * j + 1, h = j & 1;
+        if (!(ok = mbar_wait(&ctl.p_ready[t][h], (j >> 1) & 1, abort) && full(it))) break;
+        tc_fence_after();
+        const uint32_t vd = desc_mn<kKeys>(kv_tile + (it % F::kStages) * F::kTile);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int it = 2 * j + 1;
-          if (!(ok = mbar_wait(&ctl.p_ready[t][h], j & 1, abort) && (h == 1 || full(it)))) break;
-          tc_fence_after();
-          const uint32_t vd = desc_mn(kv_tile + (it % F::kStages) * F::kTile);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mma_ts(tmem + F::o(t), tmem + F::p(t, h) + i * 8, vd + step_mn(h * 4 + i), idesc_o, j > 0 || h > 0 || i > 0);
-          mma_commit(&ctl.pv_done[t]);
-          if (h == 1) mma_commit(&ctl.kv_empty[it % F::kStages]);
-          if (j + 1 < n) {
-            // DP = 128: the next scores take P's columns, so P V has to be done
-            if (!(ok = (h == 1 || full(it + 1)) && (DP == 64 || mbar_wait(&ctl.pv_done[t], h, abort)))) break;
-            tc_fence_after();
-            scores(j + 1, h);
-          }
-        }
+        for (int i = 0; i < kKeys / 16; ++i)
+          mma_ts(tmem + F::o(t), tmem + F::p(t, h) + i * 8, vd + step_mn(i), idesc_o, j > 0 || i > 0);
+        mma_commit(&ctl.pv_done[t]);
+        mma_commit(&ctl.kv_empty[it % F::kStages]);
+        // D = 128: the next scores take P's columns, so P V has to be done
+        if (j + 2 < n) ok = (DP == 64 || mbar_wait(&ctl.pv_done[t], h, abort)) && scores(j + 2);
       }
       mma_commit(&ctl.o_done[t]);
       // tiles that only the other row tile uses
@@ -146,55 +145,58 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a, co
         if ((ok = full(it))) mbar_arrive(&ctl.kv_empty[it % F::kStages]);
       mbar_drain(&ctl.o_done[t], 0);
     }
-  } else if (warp < 8) {
-    reg_inc<208>();
+  } else if (warp < NT * 4) {
+    if (NT == 2) reg_inc<208>();
     // ---- softmax: thread = row
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
-    const int r = r0 + t * kRows + row, n = n_kv[t];
-    const bool valid = row < n_rows[t];
+    const int r = r0 + t * kRows + row, n = NT == 1 ? n_max : n_kv[t], rows = NT == 1 ? n_rows[0] : n_rows[t];
+    const bool valid = row < rows;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const int tok = r / pack, pos = tok + off;
     const int limit = valid && a.causal ? min(s.lk, pos + 1) : s.lk;  // keys this row sees
     const float c2 = a.scale * kLog2e;
-    const float* bias = sbias + (a.table != nullptr ? (r - tok * pack) * bias_floats(a.span) + a.span + kBiasPad : 0);
-    float m = -CUDART_INF_F, l = 0.f;
-    bool ok = true;
-    load_tile_async<DP, kRows>(q_tile + t * F::kTile, static_cast<const __nv_bfloat16*>(a.q.p) + (int64_t)s.q0 * a.q.row + head0 * a.q.head,
-                               a.q.row, a.q.head, pack, r0 + t * kRows, n_rows[t], a.dim, row);
+    load_tile_async<DP, kRows>(q_tile + t * F::kQTile,
+                               static_cast<const __nv_bfloat16*>(a.q.p) + (int64_t)s.q0 * a.q.row + head0 * a.q.head, a.q.row,
+                               a.q.head, pack, r0 + t * kRows, rows, a.dim, row);
     cp_async_commit();
+    if (a.table != nullptr) expand_bias_padded(a, head0, pack, sbias, threadIdx.x, F::kSoftmax);
     cp_async_wait<0>();
     fence_proxy_async_smem();
     mbar_arrive(&ctl.q_full);
-    for (int i = 0; i < 2 * n; ++i) {
-      const int j = i >> 1, h = i & 1;
-      if (!(ok = mbar_wait_warp(&ctl.s_full[t][h], j & 1, abort))) break;
+    if (a.table != nullptr) named_bar_and(1, F::kSoftmax, true);
+    const float* bias = sbias + (a.table != nullptr ? (r - tok * pack) * bias_floats(a.span) + a.span + kBiasPad : 0);
+    float m = -CUDART_INF_F, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int h = j & 1;
+      if (!(ok = mbar_wait_warp(&ctl.s_full[t][h], (j >> 1) & 1, abort))) break;
       tc_fence_after();
-      float x[kHalf];
+      float x[kKeys];
 #pragma unroll
       for (int c = 0; c < 2; ++c) tmem_ld32_issue(lanes + F::s(t, h) + c * 32, x + c * 32);
       tmem_wait_ld(x);
-      const int k0 = j * kRows + h * kHalf;
+      const int k0 = j * kKeys;
       float mul = c2, add = 0.f;
       if (a.table != nullptr) {
         const int dist = pos - k0;  // to the first of the keys
-        const bool far = dist - (kHalf - 1) >= a.span || dist <= -a.span;
+        const bool far = dist - (kKeys - 1) >= a.span || dist <= -a.span;
         if (__all_sync(0xffffffffu, far)) {
           add = dist > 0 ? bias[a.span] : bias[-a.span];
         } else {
-          const float* b = bias + max(-a.span - kBiasPad + kHalf - 1, min(dist, a.span + kBiasPad));
+          const float* b = bias + max(-a.span - kBiasPad + kKeys - 1, min(dist, a.span + kBiasPad));
 #pragma unroll
-          for (int c = 0; c < kHalf; ++c) x[c] = fmaf(x[c], c2, b[-c]);
+          for (int c = 0; c < kKeys; ++c) x[c] = fmaf(x[c], c2, b[-c]);
           mul = 1.f;
         }
       }
-      if (__any_sync(0xffffffffu, limit - k0 < kHalf)) {
+      if (__any_sync(0xffffffffu, limit - k0 < kKeys)) {
         const int seen = limit - k0;
 #pragma unroll
-        for (int c = 0; c < kHalf; ++c) x[c] = c < seen ? x[c] : -CUDART_INF_F;
+        for (int c = 0; c < kKeys; ++c) x[c] = c < seen ? x[c] : -CUDART_INF_F;
       }
       float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int c = 4; c < kHalf; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
+      for (int c = 4; c < kKeys; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
       const float high = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mul, add);
       if (__any_sync(0xffffffffu, high > m + kLazy)) {
         // some row's maximum moves: its sum and, once the last P V is done, its output follow
@@ -202,8 +204,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a, co
         const float fix = m == -CUDART_INF_F ? 0.f : ex2(m - m_new);
         m = m_new;
         l *= fix;
-        if (i > 0) {
-          if (!(ok = mbar_wait_warp(&ctl.pv_done[t], (i - 1) & 1, abort))) break;
+        if (j > 0) {
+          if (!(ok = mbar_wait_warp(&ctl.pv_done[t], (j - 1) & 1, abort))) break;
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < DP / 32; ++c) {
@@ -218,9 +220,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a, co
       }
       const float base = add - (m == -CUDART_INF_F ? 0.f : m);  // a row without a visible key yet: 2^-inf = 0
       float sum[2] = {0.f, 0.f};
-      uint32_t p[kHalf / 2];
+      uint32_t p[kKeys / 2];
 #pragma unroll
-      for (int c = 0; c < kHalf / 2; ++c) {
+      for (int c = 0; c < kKeys / 2; ++c) {
         const float e0 = ex2(fmaf(x[2 * c], mul, base)), e1 = ex2(fmaf(x[2 * c + 1], mul, base));
         sum[0] += e0;
         sum[1] += e1;
@@ -273,9 +275,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_fwd_tc(const Args a, co
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 11) {
+  if (warp == F::kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, F::kCols);
   }
 }
 
@@ -287,7 +289,7 @@ int launch(const Args& a, int n_tiles, cudaStream_t st) {
   const bool keys = a.tk > 0;  // without keys no tile is loaded
   if (int rc = make_tile_map(&k_map, keys ? a.k.p : a.q.p, keys ? a.tk : 1, keys ? a.kv_heads : 1, a.dim, a.k.row, a.k.head)) return rc;
   if (int rc = make_tile_map(&v_map, keys ? a.v.p : a.q.p, keys ? a.tk : 1, keys ? a.kv_heads : 1, a.dim, a.v.row, a.v.head)) return rc;
-  attention_fwd_tc<DP><<<dim3(n_tiles, a.heads / a.pack), kThreads, smem, st>>>(a, k_map, v_map);
+  attention_fwd_tc<DP><<<dim3(n_tiles, a.heads / a.pack), Fwd<DP>::kThreads, smem, st>>>(a, k_map, v_map);
   return check_launch("kf_attention_fwd");
 }
 

@@ -11,13 +11,13 @@ namespace attn {
 
 using namespace umma;
 
-constexpr int kRows = 128;             // rows of an MMA tile, and keys or queries of a streamed tile
-constexpr int kPanel = kRows * 128;    // bytes of 128 rows x 64 bf16
+constexpr int kRows = 128;             // rows of an MMA tile
+constexpr int kBoxRows = 64;           // rows of a TMA box
 constexpr int kBiasPad = 160;          // distances a tile may lie past the span where it still reads the table
-constexpr int kBiasBytes = 32 * 1024;  // shared memory for bias tables
 
+// bytes of `rows` x DP bf16, stored as panels of 64 columns
 template <int DP>
-constexpr int tile_bytes() { return kPanel * (DP / 64); }
+__host__ __device__ constexpr int tile_bytes(int rows) { return rows * 128 * (DP / 64); }
 
 __host__ __device__ constexpr int bias_floats(int span) { return 2 * span + 1 + 2 * kBiasPad; }
 
@@ -140,11 +140,23 @@ __device__ __forceinline__ void load_tile_async(uint32_t dst, const __nv_bfloat1
         src += (int64_t)tok * row_stride + (int64_t)(r - tok * pack) * head_stride + ch * 8;
       }
     }
-    cp_async16(dst + (ch >> 3) * kPanel + sw128_offset(row, ch & 7), src, ok ? 16 : 0);
+    cp_async16(dst + (ch >> 3) * (kRows * 128) + sw128_offset(row, ch & 7), src, ok ? 16 : 0);
   }
 }
 
-// 3-D tiled load (column, head, row) of 64 columns x 128 rows of one head.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// 3-D tiled load (column, head, row) of 64 columns x 64 rows of one head.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
@@ -156,60 +168,89 @@ __device__ __forceinline__ void st_zero16(uint32_t dst) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
 }
 
-// One warp's loads of 128-row tiles by TMA.  Rows past the sequence belong to
-// its neighbour in the packed tensor: a tile that has such rows lands on a
+// One warp's loads of tiles of ROWS rows by TMA.  Rows past the sequence belong
+// to its neighbour in the packed tensor: a tile that has such rows lands on a
 // barrier of the warp's own and is signalled once they are overwritten by
-// zeros, so that nothing outside a sequence enters an MMA.
+// zeros, so that nothing outside a sequence enters an MMA.  That last step of a
+// tile is left until the next tile is on its way.
 template <int DP>
 struct TileLoader {
-  uint64_t* part;  // count 1
+  uint64_t* part;  // two barriers, count 1
   volatile int* abort;
-  uint32_t parity = 0;
+  int used = 0;           // partial tiles so far
+  bool pending = false;   // one of them is not signalled yet:
+  uint32_t p_dst = 0;
+  int p_rows = 0, p_n = 0;
+  uint64_t* p_full = nullptr;
 
-  // The n first rows of the tile at `row` of head `head`; one arrival on `full` when it is there.
-  __device__ __forceinline__ bool load(uint32_t dst, const CUtensorMap* map, uint64_t* full, int head, int row, int n) {
+  __device__ __forceinline__ TileLoader(uint64_t* part_, volatile int* abort_) : part(part_), abort(abort_) {}
+
+  __device__ __forceinline__ bool finish() {
+    if (!pending) return true;
+    pending = false;
     const int lane = threadIdx.x & 31;
-    uint64_t* bar = n < kRows ? part : full;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(bar, tile_bytes<DP>());
-#pragma unroll
-      for (int p = 0; p < DP / 64; ++p) tma_load_3d(dst + p * kPanel, map, bar, p * 64, head, row);
-    }
-    if (n >= kRows) return true;
-    const bool ok = mbar_wait_warp(part, parity, abort);
-    if (!ok) mbar_drain(part, parity);
-    parity ^= 1;
+    uint64_t* bar = part + ((used - 1) & 1);
+    const uint32_t parity = ((used - 1) >> 1) & 1;
+    const bool ok = mbar_wait_warp(bar, parity, abort);
+    if (!ok) mbar_drain(bar, parity);
 #pragma unroll
     for (int p = 0; p < DP / 64; ++p)
-      for (int i = lane; i < (kRows - n) * 8; i += 32) st_zero16(dst + p * kPanel + n * 128 + i * 16);
+      for (int i = lane; i < (p_rows - p_n) * 8; i += 32) st_zero16(p_dst + p * p_rows * 128 + p_n * 128 + i * 16);
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(full);
+    if (lane == 0) mbar_arrive(p_full);
+    return ok;
+  }
+
+  // The n (at least 1) first rows of the tile at `row` of head `head`; one arrival on `full` when it is there.
+  template <int ROWS>
+  __device__ __forceinline__ bool load(uint32_t dst, const CUtensorMap* map, uint64_t* full, int head, int row, int n) {
+    n = min(n, ROWS);
+    const bool partial = n < ROWS;
+    uint64_t* bar = partial ? part + (used & 1) : full;
+    if ((threadIdx.x & 31) == 0) {
+      const int boxes = (n + kBoxRows - 1) / kBoxRows;
+      mbar_arrive_expect_tx(bar, boxes * kBoxRows * 128 * (DP / 64));
+#pragma unroll
+      for (int p = 0; p < DP / 64; ++p)
+        for (int b = 0; b < boxes; ++b)
+          tma_load_3d(dst + p * ROWS * 128 + b * kBoxRows * 128, map, bar, p * 64, head, row + b * kBoxRows);
+    }
+    bool ok = true;
+    if (pending) ok = finish();  // the tile before: of the other barrier, if this one is partial too
+    if (partial) ++used, pending = true, p_dst = dst, p_rows = ROWS, p_n = n, p_full = full;
     return ok;
   }
 };
 
 // A ring of STAGES tiles: tile it goes to stage it % STAGES once that is free.
 // load(it, stage) starts one; after an abort the loads in flight are waited for.
-template <int STAGES, typename Load>
-__device__ __forceinline__ void feed_ring(int n_items, uint64_t* full, uint64_t* empty, volatile int* abort, Load&& load) {
+template <int STAGES, int DP, typename Load>
+__device__ __forceinline__ void feed_ring(TileLoader<DP>& loader, int n_items, uint64_t* full, uint64_t* empty, volatile int* abort,
+                                          Load&& load) {
   int it = 0;
   for (; it < n_items; ++it) {
-    if (!mbar_wait_warp(empty + it % STAGES, ((it / STAGES) & 1) ^ 1, abort)) break;
+    const uint32_t parity = ((it / STAGES) & 1) ^ 1;
+    if (!__all_sync(0xffffffffu, mbar_test(empty + it % STAGES, parity))) {
+      if (!loader.finish() || !mbar_wait_warp(empty + it % STAGES, parity, abort)) break;
+    }
     if (!load(it, it % STAGES)) break;
   }
+  loader.finish();
   if (*abort)
     for (int i = max(0, it - STAGES); i < it; ++i) mbar_drain(full + i % STAGES, (i / STAGES) & 1);
 }
 
-// Low words.  K-major operand (rows x DP, contraction over DP): k-step j of 16 columns.
+// Low words of operands of ROWS rows.  K-major (contraction over DP): k-step j of 16 columns.
 __device__ __forceinline__ uint32_t desc_k(uint32_t tile) { return ((tile >> 4) & 0x3FFFu) | (1u << 16); }
-__host__ __device__ constexpr uint32_t step_k(int j) { return ((j >> 2) * kPanel + (j & 3) * 32) >> 4; }
-// MN-major operand (contraction over its 128 rows, panels of 64 columns): k-step j of 16 rows.
-__device__ __forceinline__ uint32_t desc_mn(uint32_t tile) { return ((tile >> 4) & 0x3FFFu) | ((uint32_t)(kPanel >> 4) << 16); }
+template <int ROWS>
+__host__ __device__ constexpr uint32_t step_k(int j) { return ((j >> 2) * ROWS * 128 + (j & 3) * 32) >> 4; }
+// MN-major (contraction over the rows, panels of 64 columns): k-step j of 16 rows.
+template <int ROWS>
+__device__ __forceinline__ uint32_t desc_mn(uint32_t tile) { return ((tile >> 4) & 0x3FFFu) | ((uint32_t)(ROWS * 128 >> 4) << 16); }
 __host__ __device__ constexpr uint32_t step_mn(int j) { return j * (2048 >> 4); }
 
-// Map of a (tokens, heads, dim) bf16 tensor, boxes of 64 columns x 1 head x 128 rows.
+// Map of a (tokens, heads, dim) bf16 tensor, boxes of 64 columns x 1 head x 64 rows.
 int make_tile_map(CUtensorMap* map, const void* p, int64_t rows, int heads, int dim, int64_t row_stride, int64_t head_stride);
 
 // ---- softmax arithmetic ---------------------------------------------------------

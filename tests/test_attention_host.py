@@ -87,10 +87,10 @@ def test_entry_points_check_their_arguments_before_any_cuda_call():
 
     lib = _lib.load()
     d = _lib.AttentionDesc(heads=4, kv_heads=3, dim=64)
-    assert lib.kf_attention_fwd(*[None] * 5, 1, *[None] * 5, ctypes.byref(d), None) == 1
+    assert lib.kf_attention_fwd(*[None] * 4, 1, *[None] * 5, ctypes.byref(d), None) == 1
     assert "do not divide" in _lib.last_error()
     d = _lib.AttentionDesc(heads=4, kv_heads=2, dim=65)
-    assert lib.kf_attention_fwd(*[None] * 5, 1, *[None] * 5, ctypes.byref(d), None) == 1
+    assert lib.kf_attention_fwd(*[None] * 4, 1, *[None] * 5, ctypes.byref(d), None) == 1
     d = _lib.DecodeDesc(heads=4, kv_heads=2, dim=64, batch=1, capacity=8)
     assert lib.kf_attention_decode(*[None] * 7, ctypes.byref(d), None) == 1
     d = _lib.ResidualNormDesc(width=9000)
