@@ -30,12 +30,17 @@ struct Bwd {
   static constexpr int kRing = 2 * kFixed, kFloats = kRing + kStages * kTile;  // byte offsets behind the fixed tiles
   static constexpr int kGroups = kCols / 64, kSoftmax = kGroups * 128;
   static constexpr int kLoadWarp = kGroups * 4, kMmaWarp = DP == 64 ? 5 : 10;
-  static constexpr int kThreads = DP == 64 ? 224 : 384, kCtas = DP == 64 ? 2 : 1;
+  static constexpr int kThreads = DP == 64 ? 256 : 384, kCtas = DP == 64 ? 2 : 1;
+  // registers: 256 x 128 at launch = 128 x 192 + 128 x 64; 384 x 168 = 256 x 208 + 128 x 88
+  static constexpr int kSoftmaxRegs = DP == 64 ? 192 : 208, kOtherRegs = DP == 64 ? 64 : 88;
   static constexpr uint32_t kTmem = DP == 64 ? 256 : 512;
 };
 
+// Every barrier alternates between two phases, so a waiter must not fall two
+// behind: dS has a barrier for odd and one for even tiles, since in dQ the scores
+// of the next tile are made before dS of this one is waited for.
 struct Ctl {
-  uint64_t fixed_full, part[2], full[8], empty[8], stat_full[8], s_full, dp_full, s_read, p_ready, ds_ready, dv_done, dk_done, fin[2];
+  uint64_t fixed_full, part[2], full[8], empty[8], stat_full[8], s_full, dp_full, s_read, p_ready, ds_ready[2], dv_done, dk_done, fin[2];
   uint32_t tmem;
   int abort;
 };
@@ -47,7 +52,7 @@ __device__ __forceinline__ void init_barriers(Ctl* c, int stages, int users, int
   mbar_init(&c->part[0], 1), mbar_init(&c->part[1], 1);
   for (int i = 0; i < stages; ++i) mbar_init(&c->full[i], 1), mbar_init(&c->empty[i], users), mbar_init(&c->stat_full[i], 32);
   mbar_init(&c->s_full, 1), mbar_init(&c->dp_full, 1), mbar_init(&c->dv_done, 1), mbar_init(&c->dk_done, 1);
-  mbar_init(&c->s_read, softmax), mbar_init(&c->p_ready, softmax), mbar_init(&c->ds_ready, softmax);
+  mbar_init(&c->s_read, softmax), mbar_init(&c->p_ready, softmax), mbar_init(&c->ds_ready[0], softmax), mbar_init(&c->ds_ready[1], softmax);
   mbar_init(&c->fin[0], 1), mbar_init(&c->fin[1], 1);
   fence_barrier_init();
 }
@@ -132,8 +137,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   tc_fence_after();
   const uint32_t tmem = ctl.tmem, q_tile = smem_u32(smem), ring = q_tile + F::kRing;
 
-  // registers with D = 128: 384 x 168 at launch = 256 x 208 + 128 x 88
-  if (DP == 128 && warp >= 8) reg_dec<88>();
+  if (warp >= F::kLoadWarp) reg_dec<F::kOtherRegs>();
   if (warp == F::kLoadWarp) {
     // ---- loads: Q and dO, then K and V tiles in turn
     TileLoader<DP> loader(ctl.part, abort);
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
                                               s.k0 + j * F::kCols, s.lk - j * F::kCols);
       });
     mbar_drain(&ctl.fixed_full, 0);
-  } else if (warp >= F::kMmaWarp) {
+  } else if (warp >= F::kMmaWarp && warp < F::kMmaWarp + 2) {
     // ---- MMAs: one warp S, then dQ, the other dP.  S of the next tile goes ahead of dQ of this one.
     if (lane == 0) {
       const uint32_t idesc_s = idesc_bf16_f32(kRows, F::kCols, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
@@ -163,7 +167,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         if (ok && n > 0) ok = product(0, tmem + C::s, q_tile, &ctl.s_full);
         for (int j = 0; j < n && ok; ++j) {
           if (j + 1 < n && !(ok = mbar_wait(&ctl.s_read, j & 1, abort) && product(2 * (j + 1), tmem + C::s, q_tile, &ctl.s_full))) break;
-          if (!(ok = mbar_wait(&ctl.ds_ready, j & 1, abort))) break;
+          if (!(ok = mbar_wait(&ctl.ds_ready[j & 1], (j >> 1) & 1, abort))) break;
           tc_fence_after();
           const uint32_t kd = desc_mn<F::kCols>(ring + (2 * j % F::kStages) * F::kTile);
 #pragma unroll
@@ -174,7 +178,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         mma_commit(&ctl.dk_done);
       } else {
         for (int j = 0; j < n && ok; ++j) {
-          if (j > 0 && !(ok = mbar_wait(&ctl.ds_ready, (j - 1) & 1, abort))) break;
+          if (j > 0 && !(ok = mbar_wait(&ctl.ds_ready[(j - 1) & 1], ((j - 1) >> 1) & 1, abort))) break;
           ok = product(2 * j + 1, tmem + C::dp, q_tile + F::kFixed, &ctl.dp_full);
           if (ok) mma_commit(&ctl.empty[(2 * j + 1) % F::kStages]);
         }
@@ -183,7 +187,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       mbar_drain(&ctl.fin[warp - F::kMmaWarp], 0);
     }
   } else if (warp < F::kLoadWarp) {
-    if (DP == 128) reg_inc<208>();
+    reg_inc<F::kSoftmaxRegs>();
     // ---- softmax arithmetic: thread = query, a warpgroup per half of a tile's keys
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
     const bool valid = row < n_rows;
@@ -298,7 +302,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       tmem_st32(lanes + C::ds + (j & 1) * C::ds_buffer + half * 32, w);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&ctl.ds_ready);
+      mbar_arrive(&ctl.ds_ready[j & 1]);
       if (!grad) continue;
       // ---- the bias gradient.  A tile farther than the span from all its keys adds to one bucket.
       const int d0 = r0 + off - j * F::kCols;  // distance of the tile's first query and key
@@ -433,7 +437,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   tc_fence_after();
   const uint32_t tmem = ctl.tmem, k_tile = smem_u32(smem), ring = k_tile + F::kRing;
 
-  if (DP == 128 && warp >= 8) reg_dec<88>();
+  if (warp >= F::kLoadWarp) reg_dec<F::kOtherRegs>();
   if (warp == F::kLoadWarp) {
     // ---- loads: K and V, then Q (with lse and delta) and dO tiles in turn
     TileLoader<DP> loader(ctl.part, abort);
@@ -458,13 +462,13 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       });
     cp_async_wait<0>();
     mbar_drain(&ctl.fixed_full, 0);
-  } else if (warp >= F::kMmaWarp) {
+  } else if (warp >= F::kMmaWarp && warp < F::kMmaWarp + 2) {
     // ---- MMAs: one warp S^T and dV, the other dP^T and dK
     if (lane == 0) {
       const uint32_t idesc_s = idesc_bf16_f32(kRows, F::kCols, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
       const int w = warp - F::kMmaWarp;  // the product takes item 2 i + w, the sum item 2 i + 1 - w
       const uint32_t d = tmem + (w == 0 ? C::s : C::dp), fixed = desc_k(k_tile + w * F::kFixed), acc = tmem + (w == 0 ? C::dv : C::dk);
-      uint64_t *made = w == 0 ? &ctl.s_full : &ctl.dp_full, *ready = w == 0 ? &ctl.p_ready : &ctl.ds_ready,
+      uint64_t *made = w == 0 ? &ctl.s_full : &ctl.dp_full, *ready = w == 0 ? &ctl.p_ready : &ctl.ds_ready[0],
                *done = w == 0 ? &ctl.dv_done : &ctl.dk_done;
       auto full = [&](int it) { return mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort); };
       auto product = [&](int it) {
@@ -494,7 +498,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       mbar_drain(&ctl.fin[w], 0);
     }
   } else if (warp < F::kLoadWarp) {
-    if (DP == 128) reg_inc<208>();
+    reg_inc<F::kSoftmaxRegs>();
     // ---- softmax arithmetic: thread = key, a warpgroup per half of a tile's queries
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, key = r0 + row;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -578,7 +582,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       tmem_st32(lanes + C::dp + half * 64, w);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&ctl.ds_ready);
+      mbar_arrive(&ctl.ds_ready[0]);
     }
     if (ok && together && n > 0)
       ok = mbar_wait_warp(&ctl.dv_done, (n - 1) & 1, abort) && mbar_wait_warp(&ctl.dk_done, (n - 1) & 1, abort);

@@ -16,8 +16,9 @@
 // row tiles, all that tensor memory has room for: with D = 128 as one CTA, which
 // reads K and V once for both; with D <= 64, where the exponentials and not the
 // loads bound the loop, as two CTAs, so that one starts and ends under the other.
-// Warps: softmax (four a row tile), one that loads, one a row tile that issues
-// MMAs.
+// Warps: softmax (four a row tile), one that loads, and for each row tile one that
+// issues Q K^T and one that issues P V: issuing blocks while the tensor cores
+// are behind, and neither product should wait for the other's turn.
 #include "attention_tc.cuh"
 
 namespace kf {
@@ -26,16 +27,19 @@ namespace {
 using namespace attn;
 
 constexpr float kLazy = 8.f;
-constexpr int kKeys = 64;  // of a streamed tile
+constexpr int kKeys = 64;  // of one set of scores
 
 template <int DP>
 struct Fwd {
   static constexpr int NT = DP == 64 ? 1 : 2;          // row tiles
-  static constexpr int kStages = DP == 64 ? 10 : 8;    // K and V tiles in flight
-  static constexpr int kTile = tile_bytes<DP>(kKeys), kQTile = tile_bytes<DP>(kRows);
+  static constexpr int kUnit = DP == 64 ? 64 : 128;    // keys of a streamed tile
+  static constexpr int kStages = DP == 64 ? 10 : 4;    // K and V tiles in flight
+  static constexpr int kTile = tile_bytes<DP>(kUnit), kQTile = tile_bytes<DP>(kRows);
   static constexpr int kSmem = 1024 + NT * kQTile + kStages * kTile;  // + bias tables
-  static constexpr int kSoftmax = NT * 128, kLoadWarp = NT * 4, kMmaWarp = DP == 64 ? 5 : 10;
-  static constexpr int kThreads = DP == 64 ? 192 : 384;
+  static constexpr int kSoftmax = NT * 128, kLoadWarp = NT * 4, kMmaWarp = DP == 64 ? 5 : 12;
+  static constexpr int kThreads = DP == 64 ? 256 : 512;
+  // registers: 128 a thread at launch, as many for the softmax and the other half of the warps together
+  static constexpr int kSoftmaxRegs = DP == 64 ? 192 : 200, kOtherRegs = 256 - kSoftmaxRegs;
   static constexpr uint32_t kCols = DP == 64 ? 256 : 512;
   // tensor memory columns; with D <= 64 there is room for P beside S, with 128 it takes the columns of its scores
   __device__ static constexpr uint32_t s(int t, int h) { return t * 128 + h * kKeys; }
@@ -43,8 +47,11 @@ struct Fwd {
   __device__ static constexpr uint32_t p(int t, int h) { return DP == 64 ? 192 + h * 32 : s(t, h); }
 };
 
+// Every barrier alternates between two phases, so a waiter must not fall two
+// behind.  The two sets of a row tile have barriers of their own: set j + 2 is
+// not made before P V of set j is done, hence seen.
 struct Ctl {
-  uint64_t q_full, part[2], kv_full[10], kv_empty[10], s_full[2][2], p_ready[2][2], pv_done[2], o_done[2];
+  uint64_t q_full, part[2], kv_full[10], kv_empty[10], s_full[2][2], p_ready[2][2], pv_done[2][2], o_done[2], fin[4];
   uint32_t tmem;
   int abort;
 };
@@ -82,9 +89,11 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
     mbar_init(&ctl.part[0], 1), mbar_init(&ctl.part[1], 1);
     for (int i = 0; i < F::kStages; ++i) mbar_init(&ctl.kv_full[i], 1), mbar_init(&ctl.kv_empty[i], NT);
     for (int t = 0; t < NT; ++t) {
-      mbar_init(&ctl.pv_done[t], 1), mbar_init(&ctl.o_done[t], 1);
-      for (int h = 0; h < 2; ++h) mbar_init(&ctl.s_full[t][h], 1), mbar_init(&ctl.p_ready[t][h], kRows);
+      mbar_init(&ctl.o_done[t], 1);
+      for (int h = 0; h < 2; ++h)
+        mbar_init(&ctl.s_full[t][h], 1), mbar_init(&ctl.p_ready[t][h], kRows), mbar_init(&ctl.pv_done[t][h], 1);
     }
+    for (int i = 0; i < 2 * NT; ++i) mbar_init(&ctl.fin[i], 1);
     fence_barrier_init();
   }
   if (warp == F::kMmaWarp) {
@@ -94,59 +103,69 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  constexpr int U = F::kUnit / kKeys;
+  auto units = [](int n) { return (n + U - 1) / U; };  // streamed tiles that hold n sets of 64 keys
   const uint32_t tmem = ctl.tmem, q_tile = smem_u32(smem), kv_tile = q_tile + NT * F::kQTile;
 
-  // registers with D = 128: 384 x 168 at launch = 256 x 208 + 128 x 88
-  if (NT == 2 && warp >= F::kLoadWarp) reg_dec<88>();
+  if (warp >= F::kLoadWarp) reg_dec<F::kOtherRegs>();
   if (warp == F::kLoadWarp) {
     // ---- loads: K and V tiles in turn
     TileLoader<DP> loader(ctl.part, abort);
-    feed_ring<F::kStages>(loader, 2 * n_max, ctl.kv_full, ctl.kv_empty, abort, [&](int it, int st) {
+    feed_ring<F::kStages>(loader, 2 * units(n_max), ctl.kv_full, ctl.kv_empty, abort, [&](int it, int st) {
       const int j = it >> 1;
-      return loader.template load<kKeys>(kv_tile + st * F::kTile, it & 1 ? &v_map : &k_map, &ctl.kv_full[st], kv_head,
-                                         s.k0 + j * kKeys, s.lk - j * kKeys);
+      return loader.template load<F::kUnit>(kv_tile + st * F::kTile, it & 1 ? &v_map : &k_map, &ctl.kv_full[st], kv_head,
+                                            s.k0 + j * F::kUnit, s.lk - j * F::kUnit);
     });
-  } else if (warp >= F::kMmaWarp) {
+  } else if (warp >= F::kMmaWarp && warp < F::kMmaWarp + 2 * NT) {
     // ---- MMAs of row tile t
     if (lane == 0 && n_max > 0) {
-      const int t = warp - F::kMmaWarp, n = NT == 1 ? n_max : n_kv[t];
-      const uint32_t idesc_s = idesc_bf16_f32(kRows, kKeys, false, false), idesc_o = idesc_bf16_f32(kRows, DP, false, true);
-      const uint32_t qd = desc_k(q_tile + t * F::kQTile);
+      const int t = (warp - F::kMmaWarp) % NT, n = NT == 1 ? n_max : n_kv[t];
       auto full = [&](int it) { return mbar_wait(&ctl.kv_full[it % F::kStages], (it / F::kStages) & 1, abort); };
-      auto scores = [&](int j) {
-        if (!full(2 * j)) return false;
-        tc_fence_after();
-        const uint32_t kd = desc_k(kv_tile + (2 * j % F::kStages) * F::kTile);
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i)
-          mma_ss(tmem + F::s(t, j & 1), qd + step_k<kRows>(i), kd + step_k<kKeys>(i), idesc_s, i > 0);
-        mma_commit(&ctl.s_full[t][j & 1]);
-        mma_commit(&ctl.kv_empty[2 * j % F::kStages]);
-        return true;
-      };
+      // the last set of scores that uses its streamed tile
+      auto last_of = [&](int j) { return j % U == U - 1 || j == n - 1; };
       bool ok = mbar_wait(&ctl.q_full, 0, abort);
-      for (int j = 0; j < min(n, 2) && ok; ++j) ok = scores(j);
-      for (int j = 0; j < n && ok; ++j) {
-        const int it = 2 * j + 1, h = j & 1;
-        if (!(ok = mbar_wait(&ctl.p_ready[t][h], (j >> 1) & 1, abort) && full(it))) break;
-        tc_fence_after();
-        const uint32_t vd = desc_mn<kKeys>(kv_tile + (it % F::kStages) * F::kTile);
+      int item;  // this warp's first streamed tile that only the other row tile uses
+      if (warp - F::kMmaWarp < NT) {
+        const uint32_t idesc = idesc_bf16_f32(kRows, DP, false, true);
+        for (int j = 0; j < n && ok; ++j) {
+          const int it = 2 * (j / U) + 1, h = j & 1;
+          if (!(ok = (j % U > 0 || full(it)) && mbar_wait(&ctl.p_ready[t][h], (j >> 1) & 1, abort))) break;
+          tc_fence_after();
+          const uint32_t vd = desc_mn<F::kUnit>(kv_tile + (it % F::kStages) * F::kTile) + step_mn(j % U * (kKeys / 16));
 #pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i)
-          mma_ts(tmem + F::o(t), tmem + F::p(t, h) + i * 8, vd + step_mn(i), idesc_o, j > 0 || i > 0);
-        mma_commit(&ctl.pv_done[t]);
-        mma_commit(&ctl.kv_empty[it % F::kStages]);
-        // D = 128: the next scores take P's columns, so P V has to be done
-        if (j + 2 < n) ok = (DP == 64 || mbar_wait(&ctl.pv_done[t], h, abort)) && scores(j + 2);
+          for (int i = 0; i < kKeys / 16; ++i)
+            mma_ts(tmem + F::o(t), tmem + F::p(t, h) + i * 8, vd + step_mn(i), idesc, j > 0 || i > 0);
+          mma_commit(&ctl.pv_done[t][h]);
+          if (last_of(j)) mma_commit(&ctl.kv_empty[it % F::kStages]);
+        }
+        mma_commit(&ctl.o_done[t]);
+        item = 2 * units(n) + 1;
+      } else {
+        const uint32_t idesc = idesc_bf16_f32(kRows, kKeys, false, false), qd = desc_k(q_tile + t * F::kQTile);
+        for (int j = 0; j < n && ok; ++j) {
+          const int it = 2 * (j / U), h = j & 1;
+          if (j % U == 0 && !(ok = full(it))) break;
+          // The scores of two sets before are read.  D = 128: they hold P by now, which P V has to be done with.
+          if (j >= 2 && !(ok = mbar_wait(DP == 64 ? &ctl.p_ready[t][h] : &ctl.pv_done[t][h], ((j >> 1) + 1) & 1, abort))) break;
+          tc_fence_after();
+          const uint32_t kd = desc_k(kv_tile + (it % F::kStages) * F::kTile) + j % U * (kKeys * 128 >> 4);
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i)
+            mma_ss(tmem + F::s(t, h), qd + step_k<kRows>(i), kd + step_k<F::kUnit>(i), idesc, i > 0);
+          if (last_of(j)) mma_commit(&ctl.kv_empty[it % F::kStages]);
+          // D <= 64: the softmax writes P over that of two sets before, once P V is done with it
+          if (DP == 64 && j >= 2 && !(ok = mbar_wait(&ctl.pv_done[t][h], ((j >> 1) + 1) & 1, abort))) break;
+          mma_commit(&ctl.s_full[t][h]);
+        }
+        item = 2 * units(n);
       }
-      mma_commit(&ctl.o_done[t]);
-      // tiles that only the other row tile uses
-      for (int it = 2 * n; it < 2 * n_max && ok; ++it)
-        if ((ok = full(it))) mbar_arrive(&ctl.kv_empty[it % F::kStages]);
-      mbar_drain(&ctl.o_done[t], 0);
+      for (; item < 2 * units(n_max) && ok; item += 2)
+        if ((ok = full(item))) mbar_arrive(&ctl.kv_empty[item % F::kStages]);
+      mma_commit(&ctl.fin[warp - F::kMmaWarp]);
+      mbar_drain(&ctl.fin[warp - F::kMmaWarp], 0);
     }
   } else if (warp < NT * 4) {
-    if (NT == 2) reg_inc<208>();
+    reg_inc<F::kSoftmaxRegs>();
     // ---- softmax: thread = row
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const int r = r0 + t * kRows + row, n = NT == 1 ? n_max : n_kv[t], rows = NT == 1 ? n_rows[0] : n_rows[t];
@@ -196,8 +215,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
       }
       float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int c = 4; c < kKeys; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
-      const float high = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mul, add);
+      for (int c = 4; c + 1 < kKeys; c += 2) top[c / 2 & 3] = max3(top[c / 2 & 3], x[c], x[c + 1]);
+      const float high = fmaf(max3(fmaxf(top[0], top[1]), top[2], top[3]), mul, add);
       if (__any_sync(0xffffffffu, high > m + kLazy)) {
         // some row's maximum moves: its sum and, once the last P V is done, its output follow
         const float m_new = fmaxf(m, high);
@@ -205,7 +224,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
         m = m_new;
         l *= fix;
         if (j > 0) {
-          if (!(ok = mbar_wait_warp(&ctl.pv_done[t], (j - 1) & 1, abort))) break;
+          if (!(ok = mbar_wait_warp(&ctl.pv_done[t][h ^ 1], ((j - 1) >> 1) & 1, abort))) break;
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < DP / 32; ++c) {
@@ -219,17 +238,21 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
         }
       }
       const float base = add - (m == -CUDART_INF_F ? 0.f : m);  // a row without a visible key yet: 2^-inf = 0
-      float sum[2] = {0.f, 0.f};
+      const uint64_t mul_2 = pair(mul, mul), base_2 = pair(base, base);
+      uint64_t sum[2] = {0, 0};  // two pairs of float32 zeros
       uint32_t p[kKeys / 2];
 #pragma unroll
       for (int c = 0; c < kKeys / 2; ++c) {
-        const float e0 = ex2(fmaf(x[2 * c], mul, base)), e1 = ex2(fmaf(x[2 * c + 1], mul, base));
-        sum[0] += e0;
-        sum[1] += e1;
+        float e0, e1;
+        unpair(fma2(pair(x[2 * c], x[2 * c + 1]), mul_2, base_2), e0, e1);
+        e0 = ex2(e0), e1 = ex2(e1);
+        sum[c & 1] = add2(sum[c & 1], pair(e0, e1));
         p[c] = pack_bf16x2(e0, e1);
       }
       tmem_st32(lanes + F::p(t, h), p);
-      l += sum[0] + sum[1];
+      float s0, s1;
+      unpair(add2(sum[0], sum[1]), s0, s1);
+      l += s0 + s1;
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&ctl.p_ready[t][h]);
