@@ -106,7 +106,7 @@ extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, con
   clear_error();
   if (int rc = check_attention("kf_attention_fwd", d)) return rc;
   if (n_q_tiles == 0) return KF_OK;
-  KF_CHECK_ARG(n_q_tiles > 0, "kf_attention_fwd: negative tile count");
+  KF_CHECK_ARG(n_q_tiles > 0 && (int64_t)n_q_tiles * d->heads < (1ll << 31), "kf_attention_fwd: bad tile count");
   KF_CHECK_ARG(q && o && q_tiles && (d->tk == 0 || (k && v)), "kf_attention_fwd: null argument");
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_fwd: the bias needs a table and buckets");
   if (int rc = bind_device(q)) return rc;
@@ -121,7 +121,7 @@ extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, con
 
 extern "C" int64_t kf_attention_bwd_workspace(int32_t n_q_tiles, const kf_attention_desc* d) {
   if (d == nullptr || n_q_tiles < 0) return 0;
-  return (int64_t)d->heads * d->tq + (int64_t)n_q_tiles * d->heads * d->n_buckets;
+  return 2 * (int64_t)d->heads * d->tq + (int64_t)n_q_tiles * d->heads * d->n_buckets;
 }
 
 extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout, const float* lse,
@@ -131,7 +131,8 @@ extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, con
   using namespace kf;
   clear_error();
   if (int rc = check_attention("kf_attention_bwd", d)) return rc;
-  KF_CHECK_ARG(n_q_tiles >= 0 && n_k_tiles >= 0, "kf_attention_bwd: negative tile count");
+  KF_CHECK_ARG(n_q_tiles >= 0 && n_k_tiles >= 0 && (int64_t)std::max(n_q_tiles, n_k_tiles) * d->heads < (1ll << 31),
+               "kf_attention_bwd: bad tile count");
   KF_CHECK_ARG(n_q_tiles == 0 || (q && o && dout && lse && dq && workspace && q_tiles), "kf_attention_bwd: null argument");
   KF_CHECK_ARG(n_k_tiles == 0 || (k && v && dk && dv && k_tiles), "kf_attention_bwd: null argument");
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_bwd: the bias needs a table and buckets");
@@ -143,7 +144,7 @@ extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, con
   a.dq = dq, a.dk = dk, a.dv = dv, a.table = table, a.buckets = buckets;
   a.tiles = reinterpret_cast<const Tile*>(q_tiles);
   a.delta = workspace;
-  a.dtable_part = dtable != nullptr ? workspace + (int64_t)d->heads * d->tq : nullptr;
+  a.dtable_part = dtable != nullptr ? workspace + 2 * (int64_t)d->heads * d->tq : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Tile* kt = reinterpret_cast<const Tile*>(k_tiles);
   int rows;

@@ -40,7 +40,7 @@ struct Args {
   void* o_rest; // bf16: what the rounding of o left out, for delta; may be null
   void *dq, *dk, *dv;
   float* lse;   // (H, Tq)
-  float* delta; // (H, Tq): dO . O
+  float* delta; // (H, Tq): dO . O; bf16: minus that, then (H, Tq) minus lse
   const Tile* tiles;
   const void* table;  // (buckets, H) bias, or null
   const int* buckets; // (2 span + 1): bucket of distance index - span

@@ -3,8 +3,9 @@
 // Two kernels, so that every sum has one order without atomics: both form the
 // scores again, P = 2^(t - lse), and dS = P (dP - delta) with dP = dO V^T.
 //   dQ    rows = 128 queries of a head, walks over key tiles:
-//         S, dP -> dS -> dQ += dS K; first it makes delta = dO . O, which the
-//         second kernel reads, and it sums dS by distance for the bias gradient.
+//         S, dP -> dS -> dQ += dS K; first it makes delta = dO . O, and it sums
+//         dS by distance for the bias gradient.  The second kernel reads -delta
+//         and -lse, which this one leaves in the workspace.
 //   dK dV rows = 128 keys of a key head, walks over the query tiles of all heads
 //         that share it: S^T, dP^T -> P^T, dS^T -> dV += P^T dO, dK += dS^T Q.
 // Seven products of 128 x 128 x D a tile pair against five with one kernel;
@@ -95,10 +96,10 @@ struct QCols {
 };
 
 // Floats behind the tiles: halves of delta, bias table, sums by distance, block diagonals, bucket ids.
-constexpr int kDiag = 64;  // of a block of 32 x 32 scores: 63 diagonals
+constexpr int kDiag = 48;  // of a block of 32 x 16 scores: 47 diagonals
 template <int DP>
 __host__ __device__ constexpr int dq_floats(bool bias, bool grad, int span) {
-  return 2 * kRows + (bias ? bias_floats(span) : 0) + (grad ? 2 * span + 1 + Bwd<DP>::kCols / 8 * kDiag + (2 * span + 4) / 4 : 0);
+  return 2 * kRows + (bias ? bias_floats(span) : 0) + (grad ? 2 * span + 1 + Bwd<DP>::kCols / 4 * kDiag + (2 * span + 4) / 4 : 0);
 }
 
 template <int DP>
@@ -115,12 +116,12 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   float* sbias = sdelta + 2 * kRows;
   float* ssum = sbias + (a.table != nullptr ? bias_floats(a.span) : 0);
   float* sdiag = ssum + 2 * a.span + 1;
-  uint8_t* sbucket = reinterpret_cast<uint8_t*>(sdiag + F::kCols / 8 * kDiag);
+  uint8_t* sbucket = reinterpret_cast<uint8_t*>(sdiag + F::kCols / 4 * kDiag);
   volatile int* abort = &ctl.abort;
 
   int tile;
-  const Seq s = load_tile(a, blockIdx.x, &tile);
-  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+  const Seq s = load_tile(a, blockIdx.x / a.heads, &tile);
+  const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const int r0 = tile * kRows, off = s.lk - s.lq, n_rows = min(kRows, s.lq - r0);
   const int keys = a.causal ? max(0, min(s.lk, r0 + n_rows + off)) : s.lk;
   const int n = (keys + F::kCols - 1) / F::kCols;
@@ -224,9 +225,10 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     // O carries the rounding of P, which weighs most where a row sees few keys:
     // rows whose keys all lie in the first tile get delta = sum P dP there.
     const bool short_rows = (a.causal ? r0 + off + 1 : s.lk) <= F::kCols;
-    if (valid && half == 0 && !(short_rows && n > 0)) a.delta[stat] = delta;
+    if (valid && half == 0 && !(short_rows && n > 0)) a.delta[stat] = -delta;
     // a row that sees one key has dS = 0; rows past the sequence likewise
-    const float lse = valid && !one_key(a, s, pos) ? a.lse[stat] : CUDART_INF_F;
+    const float lse_row = valid ? a.lse[stat] : 0.f, lse = valid && !one_key(a, s, pos) ? lse_row : CUDART_INF_F;
+    if (valid && half == 0) a.delta[(int64_t)a.heads * a.tq + stat] = -lse_row;
     const float c2 = a.scale * kLog2e;
     const float* bias = sbias + a.span + kBiasPad;
     float far_sum[2] = {0.f, 0.f};  // dS at distances >= span, <= -span
@@ -255,8 +257,9 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         }
       }
       if (!near) {
+        const uint64_t c2_2 = pair(c2, c2), base_2 = pair(base, base);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) x[i] = fmaf(x[i], c2, base);
+        for (int i = 0; i < 64; i += 2) unpair(fma2(pair(x[i], x[i + 1]), c2_2, base_2), x[i], x[i + 1]);
       }
 #pragma unroll
       for (int i = 0; i < 64; ++i) x[i] = ex2(x[i]);
@@ -282,15 +285,19 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
           all = sdelta[row] + sdelta[kRows + row];
         }
         if (limit <= F::kCols) delta = all;
-        if (valid && half == 0) a.delta[stat] = delta;
+        if (valid && half == 0) a.delta[stat] = -delta;
       }
+      const uint64_t minus_delta = pair(-delta, -delta);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float d[32];
         tmem_ld32_issue(lanes + C::dp + half * 64 + h * 32, d);
         tmem_wait_ld(d);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[h * 32 + i] *= d[i] - delta;
+        for (int i = 0; i < 32; i += 2) {
+          float *x0 = &x[h * 32 + i], *x1 = x0 + 1;
+          unpair(mul2(pair(*x0, *x1), add2(pair(d[i], d[i + 1]), minus_delta)), *x0, *x1);
+        }
       }
       if (masked) {
 #pragma unroll
@@ -313,20 +320,21 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         far_sum[d0 > 0 ? 0 : 1] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       } else {
         // A partial sum moves along its diagonal, one lane up for each column; lane 31's is complete.
+        // Four blocks of 32 rows x 16 columns at a time, to have four such chains in flight.
+        const float keep = lane == 0 ? 0.f : 1.f;
+        float* out = sdiag + ((warp & 3) * (F::kCols / 16) + half * 4) * kDiag;  // index row - column + 15
+        float acc[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float* out = sdiag + ((warp & 3) * (F::kCols / 32) + half * 2 + h) * kDiag;  // index row - column + 31
-          float acc = 0.f;
+        for (int c = 0; c < 16; ++c) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if (c > 0) {
-              acc = __shfl_up_sync(0xffffffffu, acc, 1);
-              if (lane == 0) acc = 0.f;
-            }
-            acc += x[h * 32 + c];
-            if (lane == 31) out[62 - c] = acc;
+          for (int h = 0; h < 4; ++h) {
+            acc[h] = c == 0 ? x[h * 16] : fmaf(__shfl_up_sync(0xffffffffu, acc[h], 1), keep, x[h * 16 + c]);
+            if (lane == 31) out[h * kDiag + 46 - c] = acc[h];
           }
-          if (lane < 31) out[lane] = acc;
+        }
+        if (lane < 31) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) out[h * kDiag + lane] = acc[h];
         }
         if (!(together = softmax_sync<DP>())) break;
         // a thread takes the diagonal row - column = i of the tile over its blocks, in order; no other thread has it
@@ -334,9 +342,9 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
           const int i = at - (F::kCols - 1), dd = d0 + i;
           float sum = 0.f;
 #pragma unroll
-          for (int b = 0; b < 4 * (F::kCols / 32); ++b) {
-            const int e = i - (b / (F::kCols / 32) - b % (F::kCols / 32)) * 32 + 31;
-            if (e >= 0 && e < 63) sum += sdiag[b * kDiag + e];
+          for (int b = 0; b < F::kCols / 4; ++b) {
+            const int e = i - b / (F::kCols / 16) * 32 + b % (F::kCols / 16) * 16 + 15;
+            if (e >= 0 && e < 47) sum += sdiag[b * kDiag + e];
           }
           if (dd >= a.span)
             far_sum[0] += sum;
@@ -370,7 +378,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         }
         softmax_sync<DP>();
         // a warp per bucket in turn
-        float* out = a.dtable_part + ((int64_t)blockIdx.x * a.heads + head) * a.n_buckets;
+        float* out = a.dtable_part + (int64_t)blockIdx.x * a.n_buckets;
         for (int b = warp; b < a.n_buckets; b += F::kLoadWarp) {
           float sum = 0.f;
           for (int e = lane; e < 2 * a.span + 1; e += 32)
@@ -420,8 +428,8 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   volatile int* abort = &ctl.abort;
 
   int tile;
-  const Seq s = load_tile(a, blockIdx.x, &tile);
-  const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
+  const Seq s = load_tile(a, blockIdx.x / a.kv_heads, &tile);
+  const int kv_head = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
   const int r0 = tile * kRows, off = s.lk - s.lq, n_rows = min(kRows, s.lk - r0);
   const int first = a.causal ? max(0, r0 - off) / F::kCols : 0;  // earlier query tiles see none of these keys
   const int per_head = max(0, (s.lq + F::kCols - 1) / F::kCols - first), n = group * per_head;
@@ -451,7 +459,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
           for (int c = lane; c < 2 * F::kCols; c += 32) {
             const int col = c & (F::kCols - 1);
             const bool in = col < n_q;
-            const float* f = (c < F::kCols ? a.lse : a.delta) + stat + (in ? col : 0);
+            const float* f = a.delta + (c < F::kCols ? (int64_t)a.heads * a.tq : 0) + stat + (in ? col : 0);
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(sstat + st * 2 * F::kCols + c)), "l"(f),
                          "r"(in ? 4 : 0)
                          : "memory");
@@ -519,8 +527,8 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
 #pragma unroll
       for (int h = 0; h < 2; ++h) tmem_ld32_issue(lanes + C::s + half * 64 + h * 32, x + h * 32);
       tmem_wait_ld(x);
-      const float4* lse = reinterpret_cast<const float4*>(sstat + st * 2 * F::kCols + half * 64);
-      const float4* delta = lse + F::kCols / 4;
+      const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(sstat + st * 2 * F::kCols + half * 64);
+      const ulonglong2* delta = lse + F::kCols / 4;
       const int dist = q0 + off - key;  // of the first column
       float mul = c2, add = 0.f;
       if (a.table != nullptr) {
@@ -533,14 +541,15 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
           mul = 1.f;
         }
       }
+      const uint64_t mul_2 = pair(mul, mul), add_2 = pair(add, add);
 #pragma unroll
       for (int c = 0; c < 64; c += 4) {
-        const float4 e = lse[c / 4];
-        x[c] = ex2(fmaf(x[c], mul, add - e.x));
-        x[c + 1] = ex2(fmaf(x[c + 1], mul, add - e.y));
-        x[c + 2] = ex2(fmaf(x[c + 2], mul, add - e.z));
-        x[c + 3] = ex2(fmaf(x[c + 3], mul, add - e.w));
+        const ulonglong2 e = lse[c / 4];  // two pairs of -lse
+        unpair(fma2(pair(x[c], x[c + 1]), mul_2, add2(add_2, e.x)), x[c], x[c + 1]);
+        unpair(fma2(pair(x[c + 2], x[c + 3]), mul_2, add2(add_2, e.y)), x[c + 2], x[c + 3]);
       }
+#pragma unroll
+      for (int c = 0; c < 64; ++c) x[c] = ex2(x[c]);
       // columns of queries that see this key: [from, to)
       const int from = a.causal ? key - off - q0 : 0, to = s.lq - q0;
       const bool masked = __any_sync(0xffffffffu, from > 0 || to < 64 || s.lk == 1 || (a.causal && q0 + off <= 0));
@@ -565,11 +574,10 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         tmem_wait_ld(d);
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-          const float4 e = delta[(h * 32 + c) / 4];
-          x[h * 32 + c] *= d[c] - e.x;
-          x[h * 32 + c + 1] *= d[c + 1] - e.y;
-          x[h * 32 + c + 2] *= d[c + 2] - e.z;
-          x[h * 32 + c + 3] *= d[c + 3] - e.w;
+          const ulonglong2 e = delta[(h * 32 + c) / 4];  // two pairs of -delta
+          float* y = &x[h * 32 + c];
+          unpair(mul2(pair(y[0], y[1]), add2(pair(d[c], d[c + 1]), e.x)), y[0], y[1]);
+          unpair(mul2(pair(y[2], y[3]), add2(pair(d[c + 2], d[c + 3]), e.y)), y[2], y[3]);
         }
       }
       if (masked) {
@@ -621,14 +629,14 @@ int launch(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t s
   if (n_q > 0) {
     const size_t smem = 1024 + Bwd<DP>::kFloats + dq_floats<DP>(bias, a.dtable_part != nullptr, a.span) * sizeof(float);
     KF_CUDA_RET(cudaFuncSetAttribute(attention_dq_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attention_dq_tc<DP><<<dim3(n_q, a.heads), Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
+    attention_dq_tc<DP><<<(unsigned)n_q * a.heads, Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     if (int rc = check_launch("kf_attention_bwd")) return rc;
   }
   if (n_k > 0) {
     a.tiles = k_tiles;
     const size_t smem = 1024 + Bwd<DP>::kFloats + dkdv_floats<DP>(bias, a.span) * sizeof(float);
     KF_CUDA_RET(cudaFuncSetAttribute(attention_dkdv_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attention_dkdv_tc<DP><<<dim3(n_k, a.kv_heads), Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
+    attention_dkdv_tc<DP><<<(unsigned)n_k * a.kv_heads, Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     return check_launch("kf_attention_bwd");
   }
   return KF_OK;

@@ -117,8 +117,8 @@ __global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
   float* sp = sv + kTile * Ld<D>::row;
   float* sbias = sp + kTile * kLdP;
   int tile;
-  const Seq s = load_tile(a, blockIdx.x, &tile);
-  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+  const Seq s = load_tile(a, blockIdx.x / a.heads, &tile);
+  const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const int r0 = tile * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   load_rows<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
   float* sbias = sp + kTile * kLdP;
   float* ssum = sbias + 2 * a.span + 1;  // gradient sums by clamped distance
   int tile;
-  const Seq s = load_tile(a, blockIdx.x, &tile);
-  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+  const Seq s = load_tile(a, blockIdx.x / a.heads, &tile);
+  const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const int r0 = tile * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   load_rows<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
   store_rows<T, D>(static_cast<T*>(a.dq), s.q0 + r0, n_rows, a.heads, head, a.dim, ty, tx, dq, mul);
   if (a.dtable_part != nullptr) {
     __syncthreads();
-    float* out = a.dtable_part + ((int64_t)blockIdx.x * a.heads + head) * a.n_buckets;
+    float* out = a.dtable_part + (int64_t)blockIdx.x * a.n_buckets;
     for (int b = threadIdx.x; b < a.n_buckets; b += kThreads) {
       float sum = 0.f;
       for (int e = 0; e < 2 * a.span + 1; ++e)
@@ -303,8 +303,8 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
   float* sdelta = slse + kTile;
   float* sbias = sdelta + kTile;
   int tile;
-  const Seq s = load_tile(a, blockIdx.x, &tile);
-  const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
+  const Seq s = load_tile(a, blockIdx.x / a.kv_heads, &tile);
+  const int kv_head = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
   const int r0 = tile * kTile, n_rows = min(kTile, s.lk - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   load_rows<T, D>(sk, a.k, s.k0 + r0, n_rows, kv_head, a.dim);
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
 }
 
 template <typename K>
-int run(K* kernel, dim3 grid, size_t floats, const Args& a, cudaStream_t st, const char* what) {
+int run(K* kernel, unsigned grid, size_t floats, const Args& a, cudaStream_t st, const char* what) {
   KF_CUDA_RET(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(floats * sizeof(float))));
   kernel<<<grid, kThreads, floats * sizeof(float), st>>>(a);
   return check_launch(what);
@@ -367,7 +367,7 @@ int run(K* kernel, dim3 grid, size_t floats, const Args& a, cudaStream_t st, con
 template <typename T, int D>
 int fwd(const Args& a, int n_tiles, cudaStream_t st) {
   const size_t bias = a.table != nullptr ? 2 * a.span + 1 : 0;
-  return run(attention_fwd<T, D>, dim3(n_tiles, a.heads), 3 * kTile * Ld<D>::row + kTile * kLdP + bias, a, st, "kf_attention_fwd");
+  return run(attention_fwd<T, D>, (unsigned)n_tiles * a.heads, 3 * kTile * Ld<D>::row + kTile * kLdP + bias, a, st, "kf_attention_fwd");
 }
 
 template <typename T, int D>
@@ -379,11 +379,11 @@ int bwd(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) 
     if (int rc = check_launch("kf_attention_bwd")) return rc;
   }
   if (n_q > 0)
-    if (int rc = run(attention_dq<T, D>, dim3(n_q, a.heads), 4 * kTile * Ld<D>::row + kTile * kLdP + 2 * bias, a, st, "kf_attention_bwd"))
+    if (int rc = run(attention_dq<T, D>, (unsigned)n_q * a.heads, 4 * kTile * Ld<D>::row + kTile * kLdP + 2 * bias, a, st, "kf_attention_bwd"))
       return rc;
   a.tiles = k_tiles;
   if (n_k > 0)
-    return run(attention_dkdv<T, D>, dim3(n_k, a.kv_heads), 4 * kTile * Ld<D>::row + 2 * kTile * kLdP + 2 * kTile + bias, a, st,
+    return run(attention_dkdv<T, D>, (unsigned)n_k * a.kv_heads, 4 * kTile * Ld<D>::row + 2 * kTile * kLdP + 2 * kTile + bias, a, st,
                "kf_attention_bwd");
   return KF_OK;
 }

@@ -68,8 +68,9 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
   volatile int* abort = &ctl.abort;
 
   int tile;
-  const Seq s = load_tile(a, blockIdx.x, &tile);
-  const int pack = a.pack, head0 = blockIdx.y * pack, kv_head = head0 / (a.heads / a.kv_heads);
+  const int pack = a.pack, packs = a.heads / pack;
+  const Seq s = load_tile(a, blockIdx.x / packs, &tile);
+  const int head0 = blockIdx.x % packs * pack, kv_head = head0 / (a.heads / a.kv_heads);
   const int r0 = tile * NT * kRows, off = s.lk - s.lq, total = s.lq * pack;
   // key tiles of each row tile
   int n_rows[NT], n_kv[NT], n_max = 0;
@@ -312,7 +313,7 @@ int launch(const Args& a, int n_tiles, cudaStream_t st) {
   const bool keys = a.tk > 0;  // without keys no tile is loaded
   if (int rc = make_tile_map(&k_map, keys ? a.k.p : a.q.p, keys ? a.tk : 1, keys ? a.kv_heads : 1, a.dim, a.k.row, a.k.head)) return rc;
   if (int rc = make_tile_map(&v_map, keys ? a.v.p : a.q.p, keys ? a.tk : 1, keys ? a.kv_heads : 1, a.dim, a.v.row, a.v.head)) return rc;
-  attention_fwd_tc<DP><<<dim3(n_tiles, a.heads / a.pack), Fwd<DP>::kThreads, smem, st>>>(a, k_map, v_map);
+  attention_fwd_tc<DP><<<(unsigned)n_tiles * (a.heads / a.pack), Fwd<DP>::kThreads, smem, st>>>(a, k_map, v_map);
   return check_launch("kf_attention_fwd");
 }
 
