@@ -534,7 +534,7 @@ int kf_residual_norm_bwd(const void* x, const void* branch, const void* gate, co
  *   table   (n_buckets, heads) in table_dtype, buckets (2 span + 1) int32; null: no bias
  *   o       (tq, heads, dim) contiguous; lse (heads, tq) float32, base 2 (null: not written);
  *           o_rest like o, bf16 only: what o's rounding left out, which the
- *           backward reads for dout . o (null: not written, not read)
+ *           backward needs for dout . o (null: not written)
  * q, k, v in dtype with the strides of the descriptor (elements; head width
  * contiguous).  Backward: dout like o; dq, dk, dv contiguous; dtable
  * (n_buckets, heads) in table_dtype or null; workspace

@@ -22,7 +22,7 @@ from . import _lib
 from .kernels import _check_cuda, _launch
 
 ATTENTION_MAX_DIM = 128
-BIAS_MAX_DISTANCE, BIAS_MAX_BUCKETS = 1024, 256
+BIAS_MAX_DISTANCE, BIAS_MAX_BUCKETS = 512, 256
 
 _DTYPE_CODE = {torch.float32: _lib.KF_DTYPE_F32, torch.bfloat16: _lib.KF_DTYPE_BF16}
 
@@ -279,7 +279,7 @@ class _Attention(torch.autograd.Function):
                     q_tiles, n_q, k_tiles, n_k, None if tab is None else tab.data_ptr(),
                     None if tab is None else bias.buckets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                     None if dtable is None else dtable.data_ptr(), ws.data_ptr(), plan.ref, _raw_stream(q),
-                    kernels=2 + (q.dtype == torch.float32) + want)
+                    kernels=2 + (q.dtype == torch.float32) + 2 * want)
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None, None, None)
 
 

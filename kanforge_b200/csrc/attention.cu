@@ -7,21 +7,39 @@ namespace {
 
 using namespace attn;
 
-// The bias gradient: the tiles' sums of one (bucket, head) in tile order, over 32 lanes.
-__global__ void __launch_bounds__(256) attention_dtable(const float* part, int n_tiles, int heads, int n_buckets, void* out,
-                                                        bool bf16) {
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;  // head * n_buckets + bucket
-  if (i >= heads * n_buckets) return;
+// The bias gradient by distance: the tiles' sums of one (head, distance), 32
+// distances by 8 slices of the tiles, joined in order.
+__global__ void __launch_bounds__(256) attention_dist(const float* part, int n_tiles, int heads, int n_dist, float* out) {
+  __shared__ float s[8][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, e = blockIdx.x * 32 + lane, head = blockIdx.y;
   float v = 0.f;
-  for (int t = lane; t < n_tiles; t += 32) v += part[(int64_t)t * heads * n_buckets + i];
+  if (e < n_dist) {
+#pragma unroll 8
+    for (int t = slice; t < n_tiles; t += 8) v += part[((int64_t)t * heads + head) * n_dist + e];
+  }
+  s[slice][lane] = v;
+  __syncthreads();
+  if (slice != 0 || e >= n_dist) return;
+  for (int i = 1; i < 8; ++i) v += s[i][lane];
+  out[(int64_t)head * n_dist + e] = v;
+}
+
+// ... and by bucket: a warp per (bucket, head), lanes over the distances.
+__global__ void __launch_bounds__(256) attention_dtable(const float* dist, const int* buckets, int n_dist, int heads, int n_buckets,
+                                                        void* out, bool bf16) {
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (i >= heads * n_buckets) return;
+  const int bucket = i / heads, head = i - bucket * heads;
+  float v = 0.f;
+#pragma unroll 4
+  for (int e = lane; e < n_dist; e += 32) v += buckets[e] == bucket ? dist[(int64_t)head * n_dist + e] : 0.f;
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
   if (lane != 0) return;
-  const int64_t at = (int64_t)(i % n_buckets) * heads + i / n_buckets;
   if (bf16)
-    static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+    static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
   else
-    static_cast<float*>(out)[at] = v;
+    static_cast<float*>(out)[i] = v;
 }
 
 int check_attention(const char* fn, const kf_attention_desc* d) {
@@ -47,7 +65,7 @@ void tiling(const kf_attention_desc* d, int pass, int32_t* rows, int32_t* pack) 
   *rows = d->dtype == KF_DTYPE_F32 ? 64 : pass == 0 && d->dim > 64 ? 256 : 128;
   if (d->dtype == KF_DTYPE_F32 || pass > 0) return;
   const int group = d->heads / d->kv_heads;
-  if (d->n_buckets == 0 || group * bias_floats(d->span) * (int)sizeof(float) <= fwd_bias_bytes(d->dim)) *pack = group;
+  if (d->n_buckets == 0 || group * bias_floats(d->span, d->n_buckets) * (int)sizeof(float) <= fwd_bias_bytes(d->dim)) *pack = group;
 }
 
 Args make_args(const kf_attention_desc* d) {
@@ -121,7 +139,7 @@ extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, con
 
 extern "C" int64_t kf_attention_bwd_workspace(int32_t n_q_tiles, const kf_attention_desc* d) {
   if (d == nullptr || n_q_tiles < 0) return 0;
-  return 2 * (int64_t)d->heads * d->tq + (int64_t)n_q_tiles * d->heads * d->n_buckets;
+  return 2 * (int64_t)d->heads * d->tq + (d->n_buckets > 0 ? ((int64_t)n_q_tiles + 1) * d->heads * (2 * d->span + 1) : 0);
 }
 
 extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout, const float* lse,
@@ -137,6 +155,7 @@ extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, con
   KF_CHECK_ARG(n_k_tiles == 0 || (k && v && dk && dv && k_tiles), "kf_attention_bwd: null argument");
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_bwd: the bias needs a table and buckets");
   KF_CHECK_ARG(dtable == nullptr || (table != nullptr && workspace != nullptr), "kf_attention_bwd: dtable needs a table and workspace");
+  KF_CHECK_ARG(n_q_tiles == 0 || d->dtype == KF_DTYPE_F32 || o_rest != nullptr, "kf_attention_bwd: bf16 needs o_rest");
   if (n_q_tiles == 0 && n_k_tiles == 0 && dtable == nullptr) return KF_OK;
   if (int rc = bind_device(n_q_tiles ? q : n_k_tiles ? k : dtable)) return rc;
   Args a = make_args(d);
@@ -144,14 +163,17 @@ extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, con
   a.dq = dq, a.dk = dk, a.dv = dv, a.table = table, a.buckets = buckets;
   a.tiles = reinterpret_cast<const Tile*>(q_tiles);
   a.delta = workspace;
-  a.dtable_part = dtable != nullptr ? workspace + 2 * (int64_t)d->heads * d->tq : nullptr;
+  float* dist = workspace + 2 * (int64_t)d->heads * d->tq;  // (H, 2 span + 1), then the tiles' parts
+  const int n_dist = 2 * d->span + 1;
+  a.dist_part = dtable != nullptr ? dist + (int64_t)d->heads * n_dist : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Tile* kt = reinterpret_cast<const Tile*>(k_tiles);
   int rows;
   tiling(d, 1, &rows, &a.pack);
   int rc = d->dtype == KF_DTYPE_BF16 ? bwd_bf16(a, kt, n_q_tiles, n_k_tiles, st) : bwd_f32(a, kt, n_q_tiles, n_k_tiles, st);
   if (rc || dtable == nullptr) return rc;
-  attention_dtable<<<(unsigned)cdiv(d->heads * d->n_buckets, 8), 256, 0, st>>>(a.dtable_part, n_q_tiles, d->heads, d->n_buckets, dtable,
+  attention_dist<<<dim3((unsigned)cdiv(n_dist, 32), d->heads), 256, 0, st>>>(a.dist_part, n_q_tiles, d->heads, n_dist, dist);
+  attention_dtable<<<(unsigned)cdiv(d->heads * d->n_buckets, 8), 256, 0, st>>>(dist, buckets, n_dist, d->heads, d->n_buckets, dtable,
                                                                                a.table_bf16);
   return check_launch("kf_attention_bwd");
 }

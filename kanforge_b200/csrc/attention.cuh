@@ -15,7 +15,7 @@ namespace kf {
 namespace attn {
 
 constexpr int kMaxDim = 128;
-constexpr int kMaxSpan = 1024;    // largest distance with a bias of its own
+constexpr int kMaxSpan = 512;    // largest distance with a bias of its own
 constexpr int kMaxBuckets = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -44,7 +44,7 @@ struct Args {
   const Tile* tiles;
   const void* table;  // (buckets, H) bias, or null
   const int* buckets; // (2 span + 1): bucket of distance index - span
-  float* dtable_part; // (tiles, H, buckets)
+  float* dist_part;   // (tiles, H, 2 span + 1): bias gradient by distance, or null
   int64_t tq, tk;
   int heads, kv_heads, dim, span, n_buckets;
   int pack;  // heads that are neighbouring rows of a tile (bf16)
@@ -68,7 +68,7 @@ __device__ __forceinline__ float bias_base2(float b) {
 }
 
 // Bias of one head in base 2, by clamped distance.
-__device__ __forceinline__ void expand_bias(const Args& a, int head, float* out, int thread, int n_threads) {
+__device__ __forceinline__ void expand_bias_f32(const Args& a, int head, float* out, int thread, int n_threads) {
   for (int i = thread; i < 2 * a.span + 1; i += n_threads) {
     const int64_t at = (int64_t)a.buckets[i] * a.heads + head;
     const float b = a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[at])

@@ -95,11 +95,12 @@ struct QCols {
   static constexpr uint32_t s = 0, dp = Bwd<DP>::kCols, dq = 2 * Bwd<DP>::kCols, ds = dq + DP, ds_buffer = Bwd<DP>::kCols / 2;
 };
 
-// Floats behind the tiles: halves of delta, bias table, sums by distance, block diagonals, bucket ids.
+// Floats behind the tiles: parts of delta, bias table, sums by distance of each
+// block of 32 rows, block diagonals of each warp.
 constexpr int kDiag = 48;  // of a block of 32 x 16 scores: 47 diagonals
 template <int DP>
-__host__ __device__ constexpr int dq_floats(bool bias, bool grad, int span) {
-  return 2 * kRows + (bias ? bias_floats(span) : 0) + (grad ? 2 * span + 1 + Bwd<DP>::kCols / 4 * kDiag + (2 * span + 4) / 4 : 0);
+__host__ __device__ constexpr int dq_floats(bool bias, bool grad, int span, int n_buckets) {
+  return 2 * kRows + (bias ? bias_floats(span, n_buckets) : 0) + (grad ? 4 * (2 * span + 1) + Bwd<DP>::kLoadWarp * 4 * kDiag : 0);
 }
 
 template <int DP>
@@ -114,9 +115,9 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* sdelta = reinterpret_cast<float*>(smem + F::kFloats);  // (groups, 128) parts of delta
   float* sbias = sdelta + 2 * kRows;
-  float* ssum = sbias + (a.table != nullptr ? bias_floats(a.span) : 0);
-  float* sdiag = ssum + 2 * a.span + 1;
-  uint8_t* sbucket = reinterpret_cast<uint8_t*>(sdiag + F::kCols / 4 * kDiag);
+  const int n_dist = 2 * a.span + 1;
+  float* ssum = sbias + (a.table != nullptr ? bias_floats(a.span, a.n_buckets) : 0);  // (4, n_dist)
+  float* sdiag = ssum + 4 * n_dist;                                                   // (warps, 4, kDiag)
   volatile int* abort = &ctl.abort;
 
   int tile;
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   const int keys = a.causal ? max(0, min(s.lk, r0 + n_rows + off)) : s.lk;
   const int n = (keys + F::kCols - 1) / F::kCols;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool grad = a.dtable_part != nullptr;
+  const bool grad = a.dist_part != nullptr;
 
   if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, 1, F::kSoftmax);
   if (warp == F::kMmaWarp) {
@@ -196,32 +197,46 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     const int pos = r + off;
     const int limit = valid && a.causal ? min(s.lk, pos + 1) : s.lk;
     const int64_t stat = (int64_t)head * a.tq + s.q0 + r;
-    if (a.table != nullptr) expand_bias_padded(a, head, 1, sbias, threadIdx.x, F::kSoftmax);
-    if (grad)
-      for (int i = threadIdx.x; i < 2 * a.span + 1; i += F::kSoftmax) ssum[i] = 0.f, sbucket[i] = (uint8_t)a.buckets[i];
-    // delta = dO . O, a part of the columns for each warpgroup
-    float delta = 0.f;
-    if (valid) {
-      const int64_t at = ((int64_t)(s.q0 + r) * a.heads + head) * a.dim;
-      const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(a.dout.p) + (int64_t)(s.q0 + r) * a.dout.row + head * a.dout.head;
-      const __nv_bfloat16* o = static_cast<const __nv_bfloat16*>(a.o) + at;
-      const __nv_bfloat16* e = a.o_rest == nullptr ? nullptr : static_cast<const __nv_bfloat16*>(a.o_rest) + at;
-#pragma unroll 4
-      for (int c = half * 8; c < a.dim; c += F::kGroups * 8) {
-        const uint4 gv = *reinterpret_cast<const uint4*>(g + c), ov = *reinterpret_cast<const uint4*>(o + c);
-        const uint4 ev = e == nullptr ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(e + c);
-        const uint32_t *gw = &gv.x, *ow = &ov.x, *ew = &ev.x;
+    // delta = dO . O: D/8 lanes to a row, a warp has 32 rows or, with two warpgroups, 16 of them
+    constexpr int LPR = DP / 8, RPP = 32 / LPR, PASSES = 32 / F::kGroups / RPP;
+    {
+      // all loads of four passes go out together; rows and columns that are not there read one that is
+      const int c = lane % LPR * 8, first_row = (warp & 3) * 32 + half * 16 + lane / LPR, c_in = c < a.dim ? c : 0;
+      const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(a.dout.p) + (int64_t)(s.q0 + r0) * a.dout.row + head * a.dout.head + c_in;
+      const int64_t at = ((int64_t)(s.q0 + r0) * a.heads + head) * a.dim + c_in, o_row = (int64_t)a.heads * a.dim;
+      const __nv_bfloat16 *o = static_cast<const __nv_bfloat16*>(a.o) + at, *e = static_cast<const __nv_bfloat16*>(a.o_rest) + at;
+#pragma unroll
+      for (int i0 = 0; i0 < PASSES; i0 += 4) {
+        uint4 gv[4], ov[4], ev[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          delta = fmaf(__uint_as_float(gw[i] << 16), __uint_as_float(ow[i] << 16) + __uint_as_float(ew[i] << 16), delta);
-          delta = fmaf(__uint_as_float(gw[i] & 0xffff0000u),
-                       __uint_as_float(ow[i] & 0xffff0000u) + __uint_as_float(ew[i] & 0xffff0000u), delta);
+          const int64_t from = min(first_row + (i0 + i) * RPP, n_rows - 1);
+          gv[i] = *reinterpret_cast<const uint4*>(g + from * a.dout.row);
+          ov[i] = *reinterpret_cast<const uint4*>(o + from * o_row);
+          ev[i] = *reinterpret_cast<const uint4*>(e + from * o_row);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t *gw = &gv[i].x, *ow = &ov[i].x, *ew = &ev[i].x;
+          float d = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            d = fmaf(__uint_as_float(gw[k] << 16), __uint_as_float(ow[k] << 16) + __uint_as_float(ew[k] << 16), d);
+            d = fmaf(__uint_as_float(gw[k] & 0xffff0000u), __uint_as_float(ow[k] & 0xffff0000u) + __uint_as_float(ew[k] & 0xffff0000u), d);
+          }
+          if (c >= a.dim) d = 0.f;
+#pragma unroll
+          for (int k = LPR / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
+          if (lane % LPR == 0) sdelta[first_row + (i0 + i) * RPP] = d;
         }
       }
     }
-    sdelta[half * kRows + row] = delta;
-    softmax_sync<DP>();  // the bias table is complete, too
-    if (F::kGroups == 2) delta = sdelta[row] + sdelta[kRows + row];
+    if (grad)
+      for (int i = threadIdx.x; i < 4 * n_dist; i += F::kSoftmax) ssum[i] = 0.f;
+    if (a.table != nullptr) expand_bias(a, head, 1, sbias, threadIdx.x, F::kSoftmax, [] { softmax_sync<DP>(); });
+    softmax_sync<DP>();
+    float delta = sdelta[row];
+    if (F::kGroups == 2) softmax_sync<DP>();  // sdelta is written again below
     // O carries the rounding of P, which weighs most where a row sees few keys:
     // rows whose keys all lie in the first tile get delta = sum P dP there.
     const bool short_rows = (a.causal ? r0 + off + 1 : s.lk) <= F::kCols;
@@ -322,7 +337,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         // A partial sum moves along its diagonal, one lane up for each column; lane 31's is complete.
         // Four blocks of 32 rows x 16 columns at a time, to have four such chains in flight.
         const float keep = lane == 0 ? 0.f : 1.f;
-        float* out = sdiag + ((warp & 3) * (F::kCols / 16) + half * 4) * kDiag;  // index row - column + 15
+        float* out = sdiag + warp * 4 * kDiag;  // index row - column + 15
         float acc[4];
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
@@ -336,24 +351,34 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
 #pragma unroll
           for (int h = 0; h < 4; ++h) out[h * kDiag + lane] = acc[h];
         }
-        if (!(together = softmax_sync<DP>())) break;
-        // a thread takes the diagonal row - column = i of the tile over its blocks, in order; no other thread has it
-        for (int at = threadIdx.x; at < kRows + F::kCols - 1; at += F::kSoftmax) {
-          const int i = at - (F::kCols - 1), dd = d0 + i;
+        __syncwarp();
+        // The warp adds its 95 diagonals to the sums of its 32 rows, which with two warpgroups it
+        // shares with one other warp: that one's turn comes after a barrier.
+        if (F::kGroups == 2 && half == 1 && !(together = softmax_sync<DP>())) break;
+        float* sums = ssum + (warp & 3) * n_dist + a.span;
+        const int dw = d0 + (warp & 3) * 32 - half * 64;  // distance of the warp's first row and column
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const int i = k * 32 + lane - 63;  // row - column
           float sum = 0.f;
 #pragma unroll
-          for (int b = 0; b < F::kCols / 4; ++b) {
-            const int e = i - b / (F::kCols / 16) * 32 + b % (F::kCols / 16) * 16 + 15;
-            if (e >= 0 && e < 47) sum += sdiag[b * kDiag + e];
+          for (int h = 0; h < 4; ++h) {
+            const int e = i + h * 16 + 15;
+            if (e >= 0 && e < 47) sum += out[h * kDiag + e];
           }
+          const int dd = dw + i;
           if (dd >= a.span)
             far_sum[0] += sum;
           else if (dd <= -a.span)
             far_sum[1] += sum;
           else
-            ssum[dd + a.span] += sum;
+            sums[dd] += sum;
         }
-        if (!(together = softmax_sync<DP>())) break;
+        __syncwarp();
+        if (F::kGroups == 2) {
+          if (half == 0 && !(together = softmax_sync<DP>())) break;
+          if (!(together = softmax_sync<DP>())) break;
+        }
       }
     }
     if (ok && together && n > 0) ok = mbar_wait_warp(&ctl.dk_done, 0, abort);
@@ -370,22 +395,15 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
           for (int o = 16; o > 0; o >>= 1) far_sum[f] += __shfl_xor_sync(0xffffffffu, far_sum[f], o);
           if (lane == 0) sdiag[f * 8 + warp] = far_sum[f];
         }
-        softmax_sync<DP>();
-        if (threadIdx.x < 2) {
-          float sum = 0.f;
-          for (int w = 0; w < F::kLoadWarp; ++w) sum += sdiag[threadIdx.x * 8 + w];
-          ssum[threadIdx.x == 0 ? 2 * a.span : 0] += sum;
-        }
-        softmax_sync<DP>();
-        // a warp per bucket in turn
-        float* out = a.dtable_part + (int64_t)blockIdx.x * a.n_buckets;
-        for (int b = warp; b < a.n_buckets; b += F::kLoadWarp) {
-          float sum = 0.f;
-          for (int e = lane; e < 2 * a.span + 1; e += 32)
-            if (sbucket[e] == b) sum += ssum[e];
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          if (lane == 0) out[b] = sum;
+        softmax_sync<DP>();  // the sums of all warps, too
+        float* out = a.dist_part + (int64_t)blockIdx.x * n_dist;
+        for (int e = threadIdx.x; e < n_dist; e += F::kSoftmax) {
+          float sum = (ssum[e] + ssum[n_dist + e]) + (ssum[2 * n_dist + e] + ssum[3 * n_dist + e]);
+          if (e == 0 || e == 2 * a.span) {
+            const float* far = sdiag + (e == 0 ? 8 : 0);
+            for (int w = 0; w < F::kLoadWarp; ++w) sum += far[w];
+          }
+          out[e] = sum;
         }
       }
     }
@@ -409,8 +427,8 @@ struct KvCols {
 };
 
 template <int DP>
-__host__ __device__ constexpr int dkdv_floats(bool bias, int span) {
-  return Bwd<DP>::kStages * 2 * Bwd<DP>::kCols + (bias ? bias_floats(span) : 0);
+__host__ __device__ constexpr int dkdv_floats(bool bias, int span, int n_buckets) {
+  return Bwd<DP>::kStages * 2 * Bwd<DP>::kCols + (bias ? bias_floats(span, n_buckets) : 0);
 }
 
 template <int DP>
@@ -517,8 +535,9 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       const int st = 2 * i % F::kStages, q0 = (first + i % per_head) * F::kCols + half * 64;
       if (a.table != nullptr && i % per_head == 0) {  // another head's table
         if (!(together = softmax_sync<DP>())) break;
-        expand_bias_padded(a, kv_head * group + i / per_head, 1, sbias, threadIdx.x, F::kSoftmax);
-        if (!(together = softmax_sync<DP>())) break;
+        expand_bias(a, kv_head * group + i / per_head, 1, sbias, threadIdx.x, F::kSoftmax,
+                    [&] { together = softmax_sync<DP>(); });
+        if (!together || !(together = softmax_sync<DP>())) break;
       }
       ok = mbar_wait_warp(&ctl.stat_full[st], (2 * i / F::kStages) & 1, abort) && mbar_wait_warp(&ctl.s_full, i & 1, abort);
       if (!ok) break;
@@ -627,14 +646,14 @@ int launch(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t s
   if (int rc = map(&k_map, a.k, a.tk, a.kv_heads)) return rc;
   if (int rc = map(&v_map, a.v, a.tk, a.kv_heads)) return rc;
   if (n_q > 0) {
-    const size_t smem = 1024 + Bwd<DP>::kFloats + dq_floats<DP>(bias, a.dtable_part != nullptr, a.span) * sizeof(float);
+    const size_t smem = 1024 + Bwd<DP>::kFloats + dq_floats<DP>(bias, a.dist_part != nullptr, a.span, a.n_buckets) * sizeof(float);
     KF_CUDA_RET(cudaFuncSetAttribute(attention_dq_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     attention_dq_tc<DP><<<(unsigned)n_q * a.heads, Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     if (int rc = check_launch("kf_attention_bwd")) return rc;
   }
   if (n_k > 0) {
     a.tiles = k_tiles;
-    const size_t smem = 1024 + Bwd<DP>::kFloats + dkdv_floats<DP>(bias, a.span) * sizeof(float);
+    const size_t smem = 1024 + Bwd<DP>::kFloats + dkdv_floats<DP>(bias, a.span, a.n_buckets) * sizeof(float);
     KF_CUDA_RET(cudaFuncSetAttribute(attention_dkdv_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     attention_dkdv_tc<DP><<<(unsigned)n_k * a.kv_heads, Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     return check_launch("kf_attention_bwd");

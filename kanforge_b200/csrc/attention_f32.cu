@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
   const int r0 = tile * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   load_rows<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
-  if (a.table != nullptr) expand_bias(a, head, sbias, threadIdx.x, kThreads);
+  if (a.table != nullptr) expand_bias_f32(a, head, sbias, threadIdx.x, kThreads);
   float m[4], l[4], o[4][D / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
   load_rows<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
   load_rows<T, D>(sg, a.dout, s.q0 + r0, n_rows, head, a.dim);
   if (a.table != nullptr) {
-    expand_bias(a, head, sbias, threadIdx.x, kThreads);
+    expand_bias_f32(a, head, sbias, threadIdx.x, kThreads);
     for (int i = threadIdx.x; i < 2 * a.span + 1; i += kThreads) ssum[i] = 0.f;
   }
   float lse[4], delta[4], dq[4][D / 16];
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
     }
     __syncwarp();
     dot_cols<D>(sp, sk, ty, tx, dq);
-    if (a.dtable_part != nullptr) {
+    if (a.dist_part != nullptr) {
       // thread d sums the diagonal row - column = d - 63 of dS
       __syncthreads();
       float sum = 0.f;
@@ -277,15 +277,10 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
   }
   const float mul[4] = {a.scale, a.scale, a.scale, a.scale};
   store_rows<T, D>(static_cast<T*>(a.dq), s.q0 + r0, n_rows, a.heads, head, a.dim, ty, tx, dq, mul);
-  if (a.dtable_part != nullptr) {
+  if (a.dist_part != nullptr) {
     __syncthreads();
-    float* out = a.dtable_part + (int64_t)blockIdx.x * a.n_buckets;
-    for (int b = threadIdx.x; b < a.n_buckets; b += kThreads) {
-      float sum = 0.f;
-      for (int e = 0; e < 2 * a.span + 1; ++e)
-        if (a.buckets[e] == b) sum += ssum[e];
-      out[b] = sum;
-    }
+    float* out = a.dist_part + (int64_t)blockIdx.x * (2 * a.span + 1);
+    for (int e = threadIdx.x; e < 2 * a.span + 1; e += kThreads) out[e] = ssum[e];
   }
 }
 
@@ -318,7 +313,7 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
   const float c2 = a.scale * kLog2e;
   for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
     __syncthreads();
-    if (a.table != nullptr) expand_bias(a, head, sbias, threadIdx.x, kThreads);
+    if (a.table != nullptr) expand_bias_f32(a, head, sbias, threadIdx.x, kThreads);
     for (int q0 = q_first; q0 < s.lq; q0 += kTile) {
       const int n_q = min(kTile, s.lq - q0);
       __syncthreads();

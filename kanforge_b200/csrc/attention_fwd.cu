@@ -179,12 +179,13 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
                                static_cast<const __nv_bfloat16*>(a.q.p) + (int64_t)s.q0 * a.q.row + head0 * a.q.head, a.q.row,
                                a.q.head, pack, r0 + t * kRows, rows, a.dim, row);
     cp_async_commit();
-    if (a.table != nullptr) expand_bias_padded(a, head0, pack, sbias, threadIdx.x, F::kSoftmax);
+    if (a.table != nullptr)
+      expand_bias(a, head0, pack, sbias, threadIdx.x, F::kSoftmax, [] { named_bar_and(1, F::kSoftmax, true); });
     cp_async_wait<0>();
     fence_proxy_async_smem();
     mbar_arrive(&ctl.q_full);
     if (a.table != nullptr) named_bar_and(1, F::kSoftmax, true);
-    const float* bias = sbias + (a.table != nullptr ? (r - tok * pack) * bias_floats(a.span) + a.span + kBiasPad : 0);
+    const float* bias = sbias + (a.table != nullptr ? (r - tok * pack) * bias_stride(a.span) + a.span + kBiasPad : 0);
     float m = -CUDART_INF_F, l = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
 
 template <int DP>
 int launch(const Args& a, int n_tiles, cudaStream_t st) {
-  const size_t smem = Fwd<DP>::kSmem + (a.table != nullptr ? a.pack * bias_floats(a.span) * sizeof(float) : 0);
+  const size_t smem = Fwd<DP>::kSmem + (a.table != nullptr ? a.pack * bias_floats(a.span, a.n_buckets) * sizeof(float) : 0);
   KF_CUDA_RET(cudaFuncSetAttribute(attention_fwd_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   CUtensorMap k_map, v_map;
   const bool keys = a.tk > 0;  // without keys no tile is loaded

@@ -19,7 +19,7 @@ constexpr int kBiasPad = 160;          // distances a tile may lie past the span
 template <int DP>
 __host__ __device__ constexpr int tile_bytes(int rows) { return rows * 128 * (DP / 64); }
 
-__host__ __device__ constexpr int bias_floats(int span) { return 2 * span + 1 + 2 * kBiasPad; }
+__host__ __device__ constexpr int bias_stride(int span) { return 2 * span + 1 + 2 * kBiasPad; }
 
 // ---- tcgen05, one CTA --------------------------------------------------------
 
@@ -289,14 +289,40 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// The padded bias tables of `pack` heads: index distance + span + kBiasPad.
-__device__ __forceinline__ void expand_bias_padded(const Args& a, int head0, int pack, float* out, int thread, int n_threads) {
-  const int n = bias_floats(a.span);
-  for (int i = thread; i < pack * n; i += n_threads) {
-    const int at = min(max(i % n - kBiasPad, 0), 2 * a.span);
-    const int64_t e = (int64_t)a.buckets[at] * a.heads + head0 + i / n;
-    out[i] = bias_base2(a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[e])
-                                     : static_cast<const float*>(a.table)[e]);
+// The padded bias tables of `pack` heads (index distance + span + kBiasPad), with
+// room behind them for the heads' columns of the learned table.  The columns and
+// the bucket numbers are read side by side, so that one trip to memory is waited
+// for; sync() is a barrier of the `n_threads` threads.
+__host__ __device__ constexpr int bias_floats(int span, int n_buckets) { return bias_stride(span) + n_buckets; }
+
+template <typename Sync>
+__device__ __forceinline__ void expand_bias(const Args& a, int head0, int pack, float* out, int thread, int n_threads, Sync&& sync) {
+  const int n = bias_stride(a.span);
+  float* column = out + pack * n;
+  for (int i = thread; i < pack * a.n_buckets; i += n_threads) {
+    const int64_t e = (int64_t)(i % a.n_buckets) * a.heads + head0 + i / a.n_buckets;
+    column[i] = bias_base2(a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[e])
+                                        : static_cast<const float*>(a.table)[e]);
+  }
+  constexpr int U = 4;
+  int id[U];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * n_threads;
+      id[u] = a.buckets[min(max(i - kBiasPad, 0), 2 * a.span)];
+    }
+  };
+  load(thread);
+  sync();
+  for (int i0 = thread; i0 < n; i0 += U * n_threads) {
+    if (i0 != thread) load(i0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * n_threads;
+      if (i >= n) break;
+      for (int g = 0; g < pack; ++g) out[g * n + i] = column[g * a.n_buckets + min(max(id[u], 0), a.n_buckets - 1)];
+    }
   }
 }
 
