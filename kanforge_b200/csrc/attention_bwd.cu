@@ -11,11 +11,11 @@
 // Seven products of 128 x 128 x D a tile pair against five with one kernel;
 // the five would add every dQ tile into memory in an order that varies.
 // All scores live in tensor memory; P and dS go back there as bf16 (2^-9 of
-// each term) and are the A operands of the products that sum them.  A streamed
-// tile has 128 rows with D = 128 and a CTA has an SM to itself; with D <= 64 it has
-// 64 and two CTAs share an SM, so that one's chain of products and softmax runs
-// under the other's.  Warps: softmax arithmetic (thread = row, a warpgroup for
-// each 64 columns), one that loads, two that issue the MMAs of one chain each.
+// each term) and are the A operands of the products that sum them.  With D = 128 a
+// CTA has an SM to itself; with D <= 64 two CTAs share one, so that one's chain of
+// products and softmax runs under the other's.  Warps: softmax arithmetic (thread
+// = row, 64 columns each), one that loads, and some that issue MMAs, one chain
+// each.
 #include "attention_tc.cuh"
 
 namespace kf {
@@ -38,22 +38,21 @@ struct Bwd {
 };
 
 // Every barrier alternates between two phases, so a waiter must not fall two
-// behind: dS has a barrier for odd and one for even tiles, since in dQ the scores
-// of the next tile are made before dS of this one is waited for.
+// behind: dS has a barrier for odd and one for even tiles, since the scores of
+// the next tile are made before dS of this one is waited for.
 struct Ctl {
-  uint64_t fixed_full, part[2], full[8], empty[8], stat_full[8], s_full, dp_full, s_read, p_ready, ds_ready[2], dv_done, dk_done, fin[2];
+  uint64_t fixed_full, part[2], full[8], empty[8], s_full, dp_full, s_read, ds_ready[2], dq_done, fin[2];
   uint32_t tmem;
   int abort;
 };
 
-// `users`: how many MMA warps read a streamed tile
-__device__ __forceinline__ void init_barriers(Ctl* c, int stages, int users, int softmax) {
+__device__ __forceinline__ void init_barriers(Ctl* c, int stages, int softmax) {
   c->abort = 0;
   mbar_init(&c->fixed_full, 2);
   mbar_init(&c->part[0], 1), mbar_init(&c->part[1], 1);
-  for (int i = 0; i < stages; ++i) mbar_init(&c->full[i], 1), mbar_init(&c->empty[i], users), mbar_init(&c->stat_full[i], 32);
-  mbar_init(&c->s_full, 1), mbar_init(&c->dp_full, 1), mbar_init(&c->dv_done, 1), mbar_init(&c->dk_done, 1);
-  mbar_init(&c->s_read, softmax), mbar_init(&c->p_ready, softmax), mbar_init(&c->ds_ready[0], softmax), mbar_init(&c->ds_ready[1], softmax);
+  for (int i = 0; i < stages; ++i) mbar_init(&c->full[i], 1), mbar_init(&c->empty[i], 1);
+  mbar_init(&c->s_full, 1), mbar_init(&c->dp_full, 1), mbar_init(&c->dq_done, 1);
+  mbar_init(&c->s_read, softmax), mbar_init(&c->ds_ready[0], softmax), mbar_init(&c->ds_ready[1], softmax);
   mbar_init(&c->fin[0], 1), mbar_init(&c->fin[1], 1);
   fence_barrier_init();
 }
@@ -97,10 +96,11 @@ struct QCols {
 
 // Floats behind the tiles: parts of delta, bias table, sums by distance of each
 // block of 32 rows, block diagonals of each warp.
-constexpr int kDiag = 48;  // of a block of 32 x 16 scores: 47 diagonals
+constexpr int kDiag = 48;                       // of a block of 32 x 16 scores: 47 diagonals
+constexpr int kDiagWarp = 7 * kDiag + 32;       // four blocks, and what their unused stores reach
 template <int DP>
 __host__ __device__ constexpr int dq_floats(bool bias, bool grad, int span, int n_buckets) {
-  return 2 * kRows + (bias ? bias_floats(span, n_buckets) : 0) + (grad ? 4 * (2 * span + 1) + Bwd<DP>::kLoadWarp * 4 * kDiag : 0);
+  return 2 * kRows + (bias ? bias_floats(span, n_buckets) : 0) + (grad ? 4 * (2 * span + 1) + Bwd<DP>::kLoadWarp * kDiagWarp : 0);
 }
 
 template <int DP>
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   float* sbias = sdelta + 2 * kRows;
   const int n_dist = 2 * a.span + 1;
   float* ssum = sbias + (a.table != nullptr ? bias_floats(a.span, a.n_buckets) : 0);  // (4, n_dist)
-  float* sdiag = ssum + 4 * n_dist;                                                   // (warps, 4, kDiag)
+  float* sdiag = ssum + 4 * n_dist;                                                   // (warps, kDiagWarp)
   volatile int* abort = &ctl.abort;
 
   int tile;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool grad = a.dist_part != nullptr;
 
-  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, 1, F::kSoftmax);
+  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, F::kSoftmax);
   if (warp == F::kMmaWarp) {
     tmem_alloc(&ctl.tmem, F::kTmem);
     tmem_relinquish();
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
             mma_ts(tmem + C::dq, tmem + C::ds + (j & 1) * C::ds_buffer + i * 8, kd + step_mn(i), idesc_d, j > 0 || i > 0);
           mma_commit(&ctl.empty[2 * j % F::kStages]);
         }
-        mma_commit(&ctl.dk_done);
+        mma_commit(&ctl.dq_done);
       } else {
         for (int j = 0; j < n && ok; ++j) {
           if (j > 0 && !(ok = mbar_wait(&ctl.ds_ready[(j - 1) & 1], ((j - 1) >> 1) & 1, abort))) break;
@@ -200,35 +200,32 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     // delta = dO . O: D/8 lanes to a row, a warp has 32 rows or, with two warpgroups, 16 of them
     constexpr int LPR = DP / 8, RPP = 32 / LPR, PASSES = 32 / F::kGroups / RPP;
     {
-      // all loads of four passes go out together; rows and columns that are not there read one that is
+      // all loads go out together; rows and columns that are not there read one that is
       const int c = lane % LPR * 8, first_row = (warp & 3) * 32 + half * 16 + lane / LPR, c_in = c < a.dim ? c : 0;
       const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(a.dout.p) + (int64_t)(s.q0 + r0) * a.dout.row + head * a.dout.head + c_in;
       const int64_t at = ((int64_t)(s.q0 + r0) * a.heads + head) * a.dim + c_in, o_row = (int64_t)a.heads * a.dim;
       const __nv_bfloat16 *o = static_cast<const __nv_bfloat16*>(a.o) + at, *e = static_cast<const __nv_bfloat16*>(a.o_rest) + at;
+      uint4 gv[PASSES], ov[PASSES], ev[PASSES];
 #pragma unroll
-      for (int i0 = 0; i0 < PASSES; i0 += 4) {
-        uint4 gv[4], ov[4], ev[4];
+      for (int i = 0; i < PASSES; ++i) {
+        const int64_t from = min(first_row + i * RPP, n_rows - 1);
+        gv[i] = *reinterpret_cast<const uint4*>(g + from * a.dout.row);
+        ov[i] = *reinterpret_cast<const uint4*>(o + from * o_row);
+        ev[i] = *reinterpret_cast<const uint4*>(e + from * o_row);
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t from = min(first_row + (i0 + i) * RPP, n_rows - 1);
-          gv[i] = *reinterpret_cast<const uint4*>(g + from * a.dout.row);
-          ov[i] = *reinterpret_cast<const uint4*>(o + from * o_row);
-          ev[i] = *reinterpret_cast<const uint4*>(e + from * o_row);
+      for (int i = 0; i < PASSES; ++i) {
+        const uint32_t *gw = &gv[i].x, *ow = &ov[i].x, *ew = &ev[i].x;
+        float d = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          d = fmaf(__uint_as_float(gw[k] << 16), __uint_as_float(ow[k] << 16) + __uint_as_float(ew[k] << 16), d);
+          d = fmaf(__uint_as_float(gw[k] & 0xffff0000u), __uint_as_float(ow[k] & 0xffff0000u) + __uint_as_float(ew[k] & 0xffff0000u), d);
         }
+        if (c >= a.dim) d = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t *gw = &gv[i].x, *ow = &ov[i].x, *ew = &ev[i].x;
-          float d = 0.f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            d = fmaf(__uint_as_float(gw[k] << 16), __uint_as_float(ow[k] << 16) + __uint_as_float(ew[k] << 16), d);
-            d = fmaf(__uint_as_float(gw[k] & 0xffff0000u), __uint_as_float(ow[k] & 0xffff0000u) + __uint_as_float(ew[k] & 0xffff0000u), d);
-          }
-          if (c >= a.dim) d = 0.f;
-#pragma unroll
-          for (int k = LPR / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
-          if (lane % LPR == 0) sdelta[first_row + (i0 + i) * RPP] = d;
-        }
+        for (int k = LPR / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
+        if (lane % LPR == 0) sdelta[first_row + i * RPP] = d;
       }
     }
     if (grad)
@@ -336,16 +333,20 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       } else {
         // A partial sum moves along its diagonal, one lane up for each column; lane 31's is complete.
         // Four blocks of 32 rows x 16 columns at a time, to have four such chains in flight.
+        // The other lanes store beside it what nothing reads: a store by one lane would be a branch.
         const float keep = lane == 0 ? 0.f : 1.f;
-        float* out = sdiag + warp * 4 * kDiag;  // index row - column + 15
+        float* out = sdiag + warp * kDiagWarp;  // of block h: index row - column + 15
+        float* put = lane == 31 ? out + 46 : out + 4 * kDiag + lane;
+        const int back = lane == 31 ? 1 : 0;
         float acc[4];
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             acc[h] = c == 0 ? x[h * 16] : fmaf(__shfl_up_sync(0xffffffffu, acc[h], 1), keep, x[h * 16 + c]);
-            if (lane == 31) out[h * kDiag + 46 - c] = acc[h];
+            put[h * kDiag] = acc[h];
           }
+          put -= back;
         }
         if (lane < 31) {
 #pragma unroll
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         }
       }
     }
-    if (ok && together && n > 0) ok = mbar_wait_warp(&ctl.dk_done, 0, abort);
+    if (ok && together && n > 0) ok = mbar_wait_warp(&ctl.dq_done, 0, abort);
     if ((grad || owed) && together) together = softmax_sync<DP>(ok);
     if (ok && together) {
       tc_fence_after();
@@ -417,32 +418,50 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
 }
 
 // ---- dK, dV -----------------------------------------------------------------------
-// Tensor memory: S^T, dP^T, dV, dK.  P^T and dS^T lie in their scores' columns,
-// and the next scores wait for the product that reads them.
+// A tile of 64 queries is one warpgroup's.  With D = 128 two warpgroups take the
+// tiles in turn, so that one's softmax runs under the products of the other's
+// tile; with D <= 64 the other CTA of the SM does that.  Tensor memory: S^T and dP^T
+// of each group, dV, dK.  P^T and dS^T lie in their scores' columns, and the next
+// scores of the group wait for the product that reads them.  The MMA warps: one
+// makes S^T and dP^T, one dV, one dK.
 template <int DP>
-struct KvCols {
-  static constexpr uint32_t s = 0, dp = Bwd<DP>::kCols, dv = 2 * Bwd<DP>::kCols, dk = dv + DP;
-  // k-step i of 16 columns: a warpgroup's 64 scores become 32 columns at their start
-  __device__ static constexpr uint32_t step(int i) { return (i >> 2) * 64 + (i & 3) * 8; }
+struct Kv {
+  static constexpr int kGroups = DP == 64 ? 1 : 2, kCols = 64;
+  static constexpr int kStages = DP == 64 ? 6 : 8;
+  static constexpr int kFixed = tile_bytes<DP>(kRows), kTile = tile_bytes<DP>(kCols);
+  static constexpr int kRing = 2 * kFixed, kFloats = kRing + kStages * kTile;
+  static constexpr int kLoadWarp = kGroups * 4, kMmaWarp = kLoadWarp + 1;
+  static constexpr int kThreads = kGroups * 128 + 128, kCtas = DP == 64 ? 2 : 1;
+  // registers: 256 x 128 at launch = 128 x 192 + 128 x 64; 384 x 168 = 256 x 208 + 128 x 88
+  static constexpr int kSoftmaxRegs = DP == 64 ? 192 : 208, kOtherRegs = DP == 64 ? 64 : 88;
+  static constexpr uint32_t kTmem = DP == 64 ? 256 : 512;
+  __device__ static constexpr uint32_t s(int g) { return g * kCols; }
+  __device__ static constexpr uint32_t dp(int g) { return (kGroups + g) * kCols; }
+  static constexpr uint32_t dv = 2 * kGroups * kCols, dk = dv + DP;
+};
+
+struct KvCtl {
+  uint64_t fixed_full, part[2], full[8], empty[8], stat_full[8];
+  uint64_t s_full[2], dp_full[2], p_ready[2], ds_ready[2], dv_done[2], dk_done[2], dv_all, dk_all, fin;
+  uint32_t tmem;
+  int abort;
 };
 
 template <int DP>
 __host__ __device__ constexpr int dkdv_floats(bool bias, int span, int n_buckets) {
-  return Bwd<DP>::kStages * 2 * Bwd<DP>::kCols + (bias ? bias_floats(span, n_buckets) : 0);
+  return Kv<DP>::kStages * 2 * Kv<DP>::kCols + (bias ? Kv<DP>::kGroups * bias_floats(span, n_buckets) : 0);
 }
 
 template <int DP>
-__global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_dkdv_tc(const Args a, const __grid_constant__ CUtensorMap q_map,
-                                                                 const __grid_constant__ CUtensorMap g_map,
-                                                                 const __grid_constant__ CUtensorMap k_map,
-                                                                 const __grid_constant__ CUtensorMap v_map) {
-  using F = Bwd<DP>;
-  using C = KvCols<DP>;
+__global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
+    attention_dkdv_tc(const Args a, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap g_map,
+                      const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using F = Kv<DP>;
+  constexpr int G = F::kGroups;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ Ctl ctl;
+  __shared__ KvCtl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sstat = reinterpret_cast<float*>(smem + F::kFloats);  // lse, delta of each stage in the ring
-  float* sbias = sstat + F::kStages * 2 * F::kCols;
+  float* sstat = reinterpret_cast<float*>(smem + F::kFloats);  // -lse, -delta of each stage in the ring
   volatile int* abort = &ctl.abort;
 
   int tile;
@@ -453,7 +472,18 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   const int per_head = max(0, (s.lq + F::kCols - 1) / F::kCols - first), n = group * per_head;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) init_barriers(&ctl, F::kStages, 2, F::kSoftmax);
+  if (threadIdx.x == 0) {
+    ctl.abort = 0;
+    mbar_init(&ctl.fixed_full, 2);
+    mbar_init(&ctl.part[0], 1), mbar_init(&ctl.part[1], 1);
+    for (int i = 0; i < F::kStages; ++i) mbar_init(&ctl.full[i], 1), mbar_init(&ctl.empty[i], 2), mbar_init(&ctl.stat_full[i], 32);
+    for (int g = 0; g < G; ++g) {
+      mbar_init(&ctl.s_full[g], 1), mbar_init(&ctl.dp_full[g], 1), mbar_init(&ctl.dv_done[g], 1), mbar_init(&ctl.dk_done[g], 1);
+      mbar_init(&ctl.p_ready[g], 128), mbar_init(&ctl.ds_ready[g], 128);
+    }
+    mbar_init(&ctl.dv_all, 1), mbar_init(&ctl.dk_all, 1), mbar_init(&ctl.fin, 1);
+    fence_barrier_init();
+  }
   if (warp == F::kMmaWarp) {
     tmem_alloc(&ctl.tmem, F::kTmem);
     tmem_relinquish();
@@ -465,7 +495,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
 
   if (warp >= F::kLoadWarp) reg_dec<F::kOtherRegs>();
   if (warp == F::kLoadWarp) {
-    // ---- loads: K and V, then Q (with lse and delta) and dO tiles in turn
+    // ---- loads: K and V, then Q (with -lse and -delta) and dO tiles in turn
     TileLoader<DP> loader(ctl.part, abort);
     if (loader.template load<kRows>(k_tile, &k_map, &ctl.fixed_full, kv_head, s.k0 + r0, n_rows) &&
         loader.template load<kRows>(k_tile + F::kFixed, &v_map, &ctl.fixed_full, kv_head, s.k0 + r0, n_rows))
@@ -488,112 +518,128 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       });
     cp_async_wait<0>();
     mbar_drain(&ctl.fixed_full, 0);
-  } else if (warp >= F::kMmaWarp && warp < F::kMmaWarp + 2) {
-    // ---- MMAs: one warp S^T and dV, the other dP^T and dK
+  } else if (warp >= F::kMmaWarp) {
+    // ---- MMAs
     if (lane == 0) {
-      const uint32_t idesc_s = idesc_bf16_f32(kRows, F::kCols, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
-      const int w = warp - F::kMmaWarp;  // the product takes item 2 i + w, the sum item 2 i + 1 - w
-      const uint32_t d = tmem + (w == 0 ? C::s : C::dp), fixed = desc_k(k_tile + w * F::kFixed), acc = tmem + (w == 0 ? C::dv : C::dk);
-      uint64_t *made = w == 0 ? &ctl.s_full : &ctl.dp_full, *ready = w == 0 ? &ctl.p_ready : &ctl.ds_ready[0],
-               *done = w == 0 ? &ctl.dv_done : &ctl.dk_done;
+      const int role = warp - F::kMmaWarp;
       auto full = [&](int it) { return mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort); };
-      auto product = [&](int it) {
-        if (!full(it)) return false;
-        tc_fence_after();
-        const uint32_t bd = desc_k(ring + (it % F::kStages) * F::kTile);
+      bool ok = mbar_wait(&ctl.fixed_full, 0, abort);
+      if (role == 0) {
+        const uint32_t idesc = idesc_bf16_f32(kRows, F::kCols, false, false), kd = desc_k(k_tile), vd = desc_k(k_tile + F::kFixed);
+        auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* made) {
+          if (!full(it)) return false;
+          tc_fence_after();
+          const uint32_t bd = desc_k(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) mma_ss(d, fixed + step_k<kRows>(i), bd + step_k<F::kCols>(i), idesc_s, i > 0);
-        mma_commit(made);
-        mma_commit(&ctl.empty[it % F::kStages]);
-        return true;
-      };
-      bool ok = mbar_wait(&ctl.fixed_full, 0, abort) && (n == 0 || product(w));
-      for (int i = 0; i < n && ok; ++i) {
-        const int it = 2 * i + 1 - w;
-        if (!(ok = mbar_wait(ready, i & 1, abort) && full(it))) break;
-        tc_fence_after();
-        const uint32_t bd = desc_mn<F::kCols>(ring + (it % F::kStages) * F::kTile);
+          for (int c = 0; c < DP / 16; ++c) mma_ss(d, fixed + step_k<kRows>(c), bd + step_k<F::kCols>(c), idesc, c > 0);
+          mma_commit(made);
+          mma_commit(&ctl.empty[it % F::kStages]);
+          return true;
+        };
+        for (int i = 0; i < n && ok; ++i) {
+          const int g = i % G;
+          const uint32_t before = (i / G - 1) & 1;  // phase of the group's tile before
+          if (i >= G && !(ok = mbar_wait(&ctl.dv_done[g], before, abort))) break;
+          if (!(ok = product(2 * i, tmem + F::s(g), kd, &ctl.s_full[g]))) break;
+          if (i >= G && !(ok = mbar_wait(&ctl.dk_done[g], before, abort))) break;
+          ok = product(2 * i + 1, tmem + F::dp(g), vd, &ctl.dp_full[g]);
+        }
+        mma_commit(&ctl.fin);
+        mbar_drain(&ctl.fin, 0);
+      } else {
+        const bool v = role == 1;  // dV takes dO, dK takes Q
+        const uint32_t idesc = idesc_bf16_f32(kRows, DP, false, true), acc = tmem + (v ? F::dv : F::dk);
+        for (int i = 0; i < n && ok; ++i) {
+          const int g = i % G, it = 2 * i + v;
+          if (!(ok = mbar_wait(v ? &ctl.p_ready[g] : &ctl.ds_ready[g], (i / G) & 1, abort) && full(it))) break;
+          tc_fence_after();
+          const uint32_t bd = desc_mn<F::kCols>(ring + (it % F::kStages) * F::kTile), p = tmem + (v ? F::s(g) : F::dp(g));
 #pragma unroll
-        for (int c = 0; c < F::kCols / 16; ++c) mma_ts(acc, d + C::step(c), bd + step_mn(c), idesc_d, i > 0 || c > 0);
-        mma_commit(done);
-        mma_commit(&ctl.empty[it % F::kStages]);
-        // the next scores take the columns this sum reads
-        if (i + 1 < n) ok = mbar_wait(done, i & 1, abort) && product(2 * (i + 1) + w);
+          for (int c = 0; c < F::kCols / 16; ++c) mma_ts(acc, p + c * 8, bd + step_mn(c), idesc, i > 0 || c > 0);
+          mma_commit(v ? &ctl.dv_done[g] : &ctl.dk_done[g]);
+          mma_commit(&ctl.empty[it % F::kStages]);
+        }
+        uint64_t* all = v ? &ctl.dv_all : &ctl.dk_all;
+        mma_commit(all);
+        mbar_drain(all, 0);
       }
-      mma_commit(&ctl.fin[w]);
-      mbar_drain(&ctl.fin[w], 0);
     }
-  } else if (warp < F::kLoadWarp) {
+  } else {
     reg_inc<F::kSoftmaxRegs>();
-    // ---- softmax arithmetic: thread = key, a warpgroup per half of a tile's queries
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane, key = r0 + row;
+    // ---- softmax arithmetic: thread = key
+    const int g = warp >> 2, row = (warp & 3) * 32 + lane, key = r0 + row;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c2 = a.scale * kLog2e;
+    float* sbias = sstat + F::kStages * 2 * F::kCols + g * bias_floats(a.span, a.n_buckets);
     const float* bias = sbias + a.span + kBiasPad;
+    // barrier of the group: see softmax_sync
+    auto group_sync = [&](bool ok) { return named_bar_and(1 + g, 128, ok); };
     bool ok = true, together = true;
-    for (int i = 0; i < n; ++i) {
-      const int st = 2 * i % F::kStages, q0 = (first + i % per_head) * F::kCols + half * 64;
-      if (a.table != nullptr && i % per_head == 0) {  // another head's table
-        if (!(together = softmax_sync<DP>())) break;
-        expand_bias(a, kv_head * group + i / per_head, 1, sbias, threadIdx.x, F::kSoftmax,
-                    [&] { together = softmax_sync<DP>(); });
-        if (!together || !(together = softmax_sync<DP>())) break;
+    int head_in = -1;  // whose bias table is there
+    for (int i = g; i < n; i += G) {
+      const int st = 2 * i % F::kStages, q0 = (first + i % per_head) * F::kCols, head = kv_head * group + i / per_head;
+      const uint32_t phase = (i / G) & 1;
+      if (a.table != nullptr && head != head_in) {
+        head_in = head;
+        if (!(together = group_sync(true))) break;
+        expand_bias(a, head, 1, sbias, threadIdx.x & 127, 128, [&] { together = group_sync(true); });
+        if (!together || !(together = group_sync(true))) break;
       }
-      ok = mbar_wait_warp(&ctl.stat_full[st], (2 * i / F::kStages) & 1, abort) && mbar_wait_warp(&ctl.s_full, i & 1, abort);
+      ok = mbar_wait_warp(&ctl.stat_full[st], (2 * i / F::kStages) & 1, abort) && mbar_wait_warp(&ctl.s_full[g], phase, abort);
       if (!ok) break;
       tc_fence_after();
-      float x[64];
+      float x[F::kCols];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) tmem_ld32_issue(lanes + C::s + half * 64 + h * 32, x + h * 32);
+      for (int h = 0; h < 2; ++h) tmem_ld32_issue(lanes + F::s(g) + h * 32, x + h * 32);
       tmem_wait_ld(x);
-      const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(sstat + st * 2 * F::kCols + half * 64);
+      const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(sstat + st * 2 * F::kCols);  // pairs of -lse
       const ulonglong2* delta = lse + F::kCols / 4;
       const int dist = q0 + off - key;  // of the first column
       float mul = c2, add = 0.f;
       if (a.table != nullptr) {
-        if (__all_sync(0xffffffffu, dist >= a.span || dist + 63 <= -a.span)) {
+        if (__all_sync(0xffffffffu, dist >= a.span || dist + F::kCols - 1 <= -a.span)) {
           add = dist > 0 ? bias[a.span] : bias[-a.span];
         } else {
-          const float* b = bias + max(-a.span - kBiasPad, min(dist, a.span + kBiasPad - 63));
+          const float* b = bias + max(-a.span - kBiasPad, min(dist, a.span + kBiasPad - F::kCols + 1));
 #pragma unroll
-          for (int c = 0; c < 64; ++c) x[c] = fmaf(x[c], c2, b[c]);
+          for (int c = 0; c < F::kCols; ++c) x[c] = fmaf(x[c], c2, b[c]);
           mul = 1.f;
         }
       }
       const uint64_t mul_2 = pair(mul, mul), add_2 = pair(add, add);
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const ulonglong2 e = lse[c / 4];  // two pairs of -lse
+      for (int c = 0; c < F::kCols; c += 4) {
+        const ulonglong2 e = lse[c / 4];
         unpair(fma2(pair(x[c], x[c + 1]), mul_2, add2(add_2, e.x)), x[c], x[c + 1]);
         unpair(fma2(pair(x[c + 2], x[c + 3]), mul_2, add2(add_2, e.y)), x[c + 2], x[c + 3]);
       }
 #pragma unroll
-      for (int c = 0; c < 64; ++c) x[c] = ex2(x[c]);
+      for (int c = 0; c < F::kCols; ++c) x[c] = ex2(x[c]);
       // columns of queries that see this key: [from, to)
       const int from = a.causal ? key - off - q0 : 0, to = s.lq - q0;
-      const bool masked = __any_sync(0xffffffffu, from > 0 || to < 64 || s.lk == 1 || (a.causal && q0 + off <= 0));
+      const bool masked = __any_sync(0xffffffffu, from > 0 || to < F::kCols || s.lk == 1 || (a.causal && q0 + off <= 0));
       if (masked) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) x[c] = c >= from && c < to ? x[c] : 0.f;
+        for (int c = 0; c < F::kCols; ++c) x[c] = c >= from && c < to ? x[c] : 0.f;
       }
-      uint32_t w[32];
+      uint32_t w[F::kCols / 2];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) w[c] = pack_bf16x2(x[2 * c], x[2 * c + 1]);
-      tmem_st32(lanes + C::s + half * 64, w);
+      for (int c = 0; c < F::kCols / 2; ++c) w[c] = pack_bf16x2(x[2 * c], x[2 * c + 1]);
+      tmem_st32(lanes + F::s(g), w);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&ctl.p_ready);
+      mbar_arrive(&ctl.p_ready[g]);
 
-      if (!(ok = mbar_wait_warp(&ctl.dp_full, i & 1, abort))) break;
+      if (!(ok = mbar_wait_warp(&ctl.dp_full[g], phase, abort))) break;
       tc_fence_after();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float d[32];
-        tmem_ld32_issue(lanes + C::dp + half * 64 + h * 32, d);
+        tmem_ld32_issue(lanes + F::dp(g) + h * 32, d);
         tmem_wait_ld(d);
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-          const ulonglong2 e = delta[(h * 32 + c) / 4];  // two pairs of -delta
+          const ulonglong2 e = delta[(h * 32 + c) / 4];  // pairs of -delta
           float* y = &x[h * 32 + c];
           unpair(mul2(pair(y[0], y[1]), add2(pair(d[c], d[c + 1]), e.x)), y[0], y[1]);
           unpair(mul2(pair(y[2], y[3]), add2(pair(d[c + 2], d[c + 3]), e.y)), y[2], y[3]);
@@ -602,25 +648,22 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       if (masked) {
         const int one = a.causal ? -off - q0 : -1;  // the query that sees one key
 #pragma unroll
-        for (int c = 0; c < 64; ++c) x[c] = c >= from && c < to && c != one && s.lk > 1 ? x[c] : 0.f;
+        for (int c = 0; c < F::kCols; ++c) x[c] = c >= from && c < to && c != one && s.lk > 1 ? x[c] : 0.f;
       }
 #pragma unroll
-      for (int c = 0; c < 32; ++c) w[c] = pack_bf16x2(x[2 * c], x[2 * c + 1]);
-      tmem_st32(lanes + C::dp + half * 64, w);
+      for (int c = 0; c < F::kCols / 2; ++c) w[c] = pack_bf16x2(x[2 * c], x[2 * c + 1]);
+      tmem_st32(lanes + F::dp(g), w);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&ctl.ds_ready[0]);
+      mbar_arrive(&ctl.ds_ready[g]);
     }
-    if (ok && together && n > 0)
-      ok = mbar_wait_warp(&ctl.dv_done, (n - 1) & 1, abort) && mbar_wait_warp(&ctl.dk_done, (n - 1) & 1, abort);
-    if (a.table != nullptr && together) together = softmax_sync<DP>(ok);
+    if (a.table != nullptr && together) together = group_sync(ok);
+    if (ok && together && n > 0) ok = mbar_wait_warp(&ctl.dv_all, 0, abort) && mbar_wait_warp(&ctl.dk_all, 0, abort);
     if (ok && together) {
       tc_fence_after();
       const int64_t at = ((int64_t)(s.k0 + key) * a.kv_heads + kv_head) * a.dim;
-      if (half == 0)
-        store_row<DP>(lanes + C::dv, static_cast<__nv_bfloat16*>(a.dv) + at, a.dim, 1.f, n == 0, row < n_rows);
-      if (half == F::kGroups - 1)
-        store_row<DP>(lanes + C::dk, static_cast<__nv_bfloat16*>(a.dk) + at, a.dim, a.scale, n == 0, row < n_rows);
+      if (g == 0) store_row<DP>(lanes + F::dv, static_cast<__nv_bfloat16*>(a.dv) + at, a.dim, 1.f, n == 0, row < n_rows);
+      if (g == G - 1) store_row<DP>(lanes + F::dk, static_cast<__nv_bfloat16*>(a.dk) + at, a.dim, a.scale, n == 0, row < n_rows);
     }
     tc_fence_before();
   }
@@ -653,9 +696,9 @@ int launch(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t s
   }
   if (n_k > 0) {
     a.tiles = k_tiles;
-    const size_t smem = 1024 + Bwd<DP>::kFloats + dkdv_floats<DP>(bias, a.span, a.n_buckets) * sizeof(float);
+    const size_t smem = 1024 + Kv<DP>::kFloats + dkdv_floats<DP>(bias, a.span, a.n_buckets) * sizeof(float);
     KF_CUDA_RET(cudaFuncSetAttribute(attention_dkdv_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    attention_dkdv_tc<DP><<<(unsigned)n_k * a.kv_heads, Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
+    attention_dkdv_tc<DP><<<(unsigned)n_k * a.kv_heads, Kv<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     return check_launch("kf_attention_bwd");
   }
   return KF_OK;
