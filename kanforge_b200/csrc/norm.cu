@@ -433,12 +433,12 @@ __global__ void __launch_bounds__(RING ? 384 : 512, RING && sizeof(TX) == 2 ? 2 
 }
 
 // One CTA walks over rows blockIdx.x * groups + group, + gridDim.x * groups, ...
-// The column sums stay with the lane that owns the columns, in registers while
-// that is 8 columns (widths to 4096), in shared memory above, and become one partial
+// The column sums stay with the lane that owns the columns, in registers for
+// widths to 4096, in shared memory above, and become one partial
 // sum per CTA in `part`.
-template <int V, bool VEC, typename TX, typename TB>
-__global__ void __launch_bounds__(512) residual_norm_bwd(const GradArgs p, int slots, int slot_bytes) {
-  constexpr bool REGS = V == 1, RING = VEC && REGS;
+template <int V, bool REGS, bool VEC, typename TX, typename TB>
+__global__ void __launch_bounds__(REGS && V > 1 ? 256 : 512) residual_norm_bwd(const GradArgs p, int slots, int slot_bytes) {
+  constexpr bool RING = VEC && REGS;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint64_t full[16 * kMaxSlots];
   const RowArgs& a = p.f;
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(512) residual_norm_bwd(const GradArgs p, int s
   float* exch = params + (REGS ? kParams * a.width : 0);
   RowGroup g{exch + group * 2 * a.warps * 3, a.warps, warp_id - group * a.warps, lane, 1 + group, 0};
   const int wl = g.warp * 32 + lane;
-  Chunk acc[REGS ? kSums : 1] = {};
+  Chunk acc[REGS ? kSums : 1][V] = {};
   const int64_t first = (int64_t)blockIdx.x * groups + group, step = (int64_t)gridDim.x * groups;
   RowRing ring;
   const uint32_t bx = a.width * sizeof(TX), bb = a.width * sizeof(TB);
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(512) residual_norm_bwd(const GradArgs p, int s
   // sums j of chunk c, pair k
   auto add = [&](int j, int c, int k, uint64_t v, uint64_t w) {  // += v w
     if (REGS) {
-      acc[REGS ? j : 0][k] = fma2(v, w, acc[REGS ? j : 0][k]);
+      acc[REGS ? j : 0][c][k] = fma2(v, w, acc[REGS ? j : 0][c][k]);
     } else {
       float lo, hi;
       unpair(mul2(v, w), lo, hi);
@@ -621,13 +621,15 @@ __global__ void __launch_bounds__(512) residual_norm_bwd(const GradArgs p, int s
 #pragma unroll
         for (int j = 0; j < kSums; ++j)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float lo, hi;
-            unpair(acc[REGS ? j : 0][k], lo, hi);
-            const int e0 = elem<VEC>(0, 2 * k, a.warps, wl), e1 = elem<VEC>(0, 2 * k + 1, a.warps, wl);
-            if (e0 < a.width) sums[j * a.width + e0] += lo;
-            if (e1 < a.width) sums[j * a.width + e1] += hi;
-          }
+          for (int c = 0; c < V; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float lo, hi;
+              unpair(acc[REGS ? j : 0][c][k], lo, hi);
+              const int e0 = elem<VEC>(c, 2 * k, a.warps, wl), e1 = elem<VEC>(c, 2 * k + 1, a.warps, wl);
+              if (e0 < a.width) sums[j * a.width + e0] += lo;
+              if (e1 < a.width) sums[j * a.width + e1] += hi;
+            }
       }
     }
   }
@@ -714,19 +716,19 @@ int launch_fwd(RowArgs a, cudaStream_t s) {
   return check_launch("kf_residual_norm_fwd");
 }
 
-template <int V, bool VEC, typename TX, typename TB>
+template <int V, bool REGS, bool VEC, typename TX, typename TB>
 int launch_bwd(GradArgs p, int ctas, cudaStream_t s) {
   const RowArgs& a = p.f;
-  const int groups = std::max(1, 15 / a.warps);  // one named barrier each
+  const int groups = REGS && V > 1 ? 8 : std::max(1, 15 / a.warps);  // one named barrier each
   const int slot_bytes = a.width * (int)(sizeof(TX) * (1 + (p.dy != nullptr)) +
                                          sizeof(TB) * ((p.dh != nullptr) + (a.branch != nullptr) + a.gate_token));
   // what is kept beside the rings: the parameters (widths to 4096) and the exchange buffers
-  const size_t beside = (V == 1 ? sizeof(float) * kParams * a.width : 0) + groups * 2 * a.warps * 3 * sizeof(float);
+  const size_t beside = (REGS ? sizeof(float) * kParams * a.width : 0) + groups * 2 * a.warps * 3 * sizeof(float);
   int slots = 0;
-  if (VEC && V == 1)
+  if (VEC && REGS)
     for (slots = kMaxSlots; slots > 2 && slots * groups * slot_bytes + beside > 220 * 1024;) --slots;
   const size_t smem = std::max<size_t>((size_t)groups * slots * slot_bytes, sizeof(float) * kSums * a.width) + beside;
-  auto* k = residual_norm_bwd<V, VEC, TX, TB>;
+  auto* k = residual_norm_bwd<V, REGS, VEC, TX, TB>;
   if (smem > 40 * 1024) KF_CUDA_RET(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   k<<<ctas, groups * a.warps * 32, smem, s>>>(p, slots, slot_bytes);
   return check_launch("kf_residual_norm_bwd");
@@ -755,11 +757,19 @@ int dispatch_fwd(RowArgs a, cudaStream_t s) {
   return v == 2 ? launch_fwd<2, VEC, false, TX, TB>(a, s) : launch_fwd<1, VEC, false, TX, TB>(a, s);
 }
 
+// Up to 768 columns a warp has a row to itself: its column sums fill the
+// registers of 8 warps an SM, but no row waits at a barrier.
 template <bool VEC, typename TX, typename TB>
 int dispatch_bwd(GradArgs p, int ctas, cudaStream_t s) {
-  const int per_warp = p.f.width <= 4096 ? 256 : 512;
-  p.f.warps = (int)cdiv(p.f.width, per_warp);
-  return per_warp == 256 ? launch_bwd<1, VEC, TX, TB>(p, ctas, s) : launch_bwd<2, VEC, TX, TB>(p, ctas, s);
+  const int chunks = (int)cdiv(p.f.width, 256);
+  if constexpr (VEC) {
+    p.f.warps = 1;
+    if (chunks == 2) return launch_bwd<2, true, VEC, TX, TB>(p, ctas, s);
+    if (chunks == 3) return launch_bwd<3, true, VEC, TX, TB>(p, ctas, s);
+  }
+  const bool regs = p.f.width <= 4096;
+  p.f.warps = (int)cdiv(chunks, regs ? 1 : 2);
+  return regs ? launch_bwd<1, true, VEC, TX, TB>(p, ctas, s) : launch_bwd<2, false, VEC, TX, TB>(p, ctas, s);
 }
 
 int check_common(const char* fn, const kf_residual_norm_desc* d, const void* x, const void* w, int64_t rows) {
