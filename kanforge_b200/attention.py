@@ -226,7 +226,7 @@ def _plan(seqs, q, k, v, causal, scale, bias) -> _Plan:
 
 
 def _forward(q, k, v, table, seqs, causal, scale, bias, train: bool):
-    """(o, rest, lse): the output, and for the backward what the rounding of a
+    """(o, rest, lse, plan): the output, and for the backward what the rounding of a
     bf16 output leaves out (delta = dout . o keeps float32's digits) and the
     logarithms of the sums."""
     q, k, v = _vectors(q), _vectors(k), _vectors(v)
@@ -244,30 +244,27 @@ def _forward(q, k, v, table, seqs, causal, scale, bias, train: bool):
                 None if table is None else table.data_ptr(), None if table is None else bias.buckets.data_ptr(),
                 o.data_ptr(), None if rest is None else rest.data_ptr(), None if lse is None else lse.data_ptr(),
                 plan.ref, _raw_stream(q))
-    return o, rest, lse
+    return o, rest, lse, plan
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, seqs, causal, scale, bias):
-        o, rest, lse = _forward(q, k, v, table, seqs, causal, scale, bias, train=True)
+        o, rest, lse, ctx.plan = _forward(q, k, v, table, seqs, causal, scale, bias, train=True)
         ctx.save_for_backward(q, k, v, table, o, rest, lse)
-        ctx.options = (seqs, causal, scale, bias)
+        ctx.seqs, ctx.buckets = seqs, None if bias is None else bias.buckets  # the tables the plan points to
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, table, o, rest, lse = ctx.saved_tensors
-        seqs, causal, scale, bias = ctx.options
-        need = ctx.needs_input_grad
+        plan, need = ctx.plan, ctx.needs_input_grad
         q, k, v = _vectors(q), _vectors(k), _vectors(v)
-        plan = _plan(seqs, q, k, v, causal, scale, bias)
         if dout.dtype != q.dtype or not dout.is_contiguous() or dout.data_ptr() % 16:
             dout = dout.to(q.dtype).clone(memory_format=torch.contiguous_format)
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        dk = torch.empty(k.shape, device=q.device, dtype=q.dtype)
-        dv = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+        dk, dv = torch.empty((2, *k.shape), device=q.device, dtype=q.dtype).unbind(0)
         want = table is not None and need[3]
         tab = None if table is None else table.detach().contiguous()
         dtable = torch.empty_like(tab) if want else None
@@ -277,7 +274,7 @@ class _Attention(torch.autograd.Function):
             _launch("kf_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                     None if rest is None else rest.data_ptr(), dout.data_ptr(), lse.data_ptr(),
                     q_tiles, n_q, k_tiles, n_k, None if tab is None else tab.data_ptr(),
-                    None if tab is None else bias.buckets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                    None if tab is None else ctx.buckets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                     None if dtable is None else dtable.data_ptr(), ws.data_ptr(), plan.ref, _raw_stream(q),
                     kernels=2 + (q.dtype == torch.float32) + 2 * want)
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None, None, None)

@@ -690,14 +690,16 @@ int launch(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t s
   if (int rc = map(&v_map, a.v, a.tk, a.kv_heads)) return rc;
   if (n_q > 0) {
     const size_t smem = 1024 + Bwd<DP>::kFloats + dq_floats<DP>(bias, a.dist_part != nullptr, a.span, a.n_buckets) * sizeof(float);
-    KF_CUDA_RET(cudaFuncSetAttribute(attention_dq_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static SmemAllowed allowed;
+    if (int rc = allow_smem(attention_dq_tc<DP>, smem, allowed)) return rc;
     attention_dq_tc<DP><<<(unsigned)n_q * a.heads, Bwd<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     if (int rc = check_launch("kf_attention_bwd")) return rc;
   }
   if (n_k > 0) {
     a.tiles = k_tiles;
     const size_t smem = 1024 + Kv<DP>::kFloats + dkdv_floats<DP>(bias, a.span, a.n_buckets) * sizeof(float);
-    KF_CUDA_RET(cudaFuncSetAttribute(attention_dkdv_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static SmemAllowed allowed1;
+    if (int rc = allow_smem(attention_dkdv_tc<DP>, smem, allowed1)) return rc;
     attention_dkdv_tc<DP><<<(unsigned)n_k * a.kv_heads, Kv<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     return check_launch("kf_attention_bwd");
   }

@@ -352,17 +352,18 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
   store_rows<T, D>(static_cast<T*>(a.dk), s.k0 + r0, n_rows, a.kv_heads, kv_head, a.dim, ty, tx, dk, mul);
 }
 
-template <typename K>
-int run(K* kernel, unsigned grid, size_t floats, const Args& a, cudaStream_t st, const char* what) {
-  KF_CUDA_RET(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(floats * sizeof(float))));
-  kernel<<<grid, kThreads, floats * sizeof(float), st>>>(a);
+template <void (*Kernel)(const Args)>
+int run(unsigned grid, size_t floats, const Args& a, cudaStream_t st, const char* what) {
+  static SmemAllowed allowed;
+  if (int rc = allow_smem(Kernel, floats * sizeof(float), allowed)) return rc;
+  Kernel<<<grid, kThreads, floats * sizeof(float), st>>>(a);
   return check_launch(what);
 }
 
 template <typename T, int D>
 int fwd(const Args& a, int n_tiles, cudaStream_t st) {
   const size_t bias = a.table != nullptr ? 2 * a.span + 1 : 0;
-  return run(attention_fwd<T, D>, (unsigned)n_tiles * a.heads, 3 * kTile * Ld<D>::row + kTile * kLdP + bias, a, st, "kf_attention_fwd");
+  return run<attention_fwd<T, D>>((unsigned)n_tiles * a.heads, 3 * kTile * Ld<D>::row + kTile * kLdP + bias, a, st, "kf_attention_fwd");
 }
 
 template <typename T, int D>
@@ -374,11 +375,11 @@ int bwd(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) 
     if (int rc = check_launch("kf_attention_bwd")) return rc;
   }
   if (n_q > 0)
-    if (int rc = run(attention_dq<T, D>, (unsigned)n_q * a.heads, 4 * kTile * Ld<D>::row + kTile * kLdP + 2 * bias, a, st, "kf_attention_bwd"))
+    if (int rc = run<attention_dq<T, D>>((unsigned)n_q * a.heads, 4 * kTile * Ld<D>::row + kTile * kLdP + 2 * bias, a, st, "kf_attention_bwd"))
       return rc;
   a.tiles = k_tiles;
   if (n_k > 0)
-    return run(attention_dkdv<T, D>, (unsigned)n_k * a.kv_heads, 4 * kTile * Ld<D>::row + 2 * kTile * kLdP + 2 * kTile + bias, a, st,
+    return run<attention_dkdv<T, D>>((unsigned)n_k * a.kv_heads, 4 * kTile * Ld<D>::row + 2 * kTile * kLdP + 2 * kTile + bias, a, st,
                "kf_attention_bwd");
   return KF_OK;
 }

@@ -309,7 +309,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
 template <int DP>
 int launch(const Args& a, int n_tiles, cudaStream_t st) {
   const size_t smem = Fwd<DP>::kSmem + (a.table != nullptr ? a.pack * bias_floats(a.span, a.n_buckets) * sizeof(float) : 0);
-  KF_CUDA_RET(cudaFuncSetAttribute(attention_fwd_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static SmemAllowed allowed;
+  if (int rc = allow_smem(attention_fwd_tc<DP>, smem, allowed)) return rc;
   CUtensorMap k_map, v_map;
   const bool keys = a.tk > 0;  // without keys no tile is loaded
   if (int rc = make_tile_map(&k_map, keys ? a.k.p : a.q.p, keys ? a.tk : 1, keys ? a.kv_heads : 1, a.dim, a.k.row, a.k.head)) return rc;

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 #include <string>
 
@@ -46,6 +47,23 @@ int check_launch(const char* what);
 // from worker threads on which this runtime has never run, and a process may
 // drive several GPUs.
 int bind_device(const void* ptr);
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device; asks
+// the runtime only when that is more than `allowed`, a static of the caller's
+// launch site, says.
+struct SmemAllowed {
+  std::atomic<int> bytes[16];
+};
+template <typename K>
+inline int allow_smem(K* kernel, size_t bytes, SmemAllowed& allowed) {
+  int dev = 0;
+  KF_CUDA_RET(cudaGetDevice(&dev));
+  std::atomic<int>* slot = dev < 16 ? &allowed.bytes[dev] : nullptr;
+  if (slot != nullptr && slot->load(std::memory_order_relaxed) >= (int)bytes) return KF_OK;
+  KF_CUDA_RET(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (slot != nullptr) slot->store((int)bytes, std::memory_order_relaxed);
+  return KF_OK;
+}
 
 // ---- device error word ----------------------------------------------------
 // Bit set by a kernel whose bounded wait ran out; read and cleared by

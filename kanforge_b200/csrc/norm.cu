@@ -710,7 +710,8 @@ int launch_fwd(RowArgs a, cudaStream_t s) {
     for (slots = kMaxSlots; slots > 1 && slots * groups * slot_bytes > 200 * 1024 / per_sm;) --slots;
   const size_t smem = (size_t)groups * slots * slot_bytes + groups * 2 * a.warps * 3 * sizeof(float);
   auto* k = residual_norm_fwd<V, VEC, RING, TX, TB>;
-  if (smem > 40 * 1024) KF_CUDA_RET(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static SmemAllowed allowed;
+  if (int rc = allow_smem(k, smem, allowed)) return rc;
   const int64_t ctas = cdiv(a.rows, groups);
   k<<<(unsigned)(RING ? std::min<int64_t>(ctas, per_sm * sm_count()) : ctas), groups * a.warps * 32, smem, s>>>(a, slots, slot_bytes);
   return check_launch("kf_residual_norm_fwd");
@@ -729,7 +730,8 @@ int launch_bwd(GradArgs p, int ctas, cudaStream_t s) {
     for (slots = kMaxSlots; slots > 2 && slots * groups * slot_bytes + beside > 220 * 1024;) --slots;
   const size_t smem = std::max<size_t>((size_t)groups * slots * slot_bytes, sizeof(float) * kSums * a.width) + beside;
   auto* k = residual_norm_bwd<V, REGS, VEC, TX, TB>;
-  if (smem > 40 * 1024) KF_CUDA_RET(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static SmemAllowed allowed1;
+  if (int rc = allow_smem(k, smem, allowed1)) return rc;
   k<<<ctas, groups * a.warps * 32, smem, s>>>(p, slots, slot_bytes);
   return check_launch("kf_residual_norm_bwd");
 }

@@ -84,6 +84,24 @@ class _Call:
         return y, h, stats
 
 
+_workspaces: dict = {}  # floats of the backward's workspace by (rows, width)
+
+
+def _workspace(rows: int, width: int) -> int:
+    n = _workspaces.get((rows, width))
+    if n is None:
+        if len(_workspaces) >= _DESCS_MAX:
+            _workspaces.clear()
+        n = _workspaces[rows, width] = int(_lib.load().kf_residual_norm_workspace(rows, width))
+    return n
+
+
+def _like(g, like):
+    if g.dtype != like.dtype:
+        g = g.to(like.dtype)
+    return g if g.is_contiguous() else g.contiguous()
+
+
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, branch, weight, bias, branch_weight, branch_bias, gate, kind, residual_scale, eps):
@@ -103,21 +121,29 @@ class _ResidualNorm(torch.autograd.Function):
             return (None,) * 10
         need = ctx.needs_input_grad
         call = _Call(x, branch, weight, bias, branch_weight, branch_bias, gate, *ctx.options)
-        x2 = call.x
-        mat = lambda g, like: None if g is None else g.to(like.dtype).contiguous()  # noqa: E731
-        dy, dh = mat(dy, x2), mat(dh, x2 if branch is None else call.branch)
+        x2, w = call.x, call.w
+        if dy is not None:
+            dy = _like(dy, x2)
+        if dh is not None:
+            dh = _like(dh, x2 if branch is None else call.branch)
         dx = torch.empty_like(x2)
-        new = lambda p: None if p is None else torch.empty_like(p)  # noqa: E731
-        dbranch, dgate, dw, ds, dbw, dbs = map(new, (call.branch, call.gate, call.w, call.s, call.bw, call.bs))
-        n_ws = int(_lib.load().kf_residual_norm_workspace(call.rows, call.width))
-        ws = torch.empty(n_ws, device=x2.device, dtype=torch.float32)
-        _launch("kf_residual_norm_bwd", _ptr(x2), _ptr(call.branch), _ptr(call.gate), _ptr(call.w), _ptr(call.bw),
-                _ptr(call.bs), _ptr(stats), _ptr(dy), _ptr(dh), _ptr(dx), _ptr(dbranch), _ptr(dgate), _ptr(dw), _ptr(ds),
-                _ptr(dbw), _ptr(dbs), _ptr(ws), call.rows, call.desc, _raw_stream(x2), kernels=2 if call.rows else 1)
-        like = lambda g, p, n: g.to(p.dtype) if n and p is not None else None  # noqa: E731
-        return (dx if need[0] else None, dbranch if need[1] else None, like(dw, weight, need[2]), like(ds, bias, need[3]),
-                like(dbw, branch_weight, need[4]), like(dbs, branch_bias, need[5]), like(dgate, gate, need[6]), None, None,
-                None)
+        dbranch = None if branch is None else torch.empty_like(call.branch)
+        # the parameters' gradients that are asked for, rows of one tensor
+        dgate = torch.empty_like(call.gate) if call.gate_token else None
+        asked = [need[2], need[3], need[4], need[5], need[6] and not call.gate_token]
+        out = torch.empty(sum(asked), call.width, device=w.device, dtype=w.dtype).unbind(0)
+        rows = iter(out)
+        dw, ds, dbw, dbs, dchannel = (next(rows) if a else None for a in asked)
+        if not call.gate_token:
+            dgate = dchannel
+        ws = torch.empty(_workspace(call.rows, call.width), device=w.device, dtype=torch.float32)
+        _launch("kf_residual_norm_bwd", x2.data_ptr(), _ptr(call.branch), _ptr(call.gate), w.data_ptr(), _ptr(call.bw),
+                _ptr(call.bs), stats.data_ptr(), _ptr(dy), _ptr(dh), dx.data_ptr(), _ptr(dbranch), _ptr(dgate), _ptr(dw),
+                _ptr(ds), _ptr(dbw), _ptr(dbs), ws.data_ptr(), call.rows, call.desc, _raw_stream(w),
+                kernels=2 if call.rows else 1)
+        cast = lambda g, p: g if g is None or g.dtype == p.dtype else g.to(p.dtype)  # noqa: E731
+        return (dx if need[0] else None, dbranch if need[1] else None, cast(dw, weight), cast(ds, bias),
+                cast(dbw, branch_weight), cast(dbs, branch_bias), cast(dgate, gate) if need[6] else None, None, None, None)
 
 
 def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
