@@ -7,12 +7,12 @@
 // in one launch, in slice order.
 //
 // bf16 runs on mma.sync m16n8k16: the 16 rows are query heads, and one token
-// leaves no room for the 128-row tcgen05 tiles.  K and V go from global memory
-// into fragments directly.  The contraction over D and the columns of the output may be
+// leaves no room for the 128-row tcgen05 tiles.  The contraction over D and the columns of the output may be
 // taken in any order, so lane (n, t) = (lane / 4, lane % 4) reads 16 bytes of K
 // row n at 32 i + 8 t and 16 bytes of V rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 at
-// 64 h + 8 n, and the fragments are what it read: whole sectors, no shared
-// memory.  P enters as the sum of two bf16 numbers (16 bits of it): twice the
+// 64 h + 8 n: whole sectors.  Every lane copies what it will use itself into a
+// ring in shared memory (cp.async, 16 keys to a stage), so that two stages are
+// under way behind the one in use and no lane waits for another.  P enters as the sum of two bf16 numbers (16 bits of it): twice the
 // products, which a kernel bound by memory has free, and no rounding of P.
 //
 // float32 runs on the CUDA cores: a lane holds 4 of the D columns, a warp takes
@@ -205,6 +205,12 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -213,15 +219,32 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ uint4 load16(const __nv_bfloat16* p, bool ok) {
   return ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const __nv_bfloat16* src, bool ok) {  // zeros where not ok
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 take16(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+  return v;
+}
 
 constexpr int kGroupBf16 = 16;
 
+constexpr int kStages = 3;
+// bytes of a warp's stage: its lanes' 16-byte pieces of 16 keys and values
 template <int DP>
-__global__ void __launch_bounds__(kWarps * 32) attention_decode_bf16(const DecodeArgs a) {
+constexpr int stage_bytes() { return 16 * DP * 2 * 2; }
+template <int DP>
+constexpr int decode_ring() {
+  return std::max<int>(kWarps * kStages * stage_bytes<DP>(), (int)sizeof(Partial<kGroupBf16>));
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kWarps * 32, DP == 64 ? 3 : 2) attention_decode_bf16(const DecodeArgs a) {
   constexpr int GC = kGroupBf16, KC = DP / 32, VC = DP / 64;
   extern __shared__ __align__(16) uint8_t smem[];
-  Partial<GC>* sp = reinterpret_cast<Partial<GC>*>(smem);
-  float* sbias = reinterpret_cast<float*>(sp + 1);
+  Partial<GC>* sp = reinterpret_cast<Partial<GC>*>(smem);  // in the ring's place, after it
+  float* sbias = reinterpret_cast<float*>(smem + decode_ring<DP>());
   const Part<GC> p(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t = lane & 3;
   load_bias(a, p, sbias);
@@ -237,42 +260,87 @@ __global__ void __launch_bounds__(kWarps * 32) attention_decode_bf16(const Decod
   __syncthreads();
   float o[VC][8][4] = {}, m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
   const float c2 = a.scale * kLog2e;
-  for (int key0 = p.first + warp * 16; key0 < p.last; key0 += kWarps * 16) {
-    uint4 k[2][KC], v[VC][4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kStages * stage_bytes<DP>() + lane * 16;
+  // Pieces of a stage: K (h, i), then V (h, r).  The lane's first piece of the next tile to fetch;
+  // columns past dim are zeros, rows past the slice too.
+  const __nv_bfloat16* kf = kp + (int64_t)(p.first + warp * 16 + n) * a.k_row + t * 8;
+  const __nv_bfloat16* vf = vp + (int64_t)(p.first + warp * 16 + 2 * t) * a.v_row + n * 8;
+  const int64_t k8 = 8 * a.k_row, v8 = 8 * a.v_row;
+  auto fetch = [&](int key0, int stage) {
+    const uint32_t at = ring + stage * stage_bytes<DP>();
+    if (key0 + 16 <= p.last && a.dim == DP) {
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
-        const int key = key0 + h * 8 + n;
-        k[h][i] = load16(kp + (int64_t)key * a.k_row + i * 32 + t * 8, key < p.last && i * 32 + t * 8 < a.dim);
+        copy16(at + i * 512, kf + i * 32, true);
+        copy16(at + (KC + i) * 512, kf + k8 + i * 32, true);
       }
 #pragma unroll
-    for (int h = 0; h < VC; ++h)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = key0 + (r >> 1) * 8 + 2 * t + (r & 1);
-        v[h][r] = load16(vp + (int64_t)key * a.v_row + h * 64 + n * 8, key < p.last && h * 64 + n * 8 < a.dim);
+      for (int h = 0; h < VC; ++h) {
+        copy16(at + (2 * KC + h * 4) * 512, vf + h * 64, true);
+        copy16(at + (2 * KC + h * 4 + 1) * 512, vf + a.v_row + h * 64, true);
+        copy16(at + (2 * KC + h * 4 + 2) * 512, vf + v8 + h * 64, true);
+        copy16(at + (2 * KC + h * 4 + 3) * 512, vf + v8 + a.v_row + h * 64, true);
       }
+    } else if (key0 < p.last) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+          const bool ok = key0 + h * 8 + n < p.last && i * 32 + t * 8 < a.dim;
+          copy16(at + (h * KC + i) * 512, ok ? kf + h * k8 + i * 32 : kp, ok);
+        }
+#pragma unroll
+      for (int h = 0; h < VC; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool ok = key0 + (r >> 1) * 8 + 2 * t + (r & 1) < p.last && h * 64 + n * 8 < a.dim;
+          copy16(at + (2 * KC + h * 4 + r) * 512, ok ? vf + (r >> 1) * v8 + (r & 1) * a.v_row + h * 64 : vp, ok);
+        }
+    }
+    kf += (int64_t)(kWarps * 16) * a.k_row, vf += (int64_t)(kWarps * 16) * a.v_row;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  constexpr int kStep = kWarps * 16;
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(p.first + warp * 16 + i * kStep, i);
+  int stage = 0;
+  for (int key0 = p.first + warp * 16; key0 < p.last; key0 += kStep) {
+    // the stage that was used last is free: every lane reads its own pieces only
+    fetch(key0 + (kStages - 1) * kStep, stage == 0 ? kStages - 1 : stage - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    const uint32_t at = ring + stage * stage_bytes<DP>();
+    if (++stage == kStages) stage = 0;
     float s[2][4] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
-        mma_bf16(s[h], q[i][0].x, q[i][1].x, q[i][0].y, q[i][1].y, k[h][i].x, k[h][i].y);
-        mma_bf16(s[h], q[i][0].z, q[i][1].z, q[i][0].w, q[i][1].w, k[h][i].z, k[h][i].w);
+        const uint4 k = take16(at + (h * KC + i) * 512);
+        mma_bf16(s[h], q[i][0].x, q[i][1].x, q[i][0].y, q[i][1].y, k.x, k.y);
+        mma_bf16(s[h], q[i][0].z, q[i][1].z, q[i][0].w, q[i][1].w, k.z, k.w);
       }
     // s[h][2 r + e]: head n + 8 r, key key0 + 8 h + 2 t + e
     float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
+    if (a.table != nullptr || key0 + 16 > p.last) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int key = key0 + h * 8 + 2 * t + (c & 1), g = n + 8 * (c >> 1);
+          float x = s[h][c] * c2;
+          if (a.table != nullptr && g < p.n_g && key < p.last) x += sbias[g * (2 * a.span + 1) + clamp_dist(p.len - 1 - key, a.span)];
+          s[h][c] = key < p.last ? x : -CUDART_INF_F;
+        }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[h][c] *= c2;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int key = key0 + h * 8 + 2 * t + (c & 1), g = n + 8 * (c >> 1);
-        float x = s[h][c] * c2;
-        if (a.table != nullptr && g < p.n_g && key < p.last) x += sbias[g * (2 * a.span + 1) + clamp_dist(p.len - 1 - key, a.span)];
-        s[h][c] = key < p.last ? x : -CUDART_INF_F;
-        top[c >> 1] = fmaxf(top[c >> 1], s[h][c]);
-      }
+      for (int c = 0; c < 4; ++c) top[c >> 1] = fmaxf(top[c >> 1], s[h][c]);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
@@ -298,26 +366,29 @@ __global__ void __launch_bounds__(kWarps * 32) attention_decode_bf16(const Decod
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float base = m[r] == -CUDART_INF_F ? 0.f : m[r];
-        const float e0 = exp2f(s[h][2 * r] - base), e1 = exp2f(s[h][2 * r + 1] - base);
+        const float e0 = ex2(s[h][2 * r] - base), e1 = ex2(s[h][2 * r + 1] - base);
         l[r] += e0 + e1;
         const uint32_t w = pack2(e0, e1);
         hi[h * 2 + r] = w;
         lo[h * 2 + r] = pack2(e0 - __uint_as_float(w << 16), e1 - __uint_as_float(w & 0xffff0000u));
       }
 #pragma unroll
-    for (int h = 0; h < VC; ++h)
+    for (int h = 0; h < VC; ++h) {
+      uint4 v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = take16(at + (2 * KC + h * 4 + r) * 512);
+      const uint32_t *r0 = &v[0].x, *r1 = &v[1].x, *r2 = &v[2].x, *r3 = &v[3].x;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t* r0 = &v[h][0].x;
-        const uint32_t* r1 = &v[h][1].x;
-        const uint32_t* r2 = &v[h][2].x;
-        const uint32_t* r3 = &v[h][3].x;
         const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
         const uint32_t b0 = __byte_perm(r0[j >> 1], r1[j >> 1], sel), b1 = __byte_perm(r2[j >> 1], r3[j >> 1], sel);
         mma_bf16(o[h][j], hi[0], hi[1], hi[2], hi[3], b0, b1);
         mma_bf16(o[h][j], lo[0], lo[1], lo[2], lo[3], b0, b1);
       }
+    }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();  // the rings are done with
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -335,10 +406,10 @@ __global__ void __launch_bounds__(kWarps * 32) attention_decode_bf16(const Decod
   join<__nv_bfloat16>(a, p, sp);
 }
 
-// Slices per sequence: about eight CTAs an SM (sequences differ in length, and
+// Slices per sequence: about four CTAs an SM (sequences differ in length, and
 // slices even that out), none shorter than 64 keys of a full cache.
 int split_count(int batch, int capacity, int ctas_per_sequence) {
-  const int64_t want = std::min<int64_t>(cdiv(148 * 8, (int64_t)batch * ctas_per_sequence), cdiv(capacity, 64));
+  const int64_t want = std::min<int64_t>(cdiv(148 * 4, (int64_t)batch * ctas_per_sequence), cdiv(capacity, 64));
   int splits = 1;
   while (splits < want && splits < kMaxSplits) splits *= 2;
   return splits;
@@ -390,7 +461,6 @@ extern "C" int kf_attention_decode(const void* q, const void* k, const void* v, 
   a.table_bf16 = d->table_dtype == KF_DTYPE_BF16, a.scale = d->scale;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d->dtype == KF_DTYPE_F32) return launch(attention_decode_f32, kGroupF32, 0, a, d->batch, st);
-  const size_t smem = sizeof(Partial<kGroupBf16>);
-  return d->dim <= 64 ? launch(attention_decode_bf16<64>, kGroupBf16, smem, a, d->batch, st)
-                      : launch(attention_decode_bf16<128>, kGroupBf16, smem, a, d->batch, st);
+  return d->dim <= 64 ? launch(attention_decode_bf16<64>, kGroupBf16, decode_ring<64>(), a, d->batch, st)
+                      : launch(attention_decode_bf16<128>, kGroupBf16, decode_ring<128>(), a, d->batch, st);
 }
