@@ -155,20 +155,22 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     // ---- MMAs: one warp S, then dQ, the other dP.  S of the next tile goes ahead of dQ of this one.
     if (lane == 0) {
       const uint32_t idesc_s = idesc_bf16_f32(kRows, F::kCols, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
+      auto full = [&](int it) { return mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort); };
       auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* done) {
-        if (!mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort)) return false;
         tc_fence_after();
         const uint32_t ad = desc_k(fixed), bd = desc_k(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) mma_ss(d, ad + step_k<kRows>(i), bd + step_k<F::kCols>(i), idesc_s, i > 0);
         mma_commit(done);
-        return true;
       };
       bool ok = mbar_wait(&ctl.fixed_full, 0, abort);
       if (warp == F::kMmaWarp) {
-        if (ok && n > 0) ok = product(0, tmem + C::s, q_tile, &ctl.s_full);
+        if (ok && n > 0 && (ok = full(0))) product(0, tmem + C::s, q_tile, &ctl.s_full);
         for (int j = 0; j < n && ok; ++j) {
-          if (j + 1 < n && !(ok = mbar_wait(&ctl.s_read, j & 1, abort) && product(2 * (j + 1), tmem + C::s, q_tile, &ctl.s_full))) break;
+          if (j + 1 < n) {
+            if (!(ok = full(2 * (j + 1)) && mbar_wait(&ctl.s_read, j & 1, abort))) break;
+            product(2 * (j + 1), tmem + C::s, q_tile, &ctl.s_full);
+          }
           if (!(ok = mbar_wait(&ctl.ds_ready[j & 1], (j >> 1) & 1, abort))) break;
           tc_fence_after();
           const uint32_t kd = desc_mn<F::kCols>(ring + (2 * j % F::kStages) * F::kTile);
@@ -180,9 +182,9 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         mma_commit(&ctl.dq_done);
       } else {
         for (int j = 0; j < n && ok; ++j) {
-          if (j > 0 && !(ok = mbar_wait(&ctl.ds_ready[(j - 1) & 1], ((j - 1) >> 1) & 1, abort))) break;
-          ok = product(2 * j + 1, tmem + C::dp, q_tile + F::kFixed, &ctl.dp_full);
-          if (ok) mma_commit(&ctl.empty[(2 * j + 1) % F::kStages]);
+          if (!(ok = full(2 * j + 1) && (j == 0 || mbar_wait(&ctl.ds_ready[(j - 1) & 1], ((j - 1) >> 1) & 1, abort)))) break;
+          product(2 * j + 1, tmem + C::dp, q_tile + F::kFixed, &ctl.dp_full);
+          mma_commit(&ctl.empty[(2 * j + 1) % F::kStages]);
         }
       }
       mma_commit(&ctl.fin[warp - F::kMmaWarp]);
@@ -527,22 +529,20 @@ __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
       if (role == 0) {
         const uint32_t idesc = idesc_bf16_f32(kRows, F::kCols, false, false), kd = desc_k(k_tile), vd = desc_k(k_tile + F::kFixed);
         auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* made) {
-          if (!full(it)) return false;
           tc_fence_after();
           const uint32_t bd = desc_k(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
           for (int c = 0; c < DP / 16; ++c) mma_ss(d, fixed + step_k<kRows>(c), bd + step_k<F::kCols>(c), idesc, c > 0);
           mma_commit(made);
           mma_commit(&ctl.empty[it % F::kStages]);
-          return true;
         };
         for (int i = 0; i < n && ok; ++i) {
           const int g = i % G;
           const uint32_t before = (i / G - 1) & 1;  // phase of the group's tile before
-          if (i >= G && !(ok = mbar_wait(&ctl.dv_done[g], before, abort))) break;
-          if (!(ok = product(2 * i, tmem + F::s(g), kd, &ctl.s_full[g]))) break;
-          if (i >= G && !(ok = mbar_wait(&ctl.dk_done[g], before, abort))) break;
-          ok = product(2 * i + 1, tmem + F::dp(g), vd, &ctl.dp_full[g]);
+          if (!(ok = full(2 * i) && (i < G || mbar_wait(&ctl.dv_done[g], before, abort)))) break;
+          product(2 * i, tmem + F::s(g), kd, &ctl.s_full[g]);
+          if (!(ok = full(2 * i + 1) && (i < G || mbar_wait(&ctl.dk_done[g], before, abort)))) break;
+          product(2 * i + 1, tmem + F::dp(g), vd, &ctl.dp_full[g]);
         }
         mma_commit(&ctl.fin);
         mbar_drain(&ctl.fin, 0);
@@ -551,7 +551,8 @@ __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
         const uint32_t idesc = idesc_bf16_f32(kRows, DP, false, true), acc = tmem + (v ? F::dv : F::dk);
         for (int i = 0; i < n && ok; ++i) {
           const int g = i % G, it = 2 * i + v;
-          if (!(ok = mbar_wait(v ? &ctl.p_ready[g] : &ctl.ds_ready[g], (i / G) & 1, abort) && full(it))) break;
+          // the tile is there long before: its barrier is looked at first, off the way from softmax to product
+          if (!(ok = full(it) && mbar_wait(v ? &ctl.p_ready[g] : &ctl.ds_ready[g], (i / G) & 1, abort))) break;
           tc_fence_after();
           const uint32_t bd = desc_mn<F::kCols>(ring + (it % F::kStages) * F::kTile), p = tmem + (v ? F::s(g) : F::dp(g));
 #pragma unroll
