@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl.tmem, q_tile = smem_u32(smem), ring = q_tile + F::kRing;
+  const uint32_t tmem = uniform(ctl.tmem), q_tile = uniform(smem_u32(smem)), ring = q_tile + F::kRing;
 
   if (warp >= F::kLoadWarp) reg_dec<F::kOtherRegs>();
   if (warp == F::kLoadWarp) {
@@ -153,42 +153,44 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     mbar_drain(&ctl.fixed_full, 0);
   } else if (warp >= F::kMmaWarp && warp < F::kMmaWarp + 2) {
     // ---- MMAs: one warp S, then dQ, the other dP.  S of the next tile goes ahead of dQ of this one.
-    if (lane == 0) {
+    {
+      const uint32_t leader = elect_lane();
+      const int who = uniform(warp - F::kMmaWarp), n_all = uniform(n);
       const uint32_t idesc_s = idesc_bf16_f32(kRows, F::kCols, false, false), idesc_d = idesc_bf16_f32(kRows, DP, false, true);
-      auto full = [&](int it) { return mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort); };
+      auto full = [&](int it) { return mbar_wait_warp(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort); };
       auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* done) {
         tc_fence_after();
         const uint32_t ad = desc_k(fixed), bd = desc_k(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) mma_ss(d, ad + step_k<kRows>(i), bd + step_k<F::kCols>(i), idesc_s, i > 0);
-        mma_commit(done);
+        for (int i = 0; i < DP / 16; ++i) mma_ss(leader, d, ad + step_k<kRows>(i), bd + step_k<F::kCols>(i), idesc_s, i > 0);
+        mma_commit(leader, done);
       };
-      bool ok = mbar_wait(&ctl.fixed_full, 0, abort);
-      if (warp == F::kMmaWarp) {
-        if (ok && n > 0 && (ok = full(0))) product(0, tmem + C::s, q_tile, &ctl.s_full);
-        for (int j = 0; j < n && ok; ++j) {
-          if (j + 1 < n) {
-            if (!(ok = full(2 * (j + 1)) && mbar_wait(&ctl.s_read, j & 1, abort))) break;
+      bool ok = mbar_wait_warp(&ctl.fixed_full, 0, abort);
+      if (who == 0) {
+        if (ok && n_all > 0 && (ok = full(0))) product(0, tmem + C::s, q_tile, &ctl.s_full);
+        for (int j = 0; j < n_all && ok; ++j) {
+          if (j + 1 < n_all) {
+            if (!(ok = full(2 * (j + 1)) && mbar_wait_warp(&ctl.s_read, j & 1, abort))) break;
             product(2 * (j + 1), tmem + C::s, q_tile, &ctl.s_full);
           }
-          if (!(ok = mbar_wait(&ctl.ds_ready[j & 1], (j >> 1) & 1, abort))) break;
+          if (!(ok = mbar_wait_warp(&ctl.ds_ready[j & 1], (j >> 1) & 1, abort))) break;
           tc_fence_after();
           const uint32_t kd = desc_mn<F::kCols>(ring + (2 * j % F::kStages) * F::kTile);
 #pragma unroll
           for (int i = 0; i < F::kCols / 16; ++i)
-            mma_ts(tmem + C::dq, tmem + C::ds + (j & 1) * C::ds_buffer + i * 8, kd + step_mn(i), idesc_d, j > 0 || i > 0);
-          mma_commit(&ctl.empty[2 * j % F::kStages]);
+            mma_ts(leader, tmem + C::dq, tmem + C::ds + (j & 1) * C::ds_buffer + i * 8, kd + step_mn(i), idesc_d, j > 0 || i > 0);
+          mma_commit(leader, &ctl.empty[2 * j % F::kStages]);
         }
-        mma_commit(&ctl.dq_done);
+        mma_commit(leader, &ctl.dq_done);
       } else {
-        for (int j = 0; j < n && ok; ++j) {
-          if (!(ok = full(2 * j + 1) && (j == 0 || mbar_wait(&ctl.ds_ready[(j - 1) & 1], ((j - 1) >> 1) & 1, abort)))) break;
+        for (int j = 0; j < n_all && ok; ++j) {
+          if (!(ok = full(2 * j + 1) && (j == 0 || mbar_wait_warp(&ctl.ds_ready[(j - 1) & 1], ((j - 1) >> 1) & 1, abort)))) break;
           product(2 * j + 1, tmem + C::dp, q_tile + F::kFixed, &ctl.dp_full);
-          mma_commit(&ctl.empty[(2 * j + 1) % F::kStages]);
+          mma_commit(leader, &ctl.empty[(2 * j + 1) % F::kStages]);
         }
       }
-      mma_commit(&ctl.fin[warp - F::kMmaWarp]);
-      mbar_drain(&ctl.fin[warp - F::kMmaWarp], 0);
+      mma_commit(leader, &ctl.fin[who]);
+      mbar_drain(&ctl.fin[who], 0);
     }
   } else if (warp < F::kLoadWarp) {
     reg_inc<F::kSoftmaxRegs>();
@@ -493,7 +495,7 @@ __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl.tmem, k_tile = smem_u32(smem), ring = k_tile + F::kRing;
+  const uint32_t tmem = uniform(ctl.tmem), k_tile = uniform(smem_u32(smem)), ring = k_tile + F::kRing;
 
   if (warp >= F::kLoadWarp) reg_dec<F::kOtherRegs>();
   if (warp == F::kLoadWarp) {
@@ -522,46 +524,47 @@ __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
     mbar_drain(&ctl.fixed_full, 0);
   } else if (warp >= F::kMmaWarp) {
     // ---- MMAs
-    if (lane == 0) {
-      const int role = warp - F::kMmaWarp;
-      auto full = [&](int it) { return mbar_wait(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort); };
-      bool ok = mbar_wait(&ctl.fixed_full, 0, abort);
+    {
+      const uint32_t leader = elect_lane();
+      const int role = uniform(warp - F::kMmaWarp), n_all = uniform(n);
+      auto full = [&](int it) { return mbar_wait_warp(&ctl.full[it % F::kStages], (it / F::kStages) & 1, abort); };
+      bool ok = mbar_wait_warp(&ctl.fixed_full, 0, abort);
       if (role == 0) {
         const uint32_t idesc = idesc_bf16_f32(kRows, F::kCols, false, false), kd = desc_k(k_tile), vd = desc_k(k_tile + F::kFixed);
         auto product = [&](int it, uint32_t d, uint32_t fixed, uint64_t* made) {
           tc_fence_after();
           const uint32_t bd = desc_k(ring + (it % F::kStages) * F::kTile);
 #pragma unroll
-          for (int c = 0; c < DP / 16; ++c) mma_ss(d, fixed + step_k<kRows>(c), bd + step_k<F::kCols>(c), idesc, c > 0);
-          mma_commit(made);
-          mma_commit(&ctl.empty[it % F::kStages]);
+          for (int c = 0; c < DP / 16; ++c) mma_ss(leader, d, fixed + step_k<kRows>(c), bd + step_k<F::kCols>(c), idesc, c > 0);
+          mma_commit(leader, made);
+          mma_commit(leader, &ctl.empty[it % F::kStages]);
         };
-        for (int i = 0; i < n && ok; ++i) {
+        for (int i = 0; i < n_all && ok; ++i) {
           const int g = i % G;
           const uint32_t before = (i / G - 1) & 1;  // phase of the group's tile before
-          if (!(ok = full(2 * i) && (i < G || mbar_wait(&ctl.dv_done[g], before, abort)))) break;
+          if (!(ok = full(2 * i) && (i < G || mbar_wait_warp(&ctl.dv_done[g], before, abort)))) break;
           product(2 * i, tmem + F::s(g), kd, &ctl.s_full[g]);
-          if (!(ok = full(2 * i + 1) && (i < G || mbar_wait(&ctl.dk_done[g], before, abort)))) break;
+          if (!(ok = full(2 * i + 1) && (i < G || mbar_wait_warp(&ctl.dk_done[g], before, abort)))) break;
           product(2 * i + 1, tmem + F::dp(g), vd, &ctl.dp_full[g]);
         }
-        mma_commit(&ctl.fin);
+        mma_commit(leader, &ctl.fin);
         mbar_drain(&ctl.fin, 0);
       } else {
         const bool v = role == 1;  // dV takes dO, dK takes Q
         const uint32_t idesc = idesc_bf16_f32(kRows, DP, false, true), acc = tmem + (v ? F::dv : F::dk);
-        for (int i = 0; i < n && ok; ++i) {
+        for (int i = 0; i < n_all && ok; ++i) {
           const int g = i % G, it = 2 * i + v;
           // the tile is there long before: its barrier is looked at first, off the way from softmax to product
-          if (!(ok = full(it) && mbar_wait(v ? &ctl.p_ready[g] : &ctl.ds_ready[g], (i / G) & 1, abort))) break;
+          if (!(ok = full(it) && mbar_wait_warp(v ? &ctl.p_ready[g] : &ctl.ds_ready[g], (i / G) & 1, abort))) break;
           tc_fence_after();
           const uint32_t bd = desc_mn<F::kCols>(ring + (it % F::kStages) * F::kTile), p = tmem + (v ? F::s(g) : F::dp(g));
 #pragma unroll
-          for (int c = 0; c < F::kCols / 16; ++c) mma_ts(acc, p + c * 8, bd + step_mn(c), idesc, i > 0 || c > 0);
-          mma_commit(v ? &ctl.dv_done[g] : &ctl.dk_done[g]);
-          mma_commit(&ctl.empty[it % F::kStages]);
+          for (int c = 0; c < F::kCols / 16; ++c) mma_ts(leader, acc, p + c * 8, bd + step_mn(c), idesc, i > 0 || c > 0);
+          mma_commit(leader, v ? &ctl.dv_done[g] : &ctl.dk_done[g]);
+          mma_commit(leader, &ctl.empty[it % F::kStages]);
         }
         uint64_t* all = v ? &ctl.dv_all : &ctl.dk_all;
-        mma_commit(all);
+        mma_commit(leader, all);
         mbar_drain(all, 0);
       }
     }

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
   tc_fence_after();
   constexpr int U = F::kUnit / kKeys;
   auto units = [](int n) { return (n + U - 1) / U; };  // streamed tiles that hold n sets of 64 keys
-  const uint32_t tmem = ctl.tmem, q_tile = smem_u32(smem), kv_tile = q_tile + NT * F::kQTile;
+  const uint32_t tmem = uniform(ctl.tmem), q_tile = uniform(smem_u32(smem)), kv_tile = q_tile + NT * F::kQTile;
 
   if (warp >= F::kLoadWarp) reg_dec<F::kOtherRegs>();
   if (warp == F::kLoadWarp) {
@@ -119,27 +119,28 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
     });
   } else if (warp >= F::kMmaWarp && warp < F::kMmaWarp + 2 * NT) {
     // ---- MMAs of row tile t
-    if (lane == 0 && n_max > 0) {
-      const int t = (warp - F::kMmaWarp) % NT, n = NT == 1 ? n_max : n_kv[t];
-      auto full = [&](int it) { return mbar_wait(&ctl.kv_full[it % F::kStages], (it / F::kStages) & 1, abort); };
+    if (n_max > 0) {
+      const uint32_t leader = elect_lane();
+      const int who = uniform(warp - F::kMmaWarp), t = who % NT, n_all = uniform(n_max), n = NT == 1 ? n_all : uniform(n_kv[t]);
+      auto full = [&](int it) { return mbar_wait_warp(&ctl.kv_full[it % F::kStages], (it / F::kStages) & 1, abort); };
       // the last set of scores that uses its streamed tile
       auto last_of = [&](int j) { return j % U == U - 1 || j == n - 1; };
-      bool ok = mbar_wait(&ctl.q_full, 0, abort);
+      bool ok = mbar_wait_warp(&ctl.q_full, 0, abort);
       int item;  // this warp's first streamed tile that only the other row tile uses
-      if (warp - F::kMmaWarp < NT) {
+      if (who < NT) {
         const uint32_t idesc = idesc_bf16_f32(kRows, DP, false, true);
         for (int j = 0; j < n && ok; ++j) {
           const int it = 2 * (j / U) + 1, h = j & 1;
-          if (!(ok = (j % U > 0 || full(it)) && mbar_wait(&ctl.p_ready[t][h], (j >> 1) & 1, abort))) break;
+          if (!(ok = (j % U > 0 || full(it)) && mbar_wait_warp(&ctl.p_ready[t][h], (j >> 1) & 1, abort))) break;
           tc_fence_after();
           const uint32_t vd = desc_mn<F::kUnit>(kv_tile + (it % F::kStages) * F::kTile) + step_mn(j % U * (kKeys / 16));
 #pragma unroll
           for (int i = 0; i < kKeys / 16; ++i)
-            mma_ts(tmem + F::o(t), tmem + F::p(t, h) + i * 8, vd + step_mn(i), idesc, j > 0 || i > 0);
-          mma_commit(&ctl.pv_done[t][h]);
-          if (last_of(j)) mma_commit(&ctl.kv_empty[it % F::kStages]);
+            mma_ts(leader, tmem + F::o(t), tmem + F::p(t, h) + i * 8, vd + step_mn(i), idesc, j > 0 || i > 0);
+          mma_commit(leader, &ctl.pv_done[t][h]);
+          if (last_of(j)) mma_commit(leader, &ctl.kv_empty[it % F::kStages]);
         }
-        mma_commit(&ctl.o_done[t]);
+        mma_commit(leader, &ctl.o_done[t]);
         item = 2 * units(n) + 1;
       } else {
         const uint32_t idesc = idesc_bf16_f32(kRows, kKeys, false, false), qd = desc_k(q_tile + t * F::kQTile);
@@ -147,23 +148,23 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
           const int it = 2 * (j / U), h = j & 1;
           if (j % U == 0 && !(ok = full(it))) break;
           // The scores of two sets before are read.  D = 128: they hold P by now, which P V has to be done with.
-          if (j >= 2 && !(ok = mbar_wait(DP == 64 ? &ctl.p_ready[t][h] : &ctl.pv_done[t][h], ((j >> 1) + 1) & 1, abort))) break;
+          if (j >= 2 && !(ok = mbar_wait_warp(DP == 64 ? &ctl.p_ready[t][h] : &ctl.pv_done[t][h], ((j >> 1) + 1) & 1, abort))) break;
           tc_fence_after();
           const uint32_t kd = desc_k(kv_tile + (it % F::kStages) * F::kTile) + j % U * (kKeys * 128 >> 4);
 #pragma unroll
           for (int i = 0; i < DP / 16; ++i)
-            mma_ss(tmem + F::s(t, h), qd + step_k<kRows>(i), kd + step_k<F::kUnit>(i), idesc, i > 0);
-          if (last_of(j)) mma_commit(&ctl.kv_empty[it % F::kStages]);
+            mma_ss(leader, tmem + F::s(t, h), qd + step_k<kRows>(i), kd + step_k<F::kUnit>(i), idesc, i > 0);
+          if (last_of(j)) mma_commit(leader, &ctl.kv_empty[it % F::kStages]);
           // D <= 64: the softmax writes P over that of two sets before, once P V is done with it
-          if (DP == 64 && j >= 2 && !(ok = mbar_wait(&ctl.pv_done[t][h], ((j >> 1) + 1) & 1, abort))) break;
-          mma_commit(&ctl.s_full[t][h]);
+          if (DP == 64 && j >= 2 && !(ok = mbar_wait_warp(&ctl.pv_done[t][h], ((j >> 1) + 1) & 1, abort))) break;
+          mma_commit(leader, &ctl.s_full[t][h]);
         }
         item = 2 * units(n);
       }
-      for (; item < 2 * units(n_max) && ok; item += 2)
-        if ((ok = full(item))) mbar_arrive(&ctl.kv_empty[item % F::kStages]);
-      mma_commit(&ctl.fin[warp - F::kMmaWarp]);
-      mbar_drain(&ctl.fin[warp - F::kMmaWarp], 0);
+      for (; item < 2 * units(n_all) && ok; item += 2)
+        if ((ok = full(item)) && leader) mbar_arrive(&ctl.kv_empty[item % F::kStages]);
+      mma_commit(leader, &ctl.fin[who]);
+      mbar_drain(&ctl.fin[who], 0);
     }
   } else if (warp < NT * 4) {
     reg_inc<F::kSoftmaxRegs>();
