@@ -19,7 +19,7 @@ from .convert import load, save
 from .layers import GRKAN, KAN, KANLinear, layer_inputs, rebuild_kan
 from .norm import ResidualNorm, residual_norm
 from .plan import KernelPlan, plan_for
-from .transformer import KANFFN
+from .transformer import KANFFN, KANTransformer, KANTransformerBlock, KVCache
 
 __version__ = "0.1.0"
 
@@ -32,6 +32,9 @@ __all__ = [
     "KANConv3d",
     "KANFFN",
     "KANLinear",
+    "KANTransformer",
+    "KANTransformerBlock",
+    "KVCache",
     "KernelPlan",
     "PackedSequences",
     "RelativeBias",

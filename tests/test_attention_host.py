@@ -97,3 +97,29 @@ def test_entry_points_check_their_arguments_before_any_cuda_call():
     x = ctypes.c_void_p(16)
     assert lib.kf_residual_norm_fwd(x, *[None] * 2, x, *[None] * 6, 1, ctypes.byref(d), None) == 1
     assert "outside" in _lib.last_error()
+
+
+def test_transformer_refusals_and_cache():
+    for bad in (dict(dim=48, depth=0, heads=6), dict(dim=48, depth=1, heads=5), dict(dim=48, depth=1, heads=12),
+                dict(dim=272, depth=1, heads=2), dict(dim=48, depth=1, heads=6, kv_heads=4)):
+        with pytest.raises(ValueError):
+            kb.KANTransformer(**bad)
+    m = kb.KANTransformer(48, 2, 6, 2, 64)
+    assert m.bias.heads == 6 and not m.bias.bidirectional
+    assert kb.KANTransformer(48, 1, 6, num_buckets=0).bias is None
+    cache = m.new_cache(3, 4)
+    assert cache.k.shape == cache.v.shape == (2, 3, 4, 2, 8)
+    seq, slot = cache.begin([2, 0, 3])
+    assert seq.tolist() == [0, 0, 2, 2, 2] and slot.tolist() == [0, 1, 0, 1, 2]
+    seq, slot = cache.step()
+    assert seq.tolist() == [0, 1, 2] and slot.tolist() == [2, 0, 3] and cache.lengths.tolist() == [3, 1, 4]
+    with pytest.raises(ValueError):
+        cache.step()
+    for lens in ([1, 2], [1, 2, 5], [1, -1, 2]):
+        with pytest.raises(ValueError):
+            cache.begin(lens)
+    with pytest.raises(ValueError):
+        kb.KVCache(1, 0, 4, 2, 8)
+    both = kb.KANTransformer(48, 1, 6, causal=False)
+    with pytest.raises(ValueError):
+        both.decode(torch.zeros(3, 48), both.new_cache(3, 4))
