@@ -720,14 +720,18 @@ int launch_fwd(RowArgs a, cudaStream_t s) {
 template <int V, bool REGS, bool VEC, typename TX, typename TB>
 int launch_bwd(GradArgs p, int ctas, cudaStream_t s) {
   const RowArgs& a = p.f;
-  const int groups = REGS && V > 1 ? 8 : std::max(1, 15 / a.warps);  // one named barrier each
+  constexpr size_t kLimit = 226 * 1024;  // of shared memory, beside the barriers
+  int groups = REGS && V > 1 ? 8 : std::max(1, 15 / a.warps);  // one named barrier each
   const int slot_bytes = a.width * (int)(sizeof(TX) * (1 + (p.dy != nullptr)) +
                                          sizeof(TB) * ((p.dh != nullptr) + (a.branch != nullptr) + a.gate_token));
   // what is kept beside the rings: the parameters (widths to 4096) and the exchange buffers
   const size_t beside = (REGS ? sizeof(float) * kParams * a.width : 0) + groups * 2 * a.warps * 3 * sizeof(float);
   int slots = 0;
-  if (VEC && REGS)
-    for (slots = kMaxSlots; slots > 2 && slots * groups * slot_bytes + beside > 220 * 1024;) --slots;
+  if (VEC && REGS) {
+    for (slots = kMaxSlots; slots > 2 && slots * groups * slot_bytes + beside > kLimit;) --slots;
+    // float32 rows of 700 to 768 elements with a gate per token: two slots for each of 8 warps are too much
+    while (groups > 1 && slots * groups * slot_bytes + beside > kLimit) --groups;
+  }
   const size_t smem = std::max<size_t>((size_t)groups * slots * slot_bytes, sizeof(float) * kSums * a.width) + beside;
   auto* k = residual_norm_bwd<V, REGS, VEC, TX, TB>;
   static SmemAllowed allowed1;

@@ -226,3 +226,27 @@ def test_refusals():
         kb.residual_norm(torch.randn(2, 8200, device="cuda"), None, torch.ones(8200, device="cuda"))
     with pytest.raises(RuntimeError):
         kb.residual_norm(x.cpu(), x.cpu(), w.cpu())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,width", [(2371, 200), (1203, 512), (801, 768), (597, 1024), (483, 1280), (301, 2048), (397, 3000),
+                                        (151, 4096), (103, 6144), (81, 8192)])
+def test_many_rows(rows, width, dtype):
+    """Enough rows for each group of warps to walk over several, by every number of warps to a row."""
+    check(inputs((rows, width), "layer", "token", True, dtype), "layer", 0.9)
+    check(inputs((rows, width), "rms", "channel", False, dtype), "rms", 1.0)
+
+
+@pytest.mark.parametrize("width", [768, 4096])
+def test_repeats_to_the_bit(width):
+    t = inputs((3000, width), "layer", "channel", True, torch.bfloat16)
+    g = torch.randn(3000, width, device="cuda").bfloat16()
+
+    def run():
+        leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+        y, h = kb.residual_norm(leaves["x"], leaves["branch"], leaves["weight"], leaves["bias"], gate=leaves["gate"],
+                                branch_norm=True, branch_weight=leaves["branch_weight"], branch_bias=leaves["branch_bias"])
+        return [y, h, *torch.autograd.grad([y, h], list(leaves.values()), [g, g])]
+
+    for a, b in zip(run(), run()):
+        assert torch.equal(a, b)
