@@ -24,14 +24,14 @@ struct Ld {
 };
 constexpr int kLdP = kTile + 4;
 
-// A tile of up to 64 rows into shared memory as float32; rows past `n` and
+// A tile of up to 64 rows into shared memory; rows past `n` and
 // columns past `dim` are zero, so nothing outside the sequence enters a sum.
-template <typename T, int D>
+template <int D>
 __device__ __forceinline__ void load_rows(float* dst, const Strided& s, int64_t row0, int n, int head, int dim) {
-  const T* p = static_cast<const T*>(s.p) + head * s.head;
+  const float* p = static_cast<const float*>(s.p) + head * s.head;
   for (int i = threadIdx.x; i < kTile * D; i += kThreads) {
     const int r = i / D, c = i % D;
-    dst[r * Ld<D>::row + c] = (r < n && c < dim) ? to_f32<T>(p[(row0 + r) * s.row + c]) : 0.f;
+    dst[r * Ld<D>::row + c] = (r < n && c < dim) ? p[(row0 + r) * s.row + c] : 0.f;
   }
 }
 
@@ -79,20 +79,20 @@ __device__ __forceinline__ void dot_cols(const float* p, const float* m, int ty,
   }
 }
 
-template <typename T, int D>
-__device__ __forceinline__ void store_rows(T* out, int64_t row0, int n, int heads, int head, int dim, int ty, int tx,
+template <int D>
+__device__ __forceinline__ void store_rows(float* out, int64_t row0, int n, int heads, int head, int dim, int ty, int tx,
                                            const float (&acc)[4][D / 16], const float (&mul)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = ty * 4 + i;
     if (r >= n) continue;
-    T* p = out + ((row0 + r) * heads + head) * dim;
+    float* p = out + ((row0 + r) * heads + head) * dim;
 #pragma unroll
     for (int q = 0; q < D / 64; ++q)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int col = tx * 4 + 64 * q + c;
-        if (col < dim) p[col] = from_f32<T>(acc[i][4 * q + c] * mul[i]);
+        if (col < dim) p[col] = acc[i][4 * q + c] * mul[i];
       }
   }
 }
@@ -108,7 +108,7 @@ __device__ __forceinline__ float half_sum(float v) {
   return v;
 }
 
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
   extern __shared__ __align__(16) float smem[];
   float* sq = smem;
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
   const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const int r0 = tile * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  load_rows<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
+  load_rows<D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
   if (a.table != nullptr) expand_bias_f32(a, head, sbias, threadIdx.x, kThreads);
   float m[4], l[4], o[4][D / 16];
 #pragma unroll
@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
   for (int k0 = 0; k0 < k_end; k0 += kTile) {
     const int n_keys = min(kTile, s.lk - k0);
     __syncthreads();
-    load_rows<T, D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
-    load_rows<T, D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_rows<D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_rows<D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
     __syncthreads();
     float t[4][4] = {};
     dot_rows<D>(sq, sk, ty, tx, t);
@@ -178,28 +178,26 @@ __global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
     if (a.lse != nullptr && tx == 0 && r < n_rows)
       a.lse[head * a.tq + s.q0 + r0 + r] = l[i] == 0.f ? 0.f : m[i] + log2f(l[i]);
   }
-  store_rows<T, D>(static_cast<T*>(a.o), s.q0 + r0, n_rows, a.heads, head, a.dim, ty, tx, o, inv);
+  store_rows<D>(static_cast<float*>(a.o), s.q0 + r0, n_rows, a.heads, head, a.dim, ty, tx, o, inv);
 }
 
 // delta[h][i] = dO_i . O_i: one warp per (token, head).
-template <typename T>
 __global__ void __launch_bounds__(256) attention_delta(const Args a) {
   const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (i >= a.tq * a.heads) return;
   const int64_t tok = i / a.heads;
   const int head = (int)(i - tok * a.heads), lane = threadIdx.x & 31;
-  const T* o = static_cast<const T*>(a.o) + i * a.dim;
-  const T* g = static_cast<const T*>(a.dout.p) + tok * a.dout.row + head * a.dout.head;
+  const float* o = static_cast<const float*>(a.o) + i * a.dim;
+  const float* g = static_cast<const float*>(a.dout.p) + tok * a.dout.row + head * a.dout.head;
   float v = 0.f;
-  const T* rest = a.o_rest == nullptr ? nullptr : static_cast<const T*>(a.o_rest) + i * a.dim;
-  for (int c = lane; c < a.dim; c += 32) v = fmaf(to_f32<T>(o[c]) + (rest ? to_f32<T>(rest[c]) : 0.f), to_f32<T>(g[c]), v);
+  for (int c = lane; c < a.dim; c += 32) v = fmaf(o[c], g[c], v);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
   if (lane == 0) a.delta[head * a.tq + tok] = v;
 }
 
 // Rows = queries: dQ = scale dS K, and the bias gradient's sums by distance.
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
   extern __shared__ __align__(16) float smem[];
   float* sq = smem;
@@ -214,8 +212,8 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
   const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const int r0 = tile * kTile, n_rows = min(kTile, s.lq - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  load_rows<T, D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
-  load_rows<T, D>(sg, a.dout, s.q0 + r0, n_rows, head, a.dim);
+  load_rows<D>(sq, a.q, s.q0 + r0, n_rows, head, a.dim);
+  load_rows<D>(sg, a.dout, s.q0 + r0, n_rows, head, a.dim);
   if (a.table != nullptr) {
     expand_bias_f32(a, head, sbias, threadIdx.x, kThreads);
     for (int i = threadIdx.x; i < 2 * a.span + 1; i += kThreads) ssum[i] = 0.f;
@@ -234,8 +232,8 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
   for (int k0 = 0; k0 < k_end; k0 += kTile) {
     const int n_keys = min(kTile, s.lk - k0);
     __syncthreads();
-    load_rows<T, D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
-    load_rows<T, D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_rows<D>(sk, a.k, s.k0 + k0, n_keys, kv_head, a.dim);
+    load_rows<D>(sv, a.v, s.k0 + k0, n_keys, kv_head, a.dim);
     __syncthreads();
     float t[4][4] = {}, dp[4][4] = {};
     dot_rows<D>(sq, sk, ty, tx, t);
@@ -276,7 +274,7 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
     }
   }
   const float mul[4] = {a.scale, a.scale, a.scale, a.scale};
-  store_rows<T, D>(static_cast<T*>(a.dq), s.q0 + r0, n_rows, a.heads, head, a.dim, ty, tx, dq, mul);
+  store_rows<D>(static_cast<float*>(a.dq), s.q0 + r0, n_rows, a.heads, head, a.dim, ty, tx, dq, mul);
   if (a.dist_part != nullptr) {
     __syncthreads();
     float* out = a.dist_part + (int64_t)blockIdx.x * (2 * a.span + 1);
@@ -285,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
 }
 
 // Rows = keys: dV = P^T dO and dK = scale dS^T Q, summed over the heads of the group.
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
   extern __shared__ __align__(16) float smem[];
   float* sk = smem;
@@ -302,8 +300,8 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
   const int kv_head = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
   const int r0 = tile * kTile, n_rows = min(kTile, s.lk - r0), off = s.lk - s.lq;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  load_rows<T, D>(sk, a.k, s.k0 + r0, n_rows, kv_head, a.dim);
-  load_rows<T, D>(sv, a.v, s.k0 + r0, n_rows, kv_head, a.dim);
+  load_rows<D>(sk, a.k, s.k0 + r0, n_rows, kv_head, a.dim);
+  load_rows<D>(sv, a.v, s.k0 + r0, n_rows, kv_head, a.dim);
   float dk[4][D / 16], dv[4][D / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -317,8 +315,8 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
     for (int q0 = q_first; q0 < s.lq; q0 += kTile) {
       const int n_q = min(kTile, s.lq - q0);
       __syncthreads();
-      load_rows<T, D>(sq, a.q, s.q0 + q0, n_q, head, a.dim);
-      load_rows<T, D>(sg, a.dout, s.q0 + q0, n_q, head, a.dim);
+      load_rows<D>(sq, a.q, s.q0 + q0, n_q, head, a.dim);
+      load_rows<D>(sg, a.dout, s.q0 + q0, n_q, head, a.dim);
       if (threadIdx.x < kTile) {
         const bool in = (int)threadIdx.x < n_q;
         slse[threadIdx.x] = in ? a.lse[head * a.tq + s.q0 + q0 + threadIdx.x] : 0.f;
@@ -348,8 +346,8 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
     }
   }
   const float one[4] = {1.f, 1.f, 1.f, 1.f}, mul[4] = {a.scale, a.scale, a.scale, a.scale};
-  store_rows<T, D>(static_cast<T*>(a.dv), s.k0 + r0, n_rows, a.kv_heads, kv_head, a.dim, ty, tx, dv, one);
-  store_rows<T, D>(static_cast<T*>(a.dk), s.k0 + r0, n_rows, a.kv_heads, kv_head, a.dim, ty, tx, dk, mul);
+  store_rows<D>(static_cast<float*>(a.dv), s.k0 + r0, n_rows, a.kv_heads, kv_head, a.dim, ty, tx, dv, one);
+  store_rows<D>(static_cast<float*>(a.dk), s.k0 + r0, n_rows, a.kv_heads, kv_head, a.dim, ty, tx, dk, mul);
 }
 
 template <void (*Kernel)(const Args)>
@@ -360,26 +358,26 @@ int run(unsigned grid, size_t floats, const Args& a, cudaStream_t st, const char
   return check_launch(what);
 }
 
-template <typename T, int D>
+template <int D>
 int fwd(const Args& a, int n_tiles, cudaStream_t st) {
   const size_t bias = a.table != nullptr ? 2 * a.span + 1 : 0;
-  return run<attention_fwd<T, D>>((unsigned)n_tiles * a.heads, 3 * kTile * Ld<D>::row + kTile * kLdP + bias, a, st, "kf_attention_fwd");
+  return run<attention_fwd<D>>((unsigned)n_tiles * a.heads, 3 * kTile * Ld<D>::row + kTile * kLdP + bias, a, st, "kf_attention_fwd");
 }
 
-template <typename T, int D>
+template <int D>
 int bwd(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) {
   Args a = a0;
   const size_t bias = a.table != nullptr ? 2 * a.span + 1 : 0;
   if (a.tq > 0) {
-    attention_delta<T><<<(unsigned)cdiv(a.tq * a.heads, 8), 256, 0, st>>>(a);
+    attention_delta<<<(unsigned)cdiv(a.tq * a.heads, 8), 256, 0, st>>>(a);
     if (int rc = check_launch("kf_attention_bwd")) return rc;
   }
   if (n_q > 0)
-    if (int rc = run<attention_dq<T, D>>((unsigned)n_q * a.heads, 4 * kTile * Ld<D>::row + kTile * kLdP + 2 * bias, a, st, "kf_attention_bwd"))
+    if (int rc = run<attention_dq<D>>((unsigned)n_q * a.heads, 4 * kTile * Ld<D>::row + kTile * kLdP + 2 * bias, a, st, "kf_attention_bwd"))
       return rc;
   a.tiles = k_tiles;
   if (n_k > 0)
-    return run<attention_dkdv<T, D>>((unsigned)n_k * a.kv_heads, 4 * kTile * Ld<D>::row + 2 * kTile * kLdP + 2 * kTile + bias, a, st,
+    return run<attention_dkdv<D>>((unsigned)n_k * a.kv_heads, 4 * kTile * Ld<D>::row + 2 * kTile * kLdP + 2 * kTile + bias, a, st,
                "kf_attention_bwd");
   return KF_OK;
 }
@@ -388,10 +386,10 @@ int bwd(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) 
 
 namespace attn {
 int fwd_f32(const Args& a, int n_tiles, cudaStream_t st) {
-  return a.dim <= 64 ? fwd<float, 64>(a, n_tiles, st) : fwd<float, 128>(a, n_tiles, st);
+  return a.dim <= 64 ? fwd<64>(a, n_tiles, st) : fwd<128>(a, n_tiles, st);
 }
 int bwd_f32(const Args& a, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) {
-  return a.dim <= 64 ? bwd<float, 64>(a, k_tiles, n_q, n_k, st) : bwd<float, 128>(a, k_tiles, n_q, n_k, st);
+  return a.dim <= 64 ? bwd<64>(a, k_tiles, n_q, n_k, st) : bwd<128>(a, k_tiles, n_q, n_k, st);
 }
 }  // namespace attn
 }  // namespace kf

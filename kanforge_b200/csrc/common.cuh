@@ -60,7 +60,9 @@ inline int allow_smem(K* kernel, size_t bytes, SmemAllowed& allowed) {
   KF_CUDA_RET(cudaGetDevice(&dev));
   std::atomic<int>* slot = dev < 16 ? &allowed.bytes[dev] : nullptr;
   if (slot != nullptr && slot->load(std::memory_order_relaxed) >= (int)bytes) return KF_OK;
-  KF_CUDA_RET(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (err != cudaSuccess) cudaGetLastError();  // a refusal is this call's, not the next launch's
+  KF_CUDA_RET(err);
   if (slot != nullptr) slot->store((int)bytes, std::memory_order_relaxed);
   return KF_OK;
 }
