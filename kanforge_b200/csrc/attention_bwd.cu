@@ -100,7 +100,9 @@ constexpr int kDiag = 48;                       // of a block of 32 x 16 scores:
 constexpr int kDiagWarp = 7 * kDiag + 32;       // four blocks, and what their unused stores reach
 template <int DP>
 __host__ __device__ constexpr int dq_floats(bool bias, bool grad, int span, int n_buckets) {
-  return 2 * kRows + (bias ? bias_floats(span, n_buckets) : 0) + (grad ? 4 * (2 * span + 1) + Bwd<DP>::kLoadWarp * kDiagWarp : 0);
+  static_assert(Bwd<DP>::kLoadWarp * kDiagWarp >= kMaxBuckets);
+  return 2 * kRows + (bias ? bias_stride(span) : 0) +
+         (grad ? 4 * (2 * span + 1) + Bwd<DP>::kLoadWarp * kDiagWarp : bias ? n_buckets : 0);
 }
 
 template <int DP>
@@ -116,8 +118,9 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   float* sdelta = reinterpret_cast<float*>(smem + F::kFloats);  // (groups, 128) parts of delta
   float* sbias = sdelta + 2 * kRows;
   const int n_dist = 2 * a.span + 1;
-  float* ssum = sbias + (a.table != nullptr ? bias_floats(a.span, a.n_buckets) : 0);  // (4, n_dist)
-  float* sdiag = ssum + 4 * n_dist;                                                   // (warps, kDiagWarp)
+  float* ssum = sbias + (a.table != nullptr ? bias_stride(a.span) : 0);  // (4, n_dist)
+  float* sdiag = ssum + 4 * n_dist;                                      // (warps, kDiagWarp)
+  float* column = a.dist_part != nullptr ? sdiag : ssum;  // of the learned table, needed before either is
   volatile int* abort = &ctl.abort;
 
   int tile;
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     }
     if (grad)
       for (int i = threadIdx.x; i < 4 * n_dist; i += F::kSoftmax) ssum[i] = 0.f;
-    if (a.table != nullptr) expand_bias(a, head, 1, sbias, threadIdx.x, F::kSoftmax, [] { softmax_sync<DP>(); });
+    if (a.table != nullptr) expand_bias(a, head, 1, sbias, column, threadIdx.x, F::kSoftmax, [] { softmax_sync<DP>(); });
     softmax_sync<DP>();
     float delta = sdelta[row];
     if (F::kGroups == 2) softmax_sync<DP>();  // sdelta is written again below
@@ -586,7 +589,7 @@ __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
       if (a.table != nullptr && head != head_in) {
         head_in = head;
         if (!(together = group_sync(true))) break;
-        expand_bias(a, head, 1, sbias, threadIdx.x & 127, 128, [&] { together = group_sync(true); });
+        expand_bias(a, head, 1, sbias, sbias + bias_stride(a.span), threadIdx.x & 127, 128, [&] { together = group_sync(true); });
         if (!together || !(together = group_sync(true))) break;
       }
       ok = mbar_wait_warp(&ctl.stat_full[st], (2 * i / F::kStages) & 1, abort) && mbar_wait_warp(&ctl.s_full[g], phase, abort);

@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
                                a.q.head, pack, r0 + t * kRows, rows, a.dim, row);
     cp_async_commit();
     if (a.table != nullptr)
-      expand_bias(a, head0, pack, sbias, threadIdx.x, F::kSoftmax, [] { named_bar_and(1, F::kSoftmax, true); });
+      expand_bias(a, head0, pack, sbias, sbias + pack * bias_stride(a.span), threadIdx.x, F::kSoftmax,
+                  [] { named_bar_and(1, F::kSoftmax, true); });
     cp_async_wait<0>();
     fence_proxy_async_smem();
     mbar_arrive(&ctl.q_full);

@@ -289,16 +289,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// The padded bias tables of `pack` heads (index distance + span + kBiasPad), with
-// room behind them for the heads' columns of the learned table.  The columns and
+// The padded bias tables of `pack` heads (index distance + span + kBiasPad);
+// `column` has room for the heads' columns of the learned table.  The columns and
 // the bucket numbers are read side by side, so that one trip to memory is waited
 // for; sync() is a barrier of the `n_threads` threads.
 __host__ __device__ constexpr int bias_floats(int span, int n_buckets) { return bias_stride(span) + n_buckets; }
 
 template <typename Sync>
-__device__ __forceinline__ void expand_bias(const Args& a, int head0, int pack, float* out, int thread, int n_threads, Sync&& sync) {
+__device__ __forceinline__ void expand_bias(const Args& a, int head0, int pack, float* out, float* column, int thread, int n_threads,
+                                            Sync&& sync) {
   const int n = bias_stride(a.span);
-  float* column = out + pack * n;
   for (int i = thread; i < pack * a.n_buckets; i += n_threads) {
     const int64_t e = (int64_t)(i % a.n_buckets) * a.heads + head0 + i / a.n_buckets;
     column[i] = bias_base2(a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[e])

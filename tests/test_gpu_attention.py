@@ -378,3 +378,13 @@ def test_decode_refusals():
         kb.attention_decode(q.requires_grad_(), k, v, n)
     with pytest.raises(RuntimeError):
         kb.attention_decode(q.detach().cpu(), k.cpu(), v.cpu(), n.cpu())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 128), (4, 1, 96), (8, 2, 64)])
+def test_the_largest_bias_table(heads, kv_heads, dim, dtype):
+    lens = [300, 1, 700]
+    bias = kb.RelativeBias(heads, 256, 512, bidirectional=True, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        bias.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
+    check(*make(lens, lens, heads, kv_heads, dim, dtype), lens, lens, False, bias=bias)
