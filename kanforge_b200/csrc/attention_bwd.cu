@@ -251,6 +251,16 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     const float c2 = a.scale * kLog2e;
     const float* bias = sbias + a.span + kBiasPad;
     float far_sum[2] = {0.f, 0.f};  // dS at distances >= span, <= -span
+    // Sum over the keys P dP = dO . O only as far as O's P was rounded, while a row's dS add up to 0: what they do
+    // add up to goes off the sums of the tiles beyond the span, by the share of P there.  Elsewhere the keys of a
+    // bucket are too few for it to show.
+    float row_sum = 0.f, far_p[2] = {0.f, 0.f};
+    auto sum64 = [](const float (&v)[64]) {
+      uint64_t t[4] = {pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7])};
+#pragma unroll
+      for (int i = 8; i < 64; i += 2) t[i / 2 & 3] = add2(t[i / 2 & 3], pair(v[i], v[i + 1]));
+      return sum_of(add2(add2(t[0], t[1]), add2(t[2], t[3])));
+    };
     bool ok = true, together = true, owed = F::kGroups == 2 && short_rows && n > 0;  // owed: the barrier of delta is still ahead
     for (int j = 0; j < n; ++j) {
       if (!(ok = mbar_wait_warp(&ctl.s_full, j & 1, abort))) break;
@@ -283,6 +293,9 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
 #pragma unroll
       for (int i = 0; i < 64; ++i) x[i] = ex2(x[i]);
       const bool masked = __any_sync(0xffffffffu, limit - k0 < 64);
+      const int d0 = r0 + off - j * F::kCols;  // distance of the tile's first query and key
+      const bool far = d0 - (F::kCols - 1) >= a.span || d0 + kRows - 1 <= -a.span;  // farther than the span from all its keys
+      if (grad && far && !masked) far_p[d0 > 0 ? 0 : 1] += sum64(x);
       if (!(ok = mbar_wait_warp(&ctl.dp_full, j & 1, abort))) break;
       tc_fence_after();
       const int seen = limit - k0;
@@ -330,13 +343,11 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       tc_fence_before();
       mbar_arrive(&ctl.ds_ready[j & 1]);
       if (!grad) continue;
-      // ---- the bias gradient.  A tile farther than the span from all its keys adds to one bucket.
-      const int d0 = r0 + off - j * F::kCols;  // distance of the tile's first query and key
-      if (d0 - (F::kCols - 1) >= a.span || d0 + kRows - 1 <= -a.span) {
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 64; ++i) sum[i & 3] += x[i];
-        far_sum[d0 > 0 ? 0 : 1] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      // ---- the bias gradient.  A far tile adds to one bucket.
+      const float sum = sum64(x);
+      row_sum += sum;
+      if (far) {
+        far_sum[d0 > 0 ? 0 : 1] += sum;
       } else {
         // A partial sum moves along its diagonal, one lane up for each column; lane 31's is complete.
         // Four blocks of 32 rows x 16 columns at a time, to have four such chains in flight.
@@ -397,8 +408,14 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         store_row<DP>(lanes + C::dq, static_cast<__nv_bfloat16*>(a.dq) + ((int64_t)(s.q0 + r) * a.heads + head) * a.dim, a.dim,
                       a.scale, n == 0, valid);
       if (grad) {
+        if (F::kGroups == 2) {
+          sdelta[half * kRows + row] = row_sum;
+          softmax_sync<DP>();
+          row_sum = sdelta[row] + sdelta[kRows + row];
+        }
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
+          far_sum[f] -= row_sum * far_p[f];
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) far_sum[f] += __shfl_xor_sync(0xffffffffu, far_sum[f], o);
           if (lane == 0) sdiag[f * 8 + warp] = far_sum[f];
