@@ -545,6 +545,7 @@ typedef struct kf_attention_desc {
   int32_t heads, kv_heads, dim;
   int32_t dtype, causal;
   int32_t span, n_buckets, table_dtype;
+  int32_t longest; /* key rows of the longest sequence: decides how the forward divides its work */
   float scale;
 } kf_attention_desc;
 

@@ -205,7 +205,7 @@ class _Plan:
             q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
             q.shape[1], k.shape[1], q.shape[2], _DTYPE_CODE[q.dtype], int(causal),
             bias.max_distance if has else 0, bias.num_buckets if has else 0, _DTYPE_CODE[bias.weight.dtype] if has else 0,
-            scale)
+            max(seqs.kv_lens, default=0), scale)
         self.ref = ctypes.byref(self.desc)
         self.tiles = []
         for what, side in enumerate("qqk"):

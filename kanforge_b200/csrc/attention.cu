@@ -50,7 +50,7 @@ int check_attention(const char* fn, const kf_attention_desc* d) {
   KF_CHECK_ARG(d->dim >= 8 && d->dim <= kMaxDim && d->dim % 8 == 0, "%s: head width %d is not a multiple of 8 up to %d", fn, d->dim,
                kMaxDim);
   KF_CHECK_ARG(d->dtype == KF_DTYPE_F32 || d->dtype == KF_DTYPE_BF16, "%s: types must be float32 or bfloat16", fn);
-  KF_CHECK_ARG(d->tq >= 0 && d->tk >= 0, "%s: negative size", fn);
+  KF_CHECK_ARG(d->tq >= 0 && d->tk >= 0 && d->longest >= 0, "%s: negative size", fn);
   KF_CHECK_ARG(d->span >= 0 && d->span <= kMaxSpan, "%s: bias distances up to %d are outside [0, %d]", fn, d->span, kMaxSpan);
   KF_CHECK_ARG(d->n_buckets >= 0 && d->n_buckets <= kMaxBuckets, "%s: %d buckets exceed %d", fn, d->n_buckets, kMaxBuckets);
   return KF_OK;
@@ -72,7 +72,7 @@ Args make_args(const kf_attention_desc* d) {
   Args a{};
   a.heads = d->heads, a.kv_heads = d->kv_heads, a.dim = d->dim, a.span = d->span, a.n_buckets = d->n_buckets;
   a.causal = d->causal != 0, a.table_bf16 = d->table_dtype == KF_DTYPE_BF16;
-  a.scale = d->scale, a.tq = d->tq, a.tk = d->tk;
+  a.scale = d->scale, a.tq = d->tq, a.tk = d->tk, a.longest = d->longest;
   a.q = {nullptr, d->q_row, d->q_head};
   a.k = {nullptr, d->k_row, d->k_head};
   a.v = {nullptr, d->v_row, d->v_head};

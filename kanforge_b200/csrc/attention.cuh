@@ -46,6 +46,8 @@ struct Args {
   const int* buckets; // (2 span + 1): bucket of distance index - span
   float* dist_part;   // (tiles, H, 2 span + 1): bias gradient by distance, or null
   int64_t tq, tk;
+  int longest;  // keys of a sequence, at most
+  int splits;   // of the keys among CTAs (bf16 forward)
   int heads, kv_heads, dim, span, n_buckets;
   int pack;  // heads that are neighbouring rows of a tile (bf16)
   bool causal, table_bf16;

@@ -56,11 +56,46 @@ struct Ctl {
   int abort;
 };
 
-template <int DP>
+// All threads of the CTAs of a cluster, from whatever branch they are in.
+__device__ __forceinline__ void cluster_join() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float peer_load(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// 8 columns of a row of the output, and what their rounding leaves out.
+__device__ __forceinline__ void store_out(const float* o, __nv_bfloat16* out, __nv_bfloat16* rest) {
+  uint4 w, e;
+  uint32_t *u = &w.x, *f = &e.x;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) u[c] = pack_bf16x2(o[2 * c], o[2 * c + 1]);
+  *reinterpret_cast<uint4*>(out) = w;
+  if (rest == nullptr) return;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    f[c] = pack_bf16x2(o[2 * c] - __uint_as_float(u[c] << 16), o[2 * c + 1] - __uint_as_float(u[c] & 0xffff0000u));
+  *reinterpret_cast<uint4*>(rest) = e;
+}
+
+
+// SPLIT: the keys are divided among the CTAs of a cluster.  Each has a slice of
+// whole streamed tiles and the same queries; at the end they read each other's
+// row maxima and sums, put their weighted outputs into shared memory (where the
+// ring was) and each adds up some of the columns, slices in order.
+template <int DP, bool SPLIT>
 __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
     attention_fwd_tc(const Args a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using F = Fwd<DP>;
-  constexpr int NT = F::NT;
+  constexpr int NT = F::NT, U = F::kUnit / kKeys;
+  static_assert(NT * kRows * DP * 4 <= F::kStages * F::kTile);  // the weighted output of a slice
   extern __shared__ uint8_t smem_raw[];
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -69,8 +104,9 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
 
   int tile;
   const int pack = a.pack, packs = a.heads / pack;
-  const Seq s = load_tile(a, blockIdx.x / packs, &tile);
-  const int head0 = blockIdx.x % packs * pack, kv_head = head0 / (a.heads / a.kv_heads);
+  const int n_slices = SPLIT ? a.splits : 1, block = blockIdx.x / n_slices, slice = blockIdx.x - block * n_slices;
+  const Seq s = load_tile(a, block / packs, &tile);
+  const int head0 = block % packs * pack, kv_head = head0 / (a.heads / a.kv_heads);
   const int r0 = tile * NT * kRows, off = s.lk - s.lq, total = s.lq * pack;
   // key tiles of each row tile
   int n_rows[NT], n_kv[NT], n_max = 0;
@@ -81,6 +117,15 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
     const int keys = n_rows[t] == 0 ? 0 : a.causal ? min(s.lk, last + off + 1) : s.lk;
     n_kv[t] = max(0, (keys + kKeys - 1) / kKeys);
     n_max = max(n_max, n_kv[t]);
+  }
+  auto units = [](int n) { return (n + U - 1) / U; };  // streamed tiles that hold n sets of 64 keys
+  int key0 = 0;                                        // of the slice
+  if (SPLIT) {
+    const int per = (units(n_max) + n_slices - 1) / n_slices * U;
+    key0 = slice * per * kKeys;
+    n_max = max(0, min(per, n_max - slice * per));
+#pragma unroll
+    for (int t = 0; t < NT; ++t) n_kv[t] = max(0, min(per, n_kv[t] - slice * per));
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -104,8 +149,6 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  constexpr int U = F::kUnit / kKeys;
-  auto units = [](int n) { return (n + U - 1) / U; };  // streamed tiles that hold n sets of 64 keys
   const uint32_t tmem = uniform(ctl.tmem), q_tile = uniform(smem_u32(smem)), kv_tile = q_tile + NT * F::kQTile;
 
   if (warp >= F::kLoadWarp) reg_dec<F::kOtherRegs>();
@@ -115,7 +158,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
     feed_ring<F::kStages>(loader, 2 * units(n_max), ctl.kv_full, ctl.kv_empty, abort, [&](int it, int st) {
       const int j = it >> 1;
       return loader.template load<F::kUnit>(kv_tile + st * F::kTile, it & 1 ? &v_map : &k_map, &ctl.kv_full[st], kv_head,
-                                            s.k0 + j * F::kUnit, s.lk - j * F::kUnit);
+                                            s.k0 + key0 + j * F::kUnit, s.lk - key0 - j * F::kUnit);
     });
   } else if (warp >= F::kMmaWarp && warp < F::kMmaWarp + 2 * NT) {
     // ---- MMAs of row tile t
@@ -198,7 +241,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
 #pragma unroll
       for (int c = 0; c < 2; ++c) tmem_ld32_issue(lanes + F::s(t, h) + c * 32, x + c * 32);
       tmem_wait_ld(x);
-      const int k0 = j * kKeys;
+      const int k0 = key0 + j * kKeys;
       float mul = c2, add = 0.f;
       if (a.table != nullptr) {
         const int dist = pos - k0;  // to the first of the keys
@@ -263,12 +306,44 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
     }
     // ---- O / l, and the logarithm of the sum
     if (ok && n > 0) ok = mbar_wait_warp(&ctl.o_done[t], 0, abort);
-    if (ok) {
-      tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int64_t at = ((int64_t)(s.q0 + tok) * a.heads + head0 + (r - tok * pack)) * a.dim;
-      if (valid && a.lse != nullptr)
-        a.lse[(int64_t)(head0 + (r - tok * pack)) * a.tq + s.q0 + tok] = l == 0.f ? 0.f : m + log2f(l);
+    tc_fence_after();
+    const int head = head0 + (r - tok * pack);
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.o) + ((int64_t)(s.q0 + tok) * a.heads + head) * a.dim;
+    __nv_bfloat16* rest =
+        a.o_rest == nullptr ? nullptr : static_cast<__nv_bfloat16*>(a.o_rest) + ((int64_t)(s.q0 + tok) * a.heads + head) * a.dim;
+    if (!SPLIT) {
+      if (ok) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (valid && a.lse != nullptr) a.lse[(int64_t)head * a.tq + s.q0 + tok] = l == 0.f ? 0.f : m + log2f(l);
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+          float o[32];
+          __syncwarp();
+          if (n > 0) {
+            tmem_ld32_issue(lanes + F::o(t) + i * 32, o);
+            tmem_wait_ld(o);
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = n > 0 && l != 0.f ? o[c] * inv : 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (valid && i * 32 + q * 8 < a.dim) store_out(o + q * 8, out + i * 32 + q * 8, rest == nullptr ? nullptr : rest + i * 32 + q * 8);
+        }
+      }
+    } else {
+      if (!ok || n == 0) m = -CUDART_INF_F, l = 0.f;
+      const uint32_t stat = q_tile + t * F::kQTile + row * 8;  // the queries are done with
+      asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(stat), "f"(m), "f"(l) : "memory");
+      cluster_join();
+      float high = -CUDART_INF_F, sum = 0.f;
+      for (int p = 0; p < n_slices; ++p) high = fmaxf(high, peer_load(peer_addr(stat, p)));
+      for (int p = 0; p < n_slices; ++p) {
+        const float lp = peer_load(peer_addr(stat, p) + 4);
+        if (lp != 0.f) sum = fmaf(lp, ex2(peer_load(peer_addr(stat, p)) - high), sum);
+      }
+      if (slice == 0 && valid && a.lse != nullptr) a.lse[(int64_t)head * a.tq + s.q0 + tok] = sum == 0.f ? 0.f : high + log2f(sum);
+      const float weight = l == 0.f ? 0.f : ex2(m - high) / sum;
+      const uint32_t mine = kv_tile + t * DP * kRows * 4 + row * 4;  // (column, row): neighbouring lanes, neighbouring words
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) {
         float o[32];
@@ -278,29 +353,25 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
           tmem_wait_ld(o);
         }
 #pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = n > 0 && l != 0.f ? o[c] * inv : 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (!valid || i * 32 + q * 8 >= a.dim) continue;
-          uint4 w;
-          uint32_t* u = &w.x;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) u[c] = pack_bf16x2(o[q * 8 + 2 * c], o[q * 8 + 2 * c + 1]);
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o) + at + i * 32 + q * 8) = w;
-          if (a.o_rest != nullptr) {
-            uint4 e;
-            uint32_t* f = &e.x;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              f[c] = pack_bf16x2(o[q * 8 + 2 * c] - __uint_as_float(u[c] << 16),
-                                 o[q * 8 + 2 * c + 1] - __uint_as_float(u[c] & 0xffff0000u));
-            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o_rest) + at + i * 32 + q * 8) = e;
-          }
-        }
+        for (int c = 0; c < 32; ++c)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + (i * 32 + c) * kRows * 4), "f"(l == 0.f ? 0.f : o[c] * weight) : "memory");
       }
+      cluster_join();
+      for (int c0 = slice * 8; c0 < a.dim; c0 += n_slices * 8) {
+        float o[8] = {};
+        for (int p = 0; p < n_slices; ++p) {
+          const uint32_t from = peer_addr(mine, p) + c0 * kRows * 4;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) o[c] += peer_load(from + c * kRows * 4);
+        }
+        if (valid) store_out(o, out + c0, rest == nullptr ? nullptr : rest + c0);
+      }
+      cluster_join();  // the others have read what is here
     }
     tc_fence_before();
   }
+  if (SPLIT && warp >= NT * 4)
+    for (int i = 0; i < 3; ++i) cluster_join();
   __syncthreads();
   if (warp == F::kMmaWarp) {
     tc_fence_after();
@@ -308,17 +379,42 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
   }
 }
 
-template <int DP>
-int launch(const Args& a, int n_tiles, cudaStream_t st) {
+// Slices of the keys: as many, up to 8, as leave each 512 keys and an SM for each
+// CTA.  16 queries of 12 heads of 64 over 4096 keys: 51 us in one slice, 35, 25
+// and 21 in 2, 4 and 8; 129 queries of 32 heads of 128 on 8 key heads over 3129
+// keys: 64, 45 and 33 (8 slices, more CTAs than SMs: 51).  512 keys in two slices
+// gain nothing (64 CTAs with heads of 128: 22.5 us in one, 24.6 in two).
+int split_count(const Args& a, int64_t ctas) {
+  constexpr int kMaxSplits = 8, kMinKeys = 512;
+  int s = 1;
+  while (s < kMaxSplits && 2 * s * ctas <= 148 && 2 * s * kMinKeys <= a.longest) s *= 2;
+  return s;
+}
+
+template <int DP, bool SPLIT>
+int launch(const Args& a, int64_t ctas, cudaStream_t st) {
   const size_t smem = Fwd<DP>::kSmem + (a.table != nullptr ? a.pack * bias_floats(a.span, a.n_buckets) * sizeof(float) : 0);
   static SmemAllowed allowed;
-  if (int rc = allow_smem(attention_fwd_tc<DP>, smem, allowed)) return rc;
+  if (int rc = allow_smem(attention_fwd_tc<DP, SPLIT>, smem, allowed)) return rc;
   CUtensorMap k_map, v_map;
   const bool keys = a.tk > 0;  // without keys no tile is loaded
   if (int rc = make_tile_map(&k_map, keys ? a.k.p : a.q.p, keys ? a.tk : 1, keys ? a.kv_heads : 1, a.dim, a.k.row, a.k.head)) return rc;
   if (int rc = make_tile_map(&v_map, keys ? a.v.p : a.q.p, keys ? a.tk : 1, keys ? a.kv_heads : 1, a.dim, a.v.row, a.v.head)) return rc;
-  attention_fwd_tc<DP><<<(unsigned)n_tiles * (a.heads / a.pack), Fwd<DP>::kThreads, smem, st>>>(a, k_map, v_map);
-  return check_launch("kf_attention_fwd");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(ctas * a.splits)), cfg.blockDim = dim3(Fwd<DP>::kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = a.splits, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = SPLIT ? 1 : 0;
+  KF_CUDA_RET(cudaLaunchKernelEx(&cfg, attention_fwd_tc<DP, SPLIT>, a, k_map, v_map));
+  return KF_OK;
+}
+
+template <int DP>
+int launch(Args a, int n_tiles, cudaStream_t st) {
+  const int64_t ctas = (int64_t)n_tiles * (a.heads / a.pack);
+  a.splits = split_count(a, ctas);
+  return a.splits > 1 ? launch<DP, true>(a, ctas, st) : launch<DP, false>(a, ctas, st);
 }
 
 }  // namespace

@@ -388,3 +388,40 @@ def test_the_largest_bias_table(heads, kv_heads, dim, dtype):
     with torch.no_grad():
         bias.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
     check(*make(lens, lens, heads, kv_heads, dim, dtype), lens, lens, False, bias=bias)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(6, 2, 64), (4, 4, 40), (4, 1, 128), (3, 3, 104)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([16], [4100]), ([1], [8192]), ([70, 3], [2100, 1500]), ([300, 1, 0, 9], [1040, 30, 5, 0])])
+def test_few_queries_over_many_keys(q_lens, kv_lens, heads, kv_heads, dim, causal):
+    """The keys of a sequence are shared out among CTAs; short ones leave some of them none."""
+    bias = kb.RelativeBias(heads, 16, 100, bidirectional=not causal, device="cuda")
+    with torch.no_grad():
+        bias.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
+    for b in (None, bias):
+        check(*make(q_lens, kv_lens, heads, kv_heads, dim, torch.bfloat16), q_lens, kv_lens, causal, bias=b)
+
+
+def test_few_queries_repeat_to_the_bit():
+    q, k, v = make([40], [5000], 8, 2, 128, torch.bfloat16)[:3]
+    seqs = kb.PackedSequences([40], [5000])
+    first = kb.attention(q, k, v, seqs)
+    for _ in range(5):
+        assert torch.equal(first, kb.attention(q, k, v, seqs))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_with_the_largest_bias_table(dtype):
+    bias = kb.RelativeBias(32, 256, 512, bidirectional=True, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        bias.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
+    g = torch.Generator(device="cuda").manual_seed(7)
+    n = 3000
+    q, k, v = (torch.randn(1, *s, generator=g, device="cuda").to(dtype) for s in ((32, 128), (4096, 2, 128), (4096, 2, 128)))
+    got = kb.attention_decode(q, k, v, torch.tensor([n], dtype=torch.int32, device="cuda"), bias=bias.requires_grad_(False))
+    dist = torch.arange(n - 1, -1, -1, device="cuda")
+    t = torch.einsum("hd,khd->hk", q[0].double(), k[0, :n].double().repeat_interleave(16, 1)) / 128**0.5
+    t = t + bias(dist).double().T
+    want = torch.einsum("hk,khd->hd", t.softmax(-1), v[0, :n].double().repeat_interleave(16, 1))
+    # float32: sums over 128 and 3000 terms; bfloat16: one rounding of the output
+    assert (got[0].double() - want).abs().max() <= (1e-5 if dtype == torch.float32 else 2.0**-8) * want.abs().max()
