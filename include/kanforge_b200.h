@@ -536,7 +536,7 @@ int kf_residual_norm_bwd(const void* x, const void* branch, const void* gate, co
  *           o_rest like o, bf16 only: what o's rounding left out, which the
  *           backward needs for dout . o (null: not written)
  * q, k, v in dtype with the strides of the descriptor (elements; head width
- * contiguous).  Backward: dout like o; dq, dk, dv contiguous; dtable
+ * contiguous); every row of every tensor starts at a multiple of 16 bytes.  Backward: dout like o; dq, dk, dv contiguous; dtable
  * (n_buckets, heads) in table_dtype or null; workspace
  * kf_attention_bwd_workspace floats.  Every sum runs in a fixed order. */
 typedef struct kf_attention_desc {
@@ -562,7 +562,8 @@ int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o,
 /* One new token per sequence over its cache: q (batch, heads, dim) attends to
  * the first lengths[b] (clamped to [0, capacity]) rows of k, v (batch,
  * capacity, kv_heads, dim) and stands at the last of them.  Slots past the
- * length are not read.  o (batch, heads, dim) contiguous.  One launch. */
+ * length are not read.  o (batch, heads, dim) contiguous.  Rows start at
+ * multiples of 16 bytes.  One launch. */
 typedef struct kf_decode_desc {
   int64_t q_batch, q_head, k_batch, k_row, k_head, v_batch, v_row, v_head;
   int32_t batch, capacity, heads, kv_heads, dim;

@@ -68,6 +68,11 @@ void tiling(const kf_attention_desc* d, int pass, int32_t* rows, int32_t* pack) 
   if (d->n_buckets == 0 || group * bias_floats(d->span, d->n_buckets) * (int)sizeof(float) <= fwd_bias_bytes(d->dim)) *pack = group;
 }
 
+bool rows_aligned(const kf_attention_desc* d, std::initializer_list<const void*> ps) {
+  return aligned16(ps) && strides16(d->dtype == KF_DTYPE_F32 ? 4 : 2, {{d->tq, d->q_row}, {d->heads, d->q_head}, {d->tk, d->k_row},
+                                                                       {d->kv_heads, d->k_head}, {d->tk, d->v_row}, {d->kv_heads, d->v_head}});
+}
+
 Args make_args(const kf_attention_desc* d) {
   Args a{};
   a.heads = d->heads, a.kv_heads = d->kv_heads, a.dim = d->dim, a.span = d->span, a.n_buckets = d->n_buckets;
@@ -127,6 +132,7 @@ extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, con
   KF_CHECK_ARG(n_q_tiles > 0 && (int64_t)n_q_tiles * d->heads < (1ll << 31), "kf_attention_fwd: bad tile count");
   KF_CHECK_ARG(q && o && q_tiles && (d->tk == 0 || (k && v)), "kf_attention_fwd: null argument");
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_fwd: the bias needs a table and buckets");
+  KF_CHECK_ARG(rows_aligned(d, {q, k, v, o, o_rest, q_tiles}), "kf_attention_fwd: rows must start at multiples of 16 bytes");
   if (int rc = bind_device(q)) return rc;
   Args a = make_args(d);
   a.q.p = q, a.k.p = k, a.v.p = v, a.o = o, a.o_rest = o_rest, a.lse = lse, a.table = table, a.buckets = buckets;
@@ -156,6 +162,8 @@ extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, con
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_bwd: the bias needs a table and buckets");
   KF_CHECK_ARG(dtable == nullptr || (table != nullptr && workspace != nullptr), "kf_attention_bwd: dtable needs a table and workspace");
   KF_CHECK_ARG(n_q_tiles == 0 || d->dtype == KF_DTYPE_F32 || o_rest != nullptr, "kf_attention_bwd: bf16 needs o_rest");
+  KF_CHECK_ARG(rows_aligned(d, {q, k, v, o, o_rest, dout, dq, dk, dv, q_tiles, k_tiles}),
+               "kf_attention_bwd: rows must start at multiples of 16 bytes");
   if (n_q_tiles == 0 && n_k_tiles == 0 && dtable == nullptr) return KF_OK;
   if (int rc = bind_device(n_q_tiles ? q : n_k_tiles ? k : dtable)) return rc;
   Args a = make_args(d);

@@ -9,6 +9,8 @@
 
 #include <math_constants.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace kf {
@@ -79,6 +81,21 @@ __device__ __forceinline__ void expand_bias_f32(const Args& a, int head, float* 
   }
 }
 
+// The kernels read 16 bytes at a time: what the entry points check.
+inline bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  return true;
+}
+struct Extent {
+  int64_t n, stride;  // in elements
+};
+inline bool strides16(int size, std::initializer_list<Extent> es) {
+  for (const Extent& e : es)
+    if (e.n > 1 && e.stride * size % 16) return false;
+  return true;
+}
+
 // attention_f32.cu, attention_fwd.cu, attention_bwd.cu
 int fwd_f32(const Args& a, int n_tiles, cudaStream_t st);
 int bwd_f32(const Args& a, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st);
@@ -86,6 +103,12 @@ int bwd_f32(const Args& a, const Tile* k_tiles, int n_q, int n_k, cudaStream_t s
 constexpr int fwd_bias_bytes(int dim) { return dim <= 64 ? 12 * 1024 : 32 * 1024; }
 int fwd_bf16(const Args& a, int n_tiles, cudaStream_t st);
 int bwd_bf16(const Args& a, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st);
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 __device__ __forceinline__ int clamp_dist(int d, int span) { return min(max(d, -span), span) + span; }
 

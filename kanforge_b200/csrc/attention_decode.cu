@@ -205,12 +205,6 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -452,6 +446,11 @@ extern "C" int kf_attention_decode(const void* q, const void* k, const void* v, 
   if (d->batch == 0) return KF_OK;
   KF_CHECK_ARG(q && o && lengths && (d->capacity == 0 || (k && v)), "%s: null argument", fn);
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr), "%s: the bias needs a table and buckets", fn);
+  const int size = d->dtype == KF_DTYPE_F32 ? 4 : 2;
+  KF_CHECK_ARG(aligned16({q, k, v, o}) &&
+                   strides16(size, {{d->batch, d->q_batch}, {d->heads, d->q_head}, {d->batch, d->k_batch}, {d->capacity, d->k_row},
+                                    {d->kv_heads, d->k_head}, {d->batch, d->v_batch}, {d->capacity, d->v_row}, {d->kv_heads, d->v_head}}),
+               "%s: rows must start at multiples of 16 bytes", fn);
   if (int rc = bind_device(q)) return rc;
   DecodeArgs a{};
   a.q = q, a.k = k, a.v = v, a.lengths = lengths, a.table = table, a.buckets = buckets, a.o = o;

@@ -277,12 +277,6 @@ int make_tile_map(CUtensorMap* map, const void* p, int64_t rows, int heads, int 
 
 // ---- softmax arithmetic ---------------------------------------------------------
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
