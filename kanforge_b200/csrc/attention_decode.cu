@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_decode_f32(const Decode
     }
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
+      if (g >= p.n_g) break;
       float t[U], top = m[g];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -172,14 +173,14 @@ __global__ void __launch_bounds__(kWarps * 32) attention_decode_f32(const Decode
         if (key0 + u >= p.last) t[u] = -CUDART_INF_F;
         top = fmaxf(top, t[u]);
       }
-      const float base = top == -CUDART_INF_F ? 0.f : top, fix = exp2f(m[g] - base);
+      const float base = top == -CUDART_INF_F ? 0.f : top, fix = ex2(m[g] - base);
       m[g] = top;
       l[g] *= fix;
 #pragma unroll
       for (int c = 0; c < 4; ++c) o[g][c] *= fix;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float e = exp2f(t[u] - base);
+        const float e = ex2(t[u] - base);
         l[g] += e;
         o[g][0] = fmaf(e, vv[u].x, o[g][0]);
         o[g][1] = fmaf(e, vv[u].y, o[g][1]);
@@ -409,20 +410,29 @@ int split_count(int batch, int capacity, int ctas_per_sequence) {
   return splits;
 }
 
-template <typename K>
-int launch(K* kernel, int group_cap, size_t smem, const DecodeArgs& a, int batch, cudaStream_t st) {
+template <void (*Kernel)(const DecodeArgs)>
+int launch(int group_cap, size_t smem, const DecodeArgs& a, int batch, cudaStream_t st) {
+  static SmemAllowed allowed;
+  static std::atomic<bool> wide[16];  // clusters of 16 are allowed on this device
   const int per_seq = a.kv_heads * (int)cdiv(a.heads / a.kv_heads, group_cap);
   const int splits = split_count(batch, a.capacity, per_seq);
   if (a.table != nullptr) smem += (size_t)std::min(group_cap, a.heads / a.kv_heads) * (2 * a.span + 1) * sizeof(float);
-  if (smem > 16384) KF_CUDA_RET(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  if (splits > 8) KF_CUDA_RET(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (int rc = allow_smem(Kernel, smem, allowed)) return rc;
+  if (splits > 8) {
+    int dev = 0;
+    KF_CUDA_RET(cudaGetDevice(&dev));
+    if (dev >= 16 || !wide[dev].load(std::memory_order_relaxed)) {
+      KF_CUDA_RET(cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      if (dev < 16) wide[dev].store(true, std::memory_order_relaxed);
+    }
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(splits, per_seq, batch), cfg.blockDim = dim3(kWarps * 32), cfg.dynamicSmemBytes = smem, cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = splits, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr, cfg.numAttrs = splits > 1 ? 1 : 0;
-  KF_CUDA_RET(cudaLaunchKernelEx(&cfg, kernel, a));
+  KF_CUDA_RET(cudaLaunchKernelEx(&cfg, Kernel, a));
   return KF_OK;
 }
 
@@ -459,7 +469,7 @@ extern "C" int kf_attention_decode(const void* q, const void* k, const void* v, 
   a.capacity = d->capacity, a.heads = d->heads, a.kv_heads = d->kv_heads, a.dim = d->dim, a.span = d->span;
   a.table_bf16 = d->table_dtype == KF_DTYPE_BF16, a.scale = d->scale;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (d->dtype == KF_DTYPE_F32) return launch(attention_decode_f32, kGroupF32, 0, a, d->batch, st);
-  return d->dim <= 64 ? launch(attention_decode_bf16<64>, kGroupBf16, decode_ring<64>(), a, d->batch, st)
-                      : launch(attention_decode_bf16<128>, kGroupBf16, decode_ring<128>(), a, d->batch, st);
+  if (d->dtype == KF_DTYPE_F32) return launch<attention_decode_f32>(kGroupF32, 0, a, d->batch, st);
+  return d->dim <= 64 ? launch<attention_decode_bf16<64>>(kGroupBf16, decode_ring<64>(), a, d->batch, st)
+                      : launch<attention_decode_bf16<128>>(kGroupBf16, decode_ring<128>(), a, d->batch, st);
 }
