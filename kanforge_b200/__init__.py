@@ -8,6 +8,10 @@ Drop-in for the reference's torch layers on CUDA:
 The forward and backward passes, the closed derivative primitives and
 ``edge_derivative`` run hand-written CUDA kernels from ``libkanb200.so``
 (build with ``python -m kanforge_b200.build``).
+
+``KANTransformer`` puts attention over packed sequences (``attention``, with a
+learned ``RelativeBias``; ``attention_decode`` over a cache) and norms fused with
+the residual stream (``residual_norm``) around the KAN feed-forward block.
 """
 
 from . import bases, convert, kernels

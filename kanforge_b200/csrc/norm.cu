@@ -14,6 +14,13 @@
 // shuffles and warps by one exchange in shared memory.  Those dependent steps leave
 // memory idle, so each group of warps keeps its next rows coming by bulk copies
 // into a ring of its own.  Everything between the loads and the stores is float32.
+//
+// Measured, cold caches: 32768 rows of 768 bf16, both norms, a gate per channel:
+// forward 65 us (3.1 TB/s; 135 us without the rings), backward 112 us (2.7 TB/s) and
+// 7 us for the parameters; 8192 rows of 4096 float32, a gate per token: forward 136 us
+// (4.9 TB/s), backward 255 us (4.2 TB/s).  The measured copy rate is 6.6 TB/s.
+// The backward falls short of it by what a row costs between its barriers: the column
+// sums take registers that more rows in flight would need.
 #include <type_traits>
 
 #include "f32x2.cuh"
@@ -740,9 +747,11 @@ int launch_bwd(GradArgs p, int ctas, cudaStream_t s) {
   return check_launch("kf_residual_norm_bwd");
 }
 
-// A lane takes 8 V elements of a row.  With many rows a row goes to as few warps
-// as possible (a warp alone needs no exchange) and rows come through the rings;
-// with few it is spread over more warps, one row a group.
+// A lane takes 8 V elements of a row.  With many rows (16 chunks of 256 elements an
+// SM) a row goes to as few warps as possible (a warp alone needs no exchange) and rows
+// come through the rings: 32768 x 768 bf16 in 65 us, 135 us one row a group.  With
+// few it is spread over more warps, one row a group: 3 rows of 768 in 5 us, where a
+// ring has nothing to run ahead of.
 template <bool VEC, typename TX, typename TB>
 int dispatch_fwd(RowArgs a, cudaStream_t s) {
   const int chunks = (int)cdiv(a.width, 256);
@@ -764,7 +773,9 @@ int dispatch_fwd(RowArgs a, cudaStream_t s) {
 }
 
 // Up to 768 columns a warp has a row to itself: its column sums fill the
-// registers of 8 warps an SM, but no row waits at a barrier.
+// registers of 8 warps an SM, but no row waits at a barrier (32768 x 768: 112 us,
+// 126 us with three warps to a row).  Above 4096 the sums do not fit the registers
+// and are kept in shared memory.
 template <bool VEC, typename TX, typename TB>
 int dispatch_bwd(GradArgs p, int ctas, cudaStream_t s) {
   const int chunks = (int)cdiv(p.f.width, 256);

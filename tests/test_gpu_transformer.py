@@ -130,3 +130,31 @@ def test_a_few_steps_of_training_lower_the_loss():
         opt.step()
         losses.append(loss.item())
     assert all(math.isfinite(v) for v in losses) and losses[-1] < losses[0]
+
+
+def test_a_decoding_step_replays_from_a_graph():
+    heads, dim, capacity = 6, 64, 512
+    g = torch.Generator(device=DEV).manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    q, k, v = r(3, heads, dim), r(3, capacity, 2, dim), r(3, capacity, 2, dim)
+    x, w = r(3, heads * dim), r(heads * dim)
+    lengths = torch.tensor([1, 300, 77], dtype=torch.int32, device=DEV)
+
+    def step():
+        o = kb.attention_decode(q, k, v, lengths)
+        return kb.residual_norm(x, o.flatten(1), w, kind="rms")
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, h = step()
+    for n in ([1, 300, 77], [2, 512, 0]):
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        q.copy_(r(3, heads, dim))
+        graph.replay()
+        for a, b in zip((y, h), step()):
+            assert torch.equal(a, b)
