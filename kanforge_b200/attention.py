@@ -231,7 +231,7 @@ def _forward(q, k, v, table, seqs, causal, scale, bias, train: bool):
     logarithms of the sums."""
     q, k, v = _vectors(q), _vectors(k), _vectors(v)
     plan = _plan(seqs, q, k, v, causal, scale, bias)
-    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     rest = lse = None
     if train:
         lse = torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32)
@@ -312,15 +312,24 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: PackedSeq
 
 
 _DECODE_PLANS_MAX = 512
-_decode_plans: dict = {}  # descriptors by shapes, strides and types
+_decode_plans: dict = {}  # descriptors by what the arguments' checks and the launch look at
 
 
-def _decode_plan(q, k, v, scale, bias):
-    key = (q.dtype, q.shape, q.stride(), k.shape, k.stride(), v.stride(), scale,
-           None if bias is None else (bias.weight.dtype, bias.max_distance))
+def _decode_plan(q, k, v, lengths, scale, bias):
+    """The call's descriptor; arguments like those of an earlier call have been checked then."""
+    key = (q.dtype, k.dtype, v.dtype, lengths.dtype, q.device, k.device, v.device, lengths.device, q.shape, k.shape, v.shape,
+           lengths.shape, q.stride(), k.stride(), v.stride(), scale,
+           None if bias is None else (bias.weight.dtype, bias.weight.device, bias.weight.shape, bias.max_distance))
     ref = _decode_plans.get(key)
     if ref is None:
+        if q.dim() != 3 or k.dim() != 4 or v.dim() != 4:
+            raise ValueError("q must be (batch, heads, dim), the caches (batch, capacity, kv_heads, dim)")
+        _check_heads(q, k, v, bias, scale)
         batch, capacity, kv_heads, dim = k.shape
+        if q.shape[0] != batch or batch > 65535:
+            raise ValueError(f"q holds {q.shape[0]} sequences, the caches {batch} (at most 65535)")
+        if lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.device != q.device:
+            raise ValueError(f"lengths must be ({batch},) int32 on {q.device}")
         desc = _lib.DecodeDesc(q.stride(0), q.stride(1), *k.stride()[:3], *v.stride()[:3], batch, capacity, q.shape[1],
                                kv_heads, dim, _DTYPE_CODE[q.dtype], 0 if bias is None else bias.max_distance,
                                0 if bias is None else _DTYPE_CODE[bias.weight.dtype],
@@ -341,24 +350,20 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     length of 0 gives 0, one above the capacity counts as the capacity.
     Inference only: tensors that require a gradient raise.
     """
-    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4:
-        raise ValueError("q must be (batch, heads, dim), the caches (batch, capacity, kv_heads, dim)")
-    _check_heads(q, k_cache, v_cache, bias, scale)
-    batch = k_cache.shape[0]
-    if q.shape[0] != batch or batch > 65535:
-        raise ValueError(f"q holds {q.shape[0]} sequences, the caches {batch} (at most 65535)")
-    if lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.device != q.device:
-        raise ValueError(f"lengths must be ({batch},) int32 on {q.device}")
+    plan = _decode_plan(q, k_cache, v_cache, lengths, scale, bias)
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
                                     (bias is not None and bias.weight.requires_grad)):
         raise RuntimeError("attention_decode has no backward: call it under torch.no_grad(), or use attention")
-    q, k, v = _vectors(q), _vectors(k_cache), _vectors(v_cache)
-    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    if batch == 0:
+    aligned = _vectors(q), _vectors(k_cache), _vectors(v_cache)
+    if aligned[0] is not q or aligned[1] is not k_cache or aligned[2] is not v_cache:  # copies have strides of their own
+        q, k_cache, v_cache = aligned
+        plan = _decode_plan(q, k_cache, v_cache, lengths, scale, bias)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if o.numel() == 0:
         return o
     lengths = lengths.contiguous()
     table = None if bias is None else bias.weight.detach().contiguous()
-    _launch("kf_attention_decode", q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths.data_ptr(),
+    _launch("kf_attention_decode", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),
             None if table is None else table.data_ptr(), None if bias is None else bias.buckets.data_ptr(), o.data_ptr(),
-            _decode_plan(q, k, v, scale, bias), _raw_stream(q))
+            plan, _raw_stream(q))
     return o

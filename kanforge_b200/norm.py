@@ -164,14 +164,15 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, weight: torch.Te
         raise ValueError(f"kind must be one of {NORM_KINDS}")
     if eps < 0:
         raise ValueError("eps must not be negative")
-    tensors = (x, branch, weight, bias, branch_weight, branch_bias, gate)
-    given = [t for t in tensors if t is not None]
-    device = x.device
-    for t in given:
-        if not t.is_cuda:
-            _check_cuda(t)
-        if t.device != device:
-            raise ValueError(f"tensors lie on {device} and {t.device}")
+    device, grad = x.device, torch.is_grad_enabled()
+    wanted = False
+    for t in (x, branch, weight, bias, branch_weight, branch_bias, gate):
+        if t is not None:
+            if not t.is_cuda:
+                _check_cuda(t)
+            if t.device != device:
+                raise ValueError(f"tensors lie on {device} and {t.device}")
+            wanted = wanted or t.requires_grad
     if x.dim() < 1 or not 1 <= x.shape[-1] <= NORM_MAX_WIDTH:
         raise ValueError(f"rows must have 1 to {NORM_MAX_WIDTH} elements (got a tensor of shape {tuple(x.shape)})")
     width = x.shape[-1]
@@ -195,7 +196,7 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, weight: torch.Te
         if gate.dim() < 2:
             gate = gate.reshape(1, width)
     args = (x, branch, weight, bias, branch_weight, branch_bias, gate, kind, float(residual_scale), float(eps))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+    if grad and wanted:
         out = _ResidualNorm.apply(*args)
         return (x, out) if branch is None else out
     y, h, _ = _Call(*args).forward(with_stats=False)
