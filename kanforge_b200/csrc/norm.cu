@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(REGS && V > 1 ? 256 : 512) residual_norm_bwd(c
     }
     float m1 = sum_of(s1), m2 = sum_of(s2);
     g.sum2(m1, m2);
-    if (RING && row != first) ring.start();  // every lane is done with the row before
+    if (RING && !a.branch_norm && row != first) ring.start();  // every lane is done with the row before
     m1 = a.layer ? m1 * inv : 0.f;
     m2 *= inv;
 #pragma unroll
@@ -607,6 +607,7 @@ __global__ void __launch_bounds__(REGS && V > 1 ? 256 : 512) residual_norm_bwd(c
     if (!a.branch_norm) continue;
     m1 = sum_of(s1), m2 = sum_of(s2);
     g.sum2(m1, m2);
+    if (RING) ring.start();  // these sums took all that the row's slot holds
     const uint64_t rstd = pair(st.w), a1 = pair(a.layer ? -m1 * inv : 0.f), a2 = pair(-m2 * inv);
 #pragma unroll
     for (int c = 0; c < V; ++c) {
