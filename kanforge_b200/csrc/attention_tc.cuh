@@ -119,6 +119,37 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// A warp's 32 rows of results, a lane to a row, on their way to memory: through
+// shared memory, so that neighbouring lanes write whole lines (a lane that writes
+// its row itself touches 32 lines an instruction).  The rows of a tile lie
+// anywhere (heads side by side): each lane brings its row's address.
+template <int DP>
+__device__ __forceinline__ uint32_t staged(uint32_t stage, int row, int chunk) {
+  return stage + row * (DP * 2) + ((chunk ^ (row & 7)) << 4);  // 16 bytes; both ways of access meet all banks
+}
+template <int DP>
+__device__ __forceinline__ void stage_chunk(uint32_t stage, int chunk, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staged<DP>(stage, threadIdx.x & 31, chunk)), "r"(w0), "r"(w1), "r"(w2),
+               "r"(w3)
+               : "memory");
+}
+template <int DP>
+__device__ __forceinline__ void flush_rows(uint32_t stage, __nv_bfloat16* out, bool valid, int dim) {
+  constexpr int CH = DP / 8;
+  __syncwarp();
+  const uint32_t rows = __ballot_sync(0xffffffffu, valid);
+#pragma unroll 4
+  for (int k = 0; k < CH; ++k) {
+    const int i = k * 32 + (threadIdx.x & 31), row = i / CH, c = i % CH;
+    uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), row));
+    if ((rows >> row & 1) == 0 || c * 8 >= dim) continue;
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staged<DP>(stage, row, c)) : "memory");
+    *reinterpret_cast<uint4*>(to + c * 16) = v;
+  }
+  __syncwarp();
+}
+
 // Moves registers between the warpgroups of a CTA; the sum over its
 // warpgroups must not exceed what the CTA was launched with.
 template <int N>
@@ -284,40 +315,55 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // The padded bias tables of `pack` heads (index distance + span + kBiasPad);
-// `column` has room for the heads' columns of the learned table.  The columns and
-// the bucket numbers are read side by side, so that one trip to memory is waited
-// for; sync() is a barrier of the `n_threads` threads.
+// `column` has room for the heads' columns of the learned table.  begin() starts
+// the reads, so that other loads can go out before they are waited for; sync() is
+// a barrier of the `n_threads` threads.
 __host__ __device__ constexpr int bias_floats(int span, int n_buckets) { return bias_stride(span) + n_buckets; }
+
+struct BiasTable {
+  static constexpr int U = 8;
+  uint32_t raw;  // this thread's first element of the columns
+  int id[U];     // its first bucket numbers
+
+  __device__ __forceinline__ void load(const Args& a, int i0, int n_threads) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = a.buckets[min(max(i0 + u * n_threads - kBiasPad, 0), 2 * a.span)];
+  }
+  __device__ __forceinline__ uint32_t column_at(const Args& a, int head0, int i) {
+    const int64_t e = (int64_t)(i % a.n_buckets) * a.heads + head0 + i / a.n_buckets;
+    return a.table_bf16 ? static_cast<const uint16_t*>(a.table)[e] : static_cast<const uint32_t*>(a.table)[e];
+  }
+  __device__ __forceinline__ void begin(const Args& a, int head0, int pack, int thread, int n_threads) {
+    raw = column_at(a, head0, min(thread, pack * a.n_buckets - 1));
+    load(a, thread, n_threads);
+  }
+  template <typename Sync>
+  __device__ __forceinline__ void finish(const Args& a, int head0, int pack, float* out, float* column, int thread, int n_threads,
+                                         Sync&& sync) {
+    const int n = bias_stride(a.span);
+    for (int i = thread; i < pack * a.n_buckets; i += n_threads) {
+      if (i != thread) raw = column_at(a, head0, i);
+      column[i] = bias_base2(__uint_as_float(a.table_bf16 ? raw << 16 : raw));
+    }
+    sync();
+    for (int i0 = thread; i0 < n; i0 += U * n_threads) {
+      if (i0 != thread) load(a, i0, n_threads);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * n_threads;
+        if (i >= n) break;
+        for (int g = 0; g < pack; ++g) out[g * n + i] = column[g * a.n_buckets + min(max(id[u], 0), a.n_buckets - 1)];
+      }
+    }
+  }
+};
 
 template <typename Sync>
 __device__ __forceinline__ void expand_bias(const Args& a, int head0, int pack, float* out, float* column, int thread, int n_threads,
                                             Sync&& sync) {
-  const int n = bias_stride(a.span);
-  for (int i = thread; i < pack * a.n_buckets; i += n_threads) {
-    const int64_t e = (int64_t)(i % a.n_buckets) * a.heads + head0 + i / a.n_buckets;
-    column[i] = bias_base2(a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[e])
-                                        : static_cast<const float*>(a.table)[e]);
-  }
-  constexpr int U = 4;
-  int id[U];
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * n_threads;
-      id[u] = a.buckets[min(max(i - kBiasPad, 0), 2 * a.span)];
-    }
-  };
-  load(thread);
-  sync();
-  for (int i0 = thread; i0 < n; i0 += U * n_threads) {
-    if (i0 != thread) load(i0);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * n_threads;
-      if (i >= n) break;
-      for (int g = 0; g < pack; ++g) out[g * n + i] = column[g * a.n_buckets + min(max(id[u], 0), a.n_buckets - 1)];
-    }
-  }
+  BiasTable t;
+  t.begin(a, head0, pack, thread, n_threads);
+  t.finish(a, head0, pack, out, column, thread, n_threads, sync);
 }
 
 }  // namespace attn
