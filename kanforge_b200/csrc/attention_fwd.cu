@@ -20,9 +20,11 @@
 // issues Q K^T and one that issues P V: issuing blocks while the tensor cores
 // are behind, and neither product should wait for the other's turn.
 //
-// Measured, cold caches, causal: 8191 tokens, 16 heads of 128 on 4 key heads 0.28 ms
-// (1.0 PFLOP/s, 0.60 of the measured bf16 rate); 32 x 1024 tokens, 12 heads of 64
-// with a bias 0.19 ms (270 TFLOP/s).  What is left is the way of one row tile
+// Measured, cold caches, causal: 8191 tokens, 16 heads of 128 on 4 key heads 0.26 ms
+// (1.05 PFLOP/s, 0.64 of the measured bf16 rate); 32 x 1024 tokens, 12 heads of 64
+// with a bias 0.20 ms (260 TFLOP/s); 64 x 197 tokens both ways with a bias 79 us, where
+// of a CTA's 19 thousand clocks 8 are the loop and 11 its set-up, queries, bias table
+// and output.  What is left is the way of one row tile
 // through a thread (scores out of tensor memory, maximum, 64 exponentials, weights
 // back), which two row tiles an SM do not hide altogether: the tensor cores wait
 // for the weights, with D = 64 most of the time, since a product there is half as

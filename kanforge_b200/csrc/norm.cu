@@ -16,9 +16,9 @@
 // into a ring of its own.  Everything between the loads and the stores is float32.
 //
 // Measured, cold caches: 32768 rows of 768 bf16, both norms, a gate per channel:
-// forward 65 us (3.1 TB/s; 135 us without the rings), backward 112 us (2.7 TB/s) and
-// 7 us for the parameters; 8192 rows of 4096 float32, a gate per token: forward 136 us
-// (4.9 TB/s), backward 255 us (4.2 TB/s).  The measured copy rate is 6.6 TB/s.
+// forward 67 us (3.0 TB/s; 135 us without the rings), backward 113 us (2.7 TB/s) and
+// 7 us for the parameters; 8192 rows of 4096 float32, a gate per token: forward 132 us
+// (5.1 TB/s), backward 247 us (4.3 TB/s).  The measured copy rate is 6.6 TB/s.
 // The backward falls short of it by what a row costs between its barriers: the column
 // sums take registers that more rows in flight would need.
 #include <type_traits>
