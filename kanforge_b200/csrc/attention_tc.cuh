@@ -178,22 +178,21 @@ __device__ __forceinline__ void cp_async_wait() {
 template <int DP, int THREADS>
 __device__ __forceinline__ void load_tile_async(uint32_t dst, const __nv_bfloat16* base, int64_t row_stride, int64_t head_stride,
                                                 int pack, int first_row, int n, int dim, int tid) {
-  constexpr int CH = DP / 8;
-#pragma unroll 4
-  for (int i = tid; i < kRows * CH; i += THREADS) {
-    const int row = i / CH, ch = i % CH;
-    const bool ok = row < n && ch * 8 < dim;
-    const __nv_bfloat16* src = base;
-    if (ok) {
-      const int r = first_row + row;
-      if (pack == 1) {
-        src += (int64_t)r * row_stride + ch * 8;
-      } else {
-        const int tok = r / pack;
-        src += (int64_t)tok * row_stride + (int64_t)(r - tok * pack) * head_stride + ch * 8;
-      }
-    }
-    cp_async16(dst + (ch >> 3) * (kRows * 128) + sw128_offset(row, ch & 7), src, ok ? 16 : 0);
+  constexpr int CH = DP / 8, STEP = THREADS / CH;  // a thread's rows are STEP apart
+  static_assert(STEP % 8 == 0 && kRows % STEP == 0);
+  const int ch = tid % CH, row0 = tid / CH, tok = (first_row + row0) / pack;
+  int head = first_row + row0 - tok * pack;
+  const __nv_bfloat16* src = base + (int64_t)tok * row_stride + (int64_t)head * head_stride + ch * 8;
+  const int toks = STEP / pack, heads = STEP - toks * pack;
+  const int64_t step = (int64_t)toks * row_stride + (int64_t)heads * head_stride, carry = row_stride - (int64_t)pack * head_stride;
+  dst += (ch >> 3) * (kRows * 128) + sw128_offset(row0, ch & 7);
+  const int rows = ch * 8 < dim ? n : 0;
+#pragma unroll
+  for (int i = 0; i < kRows / STEP; ++i) {
+    const bool ok = row0 + i * STEP < rows;
+    cp_async16(dst + i * STEP * 128, ok ? src : base, ok ? 16 : 0);
+    src += step, head += heads;
+    if (head >= pack) head -= pack, src += carry;
   }
 }
 
