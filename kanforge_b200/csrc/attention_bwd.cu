@@ -107,7 +107,7 @@ __device__ __forceinline__ void store_row_staged(uint32_t lanes, uint32_t stage,
     return;
   }
   stage += (threadIdx.x >> 5 & 3) * 32 * (DP * 2);
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < DP / 32; ++i) {
     float o[32];
     __syncwarp();
@@ -274,7 +274,11 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     }
     if (grad)
       for (int i = threadIdx.x; i < 4 * n_dist; i += F::kSoftmax) ssum[i] = 0.f;
-    if (a.table != nullptr) expand_bias(a, head, 1, sbias, column, threadIdx.x, F::kSoftmax, [] { softmax_sync<DP>(); });
+    if (a.table != nullptr) {
+      BiasTable table;
+      table.begin(a, head, 1, sbias, threadIdx.x, F::kSoftmax);
+      table.finish<0>(a, head, 1, sbias, column, threadIdx.x, F::kSoftmax, [] { softmax_sync<DP>(); });
+    }
     softmax_sync<DP>();
     float delta = sdelta[row];
     if (F::kGroups == 2) softmax_sync<DP>();  // sdelta is written again below

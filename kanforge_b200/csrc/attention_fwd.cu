@@ -20,11 +20,12 @@
 // issues Q K^T and one that issues P V: issuing blocks while the tensor cores
 // are behind, and neither product should wait for the other's turn.
 //
-// Measured, cold caches, causal: 8191 tokens, 16 heads of 128 on 4 key heads 0.26 ms
-// (1.05 PFLOP/s, 0.64 of the measured bf16 rate); 32 x 1024 tokens, 12 heads of 64
-// with a bias 0.20 ms (260 TFLOP/s); 64 x 197 tokens both ways with a bias 79 us, where
-// of a CTA's 19 thousand clocks 8 are the loop and 11 its set-up, queries, bias table
-// and output.  What is left is the way of one row tile
+// Measured, cold caches, causal: 8191 tokens, 16 heads of 128 on 4 key heads 0.25 ms
+// (1.1 PFLOP/s, 0.68 of the measured bf16 rate); 32 x 1024 tokens, 12 heads of 64
+// with a bias 0.18 ms (290 TFLOP/s); 64 x 197 tokens both ways with a bias 67 us, where
+// about half of a CTA's time is its loop, the rest its set-up, queries, bias table
+// and output: code that runs once costs the fetching of its instructions, so it is
+// kept in loops (77 us unrolled).  What is left is the way of one row tile
 // through a thread (scores out of tensor memory, maximum, 64 exponentials, weights
 // back), which two row tiles an SM do not hide altogether: the tensor cores wait
 // for the weights, with D = 64 most of the time, since a product there is half as
@@ -230,14 +231,14 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
     const int limit = valid && a.causal ? min(s.lk, pos + 1) : s.lk;  // keys this row sees
     const float c2 = a.scale * kLog2e;
     BiasTable table;
-    if (a.table != nullptr) table.begin(a, head0, pack, threadIdx.x, F::kSoftmax);
+    if (a.table != nullptr) table.begin(a, head0, pack, sbias, threadIdx.x, F::kSoftmax);
     load_tile_async<DP, kRows>(q_tile + t * F::kQTile,
                                static_cast<const __nv_bfloat16*>(a.q.p) + (int64_t)s.q0 * a.q.row + head0 * a.q.head, a.q.row,
                                a.q.head, pack, r0 + t * kRows, rows, a.dim, row);
     cp_async_commit();
     if (a.table != nullptr)
-      table.finish(a, head0, pack, sbias, sbias + pack * bias_stride(a.span), threadIdx.x, F::kSoftmax,
-                   [] { named_bar_and(1, F::kSoftmax, true); });
+      table.finish<1>(a, head0, pack, sbias, sbias + pack * bias_stride(a.span), threadIdx.x, F::kSoftmax,
+                      [] { named_bar_and(1, F::kSoftmax, true); });
     cp_async_wait<0>();
     fence_proxy_async_smem();
     mbar_arrive(&ctl.q_full);
@@ -328,13 +329,13 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (valid && a.lse != nullptr) a.lse[(int64_t)head * a.tq + s.q0 + tok] = l == 0.f ? 0.f : m + log2f(l);
         // D = 128: in whole lines by way of shared memory, O first, what its rounding leaves out after another look at
-        // tensor memory (one document of 8191 tokens: 264 us, 279 straight from the registers).  D <= 64: straight, since
-        // the other CTA of the SM computes meanwhile (64 x 197 tokens: 79 us, 82 by way of shared memory).
+        // tensor memory (one document of 8191 tokens: 264 us against 279 straight from the registers).  D <= 64: straight,
+        // since the other CTA of the SM computes meanwhile (64 x 197 tokens: 79 us against 82 by way of shared memory).
         if constexpr (DP == 128) {
           const uint32_t stage = q_tile + t * F::kQTile + (warp & 3) * 32 * (DP * 2);  // the queries are done with
 #pragma unroll 1
           for (int what = 0; what < (rest == nullptr ? 1 : 2); ++what) {
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < DP / 32; ++i) {
               float o[32];
               __syncwarp();
@@ -357,19 +358,17 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
             flush_rows<DP>(stage, what == 0 ? out : rest, valid, a.dim);
           }
         } else {
-#pragma unroll
-          for (int i = 0; i < DP / 32; ++i) {
-            float o[32];
+#pragma unroll 1
+          for (int i = 0; i < DP; i += 8) {
+            float o[8] = {};
             __syncwarp();
             if (n > 0) {
-              tmem_ld32_issue(lanes + F::o(t) + i * 32, o);
+              tmem_ld8_issue(lanes + F::o(t) + i, o);
               tmem_wait_ld(o);
             }
 #pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] = n > 0 && l != 0.f ? o[c] * inv : 0.f;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (valid && i * 32 + q * 8 < a.dim) store_out(o + q * 8, out + i * 32 + q * 8, rest == nullptr ? nullptr : rest + i * 32 + q * 8);
+            for (int c = 0; c < 8; ++c) o[c] = l != 0.f ? o[c] * inv : 0.f;
+            if (valid && i < a.dim) store_out(o, out + i, rest == nullptr ? nullptr : rest + i);
           }
         }
       }

@@ -99,6 +99,13 @@ __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, float* v) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
+// The same for 8 columns.
+__device__ __forceinline__ void tmem_ld8_issue(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
 // Waits for this thread's TMEM loads; the registers pass through so that no use moves above the wait.
 template <int N>
 __device__ __forceinline__ void tmem_wait_ld(float (&v)[N]) {
@@ -319,7 +326,51 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // a barrier of the `n_threads` threads.
 __host__ __device__ constexpr int bias_floats(int span, int n_buckets) { return bias_stride(span) + n_buckets; }
 
+// Code that a CTA runs once costs the fetching of its instructions: the loops stay
+// loops (unrolled, with the numbers in registers, the last one took 2000 clocks).
 struct BiasTable {
+  uint32_t raw;  // this thread's first element of the columns
+
+  __device__ __forceinline__ uint32_t column_at(const Args& a, int head0, int i) {
+    const int64_t e = (int64_t)(i % a.n_buckets) * a.heads + head0 + i / a.n_buckets;
+    return a.table_bf16 ? static_cast<const uint16_t*>(a.table)[e] : static_cast<const uint32_t*>(a.table)[e];
+  }
+  // The bucket numbers come by cp.async, a group of their own, to where the first table will be.
+  __device__ __forceinline__ void begin(const Args& a, int head0, int pack, float* out, int thread, int n_threads) {
+    const int n = bias_stride(a.span);
+    raw = column_at(a, head0, min(thread, pack * a.n_buckets - 1));
+#pragma unroll 1
+    for (int i = thread; i < n; i += n_threads)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(out + i)),
+                   "l"(a.buckets + min(max(i - kBiasPad, 0), 2 * a.span))
+                   : "memory");
+    cp_async_commit();
+  }
+  // LATER: groups of cp.async since begin() that need not be complete
+  template <int LATER, typename Sync>
+  __device__ __forceinline__ void finish(const Args& a, int head0, int pack, float* out, float* column, int thread, int n_threads,
+                                         Sync&& sync) {
+    const int n = bias_stride(a.span);
+#pragma unroll 1
+    for (int i = thread; i < pack * a.n_buckets; i += n_threads) {
+      if (i != thread) raw = column_at(a, head0, i);
+      column[i] = bias_base2(__uint_as_float(a.table_bf16 ? raw << 16 : raw));
+    }
+    cp_async_wait<LATER>();
+    sync();
+#pragma unroll 1
+    for (int i = thread; i < n; i += n_threads) {
+      const int id = min(max(__float_as_int(out[i]), 0), a.n_buckets - 1);  // this thread's own copy
+#pragma unroll 1
+      for (int g = pack - 1; g >= 0; --g) out[g * n + i] = column[g * a.n_buckets + id];
+    }
+  }
+};
+
+// The same at once, with the bucket numbers in registers.  For dK dV, which expands
+// a table inside its loop over the heads: there the rolled form costs the loop
+// registers (one document of 8191 tokens: 672 us, 628 in this form).
+struct BiasTableRegs {
   static constexpr int U = 8;
   uint32_t raw;  // this thread's first element of the columns
   int id[U];     // its first bucket numbers
@@ -360,7 +411,7 @@ struct BiasTable {
 template <typename Sync>
 __device__ __forceinline__ void expand_bias(const Args& a, int head0, int pack, float* out, float* column, int thread, int n_threads,
                                             Sync&& sync) {
-  BiasTable t;
+  BiasTableRegs t;
   t.begin(a, head0, pack, thread, n_threads);
   t.finish(a, head0, pack, out, column, thread, n_threads, sync);
 }
