@@ -235,6 +235,8 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
   } else if (warp < F::kLoadWarp) {
     reg_inc<F::kSoftmaxRegs>();
     // ---- softmax arithmetic: thread = query, a warpgroup per half of a tile's keys
+    BiasTable table;
+    if (a.table != nullptr) table.begin(a, head, 1, sbias, threadIdx.x, F::kSoftmax);
     const int half = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + row;
     const bool valid = row < n_rows;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -274,11 +276,7 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     }
     if (grad)
       for (int i = threadIdx.x; i < 4 * n_dist; i += F::kSoftmax) ssum[i] = 0.f;
-    if (a.table != nullptr) {
-      BiasTable table;
-      table.begin(a, head, 1, sbias, threadIdx.x, F::kSoftmax);
-      table.finish<0>(a, head, 1, sbias, column, threadIdx.x, F::kSoftmax, [] { softmax_sync<DP>(); });
-    }
+    if (a.table != nullptr) table.finish<0>(a, head, 1, sbias, column, threadIdx.x, F::kSoftmax, [] { softmax_sync<DP>(); });
     softmax_sync<DP>();
     float delta = sdelta[row];
     if (F::kGroups == 2) softmax_sync<DP>();  // sdelta is written again below
