@@ -317,8 +317,9 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
       tc_fence_before();
       mbar_arrive(&ctl.p_ready[t][h]);
     }
-    // ---- O / l, and the logarithm of the sum
-    if (ok && n > 0) ok = mbar_wait_warp(&ctl.o_done[t], 0, abort);
+    // ---- O / l, and the logarithm of the sum.  What follows writes over the queries: the products are done with them, or,
+    // for a row tile without keys, every warp's copies of them have landed.
+    if (ok) ok = mbar_wait_warp(n > 0 ? &ctl.o_done[t] : &ctl.q_full, 0, abort);
     tc_fence_after();
     const int head = head0 + (r - tok * pack);
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.o) + ((int64_t)(s.q0 + tok) * a.heads + head) * a.dim;

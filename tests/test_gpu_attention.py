@@ -425,3 +425,30 @@ def test_decode_with_the_largest_bias_table(dtype):
     want = torch.einsum("hk,khd->hd", t.softmax(-1), v[0, :n].double().repeat_interleave(16, 1))
     # float32: sums over 128 and 3000 terms; bfloat16: one rounding of the output
     assert (got[0].double() - want).abs().max() <= (1e-5 if dtype == torch.float32 else 2.0**-8) * want.abs().max()
+
+
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("layout", [([150], [20]), ([300], [0]), ([400], [30]), ([700, 300, 20], [130, 0, 20])], ids=lambda x: f"{x[0]}over{x[1]}")
+def test_row_tiles_without_keys(layout, causal, dim):
+    """Whole tiles of queries that see no key, beside tiles that do: exactly 0, and no gradient."""
+    q_lens, kv_lens = layout
+    out, grads = check(*make(q_lens, kv_lens, 8, 2, dim, torch.bfloat16), q_lens, kv_lens, causal)
+    q0 = 0
+    for lq, lk in zip(q_lens, kv_lens):
+        empty = lq if lk == 0 else (max(0, lq - lk) if causal else 0)
+        assert (out[q0:q0 + empty] == 0).all() and (grads[0][q0:q0 + empty] == 0).all()
+        q0 += lq
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,lens", [(2, 1, 128, [2048]), (1, 1, 128, [2048]), (1, 1, 64, [2048]), (2, 1, 128, [2048, 100]),
+                                                     (1, 1, 64, [2048, 100])])
+def test_slices_of_the_keys_without_work(heads, kv_heads, dim, lens):
+    """Keys shared out among CTAs where full row tiles leave whole slices without a key, without a bias: the right
+    values, and the same bits every time."""
+    q, k, v, dout = make(lens, lens, heads, kv_heads, dim, torch.bfloat16)
+    out, _ = check(q, k, v, dout, lens, lens, True)
+    seqs = kb.PackedSequences(lens)
+    with torch.no_grad():
+        for _ in range(50):
+            assert torch.equal(kb.attention(q, k, v, seqs), out)
