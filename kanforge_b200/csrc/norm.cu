@@ -363,9 +363,10 @@ struct RowRing {
 };
 
 constexpr int kMaxSlots = 4;
+constexpr int kFwdWarps = 16, kFwdRingWarps = 12;  // of a CTA of the forward, at most
 
 template <int V, bool VEC, bool RING, typename TX, typename TB>
-__global__ void __launch_bounds__(RING ? 384 : 512, RING && sizeof(TX) == 2 ? 2 : 1) residual_norm_fwd(const RowArgs a, int slots, int slot_bytes) {
+__global__ void __launch_bounds__((RING ? kFwdRingWarps : kFwdWarps) * 32, RING && sizeof(TX) == 2 ? 2 : 1) residual_norm_fwd(const RowArgs a, int slots, int slot_bytes) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint64_t full[8 * kMaxSlots];
   const int lane = threadIdx.x & 31, warp_id = threadIdx.x >> 5, group = warp_id / a.warps;
@@ -712,6 +713,7 @@ int sm_count() {
 template <int V, bool VEC, bool RING, typename TX, typename TB>
 int launch_fwd(RowArgs a, cudaStream_t s) {
   const int groups = std::max(1, 8 / a.warps);
+  KF_CHECK_ARG(groups * a.warps <= (RING ? kFwdRingWarps : kFwdWarps), "kf_residual_norm_fwd: %d warps to a row of %d elements", a.warps, a.width);
   const int slot_bytes = a.width * (int)(sizeof(TX) + (a.branch != nullptr ? sizeof(TB) : 0) + (a.gate_token ? sizeof(TB) : 0));
   int slots = 0;
   const int per_sm = sizeof(TX) == 2 ? 3 : 2;  // CTAs
@@ -761,7 +763,7 @@ int dispatch_fwd(RowArgs a, cudaStream_t s) {
     if (a.rows * chunks >= 148 * 16) {
       int v = 1, least = 1 << 30;
       for (int t = 4; t >= 1; --t)
-        if (cdiv(chunks, t) <= 16 && cdiv(chunks, t) * t < least) least = (int)cdiv(chunks, t) * t, v = t;
+        if (cdiv(chunks, t) <= kFwdRingWarps && cdiv(chunks, t) * t < least) least = (int)cdiv(chunks, t) * t, v = t;
       a.warps = (int)cdiv(chunks, v);
       if (v == 4) return launch_fwd<4, VEC, true, TX, TB>(a, s);
       if (v == 3) return launch_fwd<3, VEC, true, TX, TB>(a, s);

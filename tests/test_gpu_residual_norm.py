@@ -250,3 +250,12 @@ def test_repeats_to_the_bit(width):
 
     for a, b in zip(run(), run()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [256 * chunks - 8 for chunks in range(1, 33)] + [3200, 6656])
+def test_many_rows_at_every_division_of_a_row(width, dtype):
+    """A row is 1 to 32 chunks of 256 elements, divided among lanes and warps; enough rows (2368 chunks) for groups
+    that walk over several."""
+    rows = -(-148 * 16 // -(-width // 256)) + 3
+    check(inputs((rows, width), "layer", "channel", True, dtype), "layer", 0.9)
