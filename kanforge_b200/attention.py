@@ -199,13 +199,12 @@ class _Plan:
 
     __slots__ = ("desc", "ref", "tiles", "workspace")
 
-    def __init__(self, seqs, q, k, v, causal, scale, bias):
-        has = bias is not None
+    def __init__(self, seqs, q, k, v, causal, scale, table):
+        dtype, buckets, span = table or (None, 0, 0)
         self.desc = _lib.AttentionDesc(
             q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
             q.shape[1], k.shape[1], q.shape[2], _DTYPE_CODE[q.dtype], int(causal),
-            bias.max_distance if has else 0, bias.num_buckets if has else 0, _DTYPE_CODE[bias.weight.dtype] if has else 0,
-            max(seqs.kv_lens, default=0), scale)
+            span, buckets, _DTYPE_CODE.get(dtype, 0), max(seqs.kv_lens, default=0), scale)
         self.ref = ctypes.byref(self.desc)
         self.tiles = []
         for what, side in enumerate("qqk"):
@@ -216,12 +215,12 @@ class _Plan:
         self.workspace = max(1, int(_lib.load().kf_attention_bwd_workspace(self.tiles[1][1], self.ref)))
 
 
-def _plan(seqs, q, k, v, causal, scale, bias) -> _Plan:
-    key = (q.dtype, q.shape, q.stride(), k.shape, k.stride(), v.stride(), causal, scale,
-           None if bias is None else (bias.weight.dtype, bias.num_buckets, bias.max_distance))
+def _plan(seqs, q, k, v, causal, scale, table) -> _Plan:
+    """``table``: type, buckets and largest distance of the bias, or None."""
+    key = (q.dtype, q.shape, q.stride(), k.shape, k.stride(), v.stride(), causal, scale, table)
     plan = seqs._plans.get(key)
     if plan is None:
-        plan = seqs._plans[key] = _Plan(seqs, q, k, v, causal, scale, bias)
+        plan = seqs._plans[key] = _Plan(seqs, q, k, v, causal, scale, table)
     return plan
 
 
@@ -230,7 +229,8 @@ def _forward(q, k, v, table, seqs, causal, scale, bias, train: bool):
     bf16 output leaves out (delta = dout . o keeps float32's digits) and the
     logarithms of the sums."""
     q, k, v = _vectors(q), _vectors(k), _vectors(v)
-    plan = _plan(seqs, q, k, v, causal, scale, bias)
+    plan = _plan(seqs, q, k, v, causal, scale,
+                 None if bias is None else (bias.weight.dtype, bias.num_buckets, bias.max_distance))
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     rest = lse = None
     if train:
@@ -250,17 +250,20 @@ def _forward(q, k, v, table, seqs, causal, scale, bias, train: bool):
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, seqs, causal, scale, bias):
-        o, rest, lse, ctx.plan = _forward(q, k, v, table, seqs, causal, scale, bias, train=True)
+        o, rest, lse, plan = _forward(q, k, v, table, seqs, causal, scale, bias, train=True)
         ctx.save_for_backward(q, k, v, table, o, rest, lse)
-        ctx.seqs, ctx.buckets = seqs, None if bias is None else bias.buckets  # the tables the plan points to
+        ctx.seqs, ctx.buckets = seqs, None if bias is None else bias.buckets
+        ctx.options = causal, scale, None if bias is None else (table.dtype, bias.num_buckets, bias.max_distance)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, table, o, rest, lse = ctx.saved_tensors
-        plan, need = ctx.plan, ctx.needs_input_grad
+        need = ctx.needs_input_grad
         q, k, v = _vectors(q), _vectors(k), _vectors(v)
+        plan = _plan(ctx.seqs, q, k, v, *ctx.options)  # saved tensors may come back with other strides
+        o, rest, lse = (t if t is None or t.is_contiguous() else t.contiguous() for t in (o, rest, lse))
         if dout.dtype != q.dtype or not dout.is_contiguous() or dout.data_ptr() % 16:
             dout = dout.to(q.dtype).clone(memory_format=torch.contiguous_format)
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)

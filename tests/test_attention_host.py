@@ -123,3 +123,25 @@ def test_transformer_refusals_and_cache():
     both = kb.KANTransformer(48, 1, 6, causal=False)
     with pytest.raises(ValueError):
         both.decode(torch.zeros(3, 48), both.new_cache(3, 4))
+
+
+def test_backward_reads_saved_tensors_by_the_strides_they_have(monkeypatch):
+    """Saved tensors may come back in another layout (offloaded to the host, say): here views of one
+    projection come back contiguous."""
+    import sys
+
+    module = sys.modules["kanforge_b200.attention"]  # the package's name of it is the function
+    calls = []
+    monkeypatch.setattr(module, "_raw_stream", lambda t: 0)
+    monkeypatch.setattr(module, "_launch", lambda name, *args, **kw: calls.append((name, args[-2]._obj)))
+    seqs = kb.PackedSequences([3, 2], device="cpu")
+    for contiguous, rows in ((False, (128, 128, 128)), (True, (64, 32, 32))):
+        qkv = torch.randn(5, 8, 16).bfloat16().requires_grad_()
+        pack = (lambda t: t.clone(memory_format=torch.contiguous_format)) if contiguous else (lambda t: t)
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            out = module._Attention.apply(*qkv.split([4, 2, 2], 1), None, seqs, True, 0.25, None)
+        torch.autograd.grad(out, qkv, torch.ones_like(out))
+        (fwd, f), (bwd, b) = calls
+        calls.clear()
+        assert (fwd, bwd) == ("kf_attention_fwd", "kf_attention_bwd")
+        assert (f.q_row, f.k_row, f.v_row) == (128, 128, 128) and (b.q_row, b.k_row, b.v_row) == rows

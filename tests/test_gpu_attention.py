@@ -452,3 +452,18 @@ def test_slices_of_the_keys_without_work(heads, kv_heads, dim, lens):
     with torch.no_grad():
         for _ in range(50):
             assert torch.equal(kb.attention(q, k, v, seqs), out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_tensors_in_another_layout(dtype):
+    """Views of one projection that come back contiguous, from the host or from any other hook."""
+    lens = [100, 57]
+    qkv = torch.randn(157, 8, 64, generator=torch.Generator(device="cuda").manual_seed(0), device="cuda").to(dtype).requires_grad_()
+    seqs = kb.PackedSequences(lens)
+    grads = []
+    for hooks in (torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t), torch.autograd.graph.save_on_cpu(),
+                  torch.autograd.graph.saved_tensors_hooks(lambda t: t.transpose(0, -1).contiguous(), lambda t: t.transpose(0, -1))):
+        with hooks:
+            out = kb.attention(*qkv.split([4, 2, 2], 1), seqs)
+        grads.append(torch.autograd.grad(out.float().square().sum(), qkv)[0])
+    assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
