@@ -121,7 +121,7 @@ class _ResidualNorm(torch.autograd.Function):
             return (None,) * 10
         need = ctx.needs_input_grad
         call = _Call(x, branch, weight, bias, branch_weight, branch_bias, gate, *ctx.options)
-        x2, w = call.x, call.w
+        x2, w, stats = call.x, call.w, stats.contiguous()  # hooks may give saved tensors back with other strides
         if dy is not None:
             dy = _like(dy, x2)
         if dh is not None:

@@ -259,3 +259,16 @@ def test_many_rows_at_every_division_of_a_row(width, dtype):
     that walk over several."""
     rows = -(-148 * 16 // -(-width // 256)) + 3
     check(inputs((rows, width), "layer", "channel", True, dtype), "layer", 0.9)
+
+
+def test_saved_tensors_in_another_layout():
+    t = inputs((40, 96), "layer", "token", True, torch.float32)
+    grads = []
+    for unpack in (lambda v: v, lambda v: v.transpose(0, -1).contiguous().transpose(0, -1)):
+        leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v, unpack):
+            y, h = kb.residual_norm(leaves["x"], leaves["branch"], leaves["weight"], leaves["bias"], gate=leaves["gate"],
+                                    branch_norm=True, branch_weight=leaves["branch_weight"], branch_bias=leaves["branch_bias"])
+        grads.append(torch.autograd.grad([y, h], list(leaves.values()), [t["x"], t["branch"]]))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
