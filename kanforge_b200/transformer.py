@@ -16,6 +16,8 @@ layers and dropout after each:
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import nn
 
@@ -52,7 +54,11 @@ class KANFFN(nn.Module):
 class KVCache:
     """Keys and values of every layer of a ``KANTransformer`` for a batch of
     sequences, (depth, batch, capacity, kv_heads, head width) each, and how many
-    slots of each sequence are filled (``lengths``, int32 on the device)."""
+    slots of each sequence are filled (``lengths``, int32 on the device).
+
+    Steps in a CUDA graph are counted on the device alone: a replay past the
+    capacity leaves ``lengths`` above it, touches the sequence's last slot and no
+    other memory, and ``KANTransformer.decode`` answers NaN for that sequence."""
 
     def __init__(self, depth: int, batch: int, capacity: int, kv_heads: int, head_dim: int, *, device=None, dtype=None):
         if min(depth, batch, capacity) < 1:
@@ -63,6 +69,7 @@ class KVCache:
         self.batch, self.capacity = batch, capacity
         self.longest = 0  # of ``lengths``, known on the host
         self._rows = torch.arange(batch, device=device)
+        self._last = torch.full((batch,), capacity - 1, device=device)
 
     def begin(self, lens: list[int]) -> tuple[torch.Tensor, torch.Tensor]:
         """Starts the sequences anew with prompts of these lengths: (sequence, slot) of each packed row."""
@@ -79,8 +86,9 @@ class KVCache:
         """Room for one more token of every sequence: its (sequence, slot) rows."""
         if self.longest >= self.capacity:
             raise ValueError(f"the cache is full: {self.capacity} slots")
-        self.longest += 1
-        slot = self.lengths.long()
+        if not (self.lengths.is_cuda and torch.cuda.is_current_stream_capturing()):
+            self.longest += 1
+        slot = torch.minimum(self.lengths, self._last)  # within the cache, whatever the host missed
         self.lengths += 1
         return self._rows, slot
 
@@ -170,4 +178,5 @@ class KANTransformer(nn.Module):
             cache.k[i][at], cache.v[i][at] = k, v
             return attention_decode(q, cache.k[i], cache.v[i], cache.lengths, bias=self.bias)
 
-        return self._run(x, attend)
+        h = self._run(x, attend)
+        return torch.where((cache.lengths > cache.capacity)[:, None], math.nan, h)

@@ -145,3 +145,14 @@ def test_backward_reads_saved_tensors_by_the_strides_they_have(monkeypatch):
         calls.clear()
         assert (fwd, bwd) == ("kf_attention_fwd", "kf_attention_bwd")
         assert (f.q_row, f.k_row, f.v_row) == (128, 128, 128) and (b.q_row, b.k_row, b.v_row) == rows
+
+
+def test_steps_the_host_does_not_count_stay_in_the_cache():
+    """A step replayed from a CUDA graph advances the lengths on the device alone."""
+    cache = kb.KVCache(1, 3, 4, 2, 8)
+    cache.begin([2, 0, 4])
+    for n in range(1, 6):
+        cache.longest = 0  # what the host knows of replays
+        seq, slot = cache.step()
+        assert seq.tolist() == [0, 1, 2] and slot.tolist() == [min(2 + n - 1, 3), min(n - 1, 3), 3]
+        assert cache.lengths.tolist() == [2 + n, n, 4 + n]  # above the capacity: a token too many

@@ -158,3 +158,33 @@ def test_a_decoding_step_replays_from_a_graph():
         graph.replay()
         for a, b in zip((y, h), step()):
             assert torch.equal(a, b)
+
+
+def test_the_models_step_replays_from_a_graph_up_to_the_capacity():
+    """Beyond it the sequences that are full answer NaN; the others go on."""
+    m = model(torch.bfloat16, gate_init=1.0)
+    lens, capacity = [5, 33, 1], 36
+    rows = torch.randn(sum(lens), 48, device=DEV, dtype=torch.bfloat16)
+    tokens = torch.randn(6, 3, 48, device=DEV, dtype=torch.bfloat16)
+    want_cache, cache = m.new_cache(3, 64), m.new_cache(3, capacity)
+    for c in (want_cache, cache):
+        m.prefill(rows, lens, c)
+    x = tokens[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        m.decode(x, cache)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h = m.decode(x, cache)
+    want = [m.decode(t, want_cache) for t in tokens]
+    for n in range(1, 6):
+        x.copy_(tokens[n])
+        graph.replay()
+        full = 33 + n + 1 > capacity
+        assert h[1].isnan().all() == full
+        for s in (0, 2) if full else (0, 1, 2):
+            close(h[s], want[n][s], TOL[torch.bfloat16])
+    assert cache.lengths.tolist() == [n + 6 for n in lens]
+    assert cache.longest == 34  # the prompt and the one step that ran outside the graph
