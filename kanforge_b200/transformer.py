@@ -154,13 +154,22 @@ class KANTransformer(nn.Module):
         block, weight = self.blocks[0], self.start.weight
         return KVCache(len(self.blocks), batch, capacity, block.kv_heads, block.head_dim, device=weight.device, dtype=weight.dtype)
 
-    def _serve(self) -> None:
+    def _serve(self, x: torch.Tensor, rows: int, cache: KVCache) -> None:
+        """The refusals, before the cache is touched."""
         if not self.causal:
             raise ValueError("a model that sees later tokens has no cache")
+        block = self.blocks[0]
+        if cache.k.shape != (len(self.blocks), cache.batch, cache.capacity, block.kv_heads, block.head_dim):
+            raise ValueError(f"a cache of shape {tuple(cache.k.shape)} is not this model's: {len(self.blocks)} layers, "
+                             f"{block.kv_heads} key heads of {block.head_dim}")
+        if cache.k.device != x.device:
+            raise ValueError(f"the cache lies on {cache.k.device}, the tokens on {x.device}")
+        if x.shape != (rows, self.start.dim):
+            raise ValueError(f"x must be ({rows}, {self.start.dim}), not {tuple(x.shape)}")
 
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, lens: list[int], cache: KVCache) -> torch.Tensor:
-        self._serve()
+        self._serve(x, sum(lens), cache)
         at, seqs = cache.begin(lens), PackedSequences(lens, device=x.device)
 
         def attend(i, q, k, v):
@@ -171,7 +180,7 @@ class KANTransformer(nn.Module):
 
     @torch.no_grad()
     def decode(self, x: torch.Tensor, cache: KVCache) -> torch.Tensor:
-        self._serve()
+        self._serve(x, cache.batch, cache)
         at = cache.step()
 
         def attend(i, q, k, v):

@@ -156,3 +156,19 @@ def test_steps_the_host_does_not_count_stay_in_the_cache():
         seq, slot = cache.step()
         assert seq.tolist() == [0, 1, 2] and slot.tolist() == [min(2 + n - 1, 3), min(n - 1, 3), 3]
         assert cache.lengths.tolist() == [2 + n, n, 4 + n]  # above the capacity: a token too many
+
+
+def test_refused_prompts_and_tokens_leave_the_cache_as_it_was():
+    m = kb.KANTransformer(48, 2, 6, 2, 64)
+    cache = m.new_cache(3, 8)
+    cache.begin([2, 1, 3])
+    cache.k.zero_(), cache.v.zero_()
+    others = (kb.KVCache(1, 3, 8, 2, 8), kb.KVCache(2, 3, 8, 6, 8), kb.KVCache(2, 3, 8, 2, 16), kb.KVCache(2, 3, 8, 2, 8, device="meta"))
+    for c in (cache, *others):
+        bad = 1 if c is cache else 3
+        with pytest.raises(ValueError):
+            m.decode(torch.randn(bad, 48), c)  # one row would be stored for all three sequences
+        with pytest.raises(ValueError):
+            m.prefill(torch.randn(1 if c is cache else 5, 48), [2, 1, 2], c)
+        assert c.longest == (3 if c is cache else 0)
+    assert cache.lengths.tolist() == [2, 1, 3] and not cache.k.any() and not cache.v.any()
