@@ -531,7 +531,8 @@ int kf_residual_norm_bwd(const void* x, const void* branch, const void* gate, co
  *           rows.  kf_attention_tiling() gives the rows of a tile for the
  *           forward's queries (pass 0), the backward's queries (1) and its keys
  *           (2), and pack: a sequence of n queries has n * pack rows
- *   table   (n_buckets, heads) in table_dtype, buckets (2 span + 1) int32; null: no bias
+ *   table   (n_buckets, heads) in table_dtype, buckets (2 span + 1) int32, beyond
+ *           [0, n_buckets) counted as the nearest; null: no bias
  *   o       (tq, heads, dim) contiguous; lse (heads, tq) float32, base 2 (null: not written);
  *           o_rest like o, bf16 only: what o's rounding left out, which the
  *           backward needs for dout . o (null: not written)
@@ -569,6 +570,7 @@ typedef struct kf_decode_desc {
   int32_t batch, capacity, heads, kv_heads, dim;
   int32_t dtype, span, table_dtype;
   float scale;
+  int32_t n_buckets; /* rows of the table: buckets beyond count as the last; 0: not given, buckets are taken as they are */
 } kf_decode_desc;
 
 int kf_attention_decode(const void* q, const void* k, const void* v, const int32_t* lengths, const void* table,

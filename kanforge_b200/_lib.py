@@ -106,7 +106,7 @@ class DecodeDesc(ctypes.Structure):
     _fields_ = (
         [(n, _c_i64) for n in ("q_batch", "q_head", "k_batch", "k_row", "k_head", "v_batch", "v_row", "v_head")]
         + [(n, _c_i32) for n in ("batch", "capacity", "heads", "kv_heads", "dim", "dtype", "span", "table_dtype")]
-        + [("scale", ctypes.c_float)]
+        + [("scale", ctypes.c_float), ("n_buckets", _c_i32)]
     )
 
 

@@ -135,13 +135,37 @@ class RelativeBias(nn.Module):
             raise ValueError("heads must be positive")
         self.heads, self.num_buckets, self.max_distance, self.bidirectional = heads, num_buckets, max_distance, bidirectional
         self.weight = nn.Parameter(torch.zeros(num_buckets, heads, device=device, dtype=dtype))
-        buckets = torch.tensor(relative_buckets(num_buckets, max_distance, bidirectional), dtype=torch.int32)
-        self.register_buffer("buckets", buckets if device is None else buckets.to(device), persistent=False)
+        self.register_buffer("buckets", None, persistent=False)
+        self._fill_buckets()
+
+    def _fill_buckets(self) -> torch.Tensor:
+        buckets = relative_buckets(self.num_buckets, self.max_distance, self.bidirectional)
+        self.buckets = torch.tensor(buckets, dtype=torch.int32, device=self.weight.device)
+        return self.buckets
+
+    def _apply(self, fn, recurse=True):
+        # the buckets follow from the arguments: a move that gives them other memory or another type makes them anew
+        # (to_empty() gives memory without contents, and from the meta device there is nothing to copy)
+        before = self._buffers["buckets"]
+        if before.is_meta:
+            self._buffers["buckets"] = None
+        super()._apply(fn, recurse)
+        if self._buffers["buckets"] is not before:
+            self._fill_buckets()
+        return self
+
+    def _tables(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The weight and, where it lies, the buckets."""
+        weight, buckets = self.weight, self.buckets
+        if buckets.device != weight.device or buckets.dtype != torch.int32 or buckets.shape != (2 * self.max_distance + 1,):
+            buckets = self._fill_buckets()  # the weight was put there by itself
+        return weight, buckets
 
     def forward(self, distance: torch.Tensor) -> torch.Tensor:
         """(..., heads): the bias of integer distances query - key."""
+        weight, buckets = self._tables()
         at = distance.clamp(-self.max_distance, self.max_distance) + self.max_distance
-        return self.weight[self.buckets[at].long()]
+        return weight[buckets[at].long()]
 
 
 def _vectors(t: torch.Tensor) -> torch.Tensor:
@@ -179,14 +203,20 @@ def _check_heads(q, k, v, bias, scale) -> tuple[int, int, int]:
     if scale is not None and not 0.0 < scale < math.inf:
         raise ValueError(f"scale must be positive, not {scale}")
     if bias is not None:
-        weight = bias.weight
-        if bias.heads != heads:
-            raise ValueError(f"the bias has {bias.heads} heads, the queries {heads}")
-        if weight.device != device:
-            raise ValueError(f"the bias lies on {weight.device}, the queries on {device}")
-        if weight.dtype not in _DTYPE_CODE:
-            raise TypeError(f"the bias must be float32 or bfloat16, not {weight.dtype}")
+        _check_bias(bias, heads, device)
     return heads, kv_heads, dim
+
+
+def _check_bias(bias: RelativeBias, heads: int, device) -> None:
+    weight = bias._tables()[0]
+    if bias.heads != heads:
+        raise ValueError(f"the bias has {bias.heads} heads, the queries {heads}")
+    if weight.shape != (bias.num_buckets, heads):
+        raise ValueError(f"the bias's weight must be ({bias.num_buckets}, {heads}), not {tuple(weight.shape)}")
+    if weight.device != device:
+        raise ValueError(f"the bias lies on {weight.device}, the queries on {device}")
+    if weight.dtype not in _DTYPE_CODE:
+        raise TypeError(f"the bias must be float32 or bfloat16, not {weight.dtype}")
 
 
 def _raw_stream(t: torch.Tensor) -> int:
@@ -318,11 +348,11 @@ _DECODE_PLANS_MAX = 512
 _decode_plans: dict = {}  # descriptors by what the arguments' checks and the launch look at
 
 
-def _decode_plan(q, k, v, lengths, scale, bias):
+def _decode_plan(q, k, v, lengths, scale, bias, weight):
     """The call's descriptor; arguments like those of an earlier call have been checked then."""
     key = (q.dtype, k.dtype, v.dtype, lengths.dtype, q.device, k.device, v.device, lengths.device, q.shape, k.shape, v.shape,
            lengths.shape, q.stride(), k.stride(), v.stride(), scale,
-           None if bias is None else (bias.weight.dtype, bias.weight.device, bias.weight.shape, bias.max_distance))
+           None if bias is None else (weight.dtype, weight.device, weight.shape, bias.num_buckets, bias.max_distance))
     ref = _decode_plans.get(key)
     if ref is None:
         if q.dim() != 3 or k.dim() != 4 or v.dim() != 4:
@@ -335,8 +365,9 @@ def _decode_plan(q, k, v, lengths, scale, bias):
             raise ValueError(f"lengths must be ({batch},) int32 on {q.device}")
         desc = _lib.DecodeDesc(q.stride(0), q.stride(1), *k.stride()[:3], *v.stride()[:3], batch, capacity, q.shape[1],
                                kv_heads, dim, _DTYPE_CODE[q.dtype], 0 if bias is None else bias.max_distance,
-                               0 if bias is None else _DTYPE_CODE[bias.weight.dtype],
-                               1.0 / math.sqrt(dim) if scale is None else float(scale))
+                               0 if bias is None else _DTYPE_CODE[weight.dtype],
+                               1.0 / math.sqrt(dim) if scale is None else float(scale),
+                               0 if bias is None else bias.num_buckets)
         if len(_decode_plans) >= _DECODE_PLANS_MAX:
             _decode_plans.clear()
         ref = _decode_plans[key] = ctypes.byref(desc)
@@ -353,20 +384,21 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     length of 0 gives 0, one above the capacity counts as the capacity.
     Inference only: tensors that require a gradient raise.
     """
-    plan = _decode_plan(q, k_cache, v_cache, lengths, scale, bias)
+    weight, buckets = (None, None) if bias is None else bias._tables()
+    plan = _decode_plan(q, k_cache, v_cache, lengths, scale, bias, weight)
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
-                                    (bias is not None and bias.weight.requires_grad)):
+                                    (bias is not None and weight.requires_grad)):
         raise RuntimeError("attention_decode has no backward: call it under torch.no_grad(), or use attention")
     aligned = _vectors(q), _vectors(k_cache), _vectors(v_cache)
     if aligned[0] is not q or aligned[1] is not k_cache or aligned[2] is not v_cache:  # copies have strides of their own
         q, k_cache, v_cache = aligned
-        plan = _decode_plan(q, k_cache, v_cache, lengths, scale, bias)
+        plan = _decode_plan(q, k_cache, v_cache, lengths, scale, bias, weight)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     if o.numel() == 0:
         return o
     lengths = lengths.contiguous()
-    table = None if bias is None else bias.weight.detach().contiguous()
+    table = None if bias is None else weight.detach().contiguous()
     _launch("kf_attention_decode", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(),
-            None if table is None else table.data_ptr(), None if bias is None else bias.buckets.data_ptr(), o.data_ptr(),
+            None if table is None else table.data_ptr(), None if bias is None else buckets.data_ptr(), o.data_ptr(),
             plan, _raw_stream(q))
     return o

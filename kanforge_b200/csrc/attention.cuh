@@ -74,7 +74,7 @@ __device__ __forceinline__ float bias_base2(float b) {
 // Bias of one head in base 2, by clamped distance.
 __device__ __forceinline__ void expand_bias_f32(const Args& a, int head, float* out, int thread, int n_threads) {
   for (int i = thread; i < 2 * a.span + 1; i += n_threads) {
-    const int64_t at = (int64_t)a.buckets[i] * a.heads + head;
+    const int64_t at = (int64_t)min(max(a.buckets[i], 0), a.n_buckets - 1) * a.heads + head;
     const float b = a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[at])
                                  : static_cast<const float*>(a.table)[at];
     out[i] = bias_base2(b);

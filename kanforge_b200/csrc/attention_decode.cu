@@ -23,6 +23,8 @@
 // 4 keys at a time (7 caches of up to 600 slots, 5 heads of 40: 12 us).
 #include <cooperative_groups.h>
 
+#include <climits>
+
 #include "attention.cuh"
 
 namespace kf {
@@ -42,7 +44,7 @@ struct DecodeArgs {
   const void* table;
   const int* buckets;
   void* o;  // (B, H, D)
-  int capacity, heads, kv_heads, dim, span;
+  int capacity, heads, kv_heads, dim, span, n_buckets;
   bool table_bf16;
   float scale;
 };
@@ -69,7 +71,7 @@ __device__ __forceinline__ void load_bias(const DecodeArgs& a, const Part<GC>& p
   if (a.table == nullptr || p.first >= p.last) return;
   const int lo = clamp_dist(p.len - p.last, a.span), n = clamp_dist(p.len - 1 - p.first, a.span) - lo + 1;
   for (int i = threadIdx.x; i < n; i += kWarps * 32) {
-    const int64_t at = (int64_t)a.buckets[lo + i] * a.heads + p.head0;
+    const int64_t at = (int64_t)min(max(a.buckets[lo + i], 0), a.n_buckets - 1) * a.heads + p.head0;
     for (int g = 0; g < p.n_g; ++g)
       sbias[g * (2 * a.span + 1) + lo + i] = bias_base2(a.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.table)[at + g])
                                                                      : static_cast<const float*>(a.table)[at + g]);
@@ -458,6 +460,7 @@ extern "C" int kf_attention_decode(const void* q, const void* k, const void* v, 
   KF_CHECK_ARG(d->dtype == KF_DTYPE_F32 || d->dtype == KF_DTYPE_BF16, "%s: types must be float32 or bfloat16", fn);
   KF_CHECK_ARG(d->batch >= 0 && d->batch <= 65535 && d->capacity >= 0, "%s: bad sizes", fn);
   KF_CHECK_ARG(d->span >= 0 && d->span <= attn::kMaxSpan, "%s: bias distances up to %d are outside [0, %d]", fn, d->span, attn::kMaxSpan);
+  KF_CHECK_ARG(d->n_buckets >= 0 && d->n_buckets <= attn::kMaxBuckets, "%s: %d buckets exceed %d", fn, d->n_buckets, attn::kMaxBuckets);
   if (d->batch == 0) return KF_OK;
   KF_CHECK_ARG(q && o && lengths && (d->capacity == 0 || (k && v)), "%s: null argument", fn);
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr), "%s: the bias needs a table and buckets", fn);
@@ -472,6 +475,7 @@ extern "C" int kf_attention_decode(const void* q, const void* k, const void* v, 
   a.q_batch = d->q_batch, a.q_head = d->q_head, a.k_batch = d->k_batch, a.k_row = d->k_row, a.k_head = d->k_head;
   a.v_batch = d->v_batch, a.v_row = d->v_row, a.v_head = d->v_head;
   a.capacity = d->capacity, a.heads = d->heads, a.kv_heads = d->kv_heads, a.dim = d->dim, a.span = d->span;
+  a.n_buckets = d->n_buckets > 0 ? d->n_buckets : INT_MAX;
   a.table_bf16 = d->table_dtype == KF_DTYPE_BF16, a.scale = d->scale;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d->dtype == KF_DTYPE_F32) return launch<attention_decode_f32>(kGroupF32, 0, a, d->batch, st);

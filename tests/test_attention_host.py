@@ -172,3 +172,42 @@ def test_refused_prompts_and_tokens_leave_the_cache_as_it_was():
             m.prefill(torch.randn(1 if c is cache else 5, 48), [2, 1, 2], c)
         assert c.longest == (3 if c is cache else 0)
     assert cache.lengths.tolist() == [2, 1, 3] and not cache.k.any() and not cache.v.any()
+
+
+def test_bias_buckets_survive_every_way_a_module_moves():
+    want = relative_buckets(8, 16, True)
+
+    def right(b):
+        return b.buckets.dtype == torch.int32 and b.buckets.device == b.weight.device and b.buckets.tolist() == want
+
+    b = kb.RelativeBias(3, 8, 16, device="meta").to_empty(device="cpu")
+    assert right(b)
+    with torch.device("meta"):
+        m = kb.KANTransformer(48, 1, 6, causal=False, num_buckets=8, max_distance=16)
+    assert right(m.to_empty(device="cpu").bias)
+    b.buckets.fill_(1 << 30)
+    assert right(b.to_empty(device="cpu")) and right(b.type(torch.float64)) and right(b.bfloat16())
+    kept = b.buckets
+    assert b.to("cpu").buckets is kept  # a move that moves nothing: what a CUDA graph holds stays
+    # weights of a checkpoint assigned to a model without memory
+    b = kb.RelativeBias(3, 8, 16, device="meta")
+    b.load_state_dict({"weight": torch.randn(8, 3)}, assign=True)
+    assert b(torch.tensor([0, -20])).shape == (2, 3) and right(b)
+
+
+def test_bias_whose_weight_has_another_shape_is_refused():
+    from kanforge_b200.attention import _check_bias
+
+    b = kb.RelativeBias(3, 8, 16)
+    _check_bias(b, 3, torch.device("cpu"))
+    b.weight = torch.nn.Parameter(torch.zeros(4, 3))
+    with pytest.raises(ValueError):
+        _check_bias(b, 3, torch.device("cpu"))
+    b.weight = torch.nn.Parameter(torch.zeros(8, 3))
+    b.buckets = b.buckets[:5]
+    _check_bias(b, 3, torch.device("cpu"))
+    assert b.buckets.tolist() == relative_buckets(8, 16, True)
+    with pytest.raises(ValueError):
+        _check_bias(b, 2, torch.device("cpu"))
+    with pytest.raises(TypeError):
+        _check_bias(b.half(), 3, torch.device("cpu"))

@@ -467,3 +467,47 @@ def test_saved_tensors_in_another_layout(dtype):
             out = kb.attention(*qkv.split([4, 2, 2], 1), seqs)
         grads.append(torch.autograd.grad(out.float().square().sum(), qkv)[0])
     assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_bias_whose_tensors_were_put_in_place_one_by_one(dtype):
+    lens = [40, 90]
+    q, k, v, dout = make(lens, lens, 4, 2, 64, dtype)
+    whole = kb.RelativeBias(4, 8, 20, bidirectional=False, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        whole.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
+    moved = kb.RelativeBias(4, 8, 20, bidirectional=False)  # the buckets stay on the host
+    moved.weight = torch.nn.Parameter(whole.weight.detach().clone())
+    emptied = kb.RelativeBias(4, 8, 20, bidirectional=False, device="meta").to_empty(device="cuda").to(dtype)
+    emptied.load_state_dict(whole.state_dict())
+    cache = [t[:100].reshape(2, 50, 2, 64).contiguous() for t in (k, v)]
+    n = torch.tensor([50, 33], dtype=torch.int32, device="cuda")
+    want = None
+    for b in (whole, moved, emptied):
+        out, grads = check(q, k, v, dout, lens, lens, True, bias=b)
+        with torch.no_grad():
+            got = [out, *grads, kb.attention_decode(q[:2], *cache, n, bias=b)]
+        want = want or got
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_buckets_outside_the_table_count_as_the_nearest(dtype):
+    lens = [40, 90]
+    q, k, v, _ = make(lens, lens, 4, 2, 64, dtype)
+    bias = kb.RelativeBias(4, 8, 20, bidirectional=False, device="cuda", dtype=dtype).requires_grad_(False)
+    bias.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
+    cache = [t[:100].reshape(2, 50, 2, 64).contiguous() for t in (k, v)]
+    n = torch.tensor([50, 33], dtype=torch.int32, device="cuda")
+
+    def run():
+        return kb.attention(q, k, v, kb.PackedSequences(lens), bias=bias), kb.attention_decode(q[:2], *cache, n, bias=bias)
+
+    near = bias.buckets.clone()
+    near[25:27], near[30:] = 0, 7
+    far = near.clone()
+    far[25], far[26], far[30:] = -1, -(1 << 31), (1 << 31) - 1
+    bias.buckets.copy_(near)
+    want = run()
+    bias.buckets.copy_(far)
+    assert all(torch.equal(x, y) for x, y in zip(run(), want))
