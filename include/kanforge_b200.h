@@ -533,7 +533,9 @@ int kf_residual_norm_bwd(const void* x, const void* branch, const void* gate, co
  *           (2), and pack: a sequence of n queries has n * pack rows
  *   table   (n_buckets, heads) in table_dtype, buckets (2 span + 1) int32, beyond
  *           [0, n_buckets) counted as the nearest; null: no bias
- *   o       (tq, heads, dim) contiguous; lse (heads, tq) float32, base 2 (null: not written);
+ *   o       (tq, heads, dim) contiguous; lse (heads, tq) float32, base 2 (null: not written; with lse_rest
+ *           two of them: without, the backward is wrong where all of a row's biases are as
+ *           large as masks are, 1e9 or the type's lowest value);
  *           o_rest like o, bf16 only: what o's rounding left out, which the
  *           backward needs for dout . o (null: not written)
  * q, k, v in dtype with the strides of the descriptor (elements; head width
@@ -548,6 +550,7 @@ typedef struct kf_attention_desc {
   int32_t span, n_buckets, table_dtype;
   int32_t longest; /* key rows of the longest sequence: decides how the forward divides its work */
   float scale;
+  int32_t lse_rest; /* 1: lse is (2, heads, tq), the second part what the rounding of the first left out */
 } kf_attention_desc;
 
 int kf_attention_tiling(const kf_attention_desc* desc, int pass, int32_t* rows, int32_t* pack);

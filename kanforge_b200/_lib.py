@@ -96,7 +96,7 @@ class AttentionDesc(ctypes.Structure):
     _fields_ = (
         [(n, _c_i64) for n in ("tq", "tk", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
         + [(n, _c_i32) for n in ("heads", "kv_heads", "dim", "dtype", "causal", "span", "n_buckets", "table_dtype", "longest")]
-        + [("scale", ctypes.c_float)]
+        + [("scale", ctypes.c_float), ("lse_rest", _c_i32)]
     )
 
 

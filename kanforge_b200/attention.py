@@ -234,7 +234,7 @@ class _Plan:
         self.desc = _lib.AttentionDesc(
             q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
             q.shape[1], k.shape[1], q.shape[2], _DTYPE_CODE[q.dtype], int(causal),
-            span, buckets, _DTYPE_CODE.get(dtype, 0), max(seqs.kv_lens, default=0), scale)
+            span, buckets, _DTYPE_CODE.get(dtype, 0), max(seqs.kv_lens, default=0), scale, 1)
         self.ref = ctypes.byref(self.desc)
         self.tiles = []
         for what, side in enumerate("qqk"):
@@ -257,14 +257,14 @@ def _plan(seqs, q, k, v, causal, scale, table) -> _Plan:
 def _forward(q, k, v, table, seqs, causal, scale, bias, train: bool):
     """(o, rest, lse, plan): the output, and for the backward what the rounding of a
     bf16 output leaves out (delta = dout . o keeps float32's digits) and the
-    logarithms of the sums."""
+    logarithms of the sums, with what their rounding leaves out."""
     q, k, v = _vectors(q), _vectors(k), _vectors(v)
     plan = _plan(seqs, q, k, v, causal, scale,
                  None if bias is None else (bias.weight.dtype, bias.num_buckets, bias.max_distance))
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     rest = lse = None
     if train:
-        lse = torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32)
+        lse = torch.empty(2, q.shape[1], q.shape[0], device=q.device, dtype=torch.float32)
         if q.dtype == torch.bfloat16:
             rest = torch.empty_like(o)
     tiles, n = plan.tiles[0]

@@ -7,6 +7,8 @@ namespace {
 
 using namespace attn;
 
+constexpr int kWorkspaceRows = 3;  // of (H, Tq) floats at Args::delta
+
 // The bias gradient by distance: the tiles' sums of one (head, distance), 32
 // distances by 8 slices of the tiles, joined in order.
 __global__ void __launch_bounds__(256) attention_dist(const float* part, int n_tiles, int heads, int n_dist, float* out) {
@@ -80,7 +82,7 @@ Args make_args(const kf_attention_desc* d) {
   Args a{};
   a.heads = d->heads, a.kv_heads = d->kv_heads, a.dim = d->dim, a.span = d->span, a.n_buckets = d->n_buckets;
   a.causal = d->causal != 0, a.table_bf16 = d->table_dtype == KF_DTYPE_BF16;
-  a.scale = d->scale, a.tq = d->tq, a.tk = d->tk, a.longest = d->longest;
+  a.lse_rest = d->lse_rest != 0, a.scale = d->scale, a.tq = d->tq, a.tk = d->tk, a.longest = d->longest;
   a.q = {nullptr, d->q_row, d->q_head};
   a.k = {nullptr, d->k_row, d->k_head};
   a.v = {nullptr, d->v_row, d->v_head};
@@ -148,7 +150,7 @@ extern "C" int kf_attention_fwd(const void* q, const void* k, const void* v, con
 
 extern "C" int64_t kf_attention_bwd_workspace(int32_t n_q_tiles, const kf_attention_desc* d) {
   if (d == nullptr || n_q_tiles < 0) return 0;
-  return 2 * (int64_t)d->heads * d->tq + (d->n_buckets > 0 ? ((int64_t)n_q_tiles + 1) * d->heads * (2 * d->span + 1) : 0);
+  return kf::kWorkspaceRows * (int64_t)d->heads * d->tq + (d->n_buckets > 0 ? ((int64_t)n_q_tiles + 1) * d->heads * (2 * d->span + 1) : 0);
 }
 
 extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout, const float* lse,
@@ -174,7 +176,7 @@ extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, con
   a.dq = dq, a.dk = dk, a.dv = dv, a.table = table, a.buckets = buckets;
   a.tiles = reinterpret_cast<const Tile*>(q_tiles);
   a.delta = workspace;
-  float* dist = workspace + 2 * (int64_t)d->heads * d->tq;  // (H, 2 span + 1), then the tiles' parts
+  float* dist = workspace + kWorkspaceRows * (int64_t)d->heads * d->tq;  // (H, 2 span + 1), then the tiles' parts
   const int n_dist = 2 * d->span + 1;
   a.dist_part = dtable != nullptr ? dist + (int64_t)d->heads * n_dist : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

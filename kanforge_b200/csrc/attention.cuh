@@ -41,8 +41,8 @@ struct Args {
   void* o;      // (Tq, H, D) contiguous; read by the backward
   void* o_rest; // bf16: what the rounding of o left out, for delta; may be null
   void *dq, *dk, *dv;
-  float* lse;   // (H, Tq)
-  float* delta; // (H, Tq): dO . O; bf16: minus that, then (H, Tq) minus lse
+  float* lse;   // (H, Tq), with lse_rest twice: see store_lse
+  float* delta; // (H, Tq): dO . O; bf16: minus that, then (H, Tq) minus lse, then (H, Tq) of which every 32nd of a sequence: beyond kDeep
   const Tile* tiles;
   const void* table;  // (buckets, H) bias, or null
   const int* buckets; // (2 span + 1): bucket of distance index - span
@@ -52,7 +52,7 @@ struct Args {
   int splits;   // of the keys among CTAs (bf16 forward)
   int heads, kv_heads, dim, span, n_buckets;
   int pack;  // heads that are neighbouring rows of a tile (bf16)
-  bool causal, table_bf16;
+  bool causal, table_bf16, lse_rest;
   float scale;
 };
 
@@ -70,6 +70,22 @@ __device__ __forceinline__ bool one_key(const Args& a, const Seq& s, int pos) { 
 __device__ __forceinline__ float bias_base2(float b) {
   return isinf(b) ? b : fminf(fmaxf(b * kLog2e, -CUDART_MAX_NORMAL_F), CUDART_MAX_NORMAL_F);
 }
+
+// With a bias, from this magnitude of it or of a row's maximum on, scores are taken as
+// the float32 numbers that product and bias round to, and lse as two of them: next to
+// a mask of 1e9 or the type's lowest value log2(sum) is less than lse's last digit, and
+// P = 2^(score - lse) would not add up to 1.  Below, P loses at most 2^-12 by that.
+// (Without a bias such scores have lost as much in their own rounding.)
+constexpr float kDeep = 4096.f;
+__device__ __forceinline__ bool deep(float x) { return fabsf(x) >= kDeep && !isinf(x); }
+
+// lse of a row with maximum m and sum l, and what its rounding leaves out.
+__device__ __forceinline__ void store_lse(const Args& a, int64_t at, float m, float l) {
+  const float log = log2f(l), lse = l == 0.f ? 0.f : m + log;
+  a.lse[at] = lse;
+  if (a.lse_rest) a.lse[a.heads * a.tq + at] = l == 0.f ? 0.f : (m - lse) + log;
+}
+__device__ __forceinline__ float load_lse_rest(const Args& a, int64_t at) { return a.lse_rest ? a.lse[a.heads * a.tq + at] : 0.f; }
 
 // Bias of one head in base 2, by clamped distance.
 __device__ __forceinline__ void expand_bias_f32(const Args& a, int head, float* out, int thread, int n_threads) {

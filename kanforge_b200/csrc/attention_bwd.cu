@@ -287,6 +287,8 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
     // a row that sees one key has dS = 0; rows past the sequence likewise
     const float lse_row = valid ? a.lse[stat] : 0.f, lse = valid && !one_key(a, s, pos) ? lse_row : CUDART_INF_F;
     if (valid && half == 0) a.delta[(int64_t)a.heads * a.tq + stat] = -lse_row;
+    const bool large = a.table != nullptr && __any_sync(0xffffffffu, deep(lse_row));  // see kDeep
+    if (valid && half == 0 && lane == 0) a.delta[2 * (int64_t)a.heads * a.tq + stat] = large ? 1.f : 0.f;
     const float c2 = a.scale * kLog2e;
     const float* bias = sbias + a.span + kBiasPad;
     float far_sum[2] = {0.f, 0.f};  // dS at distances >= span, <= -span
@@ -315,11 +317,12 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
       bool near = false;
       float base = -lse;
       if (a.table != nullptr) {
-        near = !__all_sync(0xffffffffu, dist - 63 >= a.span || dist <= -a.span);
+        near = !__all_sync(0xffffffffu, dist - 63 >= a.span || dist <= -a.span) || large;
         if (near) {
           const float* b = bias + max(-a.span - kBiasPad + 63, min(dist, a.span + kBiasPad));
+          const float minus = large ? 0.f : lse;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) x[i] = fmaf(x[i], c2, b[-i] - lse);
+          for (int i = 0; i < 64; ++i) x[i] = fmaf(x[i], c2, b[-i] - minus);
         } else {
           base = (dist > 0 ? bias[a.span] : bias[-a.span]) - lse;
         }
@@ -328,6 +331,11 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas) attention_d
         const uint64_t c2_2 = pair(c2, c2), base_2 = pair(base, base);
 #pragma unroll
         for (int i = 0; i < 64; i += 2) unpair(fma2(pair(x[i], x[i + 1]), c2_2, base_2), x[i], x[i + 1]);
+      }
+      if (large) {
+        const float minus = near ? lse : 0.f, rest = valid ? load_lse_rest(a, stat) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) x[i] = (x[i] - minus) - rest;
       }
 #pragma unroll
       for (int i = 0; i < 64; ++i) x[i] = ex2(x[i]);
@@ -515,7 +523,7 @@ __host__ __device__ constexpr int dkdv_floats(bool bias, int span, int n_buckets
   return Kv<DP>::kStages * 2 * Kv<DP>::kCols + (bias ? Kv<DP>::kGroups * bias_floats(span, n_buckets) : 0);
 }
 
-template <int DP>
+template <int DP, bool BIAS>
 __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
     attention_dkdv_tc(const Args a, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap g_map,
                       const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
@@ -639,10 +647,17 @@ __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
     auto group_sync = [&](bool ok) { return named_bar_and(1 + g, 128, ok); };
     bool ok = true, together = true;
     int head_in = -1;  // whose bias table is there
+    // Whether any row of the group's heads is beyond kDeep: what dQ left for every 32 rows.  (A look at each tile's
+    // statistics instead costs its chain up to 15%, this 1.5 to 3%, for which calls without a bias have a kernel
+    // of their own: 16 packed documents 141 us, with both in one 151.)
+    bool large = false;
+    for (int h = 0; BIAS && a.lse_rest && h < group; ++h)
+      for (int q = lane * 32; q < s.lq; q += 32 * 32) large |= a.delta[2 * (int64_t)a.heads * a.tq + (int64_t)(kv_head * group + h) * a.tq + s.q0 + q] != 0.f;
+    if (BIAS) large = __any_sync(0xffffffffu, large);
     for (int i = g; i < n; i += G) {
       const int st = 2 * i % F::kStages, q0 = (first + i % per_head) * F::kCols, head = kv_head * group + i / per_head;
       const uint32_t phase = (i / G) & 1;
-      if (a.table != nullptr && head != head_in) {
+      if (BIAS && head != head_in) {
         head_in = head;
         if (!(together = group_sync(true))) break;
         expand_bias(a, head, 1, sbias, sbias + bias_stride(a.span), threadIdx.x & 127, 128, [&] { together = group_sync(true); });
@@ -659,8 +674,8 @@ __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
       const ulonglong2* delta = lse + F::kCols / 4;
       const int dist = q0 + off - key;  // of the first column
       float mul = c2, add = 0.f;
-      if (a.table != nullptr) {
-        if (__all_sync(0xffffffffu, dist >= a.span || dist + F::kCols - 1 <= -a.span)) {
+      if (BIAS) {
+        if (__all_sync(0xffffffffu, dist >= a.span || dist + F::kCols - 1 <= -a.span) && !large) {
           add = dist > 0 ? bias[a.span] : bias[-a.span];
         } else {
           const float* b = bias + max(-a.span - kBiasPad, min(dist, a.span + kBiasPad - F::kCols + 1));
@@ -680,8 +695,17 @@ __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
       for (int c = 0; c < F::kCols; ++c) x[c] = ex2(x[c]);
       // columns of queries that see this key: [from, to)
       const int from = a.causal ? key - off - q0 : 0, to = s.lq - q0;
-      const bool masked = __any_sync(0xffffffffu, from > 0 || to < F::kCols || s.lk == 1 || (a.causal && q0 + off <= 0));
+      const bool masked = __any_sync(0xffffffffu, from > 0 || to < F::kCols || s.lk == 1 || (a.causal && q0 + off <= 0)) || large;
       if (masked) {
+        if (large) {  // the scores are their row's maximum or far below it: what is left of lse is a factor
+          const int64_t at = (int64_t)head * a.tq + s.q0 + q0 + lane;
+#pragma unroll
+          for (int h = 0; h < F::kCols / 32; ++h) {
+            const float f = q0 + h * 32 + lane < s.lq ? ex2(-load_lse_rest(a, at + h * 32)) : 0.f;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[h * 32 + c] *= __shfl_sync(0xffffffffu, f, c);
+          }
+        }
 #pragma unroll
         for (int c = 0; c < F::kCols; ++c) x[c] = c >= from && c < to ? x[c] : 0.f;
       }
@@ -720,7 +744,7 @@ __global__ void __launch_bounds__(Kv<DP>::kThreads, Kv<DP>::kCtas)
       tc_fence_before();
       mbar_arrive(&ctl.ds_ready[g]);
     }
-    if (a.table != nullptr && together) together = group_sync(ok);
+    if (BIAS && together) together = group_sync(ok);
     if (ok && together && n > 0) ok = mbar_wait_warp(&ctl.dv_all, 0, abort) && mbar_wait_warp(&ctl.dk_all, 0, abort);
     if (ok && together) {
       tc_fence_after();
@@ -761,9 +785,10 @@ int launch(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t s
   if (n_k > 0) {
     a.tiles = k_tiles;
     const size_t smem = 1024 + Kv<DP>::kFloats + dkdv_floats<DP>(bias, a.span, a.n_buckets) * sizeof(float);
-    static SmemAllowed allowed1;
-    if (int rc = allow_smem(attention_dkdv_tc<DP>, smem, allowed1)) return rc;
-    attention_dkdv_tc<DP><<<(unsigned)n_k * a.kv_heads, Kv<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
+    static SmemAllowed allowed, allowed_bias;
+    auto* kernel = bias ? attention_dkdv_tc<DP, true> : attention_dkdv_tc<DP, false>;
+    if (int rc = allow_smem(kernel, smem, bias ? allowed_bias : allowed)) return rc;
+    kernel<<<(unsigned)n_k * a.kv_heads, Kv<DP>::kThreads, smem, st>>>(a, q_map, g_map, k_map, v_map);
     return check_launch("kf_attention_bwd");
   }
   return KF_OK;

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads) attention_fwd(const Args a) {
     inv[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
     const int r = ty * 4 + i;
     if (a.lse != nullptr && tx == 0 && r < n_rows)
-      a.lse[head * a.tq + s.q0 + r0 + r] = l[i] == 0.f ? 0.f : m[i] + log2f(l[i]);
+      store_lse(a, head * a.tq + s.q0 + r0 + r, m[i], l[i]);
   }
   store_rows<D>(static_cast<float*>(a.o), s.q0 + r0, n_rows, a.heads, head, a.dim, ty, tx, o, inv);
 }
@@ -251,12 +251,13 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
     expand_bias_f32(a, head, sbias, threadIdx.x, kThreads);
     for (int i = threadIdx.x; i < 2 * a.span + 1; i += kThreads) ssum[i] = 0.f;
   }
-  float lse[4], delta[4], far[2] = {0.f, 0.f};  // far: sums beyond the span
+  float lse[4], rest[4], delta[4], far[2] = {0.f, 0.f};  // far: sums beyond the span
   uint64_t dq[4][D / 32];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = ty * 4 + i;
     lse[i] = r < n_rows ? a.lse[head * a.tq + s.q0 + r0 + r] : 0.f;
+    rest[i] = r < n_rows ? load_lse_rest(a, head * a.tq + s.q0 + r0 + r) : 0.f;
     delta[i] = r < n_rows ? a.delta[head * a.tq + s.q0 + r0 + r] : 0.f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) dq[i][c] = 0;
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) attention_dq(const Args a) {
         float v = t[i][j] * c2;
         if (a.table != nullptr) v += sbias[clamp_dist(pos - key, a.span)];
         const bool visible = ty * 4 + i < n_rows && key < s.lk && (!a.causal || key <= pos) && !one_key(a, s, pos);
-        sp[(ty * 4 + i) * kLdP + tx + 16 * j] = visible ? ex2(v - lse[i]) * (dp[i][j] - delta[i]) : 0.f;
+        sp[(ty * 4 + i) * kLdP + tx + 16 * j] = visible ? ex2((v - lse[i]) - rest[i]) * (dp[i][j] - delta[i]) : 0.f;
       }
     }
     __syncwarp();
@@ -335,7 +336,8 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
   float* sp = sg + kTile * Ld<D>::row;
   float* sds = sp + kTile * kLdP;
   float* slse = sds + kTile * kLdP;
-  float* sdelta = slse + kTile;
+  float* srest = slse + kTile;
+  float* sdelta = srest + kTile;
   float* sbias = sdelta + kTile;
   int tile;
   const Seq s = load_tile(a, blockIdx.x / a.kv_heads, &tile);
@@ -362,6 +364,7 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
       if (threadIdx.x < kTile) {
         const bool in = (int)threadIdx.x < n_q;
         slse[threadIdx.x] = in ? a.lse[head * a.tq + s.q0 + q0 + threadIdx.x] : 0.f;
+        srest[threadIdx.x] = in ? load_lse_rest(a, head * a.tq + s.q0 + q0 + threadIdx.x) : 0.f;
         sdelta[threadIdx.x] = in ? a.delta[head * a.tq + s.q0 + q0 + threadIdx.x] : 0.f;
       }
       rows_ready<0>();
@@ -377,7 +380,7 @@ __global__ void __launch_bounds__(kThreads) attention_dkdv(const Args a) {
           float v = t[i][j] * c2;
           if (a.table != nullptr) v += sbias[clamp_dist(pos - key, a.span)];
           const bool visible = c < n_q && key < s.lk && (!a.causal || key <= pos);
-          const float p = visible ? ex2(v - slse[c]) : 0.f;
+          const float p = visible ? ex2((v - slse[c]) - srest[c]) : 0.f;
           sp[(ty * 4 + i) * kLdP + c] = p;
           sds[(ty * 4 + i) * kLdP + c] = visible && !one_key(a, s, pos) ? p * (dp[i][j] - sdelta[c]) : 0.f;
         }
@@ -420,7 +423,7 @@ int bwd(const Args& a0, const Tile* k_tiles, int n_q, int n_k, cudaStream_t st) 
       return rc;
   a.tiles = k_tiles;
   if (n_k > 0)
-    return run<attention_dkdv<D>>((unsigned)n_k * a.kv_heads, 4 * kTile * Ld<D>::row + 2 * kTile * kLdP + 2 * kTile + bias, a, st,
+    return run<attention_dkdv<D>>((unsigned)n_k * a.kv_heads, 4 * kTile * Ld<D>::row + 2 * kTile * kLdP + 3 * kTile + bias, a, st,
                "kf_attention_bwd");
   return KF_OK;
 }

@@ -244,6 +244,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
     mbar_arrive(&ctl.q_full);
     if (a.table != nullptr) named_bar_and(1, F::kSoftmax, true);
     const float* bias = sbias + (a.table != nullptr ? (r - tok * pack) * bias_stride(a.span) + a.span + kBiasPad : 0);
+    // a far bias this large is added score by score, as the near ones are: see kDeep
+    const bool large = a.table != nullptr && __any_sync(0xffffffffu, deep(bias[a.span]) || deep(bias[-a.span]));
     float m = -CUDART_INF_F, l = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
       if (a.table != nullptr) {
         const int dist = pos - k0;  // to the first of the keys
         const bool far = dist - (kKeys - 1) >= a.span || dist <= -a.span;
-        if (__all_sync(0xffffffffu, far)) {
+        if (__all_sync(0xffffffffu, far) && !large) {
           add = dist > 0 ? bias[a.span] : bias[-a.span];
         } else {
           const float* b = bias + max(-a.span - kBiasPad + kKeys - 1, min(dist, a.span + kBiasPad));
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
     if (!SPLIT) {
       if (ok) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (valid && a.lse != nullptr) a.lse[(int64_t)head * a.tq + s.q0 + tok] = l == 0.f ? 0.f : m + log2f(l);
+        if (valid && a.lse != nullptr) store_lse(a, (int64_t)head * a.tq + s.q0 + tok, m, l);
         // D = 128: in whole lines by way of shared memory, O first, what its rounding leaves out after another look at
         // tensor memory (one document of 8191 tokens: 264 us against 279 straight from the registers).  D <= 64: straight,
         // since the other CTA of the SM computes meanwhile (64 x 197 tokens: 79 us against 82 by way of shared memory).
@@ -384,7 +386,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, DP == 64 ? 2 : 1)
         const float lp = peer_load(peer_addr(stat, p) + 4);
         if (lp != 0.f) sum = fmaf(lp, ex2(peer_load(peer_addr(stat, p)) - high), sum);
       }
-      if (slice == 0 && valid && a.lse != nullptr) a.lse[(int64_t)head * a.tq + s.q0 + tok] = sum == 0.f ? 0.f : high + log2f(sum);
+      if (slice == 0 && valid && a.lse != nullptr) store_lse(a, (int64_t)head * a.tq + s.q0 + tok, high, sum);
       const float weight = l == 0.f ? 0.f : ex2(m - high) / sum;
       const uint32_t mine = kv_tile + t * DP * kRows * 4 + row * 4;  // (column, row): neighbouring lanes, neighbouring words
 #pragma unroll

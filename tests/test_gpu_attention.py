@@ -511,3 +511,44 @@ def test_buckets_outside_the_table_count_as_the_nearest(dtype):
     want = run()
     bias.buckets.copy_(far)
     assert all(torch.equal(x, y) for x, y in zip(run(), want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("closed", ["a head", "the first distances", "a head but for the far ones"])
+def test_biases_of_the_lowest_value(closed, causal, heads, kv_heads, dim, dtype):
+    """Rows whose keys all have the type's lowest value as a bias: their scores round to it (in 64 bits, too), so
+    every key weighs the same, forward and backward, near and far."""
+    lens = [1, 2, 90, 400]
+    bias = kb.RelativeBias(heads, 16, 40, bidirectional=not causal, device="cuda", dtype=dtype)
+    low = torch.finfo(dtype).min
+    with torch.no_grad():
+        bias.weight.normal_(0, 0.7, generator=torch.Generator(device="cuda").manual_seed(5))
+        if closed == "the first distances":
+            bias.weight[:3] = low
+        else:
+            bias.weight[:, 1] = low
+        if closed == "a head but for the far ones":
+            bias.weight[7, 1] = bias.weight[15, 1] = 0.5
+    check(*make(lens, lens, heads, kv_heads, dim, dtype), lens, lens, causal, bias=bias)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("low", [-1e4, -1e9, -1e30])
+def test_weights_add_up_to_one_under_any_mask_value(low, dtype):
+    """sum over keys of dV = sum over queries of dO, whatever the rounding of the scores: each row's weights add up
+    to 1 in the backward as in the forward.  bfloat16: each dV is rounded once (2^-9) and the weights are (2^-9);
+    float32: P loses 2^-13 by a score of 1e4 that product and bias round to."""
+    lens = [300]
+    q, k, v, dout = make(lens, lens, 4, 2, 64, dtype)
+    bias = kb.RelativeBias(4, 16, 40, bidirectional=False, device="cuda")
+    with torch.no_grad():
+        bias.weight.fill_(low)
+    v.requires_grad_()
+    out = kb.attention(q, k, v, kb.PackedSequences(lens), bias=bias)
+    dv = torch.autograd.grad(out, v, dout)[0].double()
+    terms = dout.double().reshape(300, 2, 2, 64).sum(2)
+    err = (dv.sum(0) - terms.sum(0)).abs().max()
+    assert err <= (2.0**-8 if dtype == torch.bfloat16 else 2.0**-12) * terms.abs().sum(0).max()
+    assert (out[0].double() - v[0].double().repeat_interleave(2, 0)).abs().max() <= 2.0**-8 * v.abs().max()
