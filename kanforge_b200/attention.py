@@ -19,7 +19,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernels import _check_cuda, _launch
+from .kernels import _check_cuda, _launch, _unwatched
 
 ATTENTION_MAX_DIM = 128
 BIAS_MAX_DISTANCE, BIAS_MAX_BUCKETS = 512, 256
@@ -338,8 +338,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: PackedSeq
         raise ValueError(f"the sequences lie on {seqs.device}, the queries on {q.device}")
     table = None if bias is None else bias.weight
     args = (q, k, v, table, seqs, bool(causal), 1.0 / math.sqrt(dim) if scale is None else float(scale), bias)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
-                                    (table is not None and table.requires_grad)):
+    if not _unwatched() or torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                                        (table is not None and table.requires_grad)):
         return _Attention.apply(*args)
     return _forward(*args, train=False)[0]
 
@@ -389,6 +389,21 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
                                     (bias is not None and weight.requires_grad)):
         raise RuntimeError("attention_decode has no backward: call it under torch.no_grad(), or use attention")
+    if not _unwatched():
+        return _Decode.apply(q, k_cache, v_cache, lengths, weight, buckets, scale, bias)
+    return _decode(q, k_cache, v_cache, lengths, weight, buckets, scale, bias, plan)
+
+
+class _Decode(torch.autograd.Function):
+    """``_decode`` where something watches the call; it has no derivative."""
+
+    @staticmethod
+    def forward(ctx, q, k_cache, v_cache, lengths, weight, buckets, scale, bias):
+        return _decode(q, k_cache, v_cache, lengths, weight, buckets, scale, bias,
+                       _decode_plan(q, k_cache, v_cache, lengths, scale, bias, weight))
+
+
+def _decode(q, k_cache, v_cache, lengths, weight, buckets, scale, bias, plan):
     aligned = _vectors(q), _vectors(k_cache), _vectors(v_cache)
     if aligned[0] is not q or aligned[1] is not k_cache or aligned[2] is not v_cache:  # copies have strides of their own
         q, k_cache, v_cache = aligned

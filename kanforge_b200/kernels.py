@@ -20,6 +20,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._init import silu_derivative_polys
@@ -99,6 +100,13 @@ def _check_cuda(*ts) -> None:
     for t in ts:
         if t is not None and t.device.type != "cuda":
             raise RuntimeError(f"kanforge_b200 kernels run on CUDA tensors only (got a {t.device} tensor)")
+
+
+def _unwatched() -> bool:
+    """Whether a call that needs no gradient may go round its autograd function: inside a
+    forward-mode level an input may carry a tangent, which the function refuses to drop,
+    and a trace sees only what goes through it."""
+    return forward_ad._current_level < 0 and not torch._C._is_tracing()
 
 
 # --- raw launches (no autograd) ---------------------------------------------

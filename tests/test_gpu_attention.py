@@ -552,3 +552,42 @@ def test_weights_add_up_to_one_under_any_mask_value(low, dtype):
     err = (dv.sum(0) - terms.sum(0)).abs().max()
     assert err <= (2.0**-8 if dtype == torch.bfloat16 else 2.0**-12) * terms.abs().sum(0).max()
     assert (out[0].double() - v[0].double().repeat_interleave(2, 0)).abs().max() <= 2.0**-8 * v.abs().max()
+
+
+def derivative_calls():
+    """(name, function, inputs) of calls that need no gradient."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    seqs, w = kb.PackedSequences([5, 3]), r(32)
+    n = torch.tensor([4, 7], dtype=torch.int32, device="cuda")
+    return [("attention", lambda q, k, v: kb.attention(q, k, v, seqs), (r(8, 4, 16), r(8, 2, 16), r(8, 2, 16))),
+            ("attention_decode", lambda q, k, v: kb.attention_decode(q, k, v, n), (r(2, 4, 16), r(2, 9, 2, 16), r(2, 9, 2, 16))),
+            ("residual_norm", lambda x, b: kb.residual_norm(x, b, w, kind="rms")[1], (r(6, 32), r(6, 32))),
+            ("first norm", lambda x: kb.residual_norm(x, None, w, kind="rms")[1], (r(6, 32),))]
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_forward_mode_derivatives_are_refused_not_dropped(i):
+    from torch.autograd import forward_ad
+
+    _, f, args = derivative_calls()[i]
+    want = f(*args)
+    for j in range(len(args)):
+        with forward_ad.dual_level():
+            assert torch.equal(f(*args), want)  # no input carries a tangent
+            dual = [forward_ad.make_dual(a, torch.ones_like(a)) if k == j else a for k, a in enumerate(args)]
+            with pytest.raises(NotImplementedError):
+                f(*dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                f(*dual)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("i", range(4))
+def test_a_traced_call_computes(i):
+    _, f, args = derivative_calls()[i]
+    with torch.no_grad():
+        traced = torch.jit.trace(f, args, check_trace=False)
+        other = [a * 0.5 + 0.25 for a in args]
+        for a in (args, other):
+            assert torch.equal(traced(*a), f(*a))
