@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
+#include <mutex>
 #include <string>
 
 #include "../../include/kanforge_b200.h"
@@ -49,21 +50,27 @@ int check_launch(const char* what);
 int bind_device(const void* ptr);
 
 // Lets a kernel use `bytes` of dynamic shared memory on the current device; asks
-// the runtime only when that is more than `allowed`, a static of the caller's
-// launch site, says.
+// the runtime only when that is more than `allowed`, a static of the kernel's one
+// launch site, says.  The runtime's limit may be lowered, too, so host threads ask
+// in turn and only for more.
 struct SmemAllowed {
-  std::atomic<int> bytes[16];
+  static constexpr int kDevices = 64;
+  std::atomic<int> bytes[kDevices];
+  std::mutex asking;
 };
 template <typename K>
 inline int allow_smem(K* kernel, size_t bytes, SmemAllowed& allowed) {
   int dev = 0;
   KF_CUDA_RET(cudaGetDevice(&dev));
-  std::atomic<int>* slot = dev < 16 ? &allowed.bytes[dev] : nullptr;
-  if (slot != nullptr && slot->load(std::memory_order_relaxed) >= (int)bytes) return KF_OK;
+  KF_CHECK_ARG(dev < SmemAllowed::kDevices, "device %d: at most %d in a process", dev, SmemAllowed::kDevices);
+  std::atomic<int>& limit = allowed.bytes[dev];
+  if (limit.load(std::memory_order_acquire) >= (int)bytes) return KF_OK;
+  std::lock_guard<std::mutex> turn(allowed.asking);
+  if (limit.load(std::memory_order_relaxed) >= (int)bytes) return KF_OK;
   const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (err != cudaSuccess) cudaGetLastError();  // a refusal is this call's, not the next launch's
   KF_CUDA_RET(err);
-  if (slot != nullptr) slot->store((int)bytes, std::memory_order_relaxed);
+  limit.store((int)bytes, std::memory_order_release);
   return KF_OK;
 }
 
