@@ -33,7 +33,8 @@ class PackedSequences:
     ``q_lens`` are the query rows of each sequence and ``kv_lens`` (default: the
     same) its key and value rows; a sequence's queries stand at the last of its
     positions.  Zero lengths are allowed.  Build it once for a batch layout and
-    pass it to every layer's call; the tables lie on ``device``.
+    pass it to every layer's call, on any stream; the tables lie on ``device``.
+    A CUDA graph that holds such a call needs it kept, as it does the tensors.
     """
 
     def __init__(self, q_lens, kv_lens=None, device="cuda"):
@@ -227,7 +228,7 @@ class _Plan:
     """What a call's shapes decide: the descriptor, the tiles of the forward's
     queries, the backward's queries and its keys, the backward's workspace."""
 
-    __slots__ = ("desc", "ref", "tiles", "workspace")
+    __slots__ = ("desc", "ref", "tables", "tiles", "workspace", "streams")
 
     def __init__(self, seqs, q, k, v, causal, scale, table):
         dtype, buckets, span = table or (None, 0, 0)
@@ -236,13 +237,27 @@ class _Plan:
             q.shape[1], k.shape[1], q.shape[2], _DTYPE_CODE[q.dtype], int(causal),
             span, buckets, _DTYPE_CODE.get(dtype, 0), max(seqs.kv_lens, default=0), scale, 1)
         self.ref = ctypes.byref(self.desc)
-        self.tiles = []
+        self.tables, self.tiles, self.streams = [], [], set()
         for what, side in enumerate("qqk"):
             rows, pack = ctypes.c_int32(), ctypes.c_int32()
             _lib.call("kf_attention_tiling", self.ref, what, ctypes.byref(rows), ctypes.byref(pack))
             t = seqs._entries(side, rows.value, causal, pack.value)
+            self.tables.append(t)
             self.tiles.append((t.data_ptr(), t.shape[0]))
         self.workspace = max(1, int(_lib.load().kf_attention_bwd_workspace(self.tiles[1][1], self.ref)))
+
+
+def _plan_stream(plan: _Plan, t: torch.Tensor) -> int:
+    """The current stream of t's device, which from now on may read the plan's tables: they were
+    allocated on the stream of the first call, and when the sequences go their memory must not
+    be given away while another stream still reads it."""
+    raw = _raw_stream(t)
+    if raw not in plan.streams:
+        plan.streams.add(raw)
+        for table in plan.tables:
+            if table.is_cuda:
+                table.record_stream(torch.cuda.current_stream(table.device))
+    return raw
 
 
 def _plan(seqs, q, k, v, causal, scale, table) -> _Plan:
@@ -273,7 +288,7 @@ def _forward(q, k, v, table, seqs, causal, scale, bias, train: bool):
         _launch("kf_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), tiles, n,
                 None if table is None else table.data_ptr(), None if table is None else bias.buckets.data_ptr(),
                 o.data_ptr(), None if rest is None else rest.data_ptr(), None if lse is None else lse.data_ptr(),
-                plan.ref, _raw_stream(q))
+                plan.ref, _plan_stream(plan, q))
     return o, rest, lse, plan
 
 
@@ -308,7 +323,7 @@ class _Attention(torch.autograd.Function):
                     None if rest is None else rest.data_ptr(), dout.data_ptr(), lse.data_ptr(),
                     q_tiles, n_q, k_tiles, n_k, None if tab is None else tab.data_ptr(),
                     None if tab is None else ctx.buckets.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                    None if dtable is None else dtable.data_ptr(), ws.data_ptr(), plan.ref, _raw_stream(q),
+                    None if dtable is None else dtable.data_ptr(), ws.data_ptr(), plan.ref, _plan_stream(plan, q),
                     kernels=2 + (q.dtype == torch.float32) + 2 * want)
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable, None, None, None, None)
 

@@ -591,3 +591,24 @@ def test_a_traced_call_computes(i):
         other = [a * 0.5 + 0.25 for a in args]
         for a in (args, other):
             assert torch.equal(traced(*a), f(*a))
+
+
+def test_tables_outlive_the_calls_that_read_them_on_another_stream():
+    q = torch.randn(347, 2, 64, device="cuda")
+    seqs = kb.PackedSequences([300, 40, 7])
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        want = kb.attention(q, q, q, seqs)
+    tables = {t.data_ptr() for t in seqs._tiles.values()}
+    torch.cuda.synchronize()
+    with torch.cuda.stream(second):
+        torch.cuda._sleep(400_000_000)  # some 0.2 s
+        got = kb.attention(q, q, q, seqs)
+    del seqs
+    with torch.cuda.stream(first):
+        new = [torch.empty(8, 8, dtype=torch.int32, device="cuda") for _ in range(64)]
+    assert not second.query(), "the call was over too soon to tell"
+    assert not tables & {t.data_ptr() for t in new}
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
