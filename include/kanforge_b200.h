@@ -493,7 +493,7 @@ int kf_sparse_wgrad(const float* x, const float* dy, const float* coef, const fl
  * dh, dbranch and a token gate (rows, width) in branch_dtype (x_dtype bf16 with
  * a float32 branch is refused); w, s, bw, bs and a channel gate (width) in
  * param_dtype.  s, bs, gate may be null; branch null: h = N(x) w + s alone, y
- * is x.  stats (rows, 4) float32 receives mean and 1/std of y and of the
+ * is x.  stats (rows, 4) float32, at a multiple of 16 bytes, receives mean and 1/std of y and of the
  * branch for the backward (null: not written).  width 1 .. 8192.
  * Backward: y is formed again from x and the branch; dy or dh may be null (no gradient); dw, ds, dbw, dbs and a channel
  * gate's dgate may be null when not wanted; their sums over rows run in a fixed

@@ -162,11 +162,14 @@ extern "C" int kf_attention_bwd(const void* q, const void* k, const void* v, con
   if (int rc = check_attention("kf_attention_bwd", d)) return rc;
   KF_CHECK_ARG(n_q_tiles >= 0 && n_k_tiles >= 0 && (int64_t)std::max(n_q_tiles, n_k_tiles) * d->heads < (1ll << 31),
                "kf_attention_bwd: bad tile count");
-  KF_CHECK_ARG(n_q_tiles == 0 || (q && o && dout && lse && dq && workspace && q_tiles), "kf_attention_bwd: null argument");
-  KF_CHECK_ARG(n_k_tiles == 0 || (k && v && dk && dv && k_tiles), "kf_attention_bwd: null argument");
+  const bool any = n_q_tiles > 0 || n_k_tiles > 0;  // each pass reads the rows of both sides
+  KF_CHECK_ARG(!any || d->tq == 0 || (q && o && dout && lse && workspace), "kf_attention_bwd: null argument");
+  KF_CHECK_ARG(!any || d->tk == 0 || (k && v), "kf_attention_bwd: null argument");
+  KF_CHECK_ARG(n_q_tiles == 0 || (d->tq > 0 && dq && q_tiles), "kf_attention_bwd: null argument");
+  KF_CHECK_ARG(n_k_tiles == 0 || (d->tk > 0 && dk && dv && k_tiles), "kf_attention_bwd: null argument");
   KF_CHECK_ARG((table == nullptr) == (buckets == nullptr) && (table == nullptr || d->n_buckets > 0), "kf_attention_bwd: the bias needs a table and buckets");
   KF_CHECK_ARG(dtable == nullptr || (table != nullptr && workspace != nullptr), "kf_attention_bwd: dtable needs a table and workspace");
-  KF_CHECK_ARG(n_q_tiles == 0 || d->dtype == KF_DTYPE_F32 || o_rest != nullptr, "kf_attention_bwd: bf16 needs o_rest");
+  KF_CHECK_ARG(!any || d->tq == 0 || d->dtype == KF_DTYPE_F32 || o_rest != nullptr, "kf_attention_bwd: bf16 needs o_rest");
   KF_CHECK_ARG(rows_aligned(d, {q, k, v, o, o_rest, dout, dq, dk, dv, q_tiles, k_tiles}),
                "kf_attention_bwd: rows must start at multiples of 16 bytes");
   if (n_q_tiles == 0 && n_k_tiles == 0 && dtable == nullptr) return KF_OK;

@@ -828,6 +828,7 @@ extern "C" int kf_residual_norm_fwd(const void* x, const void* branch, const voi
                "kf_residual_norm_fwd: a gate, a branch norm or a residual scale needs a branch");
   KF_CHECK_ARG(!d->branch_norm || bw != nullptr, "kf_residual_norm_fwd: the branch norm has no weight");
   KF_CHECK_ARG(!d->gate_token || gate != nullptr, "kf_residual_norm_fwd: a gate per token is missing");
+  KF_CHECK_ARG(reinterpret_cast<uintptr_t>(stats) % 16 == 0, "kf_residual_norm_fwd: stats must start at a multiple of 16 bytes");
   if (rows == 0) return KF_OK;
   if (int rc = bind_device(x)) return rc;
   RowArgs a = row_args(d, rows);
@@ -859,6 +860,7 @@ extern "C" int kf_residual_norm_bwd(const void* x, const void* branch, const voi
   KF_CHECK_ARG(rows == 0 || gate == nullptr || !d->gate_token || dgate != nullptr, "kf_residual_norm_bwd: the token gate needs dgate");
   KF_CHECK_ARG(!d->branch_norm || bw != nullptr, "kf_residual_norm_bwd: the branch norm has no weight");
   KF_CHECK_ARG(rows == 0 || !d->gate_token || gate != nullptr, "kf_residual_norm_bwd: a gate per token is missing");
+  KF_CHECK_ARG(reinterpret_cast<uintptr_t>(stats) % 16 == 0, "kf_residual_norm_bwd: stats must start at a multiple of 16 bytes");
   if (int rc = bind_device(workspace)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int ctas = 0;

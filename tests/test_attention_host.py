@@ -211,3 +211,26 @@ def test_bias_whose_weight_has_another_shape_is_refused():
         _check_bias(b, 2, torch.device("cpu"))
     with pytest.raises(TypeError):
         _check_bias(b.half(), 3, torch.device("cpu"))
+
+
+def test_entry_points_refuse_pointers_that_would_fault():
+    import ctypes
+
+    from kanforge_b200 import _lib
+
+    lib, p, odd = _lib.load(), ctypes.c_void_p(64), ctypes.c_void_p(68)
+    # the statistics are read and written 16 bytes at a time
+    d = ctypes.byref(_lib.ResidualNormDesc(width=8, residual_scale=1.0))
+    assert lib.kf_residual_norm_fwd(p, None, None, p, None, None, None, None, p, odd, 1, d, None) == 1
+    assert "16 bytes" in _lib.last_error()
+    assert lib.kf_residual_norm_bwd(p, None, None, p, None, None, odd, p, p, p, *[None] * 6, p, 1, d, None) == 1
+    assert "16 bytes" in _lib.last_error()
+    # both passes read the rows of both sides, whichever tiles are given
+    for dtype, rest in ((0, None), (1, p)):
+        d = ctypes.byref(_lib.AttentionDesc(tq=4, tk=4, q_row=64, q_head=64, k_row=64, k_head=64, v_row=64, v_head=64, heads=1,
+                                            kv_heads=1, dim=64, dtype=dtype, scale=1.0))
+        for missing in range(7):  # q, k, v, o, dout, lse, workspace
+            q, k, v, o, g, lse, ws = (None if i == missing else p for i in range(7))
+            for n_q, n_k in ((0, 1), (1, 0), (1, 1)):
+                assert lib.kf_attention_bwd(q, k, v, o, rest, g, lse, p, n_q, p, n_k, None, None, p, p, p, None, ws, d, None) == 1, missing
+                assert "null argument" in _lib.last_error()
