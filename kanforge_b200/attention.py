@@ -89,6 +89,9 @@ class PackedSequences:
     def __len__(self) -> int:
         return len(self.q_lens)
 
+    def __getstate__(self) -> dict:  # for copies and pickles: plans hold addresses
+        return {**self.__dict__, "_tiles": {}, "_plans": {}}
+
 
 def relative_buckets(num_buckets: int, max_distance: int, bidirectional: bool) -> list[int]:
     """Bucket of every distance position - key from -max_distance to max_distance.

@@ -234,3 +234,20 @@ def test_entry_points_refuse_pointers_that_would_fault():
             for n_q, n_k in ((0, 1), (1, 0), (1, 1)):
                 assert lib.kf_attention_bwd(q, k, v, o, rest, g, lse, p, n_q, p, n_k, None, None, p, p, p, None, ws, d, None) == 1, missing
                 assert "null argument" in _lib.last_error()
+
+
+def test_sequences_copy_and_pickle_after_use():
+    """What is kept for calls stays behind: addresses, and descriptors that do not copy."""
+    import copy
+    import pickle
+
+    from kanforge_b200.attention import _plan
+
+    seqs = kb.PackedSequences([3, 2], [4, 2], device="cpu")
+    q, k = torch.randn(5, 4, 16), torch.randn(6, 2, 16)
+    _plan(seqs, q, k, k, True, 0.25, None)
+    for other in (copy.copy(seqs), copy.deepcopy(seqs), pickle.loads(pickle.dumps(seqs))):
+        assert (other.q_lens, other.kv_lens, other.total_q, other.total_kv) == ([3, 2], [4, 2], 5, 6)
+        assert other.table.tolist() == seqs.table.tolist() and other.device == seqs.device
+        plan, mine = _plan(other, q, k, k, True, 0.25, None), _plan(seqs, q, k, k, True, 0.25, None)
+        assert plan is not mine and all(a is not b for a, b in zip(plan.tables, mine.tables))
