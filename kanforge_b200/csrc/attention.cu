@@ -62,9 +62,9 @@ int check_attention(const char* fn, const kf_attention_desc* d) {
 // and its keys (2), and how many neighbouring rows are heads of one token.
 // bf16 packs the heads that share a key head, unless their bias tables would
 // not fit in shared memory (with D <= 64: twice an SM).  Few queries then fill a
-// tile: 32 x 16 queries of 32 heads of 128 on 8 key heads over 4096 keys take 123 us,
-// unpacked 360; 16 documents of up to 2000 tokens, 12 heads of 64 on 4: 98 and 101 us;
-// one of 8191, 16 heads of 128 on 4: 279 and 271 us.
+// tile: 32 x 16 queries of 32 heads of 128 on 8 key heads over 4096 keys take 120 us,
+// unpacked 353; 16 documents of up to 2000 tokens, 12 heads of 64 on 4: 85 and 91 us;
+// one of 8191, 16 heads of 128 on 4: 238 and 241 us.
 void tiling(const kf_attention_desc* d, int pass, int32_t* rows, int32_t* pack) {
   *pack = 1;
   *rows = d->dtype == KF_DTYPE_F32 ? 64 : pass == 0 && d->dim > 64 ? 256 : 128;

@@ -20,7 +20,7 @@
 // Measured, cold caches, causal: 8191 tokens, 16 heads of 128 on 4 key heads: dQ
 // 0.37 ms (1.1 PFLOP/s), dK dV 0.63 ms (0.88 PFLOP/s; of 1.63 measured for bf16);
 // 32 x 1024 tokens, 12 heads of 64 with a bias and its gradient: 0.26 ms (300 TFLOP/s)
-// and 0.27 ms (380 TFLOP/s).  The chain S -> P -> dP -> dS -> product of a tile bounds
+// and 0.28 ms (370 TFLOP/s).  The chain S -> P -> dP -> dS -> product of a tile bounds
 // them, of which tensor memory holds two an SM.  dK dV with four MMA warps (0.72 ms
 // for the first) or with P and dS in columns of their own, one CTA an SM (0.69 ms,
 // and 0.37 for the second) were slower.

@@ -20,16 +20,17 @@
 // issues Q K^T and one that issues P V: issuing blocks while the tensor cores
 // are behind, and neither product should wait for the other's turn.
 //
-// Measured, cold caches, causal: 8191 tokens, 16 heads of 128 on 4 key heads 0.25 ms
-// (1.1 PFLOP/s, 0.68 of the measured bf16 rate); 32 x 1024 tokens, 12 heads of 64
+// Measured, cold caches, causal: 8191 tokens, 16 heads of 128 on 4 key heads 0.24 ms
+// (1.15 PFLOP/s, 0.70 of the measured bf16 rate); 32 x 1024 tokens, 12 heads of 64
 // with a bias 0.18 ms (290 TFLOP/s); 64 x 197 tokens both ways with a bias 67 us, where
 // about half of a CTA's time is its loop, the rest its set-up, queries, bias table
 // and output: code that runs once costs the fetching of its instructions, so it is
-// kept in loops (77 us unrolled).  What is left is the way of one row tile
-// through a thread (scores out of tensor memory, maximum, 64 exponentials, weights
-// back), which two row tiles an SM do not hide altogether: the tensor cores wait
-// for the weights, with D = 64 most of the time, since a product there is half as
-// long and the exponentials are as many.
+// kept in loops (77 us unrolled).  No pipe is full: what the time goes to is the way
+// of one row tile through a thread (scores out of tensor memory, maximum, 64
+// exponentials, weights back), which two row tiles an SM do not hide altogether.
+// The tensor cores wait for the weights, with D = 64 most of the time, since a
+// product there is half as long and the exponentials are as many.  Two threads to
+// a row would halve that way; that has not been tried.
 #include "attention_tc.cuh"
 
 namespace kf {

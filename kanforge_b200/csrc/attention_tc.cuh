@@ -1,6 +1,7 @@
 // Building blocks of the bf16 attention kernels on the tensor cores: one-CTA
-// tcgen05 instructions, tile loads by cp.async into the 128-byte swizzled
-// layout, and the softmax arithmetic shared by forward and backward.
+// tcgen05 instructions, tile loads into the 128-byte swizzled layout (by TMA; the
+// forward's queries, whose rows may be heads of one token, by cp.async), and the
+// softmax arithmetic shared by forward and backward.
 #pragma once
 
 #include "attention.cuh"

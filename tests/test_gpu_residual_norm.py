@@ -1,9 +1,8 @@
 """Residual norm (kf_residual_norm_fwd / _bwd) against its formulas in float64.
 
 Tolerance, max|a - b| / max(1, max|b|): 1e-5 for float32 tensors and 2e-2 for
-bfloat16 ones, the framework's own.  A bfloat16 output is rounded once (2^-9);
-in the backward y is read back rounded, which moves the normed rows by 2^-9 of
-their largest element again.  The float32 parameter gradients sum up to 4096
+bfloat16 ones, the framework's own.  A bfloat16 output is rounded once (2^-9); the
+backward forms y again from x and the branch, without that rounding.  The float32 parameter gradients sum up to 4096
 rows of float32 products: 4096 * 2^-24 = 2.4e-4 of the largest term at the very
 worst, some 1e-6 of the result with errors of either sign.
 """
