@@ -603,7 +603,7 @@ def test_tables_outlive_the_calls_that_read_them_on_another_stream():
     tables = {t.data_ptr() for t in seqs._tiles.values()}
     torch.cuda.synchronize()
     with torch.cuda.stream(second):
-        torch.cuda._sleep(400_000_000)  # some 0.2 s
+        torch.cuda._sleep(1_500_000_000)  # some 0.8 s
         got = kb.attention(q, q, q, seqs)
     del seqs
     with torch.cuda.stream(first):
