@@ -153,9 +153,11 @@ class RelativeBias(nn.Module):
         before = self._buffers["buckets"]
         if before.is_meta:
             self._buffers["buckets"] = None
-        super()._apply(fn, recurse)
-        if self._buffers["buckets"] is not before:
-            self._fill_buckets()
+        try:
+            super()._apply(fn, recurse)
+        finally:
+            if self._buffers["buckets"] is not before:
+                self._fill_buckets()
         return self
 
     def _tables(self) -> tuple[torch.Tensor, torch.Tensor]:

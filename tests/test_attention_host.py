@@ -251,3 +251,11 @@ def test_sequences_copy_and_pickle_after_use():
         assert other.table.tolist() == seqs.table.tolist() and other.device == seqs.device
         plan, mine = _plan(other, q, k, k, True, 0.25, None), _plan(seqs, q, k, k, True, 0.25, None)
         assert plan is not mine and all(a is not b for a, b in zip(plan.tables, mine.tables))
+
+
+def test_bias_after_a_move_that_failed():
+    b = kb.RelativeBias(3, 8, 16, device="meta")
+    with pytest.raises(NotImplementedError):
+        b.to("cpu")  # the weight has nothing to copy
+    assert b.buckets.is_meta
+    assert b.to_empty(device="cpu").buckets.tolist() == relative_buckets(8, 16, True)
