@@ -178,7 +178,7 @@ def _vectors(t: torch.Tensor) -> torch.Tensor:
     """t, or a contiguous copy when its rows cannot be read in 16-byte vectors
     (contiguous tensors can: the head width is a multiple of 8)."""
     if t.data_ptr() % 16 == 0:
-        if t.is_contiguous():
+        if t.is_contiguous() and t.numel():  # without elements, whatever the strides
             return t
         per = 16 // t.element_size()
         if t.stride(-1) == 1 and all(s % per == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):

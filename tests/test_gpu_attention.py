@@ -612,3 +612,17 @@ def test_tables_outlive_the_calls_that_read_them_on_another_stream():
     assert not tables & {t.data_ptr() for t in new}
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_rows_with_odd_strides(dtype):
+    """Tensors without elements count as contiguous whatever their strides."""
+    full = torch.randn(3, 2, 19, device="cuda").to(dtype)[..., 2:18]
+    none = torch.randn(0, 2, 19, device="cuda").to(dtype)[..., 2:18]
+    for q, kv, lens in ((full, none, ([3], [0])), (none, full, ([0], [3]))):
+        leaves = [t.detach().requires_grad_() for t in (q, kv, kv)]
+        out = kb.attention(*leaves, kb.PackedSequences(*lens))
+        assert out.shape == q.shape and not out.any()
+        assert not any(g.any() for g in torch.autograd.grad(out, leaves, torch.ones_like(out)))
+    cache = torch.randn(3, 0, 2, 19, device="cuda").to(dtype)[..., 2:18]
+    assert not kb.attention_decode(full, cache, cache, torch.ones(3, dtype=torch.int32, device="cuda")).any()
